@@ -49,7 +49,7 @@ def listed() -> list[dict]:
         dict(name="verify_one", kind="verify", dtype="bf16", S=1, n=4, V=QWEN_VOCAB, temperature=1.0, draft="model",
              ragged=False),
         # Drafts looked up rather than sampled (no draft distribution), odd f32 rows, drafts of all lengths.
-        dict(name="verify_lookup", kind="verify", dtype="f32", S=48, n=6, V=GPT_VOCAB, temperature=0.7, draft="lookup",
+        dict(name="verify_lookup", kind="verify", dtype="f32", S=48, n=6, V=GPT_VOCAB, temperature=0.75, draft="lookup",
              ragged=True),
         # Greedy decoding of 16 rollouts: drafted tokens against the target's largest logits.
         dict(name="verify_greedy", kind="verify", dtype="f32", S=16, n=5, V=QWEN_VOCAB, temperature=0.0, draft="lookup",
@@ -76,7 +76,7 @@ def draw(rng) -> dict:
     if kind == "top":
         # Up to the largest listed rows (1.2 GB).
         R = _log_int(rng, 1, min(8192, 4096 * QWEN_VOCAB * 2 // (V * size)))
-        return dict(kind=kind, dtype=dtype, R=R, V=V, k=_log_int(rng, 1, 256), temperature=rng.choice([1.0, 0.7, 2.0]),
+        return dict(kind=kind, dtype=dtype, R=R, V=V, k=_log_int(rng, 1, 256), temperature=rng.choice([1.0, 0.75, 2.0]),
                     ids=rng.choice(["i32", "i64"]))
     if kind == "distill":
         out = rng.choice([dtype, dtype, "f32"])
@@ -91,7 +91,7 @@ def draw(rng) -> dict:
     n = rng.randint(1, 12)
     # Up to the largest listed rows (0.33 GB).
     S = _log_int(rng, 1, max(1, min(256, 64 * 17 * QWEN_VOCAB * 2 // ((2 * n + 1) * V * size))))
-    temperature = rng.choice([0.0, 0.7, 1.0, 1.0])
+    temperature = rng.choice([0.0, 0.75, 1.0, 1.0])
     return dict(kind=kind, dtype=dtype, S=S, n=n, V=V, temperature=temperature,
                 draft="lookup" if temperature == 0.0 else rng.choice(["model", "model", "lookup"]),
                 ragged=rng.random() < 0.4)
