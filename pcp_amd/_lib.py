@@ -48,6 +48,8 @@ FLAG_ASYNC = 0x1
 FLAG_NO_ZERO_FILL = 0x2
 FLAG_FORCE_STREAMING = 0x4
 FLAG_EXACT_BF16 = 0x8
+TOP_LOGITS_MAX = 256
+VERIFY_MAX_DRAFT = 64
 NOALLOC_SCRATCH_BYTES = 4 << 20
 IGNORE_INDEX = -100
 
@@ -125,6 +127,50 @@ class GradStats(ctypes.Structure):
     ]
 
 
+class TopLogitsArgs(ctypes.Structure):
+    """pcp_top_logits_args (include/pcp_distill.h)."""
+    _fields_ = [
+        ("n_rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+        ("k", ctypes.c_int32), ("logits_dtype", ctypes.c_int32), ("ids_dtype", ctypes.c_int32),
+        ("temperature", ctypes.c_float),
+        ("logits", ctypes.c_void_p), ("values", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+        ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
+    ]
+
+
+class DistillArgs(ctypes.Structure):
+    """pcp_distill_args (include/pcp_distill.h)."""
+    _fields_ = [
+        ("n_seq", ctypes.c_int64), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64),
+        ("logit_seq_stride", ctypes.c_int64), ("tok_seq_stride", ctypes.c_int64), ("tok_offset", ctypes.c_int64),
+        ("k", ctypes.c_int32), ("logits_dtype", ctypes.c_int32), ("dlogits_dtype", ctypes.c_int32),
+        ("ids_dtype", ctypes.c_int32), ("mask_dtype", ctypes.c_int32), ("divergence", ctypes.c_int32),
+        ("logits", ctypes.c_void_p), ("teacher_ids", ctypes.c_void_p), ("teacher_logits", ctypes.c_void_p),
+        ("teacher_lse", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+        ("dlogits", ctypes.c_void_p), ("token_loss", ctypes.c_void_p), ("loss", ctypes.c_void_p),
+        ("temperature", ctypes.c_float), ("weight", ctypes.c_float), ("loss_norm", ctypes.c_float),
+        ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
+    ]
+
+
+class VerifyArgs(ctypes.Structure):
+    """pcp_verify_args (include/pcp_sample.h)."""
+    _fields_ = [
+        ("n_seq", ctypes.c_int64), ("n_draft", ctypes.c_int64), ("vocab", ctypes.c_int64),
+        ("target_row_stride", ctypes.c_int64), ("draft_row_stride", ctypes.c_int64),
+        ("logits_dtype", ctypes.c_int32), ("temperature", ctypes.c_float),
+        ("target_logits", ctypes.c_void_p), ("draft_logits", ctypes.c_void_p), ("draft_ids", ctypes.c_void_p),
+        ("draft_lens", ctypes.c_void_p), ("uniforms", ctypes.c_void_p),
+        ("tokens", ctypes.c_void_p), ("accepted", ctypes.c_void_p), ("logp", ctypes.c_void_p),
+        ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
+    ]
+
+
+class Divergence(enum.IntEnum):
+    forward = 0   # sum p log(p / q)
+    reverse = 1   # sum q log(q / p)
+
+
 class NesterovMode(enum.IntEnum):
     sutskever = 0   # nesterov.zig:86-97 (RLShepherd's optimizer)
     mlir = 1        # nesterov_mlir.zig:93-99
@@ -176,6 +222,12 @@ SIGNATURES = {
     "pcp_nesterov_deserialize": (_I, [_VP, _VP, ctypes.c_size_t]),
     "pcp_sample_tokens": (_I, [_VP, _VP, _I, _I64, _I64, _I64, _F, _VP, _VP, _VP]),
     "pcp_sample_tokens_async": (_I, [_VP, _VP, _I, _I64, _I64, _I64, _F, _VP, _VP, _VP]),
+    "pcp_verify_args_init": (None, [ctypes.POINTER(VerifyArgs)]),
+    "pcp_verify_drafts": (_I, [_VP, ctypes.POINTER(VerifyArgs)]),
+    "pcp_top_logits_args_init": (None, [ctypes.POINTER(TopLogitsArgs)]),
+    "pcp_top_logits": (_I, [_VP, ctypes.POINTER(TopLogitsArgs)]),
+    "pcp_distill_args_init": (None, [ctypes.POINTER(DistillArgs)]),
+    "pcp_distill_fwd_bwd": (_I, [_VP, ctypes.POINTER(DistillArgs)]),
     "pcp_prompts_load": (_I, [_VP, ctypes.c_char_p, _VP, _I64, _VP, _I64, ctypes.POINTER(_I64),
                               ctypes.POINTER(_I64)]),
     "pcp_weights_load": (_I, [_VP, ctypes.c_char_p, _I, ctypes.POINTER(_I64), _VP, _VP]),

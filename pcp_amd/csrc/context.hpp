@@ -108,6 +108,36 @@ inline int dtype_bytes(int dt) {
 // Make `bytes` of scratch available on ctx (grow-only; synchronises before a free).
 int ensure_scratch(pcp_ctx* ctx, size_t bytes);
 
+// The same for work enqueued on `st`; a stream under capture cannot grow it
+// (PCP_ERR_INVALID_ARG, the capture left as it was).
+int ensure_scratch_on(pcp_ctx* ctx, size_t bytes, hipStream_t st);
+
+// Makes a device current for a scope and the caller's current again after it.
+class DeviceScope {
+ public:
+  explicit DeviceScope(int device) {
+    if ((err_ = hipGetDevice(&before_)) == hipSuccess && before_ != device) {
+      err_ = hipSetDevice(device);
+      changed_ = err_ == hipSuccess;
+    }
+  }
+  ~DeviceScope() {
+    if (changed_) (void)hipSetDevice(before_);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+  hipError_t error() const { return err_; }
+
+ private:
+  int before_ = 0;
+  bool changed_ = false;
+  hipError_t err_;
+};
+
+// The end of an entry point whose work is enqueued on `st`: with PCP_FLAG_ASYNC the stream
+// is recorded for pcp_sync, else it is waited for and the device-side errors returned.
+int finish_call(pcp_ctx* ctx, uint32_t flags, hipStream_t st);
+
 // After synchronising: read and clear the error slots of the context's page, map them to
 // a status.
 int collect_device_errors(pcp_ctx* ctx);

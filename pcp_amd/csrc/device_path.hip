@@ -57,6 +57,25 @@ int ensure_scratch(pcp_ctx* ctx, size_t bytes) {
   return PCP_OK;
 }
 
+int ensure_scratch_on(pcp_ctx* ctx, size_t bytes, hipStream_t st) {
+  if (bytes <= ctx->scratch_bytes) return PCP_OK;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &status) != hipSuccess) (void)hipGetLastError();
+  else if (status != hipStreamCaptureStatusNone)
+    return fail(ctx, PCP_ERR_INVALID_ARG,
+                "the stream is being captured and the context's work buffer would have to grow from %zu to %zu bytes: "
+                "make one uncaptured call of the same sizes first",
+                ctx->scratch_bytes, bytes);
+  return ensure_scratch(ctx, bytes);
+}
+
+int finish_call(pcp_ctx* ctx, uint32_t flags, hipStream_t st) {
+  if (flags & PCP_FLAG_ASYNC) return add_pending(ctx, st);
+  hipError_t e = hipStreamSynchronize(st);
+  if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
+  return collect_device_errors(ctx);
+}
+
 // Read in place: with the error word in device memory and a 4-byte hipMemcpy here, every
 // synchronous call took 12 us more (configuration 1's step 55.8 us against 44.1, 64 rows of
 // 151,936 68.9 against 56.9, 512 rows of log-probs 82 against 70).
@@ -79,6 +98,10 @@ int collect_device_errors(pcp_ctx* ctx) {
   if (h & kErrBadBase64)
     return fail(ctx, PCP_ERR_INVALID_ARG, "base64 text has a character outside the alphabet or misplaced padding "
                                           "(InvalidCharacter / InvalidPadding)");
+  if (h & kErrTeacherTwice)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "a row uses one teacher id twice");
+  if (h & kErrDraftLen)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "a sequence's draft length is outside [0, n_draft]");
   return fail(ctx, PCP_ERR_NONFINITE, "a live row has a non-finite log-sum-exp (NaN/Inf logits)");
 }
 
@@ -184,15 +207,6 @@ int validate(const pcp_grpo_args* a, Op op, Geo* g) {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline size_t round256(size_t b) { return (b + 255) & ~static_cast<size_t>(255); }
-
-int finish(pcp_ctx* ctx, const pcp_grpo_args* a, hipStream_t st) {
-  if (a->flags & PCP_FLAG_ASYNC) {
-    return add_pending(ctx, st);
-  }
-  hipError_t e = hipStreamSynchronize(st);
-  if (e != hipSuccess) return hip_fail(ctx, e, "hipStreamSynchronize");
-  return collect_device_errors(ctx);
-}
 
 // A context's flag, held until the call returns.
 struct PartClaim {
@@ -360,7 +374,7 @@ int run(pcp_ctx* ctx, const pcp_grpo_args* a, Op op, bool noalloc = false, int64
     e = launch_loss_reduce_fused(la, st);
     if (e != hipSuccess) return hip_fail(ctx, e, "loss reduction launch");
   }
-  return finish(ctx, a, st);
+  return finish_call(ctx, a->flags, st);
 }
 
 }  // namespace

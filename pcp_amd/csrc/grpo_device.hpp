@@ -28,6 +28,8 @@ constexpr int kErrNonFinite = 2;
 constexpr int kErrBadRagged = 4;   // rollout packing: offsets decrease or run past the token array
 constexpr int kErrBadBase64 = 8;   // base64: a character outside the alphabet or misplaced padding
 constexpr int kErrListedRow = 16;  // a row listed live by live_rows_kernel was not live in the row kernel
+constexpr int kErrTeacherTwice = 32;  // distillation: a row uses a teacher id twice
+constexpr int kErrDraftLen = 64;   // draft verification: a sequence's draft length outside [0, n]
 
 // A store of 1 to the condition's own slot, not an atomic OR: the page is host memory, and
 // the link to the host carries no OR.
@@ -311,6 +313,37 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return lanes_reduce<N>(v, 0.f, [](float a, float b) { return a + b; });
 }
 
+// v of the lane that DPP control CTRL names, 0 where there is none or ROWS masks the row.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// Inclusive sum over the lanes up to this one, in a fixed order (see lanes_reduce).
+__device__ __forceinline__ double wave_scan(double v) {
+  v += dpp64<0x111>(v);
+  v += dpp64<0x112>(v);
+  v += dpp64<0x114>(v);
+  v += dpp64<0x118>(v);
+  v += dpp64<0x142, 0xa>(v);
+  v += dpp64<0x143, 0xc>(v);
+  return v;
+}
+
+// v of lane `lane` (the same on every lane).
+__device__ __forceinline__ double read_lane64(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// The sum over the wave, on every lane, in a fixed order.
+__device__ __forceinline__ double wave_sum64(double v) { return read_lane64(wave_scan(v), 63); }
+
 // The merge of the first N lanes' (m, s) pairs: the largest m, then every s rescaled to it
 // once and added. NaN and -inf behave as in ms_merge.
 template <int N>
@@ -346,6 +379,86 @@ __device__ __forceinline__ void block_merge2(float& m1, float& s1, float& m2, fl
     lanes_merge<NW>(m1, s1);
     lanes_merge<NW>(m2, s2);
   }
+}
+
+// ---------------------------------------------------------------------------
+// Rows as 16-byte vectors.
+// ---------------------------------------------------------------------------
+// A row that may start off 16 bytes: its 16-byte-aligned interior of nv vectors, and
+// the head (before it) and tail (after it) of fewer than EPV elements each.
+struct RowSpan {
+  const void* vec;
+  int head, nv, tail;
+};
+
+template <typename TI>
+__device__ __forceinline__ RowSpan row_span(const void* p, int64_t vocab) {
+  constexpr int EPV = 16 / TI::kBytes;
+  RowSpan s;
+  const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u);
+  s.head = static_cast<int>(min<int64_t>(((16 - mis) & 15) / TI::kBytes, vocab));
+  s.nv = static_cast<int>((vocab - s.head) / EPV);
+  s.tail = static_cast<int>(vocab - s.head - static_cast<int64_t>(s.nv) * EPV);
+  s.vec = static_cast<const char*>(p) + s.head * TI::kBytes;
+  return s;
+}
+
+// The head or tail element that thread tid handles: threads [0, head) take the head,
+// [head, head + tail) the tail; -1 for the rest.
+template <typename TI>
+__device__ __forceinline__ int edge_index(const RowSpan& sp, int tid) {
+  constexpr int EPV = 16 / TI::kBytes;
+  return tid < sp.head ? tid : (tid - sp.head < sp.tail ? sp.head + sp.nv * EPV + (tid - sp.head) : -1);
+}
+
+// Thread tid's head or tail element of the row as a one-element online state (m, s).
+template <typename TI>
+__device__ __forceinline__ void edge_state(const void* p, const RowSpan& sp, int tid, float& m, float& s) {
+  const int k = edge_index<TI>(sp, tid);
+  m = kNegInf;
+  s = 0.f;
+  if (k < 0) return;
+  const float x = TI::load1(p, k) * kLog2e;
+  m = fmaxf(m, x);
+  s = hw_exp2(x - ms_ref(m));
+}
+
+template <typename TI, typename TO, int BLOCK>
+__device__ __forceinline__ uint32_t split_group(int tid) {
+  return (TI::kBytes == 2 && TO::kBytes == 4) ? static_cast<uint32_t>(128 * (tid >> 6) + (tid & 63)) : 0u;
+}
+
+// Chunk k of a row through its descriptor: 16 bytes at lane offset voff, or for kSplit
+// (16-bit logits, f32 dlogits) the two 8-byte halves of 4-element group sgrp, 512 bytes
+// apart (see resident_row).
+template <typename TI, typename TO, int BLOCK>
+__device__ __forceinline__ u32x4 load_chunk(const __amdgpu_buffer_rsrc_t buf, int k, uint32_t voff, uint32_t sgrp) {
+  constexpr uint32_t kChunkBytes = BLOCK * 16;
+  if constexpr (TI::kBytes == 2 && TO::kBytes == 4) {
+    const u32x2 lo = buf_ld8<true>(buf, fresh_off(sgrp * 8u, k * kChunkBytes));
+    const u32x2 hi = buf_ld8<true>(buf, fresh_off(sgrp * 8u, k * kChunkBytes + 512u));
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  } else {
+    return buf_ld16<true>(buf, fresh_off(voff, k * kChunkBytes));
+  }
+}
+
+// max(m, the EPV values of one 16-byte vector). bf16 halves come from byte permutes:
+// the same values as unpack(), but the compiler does not merge them with the sum
+// pass's unpacks, which would keep every unpacked value of the batch live.
+template <typename TI>
+__device__ __forceinline__ float vec_max(float m, const u32x4& v) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+  if constexpr (__is_same(TI, BF16T)) {
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+      m = fmaxf(fmaxf(m, __uint_as_float(__builtin_amdgcn_perm(w[h], 0u, 0x05040c0cu))),
+                __uint_as_float(__builtin_amdgcn_perm(w[h], 0u, 0x07060c0cu)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16 / TI::kBytes; ++j) m = fmaxf(m, TI::unpack(w, j));
+  }
+  return m;
 }
 
 // ---------------------------------------------------------------------------

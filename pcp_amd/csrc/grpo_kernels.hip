@@ -61,45 +61,6 @@ __device__ __forceinline__ void flag_nonfinite(const RowArgs& a, double lse, dou
     raise_error(a.err, kErrNonFinite);
 }
 
-// A row that may start off 16 bytes: its 16-byte-aligned interior of nv vectors, and
-// the head (before it) and tail (after it) of fewer than EPV elements each.
-struct RowSpan {
-  const void* vec;
-  int head, nv, tail;
-};
-
-template <typename TI>
-__device__ __forceinline__ RowSpan row_span(const void* p, int64_t vocab) {
-  constexpr int EPV = 16 / TI::kBytes;
-  RowSpan s;
-  const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u);
-  s.head = static_cast<int>(min<int64_t>(((16 - mis) & 15) / TI::kBytes, vocab));
-  s.nv = static_cast<int>((vocab - s.head) / EPV);
-  s.tail = static_cast<int>(vocab - s.head - static_cast<int64_t>(s.nv) * EPV);
-  s.vec = static_cast<const char*>(p) + s.head * TI::kBytes;
-  return s;
-}
-
-// The head or tail element that thread tid handles: threads [0, head) take the head,
-// [head, head + tail) the tail; -1 for the rest.
-template <typename TI>
-__device__ __forceinline__ int edge_index(const RowSpan& sp, int tid) {
-  constexpr int EPV = 16 / TI::kBytes;
-  return tid < sp.head ? tid : (tid - sp.head < sp.tail ? sp.head + sp.nv * EPV + (tid - sp.head) : -1);
-}
-
-// Thread tid's head or tail element of the row as a one-element online state (m, s).
-template <typename TI>
-__device__ __forceinline__ void edge_state(const void* p, const RowSpan& sp, int tid, float& m, float& s) {
-  const int k = edge_index<TI>(sp, tid);
-  m = kNegInf;
-  s = 0.f;
-  if (k < 0) return;
-  const float x = TI::load1(p, k) * kLog2e;
-  m = fmaxf(m, x);
-  s = hw_exp2(x - ms_ref(m));
-}
-
 // ---------------------------------------------------------------------------
 // Register-resident fused forward+backward.
 //   TI/TO: input / output codecs; BLOCK lanes; NCH 16-byte chunks per lane
@@ -112,26 +73,6 @@ __device__ __forceinline__ void edge_state(const void* p, const RowSpan& sp, int
 // stored as vectors, the head and tail (under EPV elements each) by threads 0..13 one
 // element each. dlogits == nullptr: forward only (log-probs).
 // ---------------------------------------------------------------------------
-// Chunk k of a row through its descriptor: 16 bytes at lane offset voff, or for kSplit
-// (16-bit logits, f32 dlogits) the two 8-byte halves of 4-element group sgrp, 512 bytes
-// apart (see resident_row).
-template <typename TI, typename TO, int BLOCK>
-__device__ __forceinline__ u32x4 load_chunk(const __amdgpu_buffer_rsrc_t buf, int k, uint32_t voff, uint32_t sgrp) {
-  constexpr uint32_t kChunkBytes = BLOCK * 16;
-  if constexpr (TI::kBytes == 2 && TO::kBytes == 4) {
-    const u32x2 lo = buf_ld8<true>(buf, fresh_off(sgrp * 8u, k * kChunkBytes));
-    const u32x2 hi = buf_ld8<true>(buf, fresh_off(sgrp * 8u, k * kChunkBytes + 512u));
-    return u32x4{lo[0], lo[1], hi[0], hi[1]};
-  } else {
-    return buf_ld16<true>(buf, fresh_off(voff, k * kChunkBytes));
-  }
-}
-
-template <typename TI, typename TO, int BLOCK>
-__device__ __forceinline__ uint32_t split_group(int tid) {
-  return (TI::kBytes == 2 && TO::kBytes == 4) ? static_cast<uint32_t>(128 * (tid >> 6) + (tid & 63)) : 0u;
-}
-
 // The policy row's descriptor for rows without EDGE handling (aligned, V % EPV == 0);
 // row < 0 gives an empty descriptor, whose loads return 0 without a memory access.
 template <typename TI>
@@ -636,24 +577,6 @@ __global__ void __launch_bounds__(256) live_rows_kernel(RowArgs a) {
 #ifndef PCP_FWD_U
 #define PCP_FWD_U 8
 #endif
-
-// max(m, the EPV values of one 16-byte vector). bf16 halves come from byte permutes:
-// the same values as unpack(), but the compiler does not merge them with the sum
-// pass's unpacks, which would keep every unpacked value of the batch live.
-template <typename TI>
-__device__ __forceinline__ float vec_max(float m, const u32x4& v) {
-  const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
-  if constexpr (__is_same(TI, BF16T)) {
-#pragma unroll
-    for (int h = 0; h < 4; ++h)
-      m = fmaxf(fmaxf(m, __uint_as_float(__builtin_amdgcn_perm(w[h], 0u, 0x05040c0cu))),
-                __uint_as_float(__builtin_amdgcn_perm(w[h], 0u, 0x07060c0cu)));
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16 / TI::kBytes; ++j) m = fmaxf(m, TI::unpack(w, j));
-  }
-  return m;
-}
 
 template <typename TI, int BLOCK, int U, bool REF>
 __global__ void __launch_bounds__(BLOCK) grpo_fwd_kernel(RowArgs a) {

@@ -97,34 +97,6 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
-// v of the lane that DPP control CTRL names, 0 where there is none or ROWS masks the row.
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ double dpp64(double v) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWS, 0xf, false);
-  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xf, false);
-  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
-}
-
-// Inclusive sum over the lanes up to this one, in a fixed order (see lanes_reduce).
-__device__ __forceinline__ double wave_scan(double v) {
-  v += dpp64<0x111>(v);
-  v += dpp64<0x112>(v);
-  v += dpp64<0x114>(v);
-  v += dpp64<0x118>(v);
-  v += dpp64<0x142, 0xa>(v);
-  v += dpp64<0x143, 0xc>(v);
-  return v;
-}
-
-// v of lane `lane` (the same on every lane).
-__device__ __forceinline__ double read_lane64(double v, int lane) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
-  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), lane);
-  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane);
-  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
-}
-
 // Greedy: (value, index), larger value wins, equal values the smaller index (the
 // reference's strict '>' scan keeps the first maximum; NaN never compares greater,
 // and -inf never beats the initial -inf, so such rows keep index 0).

@@ -95,6 +95,43 @@ def _stream_handle(stream) -> int | None:
     return s.cuda_stream or None
 
 
+class call_scope:
+    """The stream of a call on `ctx` over `tensors` (None among them allowed), all on the
+    context's device: its raw handle, as the value of the ``with``. With a torch stream or a raw
+    handle other than the device's current stream, tensors allocated inside belong to that
+    stream, and the allocator keeps the given ones until the work enqueued there is done."""
+
+    __slots__ = ("handle", "inner")
+
+    def __init__(self, ctx: Context, stream, *tensors):
+        for t in tensors:
+            if t is not None and (not t.is_cuda or t.device.index != ctx.device):
+                raise PcpError(-1, f"tensor on {t.device}, context on device {ctx.device}")
+        self.inner = None
+        current = torch.cuda.current_stream(ctx.device)
+        if isinstance(stream, int):
+            stream = (current if stream == current.cuda_stream
+                      else torch.cuda.ExternalStream(stream, device=ctx.device) if stream
+                      else torch.cuda.default_stream(ctx.device))
+        if stream is not None and stream.cuda_stream != current.cuda_stream:
+            self.inner = torch.cuda.stream(stream)
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(stream)
+            current = stream
+        self.handle = current.cuda_stream or None
+
+    def __enter__(self):
+        if self.inner is not None:
+            self.inner.__enter__()
+        return self.handle
+
+    def __exit__(self, *exc):
+        if self.inner is not None:
+            self.inner.__exit__(*exc)
+        return False
+
+
 @dataclass
 class GrpoOutputs:
     loss: torch.Tensor          # f32 scalar

@@ -8,12 +8,13 @@ Mirrors RLShepherd.trainStep (src/nodes/controllers/rl_shepherd.zig:487-515 pack
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 
 import numpy as np
 import torch
 
-from ._lib import GradStats, NesterovMode, PcpError, check, lib
-from .grpo import Context, _ptr, _stream_handle, default_context
+from ._lib import FLAG_ASYNC, GradStats, NesterovMode, PcpError, VerifyArgs, check, lib
+from .grpo import Context, _ptr, _stream_handle, call_scope, default_context, dtype_code
 
 
 def pack_rollouts(prompt_tokens: torch.Tensor, prompt_offsets: torch.Tensor, completion_tokens: torch.Tensor,
@@ -148,3 +149,70 @@ def sample_tokens(logits: torch.Tensor, temperature: float, uniforms: torch.Tens
     check(fn(ctx.handle, logits.data_ptr(), int(code), R, V, logits.stride(0), float(temperature), _ptr(uniforms),
              _ptr(ids), _stream_handle(stream)), ctx.handle)
     return ids
+
+
+@dataclass
+class Verified:
+    tokens: torch.Tensor      # int64 [S, n + 1]: accepted tokens, the one after, IGNORE_INDEX
+    accepted: torch.Tensor    # int32 [S]
+    logp: torch.Tensor        # f32 [S, n + 1]: the target's log-probs of those tokens, 0 past them
+
+
+def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_logits: torch.Tensor | None = None, *,
+                  temperature: float = 1.0, uniforms: torch.Tensor | None = None,
+                  draft_lens: torch.Tensor | None = None, outputs: Verified | None = None, sync: bool = True,
+                  stream=None, ctx: Context | None = None) -> Verified:
+    """Speculative decoding's check of drafted tokens draft_ids [S, n] (int64) against the
+    target's logits [S, n + 1, V] (f32, bf16 or f16; pcp_verify_drafts): the longest accepted
+    prefix and one more token. draft_logits [S, n, V] is the distribution the tokens were drawn
+    from, None for drafts looked up or chosen greedily; uniforms f32 [S, n + 1] in [0, 1), n
+    for the tokens and the last for the one after (None when temperature < 1e-6, which is
+    greedy); draft_lens int32 [S] the tokens drafted per sequence (None: n). The rows may lie
+    further apart than V if evenly so. sync=False only enqueues the launches."""
+    if target_logits.dim() != 3 or target_logits.shape[1] < 1:
+        raise PcpError(-1, "target_logits must be [S, n + 1, V]")
+    S, n1, V = target_logits.shape
+    n = n1 - 1
+    if draft_ids.shape != (S, n) or draft_ids.dtype != torch.int64:
+        raise PcpError(-1, "draft_ids must be int64 [S, n]")
+    if draft_logits is not None and (draft_logits.shape != (S, n, V) or draft_logits.dtype != target_logits.dtype):
+        raise PcpError(-1, "draft_logits must be [S, n, V] of the target's dtype")
+    if uniforms is not None and (uniforms.dtype != torch.float32 or uniforms.shape != (S, n1)):
+        raise PcpError(-1, "uniforms must be f32 [S, n + 1]")
+    if draft_lens is not None and (draft_lens.dtype != torch.int32 or draft_lens.shape != (S,)):
+        raise PcpError(-1, "draft_lens must be int32 [S]")
+    ctx = ctx or default_context(target_logits.device.index or 0)
+    a = VerifyArgs()
+    lib().pcp_verify_args_init(ctypes.byref(a))
+    with call_scope(ctx, stream, target_logits, draft_ids, draft_logits, uniforms, draft_lens) as handle:
+        if outputs is None:
+            dev = target_logits.device
+            outputs = Verified(torch.empty((S, n1), dtype=torch.int64, device=dev),
+                               torch.empty(S, dtype=torch.int32, device=dev),
+                               torch.empty((S, n1), dtype=torch.float32, device=dev))
+        o = outputs
+        if (o.tokens.dtype != torch.int64 or o.tokens.numel() != S * n1 or o.accepted.dtype != torch.int32
+                or o.accepted.numel() != S or o.logp.dtype != torch.float32 or o.logp.numel() != S * n1):
+            raise PcpError(-1, "outputs do not fit the call: tokens int64 and logp f32 [S, n + 1], accepted int32 [S]")
+        a.n_seq, a.n_draft, a.vocab = S, n, V
+        a.target_row_stride = _row_stride(target_logits)
+        a.draft_row_stride = _row_stride(draft_logits) if draft_logits is not None else V
+        a.logits_dtype, a.temperature = dtype_code(target_logits), temperature
+        a.target_logits = target_logits.data_ptr()
+        a.draft_logits = draft_logits.data_ptr() if draft_logits is not None and n else None
+        a.draft_ids, a.draft_lens, a.uniforms = _ptr(draft_ids), _ptr(draft_lens), _ptr(uniforms)
+        a.tokens, a.accepted, a.logp = _ptr(o.tokens), _ptr(o.accepted), _ptr(o.logp)
+        a.flags = 0 if sync else FLAG_ASYNC
+        a.stream = handle
+        check(lib().pcp_verify_drafts(ctx.handle, ctypes.byref(a)), ctx.handle)
+    return outputs
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    """Elements between the evenly spaced rows of [S, m, V]."""
+    S, m, V = t.shape
+    if V > 1 and t.stride(2) != 1:
+        raise PcpError(-1, "logits rows must be contiguous")
+    if m > 1 and S > 1 and t.stride(0) != m * t.stride(1):
+        raise PcpError(-1, "logits rows must be evenly spaced over the sequences")
+    return t.stride(1) if m > 1 else (t.stride(0) if S > 1 else V)
