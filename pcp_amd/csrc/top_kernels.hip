@@ -4,12 +4,13 @@
 // An element is ordered by a 64-bit key: its logit's bits made monotone, then the id
 // complemented, so that no two are equal and equal logits fall by rising id. A workgroup
 // streams its part of a row once. It keeps candidates in LDS and a threshold that at least
-// k of the elements seen reach: at first the k-th largest of its lanes' maxima over the
-// first batch, later the k-th candidate whenever the list is cut back. Few elements pass
-// it, so the row costs one read, the log-sum-exp's arithmetic and a comparison each; rows
-// in any order are right, falling back to cuts every 1,024 elements where they pass in
-// numbers. A row with one part is sorted and written by its workgroup; else each part
-// leaves its k best and a second kernel merges them.
+// k of the elements seen reach: first from a histogram of the maxima of the 16-byte vectors
+// of its first batch, later, as the list grows, from a histogram of the candidates. Few
+// elements pass it, so the row costs one read, the log-sum-exp's arithmetic and a comparison
+// per vector. Rows in any order are right: a batch of which too much passes is taken again
+// in small rounds, and a list that a histogram cannot thin (equal values) is sorted. A row
+// with one part is ranked and written by its workgroup; else each part leaves its
+// candidates and a second kernel merges them.
 
 #include <hip/hip_runtime.h>
 
@@ -25,9 +26,14 @@ namespace pcp {
 namespace {
 
 constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / 64;
 constexpr int kU = 8;              // 16-byte vectors per lane and batch
 constexpr int kCap = 2048;         // candidates held
-constexpr int kCut = 1024;         // cut back past this many: a cautious round adds at most kCap - kCut
+constexpr int kCut = 1024;         // thinned past this many: a cautious round adds at most kCap - kCut
+constexpr int kBins = 256;
+// A logit this low is a mask (-inf, or a type's lowest value): it stays out of the histograms,
+// whose range it would take up.
+constexpr float kMasked = -32768.f;
 
 struct TopArgs {
   const void* logits;
@@ -36,12 +42,11 @@ struct TopArgs {
   float* values;
   void* ids;
   float* lse;
-  uint64_t* part_key;     // [n_rows, parts, k]
-  float2* part_ms;        // [n_rows, parts]
+  uint64_t* part_key;     // [n_rows, parts, part_cap]
+  float4* part_ms;        // [n_rows, parts]: (m, s, candidates left, -)
   int* err;
   float k2;               // log2(e) / temperature
-  double to_nat;          // ln 2: base-2 state to natural units
-  int32_t k, ids_i64, parts, per;
+  int32_t k, ids_i64, parts, per, part_cap;
 };
 
 // Monotone in x; -0 as 0, NaN below everything.
@@ -76,9 +81,80 @@ __device__ __forceinline__ void sort_falling(uint64_t* c, int n) {
     }
 }
 
+struct Shared {
+  uint64_t key[kCap];
+  int bin[kBins];
+  float low[kWaves], high[kWaves];
+  int count;
+};
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ int lanes_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+  return v;
+}
+
+// A value that at least k of the workgroup's values v[] reach, and not many more unless they
+// lie close together: the lower edge of a bin of a histogram over their range; -inf where
+// fewer than k lie above kMasked. Called by the whole workgroup; sh.bin is free again after
+// the caller's next barrier.
+// used: the values past this many of v are no one's.
+template <int M>
+__device__ __forceinline__ float reached_by(Shared& sh, const float (&v)[M], int k, int used = M) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float lo = __builtin_inff(), hi = kNegInf;
+#pragma unroll
+  for (int i = 0; i < M; ++i) {
+    if (i >= used) break;
+    const bool plain = v[i] > kMasked && v[i] < __builtin_inff();
+    lo = plain ? fminf(lo, v[i]) : lo;
+    hi = plain ? fmaxf(hi, v[i]) : hi;
+  }
+  lo = -lanes_max<64>(-lo);
+  hi = lanes_max<64>(hi);
+  if (lane == 0) {
+    sh.low[wave] = lo;
+    sh.high[wave] = hi;
+  }
+  for (int i = threadIdx.x; i < kBins; i += kBlock) sh.bin[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    lo = fminf(lo, sh.low[w]);
+    hi = fmaxf(hi, sh.high[w]);
+  }
+  const float range = hi - lo;
+  const float scale = range > 0.f && range < __builtin_inff() ? (kBins - 1) / range : 0.f;
+#pragma unroll
+  for (int i = 0; i < M; ++i)
+    if (i < used && v[i] >= lo)   // +inf counts in the last bin
+      atomicAdd(&sh.bin[v[i] > hi ? kBins - 1 : min(static_cast<int>((v[i] - lo) * scale), kBins - 1)], 1);
+  __syncthreads();
+  // Lane l: the bins 4 (63 - l) .. + 3, from the last bin down.
+  const int first = 4 * (63 - lane);
+  const int4 c = *reinterpret_cast<const int4*>(&sh.bin[first]);
+  const int incl = lanes_scan(c.x + c.y + c.z + c.w);
+  const uint64_t enough = __ballot(incl >= k);
+  if (enough == 0) return kNegInf;
+  const int above = incl - (c.x + c.y + c.z + c.w);
+  int at = first;
+  if (above + c.w >= k) at = first + 3;
+  else if (above + c.w + c.z >= k) at = first + 2;
+  else if (above + c.w + c.z + c.y >= k) at = first + 1;
+  at = __builtin_amdgcn_readlane(at, __builtin_ctzll(enough));
+  // Below the edge by more than the rounding of the bins' arithmetic.
+  return at == 0 || scale == 0.f ? lo : lo + (at / scale - 0x1p-20f * (fabsf(lo) + fabsf(hi)));
+}
+
 struct Candidates {
-  uint64_t* key;       // LDS [kCap]
-  int* count;          // LDS
+  Shared& sh;
   uint64_t least;      // keys above this pass (0: all)
   float least_x;       // no element below this passes
 
@@ -88,34 +164,75 @@ struct Candidates {
     if (who == 0) return;
     const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32),
                                                  __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
-    int at = 0;
-    if (before == 0 && pass) at = atomicAdd(count, __popcll(who));
+    // One lane adds for all; the offset that the compiler cannot see through keeps it from
+    // wrapping the single atomic in a reduction of its own.
+    int at = 0, zero = 0;
+    asm volatile("" : "+v"(zero));
+    if (before == 0 && pass) at = atomicAdd(&sh.count + zero, __popcll(who));
     at = __builtin_amdgcn_readlane(at, __builtin_ctzll(who)) + before;
-    if (pass && at < kCap) key[at] = k;
+    if (pass && at < kCap) sh.key[at] = k;
   }
-  // Keeps the k largest of the n held, in falling order; called by the whole workgroup.
-  __device__ __forceinline__ int cut(int n, int k) {
-    sort_falling(key, n);
-    const int left = min(n, k);
-    if (n >= k) {
-      least = key[k - 1] - 1;   // the k-th itself is held already, and no other key equals it
-      least_x = from_order(static_cast<uint32_t>(key[k - 1] >> 32));
+  // The n candidates held become those of the k largest, and few more: at most `most` (>= k).
+  // Called by the whole workgroup after a barrier; ends with one.
+  __device__ __forceinline__ int thin(int n, int k, int most) {
+    constexpr int M = kCap / kBlock;
+    uint64_t key[M];
+    float v[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      key[i] = 0;
+      v[i] = kNegInf;
+      if (i * kBlock < n) {
+        const int at = i * kBlock + static_cast<int>(threadIdx.x);
+        if (at < n) {
+          key[i] = sh.key[at];
+          v[i] = from_order(static_cast<uint32_t>(key[i] >> 32));
+        }
+      }
+    }
+    const float x = reached_by(sh, v, k, (n + kBlock - 1) / kBlock);
+    least_x = fmaxf(least_x, x);
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+      if (i * kBlock < n) add(i * kBlock + static_cast<int>(threadIdx.x) < n && !(v[i] < x), key[i]);
+    __syncthreads();
+    n = sh.count;
+    if (n > most) {   // too many near the k-th: exactly
+      sort_falling(sh.key, n);
+      least = sh.key[k - 1] - 1;   // the k-th itself is held already, and no other key equals it
+      n = k;
+      __syncthreads();
+      if (threadIdx.x == 0) sh.count = k;
     }
     __syncthreads();
-    if (threadIdx.x == 0) *count = left;
-    __syncthreads();
-    return left;
+    return n;
   }
 };
 
-// A row's entries from the sorted candidates.
-__device__ __forceinline__ void write_entries(const TopArgs& a, int64_t row, const uint64_t* key) {
-  for (int i = threadIdx.x; i < a.k; i += kBlock) {
-    const uint64_t v = key[i];
+// A row's entries from its n candidates (>= k of them), each put where its rank says: the
+// number of larger ones, counted over LDS reads that every lane shares.
+__device__ __forceinline__ void write_entries(const TopArgs& a, int64_t row, Shared& sh, int n) {
+  if (n > 2 * kBlock) {
+    sort_falling(sh.key, n);
+    n = a.k;
+  } else {
+    if (threadIdx.x == 0) sh.key[n] = 0;   // pairs below
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < n; i += kBlock) {
+    const uint64_t v = sh.key[i];
+    int rank = 0;
+    for (int o = 0; o < n; o += 2) {
+      const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&sh.key[o]);
+      rank += (w.x > v) + (w.y > v);
+    }
+    if (rank >= a.k) continue;
     const int64_t id = 0xffffffffu - static_cast<uint32_t>(v);
-    a.values[row * a.k + i] = from_order(static_cast<uint32_t>(v >> 32));
-    if (a.ids_i64) static_cast<int64_t*>(a.ids)[row * a.k + i] = id;
-    else static_cast<int32_t*>(a.ids)[row * a.k + i] = static_cast<int32_t>(id);
+    a.values[row * a.k + rank] = from_order(static_cast<uint32_t>(v >> 32));
+    if (a.ids_i64) static_cast<int64_t*>(a.ids)[row * a.k + rank] = id;
+    else static_cast<int32_t*>(a.ids)[row * a.k + rank] = static_cast<int32_t>(id);
   }
 }
 
@@ -128,22 +245,16 @@ __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, float m
 template <typename TI>
 __global__ void __launch_bounds__(kBlock) top_part_kernel(TopArgs a) {
   constexpr int EPV = 16 / TI::kBytes, U = kU, BLOCK = kBlock;
-  __shared__ uint64_t key[kCap];
+  __shared__ __align__(16) Shared sh;
   __shared__ __align__(16) float lds[4 * (BLOCK / 64)];
-  __shared__ float lane_max[BLOCK];
-  __shared__ int count;
-  __shared__ float first_least;
   const int tid = threadIdx.x, part = blockIdx.x;
   const int64_t row = a.row0 + blockIdx.y;
   const char* xrow = static_cast<const char*>(a.logits) + row * a.row_stride * TI::kBytes;
   const RowSpan sp = row_span<TI>(xrow, a.vocab);
   const int v0 = part * a.per, end = min(v0 + a.per, sp.nv);
   const __amdgpu_buffer_rsrc_t xbuf = row_rsrc(sp.vec, static_cast<uint32_t>(max(end, 0)) * 16u);
-  Candidates c{key, &count, 0, kNegInf};
-  if (tid == 0) {
-    count = 0;
-    first_least = kNegInf;
-  }
+  Candidates c{sh, 0, kNegInf};
+  if (tid == 0) sh.count = 0;
   float m = kNegInf, s = 0.f;
   __syncthreads();
   if (part == 0 && tid < 64) {   // the elements outside the interior
@@ -156,119 +267,179 @@ __global__ void __launch_bounds__(kBlock) top_part_kernel(TopArgs a) {
     }
     c.add(ek >= 0, element_key(xe, static_cast<uint32_t>(ek)));
   }
-  for (int base = v0; base < end; base += BLOCK * U) {
+  // The candidates are thinned where they pass `limit`; after the last batch to about k.
+  const int room = min(kCut, 2 * a.k + 128), left = a.parts == 1 ? a.k + 64 : a.part_cap;
+  constexpr int kRounds = U * EPV / 4;                   // of 4 elements per lane
+  int n = part == 0 ? sp.head + sp.tail : 0;             // candidates before the batch
+  int round = -1;                                        // >= 0: a batch taken in rounds
+  for (int base = v0; base < end;) {
     u32x4 x[U];
     const uint32_t off = static_cast<uint32_t>(base + tid) * 16u;
 #pragma unroll
     for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
     auto held = [&](int q) { return base + q * BLOCK + tid < end; };
-    float bx = kNegInf;
+    uint64_t near[U];   // the lanes whose vector may hold an element that passes
+    bool fresh = round >= 0 || base == v0 || __any(m == kNegInf);
+    if (!fresh) {
+      // Terms against the lane's maximum so far, and the vectors compared by their largest term:
+      // no pass for a new maximum unless one has risen far above.
+      const float cut = hw_exp2(fmaf(c.least_x, a.k2, -m)) * (1.f - 0x1p-16f);
+      const float floor = cut > 0x1p-100f ? cut : 0.f;   // rounding above, underflow below
+      float acc = s, most = 0.f;
 #pragma unroll
-    for (int q = 0; q < U; ++q)
-      if (held(q)) bx = vec_max<TI>(bx, x[q]);
-    {
-      const float nm = fmaxf(m, bx * a.k2), ref = ms_ref(nm);
-      float acc = ms_rescale(s, m, nm);
-#pragma unroll
-      for (int q = 0; q < U; ++q)
+      for (int q = 0; q < U; ++q) {
+        float e[EPV], ve = 0.f;
         if (held(q)) {
           const uint32_t* w = reinterpret_cast<const uint32_t*>(&x[q]);
 #pragma unroll
-          for (int j = 0; j < EPV; ++j) acc += hw_exp2(fmaf(TI::unpack(w, j), a.k2, -ref));
-        }
-      m = nm;
-      s = acc;
-    }
-    if (base == v0) {
-      // The k-th largest of the lanes' maxima: k elements of this batch reach it.
-      lane_max[tid] = bx;
-      __syncthreads();
-      int above = 0;
-      for (int i = 0; i < BLOCK; ++i) above += lane_max[i] > bx || (lane_max[i] == bx && i < tid);
-      if (above == a.k - 1) first_least = bx;
-      __syncthreads();
-      c.least_x = first_least;
-    }
-    auto offer = [&](int q, int j0, int j1) {
+          for (int j = 0; j < EPV; ++j) {
+            e[j] = hw_exp2(fmaf(TI::unpack(w, j), a.k2, -m));
+            acc += e[j];
+          }
 #pragma unroll
-      for (int j = j0; j < j1; ++j) {
-        const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j);
-        const bool near = held(q) && !(v < c.least_x);
-        if (__any(near)) {
-          const uint32_t id = static_cast<uint32_t>(sp.head + (base + q * BLOCK + tid) * EPV + j);
-          const uint64_t k = element_key(v, id);
-          c.add(near && k > c.least, k);
+          for (int j = 0; j < EPV; j += 2) ve = max3(ve, e[j], e[j + 1]);
         }
+        near[q] = __ballot(held(q) && ve >= floor);
+        most = fmaxf(most, ve);
       }
-    };
-    __syncthreads();
-    const int before = count;
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < U; ++q) offer(q, 0, EPV);
-    __syncthreads();
-    int n = count;
-    if (n > kCap) {   // too many at once: this batch again, in rounds that are sure to fit
-      __syncthreads();
-      if (tid == 0) count = before;
-      __syncthreads();
-      n = before;
-#pragma unroll
-      for (int q = 0; q < U; ++q)
-#pragma unroll
-        for (int h = 0; h < EPV; h += 4) {
-          if (n > kCut) n = c.cut(n, a.k);
-          offer(q, h, h + 4);
-          __syncthreads();
-          n = count;
-          __syncthreads();
-        }
+      fresh = __any(most > 0x1p40f);
+      if (!fresh) s = acc;
     }
-    if (n > kCut) n = c.cut(n, a.k);
+    if (fresh) {
+      float vm[U], bx = kNegInf;
+#pragma unroll
+      for (int q = 0; q < U; ++q) {
+        vm[q] = held(q) ? vec_max<TI>(kNegInf, x[q]) : kNegInf;
+        bx = fmaxf(bx, vm[q]);
+      }
+      if (round < 0) {
+        const float nm = fmaxf(m, bx * a.k2), ref = ms_ref(nm);
+        float acc = ms_rescale(s, m, nm);
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+          if (held(q)) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(&x[q]);
+#pragma unroll
+            for (int j = 0; j < EPV; ++j) acc += hw_exp2(fmaf(TI::unpack(w, j), a.k2, -ref));
+          }
+        m = nm;
+        s = acc;
+        // k vectors of the first batch reach this, each with one element at least.
+        if (base == v0) c.least_x = reached_by(sh, vm, a.k);
+      }
+#pragma unroll
+      for (int q = 0; q < U; ++q) near[q] = __ballot(held(q) && (vm[q] >= c.least_x || c.least_x == kNegInf));
+    }
+    // While nothing is ruled out NaN is taken too, which ranks below all.
+    const bool all = c.least_x == kNegInf;
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      if (near[q] == 0) continue;
+      // Bit EPV - 1 - j: element j passes. Few lanes have any, fewer have two.
+      uint32_t bits = 0;
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) {
+        const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j);
+        bits = 2 * bits + ((v >= c.least_x || all) ? 1u : 0u);
+      }
+      if (!held(q)) bits = 0;
+      if (round >= 0) bits &= round / (EPV / 4) == q ? 0xf0u >> (EPV == 4 ? 4 : 4 * (round % 2)) : 0u;
+      while (__any(bits != 0)) {
+        const int j = EPV - 32 + __builtin_clz(bits | 1u);   // the first that is left
+        uint32_t w = x[q][0];
+        const int word = TI::kBytes == 4 ? j : j >> 1;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) w = word == i ? x[q][i] : w;
+        if constexpr (TI::kBytes == 2) w >>= 16 * (j & 1);
+        const uint64_t k = element_key(TI::unpack(&w, 0), static_cast<uint32_t>(sp.head + (base + q * BLOCK + tid) * EPV + j));
+        c.add(bits != 0 && k > c.least, k);
+        bits &= ~((1u << (EPV - 1)) >> j);
+      }
+    }
+    __syncthreads();
+    const int was = n;
+    n = sh.count;
+    __syncthreads();
+    if (round < 0 && n > kCap) {   // too many at once: this batch again, in rounds that are sure to fit
+      if (tid == 0) sh.count = was;
+      n = was;
+      round = 0;
+    } else if (round < 0 || ++round == kRounds) {
+      round = -1;
+      base += BLOCK * U;
+    }
+    if (n > (base >= end ? left : round >= 0 ? kCut : room)) n = c.thin(n, a.k, base >= end ? left : kCut);
+    else __syncthreads();
   }
   __syncthreads();
-  const int n = count;
+  n = sh.count;
   float m2 = kNegInf, s2 = 0.f;
   block_merge2<BLOCK>(m, s, m2, s2, lds);
-  sort_falling(key, n);
   if (a.parts == 1) {
-    write_entries(a, row, key);
+    write_entries(a, row, sh, n);
     if (tid == 0) write_lse(a, row, m, s);
   } else {
-    uint64_t* out = a.part_key + (row * a.parts + part) * a.k;
-    for (int i = tid; i < a.k; i += BLOCK) out[i] = i < n ? key[i] : 0;
-    if (tid == 0) a.part_ms[row * a.parts + part] = make_float2(m, s);
+    uint64_t* out = a.part_key + (row * a.parts + part) * a.part_cap;
+    for (int i = tid; i < n; i += BLOCK) out[i] = sh.key[i];
+    if (tid == 0) a.part_ms[row * a.parts + part] = make_float4(m, s, __int_as_float(n), 0.f);
   }
 }
 
+// The parts' candidates, kMergeKeys per lane at a time: a histogram of the first ones finds what
+// k of them reach, as in the first kernel.
+constexpr int kMergeKeys = 12;
+
 __global__ void __launch_bounds__(kBlock) top_merge_kernel(TopArgs a) {
-  __shared__ uint64_t key[kCap];
-  __shared__ int count;
+  constexpr int R = kMergeKeys, kPer = 4;   // keys per lane: of a round, of a cautious one
+  static_assert(R % kPer == 0 && kBlock * kPer <= kCap - kCut, "cautious rounds fit");
+  __shared__ __align__(16) Shared sh;
   const int tid = threadIdx.x;
   const int64_t row = a.row0 + blockIdx.x;
-  const uint64_t* in = a.part_key + row * a.parts * a.k;
-  const int total = a.parts * a.k;
-  Candidates c{key, &count, 0, kNegInf};
-  if (tid == 0) count = 0;
+  const uint64_t* in = a.part_key + row * a.parts * a.part_cap;
+  const float4* ms = a.part_ms + row * a.parts;
+  const int total = a.parts * a.part_cap;
+  Candidates c{sh, 0, kNegInf};
+  if (tid == 0) sh.count = 0;
   __syncthreads();
-  int n = 0;
-  for (int base = 0; base < total; base += kBlock) {
-    if (n > kCap - kBlock) n = c.cut(n, a.k);
-    const uint64_t k = base + tid < total ? in[base + tid] : 0;
-    c.add(k > c.least, k);
+  int n = 0, round = -1;
+  for (int base = 0; base < total;) {
+    uint64_t k[R];
+    float v[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int at = base + i * kBlock + tid, p = at / a.part_cap;
+      const bool is = at < total && at - p * a.part_cap < __float_as_int(ms[p].z);
+      k[i] = is ? in[at] : 0;   // no key is 0
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] = k[i] ? from_order(static_cast<uint32_t>(k[i] >> 32)) : kNegInf;
+    if (base == 0 && round < 0) c.least_x = reached_by(sh, v, a.k);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      if (round >= 0 && i / kPer != round) continue;
+      c.add(k[i] > c.least && (v[i] >= c.least_x || c.least_x == kNegInf), k[i]);
+    }
     __syncthreads();
-    n = count;
+    const int was = n;
+    n = sh.count;
     __syncthreads();
+    if (round < 0 && n > kCap) {
+      if (tid == 0) sh.count = was;
+      n = was;
+      round = 0;
+    } else if (round < 0 || ++round == R / kPer) {
+      round = -1;
+      base += kBlock * R;
+    }
+    if (n > (base >= total ? a.k + 64 : kCut)) n = c.thin(n, a.k, kCut);
+    else __syncthreads();
   }
-  sort_falling(key, n);
-  write_entries(a, row, key);
+  write_entries(a, row, sh, n);
   if (tid < 64) {
     float m = kNegInf, s = 0.f;
-    for (int p = tid; p < a.parts; p += 64) {
-      const float2 v = a.part_ms[row * a.parts + p];
-      const float M = fmaxf(m, v.x);
-      s = ms_rescale(s, m, M) + ms_rescale(v.y, v.x, M);
-      m = M;
+    if (tid < a.parts) {
+      m = ms[tid].x;
+      s = ms[tid].y;
     }
     lanes_merge<64>(m, s);
     if (tid == 0) write_lse(a, row, m, s);
@@ -332,10 +503,12 @@ int top_logits(pcp_ctx* ctx, const pcp_top_logits_args* a) {
   const int64_t batches = nv > 0 ? (nv + kBlock * kU - 1) / (kBlock * kU) : 1;
   int64_t parts = (2048 + a->n_rows - 1) / a->n_rows;
   if (parts > batches) parts = batches;
+  if (parts > 64) parts = 64;   // one wave merges their sums
   const int64_t per_batches = (batches + parts - 1) / parts;
   parts = (batches + per_batches - 1) / per_batches;
-  const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(a->n_rows) * parts * a->k : 0;
-  const size_t ms = parts > 1 ? sizeof(float2) * static_cast<size_t>(a->n_rows) * parts : 0;
+  const int64_t part_cap = a->k + 64;
+  const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(a->n_rows) * parts * part_cap : 0;
+  const size_t ms = parts > 1 ? sizeof(float4) * static_cast<size_t>(a->n_rows) * parts + 16 : 0;
   const int rc = ensure_scratch_on(ctx, keys + ms, st);
   if (rc != PCP_OK) return rc;
 
@@ -349,13 +522,14 @@ int top_logits(pcp_ctx* ctx, const pcp_top_logits_args* a) {
   t.ids = a->ids;
   t.lse = a->lse;
   t.part_key = static_cast<uint64_t*>(ctx->scratch);
-  t.part_ms = reinterpret_cast<float2*>(static_cast<char*>(ctx->scratch) + keys);
+  t.part_ms = reinterpret_cast<float4*>(static_cast<char*>(ctx->scratch) + ((keys + 15) & ~static_cast<size_t>(15)));
   t.err = ctx->d_page->err;
   t.k2 = k2;
   t.k = a->k;
   t.ids_i64 = a->ids_dtype == PCP_I64;
   t.parts = static_cast<int32_t>(parts);
   t.per = static_cast<int32_t>(per_batches * kBlock * kU);
+  t.part_cap = static_cast<int32_t>(part_cap);
   const bool timed = prof_begin(ctx, st);
   const hipError_t e = a->logits_dtype == PCP_F32    ? launch_top<F32T>(t, st)
                        : a->logits_dtype == PCP_BF16 ? launch_top<BF16T>(t, st)

@@ -87,6 +87,30 @@ def test_top_logits_orders(kind, dtype, R, V, k):
     check_top(x, k, 1.0, distill.top_logits(x, k))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("R,V,k", [(3, 40000, 200), (2100, 5000, 30), (2, 600, 256)])
+def test_top_logits_masks_of_the_lowest_value(dtype, R, V, k):
+    """Two thirds of the vocabulary at the type's lowest value or -inf, in runs and scattered,
+    with one row of NaN between (which outranks nothing)."""
+    rng = np.random.default_rng(R + k)
+    x = rows_like_a_model(rng, (R, V))
+    low = float(torch.finfo(DT[dtype]).min)
+    x[:, V // 3:2 * V // 3] = low
+    x[rng.random((R, V)) < 0.4] = low
+    x[1::2][x[1::2] == low] = -np.inf
+    check_top(to_dev(x, dtype), k, 1.0, distill.top_logits(to_dev(x, dtype), k))
+    x[1] = np.nan
+    x[1, 5:5 + k - 1] = 1.0
+    t = to_dev(x, dtype)
+    ctx = grpo.Context(0)
+    out = distill.top_logits(t, k, sync=False, ctx=ctx)
+    with pytest.raises(PcpError):
+        ctx.sync()
+    assert torch.equal(out.ids[1, :k - 1].cpu(), torch.arange(5, 5 + k - 1, dtype=torch.int32))
+    assert torch.isnan(out.values[1, k - 1]) and int(out.ids[1, k - 1]) == 0
+    check_top(t[2:], k, 1.0, distill.TopLogits(out.values[2:], out.ids[2:], out.lse[2:]))
+
+
 def test_top_logits_rows_apart_and_long():
     """Rows further apart than the vocabulary, and offsets past 2^31 elements."""
     rng = np.random.default_rng(1)
