@@ -1288,6 +1288,8 @@ __global__ void __launch_bounds__(kSmallBlock) loss_reduce_kernel(LossReduceArgs
 // ---------------------------------------------------------------------------
 namespace {
 
+}  // namespace
+
 // How far on each stride of rows dealt in grid strides (kResStatic) starts. Where a workgroup
 // would meet three positions of a sequence or fewer over and over (sequences of 128, 256 or 96
 // rows, say), it would get rows that are all live or all dead: it then moves on by the golden
@@ -1302,6 +1304,8 @@ int32_t resident_turn(int64_t grid, int64_t seq, bool masked) {
   if (!masked || seq / std::gcd(grid, seq) > 3) return 0;
   return static_cast<int32_t>((static_cast<int64_t>(0.618034 * static_cast<double>(seq)) + seq - grid % seq) % seq % grid);
 }
+
+namespace {
 
 template <typename TI, typename TO, int BLOCK, int NCH, bool EDGE, bool CACHE>
 hipError_t launch_resident(RowArgs a, int64_t nrows, hipStream_t st) {

@@ -39,6 +39,9 @@ RowPlan plan_rows(const RowShape& shape, int64_t nrows);
 // Bytes of RowArgs::part (kParts), at most: 1,536 rows of 64 parts.
 constexpr size_t kPartScratchBytes = 1536 * (64 + 1) * 16;
 
+// Rows dealt in grid strides: how far on each stride starts (see grpo_kernels.hip).
+int32_t resident_turn(int64_t grid, int64_t seq, bool masked);
+
 hipError_t launch_seq_prep(const void* mask, int mask_u8, int64_t n_seq, int64_t rows,
                            int64_t tok_stride, int64_t tok_offset, float loss_norm,
                            float* seq_len, float* seq_scale, hipStream_t st);
