@@ -29,7 +29,8 @@ constexpr int64_t kDistillRowVecs = 1024 * 19;
 
 constexpr int kMaxEntries = PCP_TOP_LOGITS_MAX;
 constexpr int kWave = 64;
-// Entry i is slot i / 64 of lane i % 64; kernels are compiled for 1 slot (k <= 64) and for 4.
+// Entry i is slot i / 64 of lane i % 64; the kernels of rows in parts are compiled for 1 slot
+// (k <= 64) and for 4.
 constexpr int kMaxSlots = kMaxEntries / kWave;
 
 // What a row's teacher comes to, whatever the student.
@@ -94,7 +95,12 @@ __device__ __forceinline__ DistillRow distill_row(const DistillArgs& a, int64_t 
   return r;
 }
 
-// Entry i of a row: its id, or -1 when it is unused, -2 when its id is out of range.
+// An entry's id, or -1 when it is unused, -2 when its id is out of range.
+__device__ __forceinline__ int used_id(const DistillArgs& a, int64_t id, float t) {
+  if (id == PCP_IGNORE_INDEX || t == kNegInf) return -1;
+  return id >= 0 && id < a.vocab ? static_cast<int>(id) : -2;
+}
+// Entry i of a row.
 __device__ __forceinline__ int entry_id(const DistillArgs& a, int64_t row, int i, float& t) {
   t = kNegInf;
   if (i >= a.k) return -1;
@@ -102,8 +108,7 @@ __device__ __forceinline__ int entry_id(const DistillArgs& a, int64_t row, int i
   const int64_t id = a.ids_i64 ? static_cast<const int64_t*>(a.tids)[e]
                                : static_cast<int64_t>(static_cast<const int32_t*>(a.tids)[e]);
   t = a.tlogits[e];
-  if (id == PCP_IGNORE_INDEX || t == kNegInf) return -1;
-  return id >= 0 && id < a.vocab ? static_cast<int>(id) : -2;
+  return used_id(a, id, t);
 }
 
 // Where a workgroup of BLOCK lanes that holds vectors [v0, v0 + U * BLOCK) of a row's interior
@@ -293,14 +298,15 @@ __global__ void __launch_bounds__(BLOCK) distill_prepare_kernel(DistillArgs a) {
 }
 
 // ---- a row's terms -----------------------------------------------------------------------
-// A row's teacher and the student's logits there, in LDS for the whole workgroup.
+// A row's teacher and the student's logits there, in LDS for the whole workgroup. Entries go by
+// groups of 64, group w staged by wave w.
 struct Teacher {
   TeacherRow row;
   int id[kMaxEntries];
   float t[kMaxEntries];
   float p[kMaxEntries];
-  float z[kMaxEntries];     // the student's logits
-  float mk, sk;             // their log-sum-exp state, base 2
+  float z[kMaxEntries];                   // the student's logits, and
+  float mk[kMaxSlots], sk[kMaxSlots];     // per group their log-sum-exp state, base 2
 };
 
 // What a row's gradient needs: tail * 2^(x k2 - ref) outside K, g[] at the entries.
@@ -309,106 +315,120 @@ struct RowTerms {
   float g[kMaxEntries];
 };
 
-// A row's entries to LDS, by one wave, in steps: the loads, the stores, the student's part.
-template <int NS>
-struct Entries {
-  int id[NS];
-  float t[NS], p[NS];
+// A group's entries to LDS in steps: the loads, the stores, the student's part.
+struct Entry {
+  int id;
+  float t, p;
 };
-template <int NS>
-__device__ __forceinline__ void load_entries(const DistillArgs& a, int64_t row, Entries<NS>& e) {
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    const int i = static_cast<int>(threadIdx.x & 63) + kWave * s;
-    e.id[s] = entry_id(a, row, i, e.t[s]);
-    e.p[s] = i < a.k ? a.teacher_p[row * a.k + i] : 0.f;
-  }
+__device__ __forceinline__ Entry load_entry(const DistillArgs& a, int64_t row, int group) {
+  const int i = static_cast<int>(threadIdx.x & 63) + kWave * group;
+  Entry e;
+  e.id = entry_id(a, row, i, e.t);
+  e.p = i < a.k ? a.teacher_p[row * a.k + i] : 0.f;
+  return e;
 }
-template <int NS>
-__device__ __forceinline__ void put_entries(const DistillArgs& a, int64_t row, Teacher& te, const Entries<NS>& e) {
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    const int i = static_cast<int>(threadIdx.x & 63) + kWave * s;
-    te.id[i] = e.id[s];
-    te.t[i] = e.t[s];
-    te.p[i] = e.p[s];
-  }
-  if ((threadIdx.x & 63) == 0) te.row = a.teacher[row];
+__device__ __forceinline__ void put_entry(Teacher& te, int group, const Entry& e) {
+  const int i = static_cast<int>(threadIdx.x & 63) + kWave * group;
+  te.id[i] = e.id;
+  te.t[i] = e.t;
+  te.p[i] = e.p;
 }
-template <int NS>
-__device__ __forceinline__ void put_student(const DistillArgs& a, Teacher& te, const float (&z)[NS]) {
-  const int lane = threadIdx.x & 63;
-  float zmax = kNegInf, sk = 0.f;
-  bool used[NS];
-#pragma unroll
-  for (int s = 0; s < NS; ++s) {
-    used[s] = te.id[lane + kWave * s] >= 0;
-    te.z[lane + kWave * s] = z[s];
-    if (used[s]) zmax = fmaxf(zmax, z[s]);
-  }
-  const float mk = lanes_max<64>(zmax) * a.k2;
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-    if (used[s]) sk += hw_exp2(fmaf(z[s], a.k2, -ms_ref(mk)));
-  sk = lanes_sum<64>(sk);
+__device__ __forceinline__ void put_student(const DistillArgs& a, Teacher& te, int group, float z) {
+  const int lane = threadIdx.x & 63, i = lane + kWave * group;
+  const bool used = te.id[i] >= 0;
+  te.z[i] = z;
+  const float mk = lanes_max<64>(used ? z : kNegInf) * a.k2;
+  const float sk = lanes_sum<64>(used ? hw_exp2(fmaf(z, a.k2, -ms_ref(mk))) : 0.f);
   if (lane == 0) {
-    te.mk = mk;
-    te.sk = sk;
+    te.mk[group] = mk;
+    te.sk[group] = sk;
   }
+}
+__device__ __forceinline__ int groups_of(const DistillArgs& a) { return (a.k + kWave - 1) / kWave; }
+// The largest of the entries' scaled logits.
+__device__ __forceinline__ float entries_max(const Teacher& te, int groups) {
+  float m = te.mk[0];
+  for (int w = 1; w < groups; ++w) m = fmaxf(m, te.mk[w]);
+  return m;
 }
 
-// By all lanes of one wave, into LDS; returns m * l. mt, st: the state outside K.
-template <int NS>
-__device__ __forceinline__ float row_terms(const DistillArgs& a, const DistillRow& r, const Teacher& te, float mt,
-                                           float st, RowTerms& o) {
-  const int lane = threadIdx.x & 63;
-  const float m = fmaxf(mt, te.mk), rm = ms_ref(m);
-  const float ft = st == 0.f ? 0.f : hw_exp2(mt - rm);
-  const float s = (st == 0.f ? 0.f : st * ft) + (te.sk == 0.f ? 0.f : te.sk * hw_exp2(te.mk - rm));
-  const double lse = ms_lse(m, s);
-  const float inv_s = 1.f / s;
-  const float qt = st * ft * inv_s;
-  const bool tail = a.tlse != nullptr && qt >= 0x1p-126f;
-  const float pt = tail ? te.row.pt : 0.f;
-  const double tail_gap = tail ? te.row.log_pt - (ms_lse(mt, st) - lse) : 0.;   // log(p_T / q_T)
-  const float c = static_cast<float>(static_cast<double>(a.seq_scale[r.seq] * r.w) * a.inv_tau);
-  double gap[NS], l = 0.;
-  float q[NS];
-#pragma unroll
-  for (int e = 0; e < NS; ++e) {
-    const int i = lane + kWave * e;
-    q[e] = 0.f;
-    gap[e] = 0.;
-    if (kWave * e >= a.k || te.id[i] < 0) continue;
-    q[e] = hw_exp2(fmaf(te.z[i], a.k2, -rm)) * inv_s;
-    const double log_q = static_cast<double>(te.z[i]) * static_cast<double>(a.k2) * 0.69314718055994530942 - lse;
-    gap[e] = static_cast<double>(te.t[i]) * a.inv_tau - te.row.lse - log_q;   // log(p_i / q_i)
-    if (a.forward ? te.p[i] > 0.f : q[e] > 0.f) l += a.forward ? te.p[i] * gap[e] : -q[e] * gap[e];
+// A row's factors, the same in every lane of any wave that forms them.
+struct RowFactors {
+  float tail, ref;      // the gradient outside K: tail * 2^(x k2 - ref)
+  float c, rm, inv_s;   // the coefficient; q_i = 2^(z k2 - rm) inv_s
+  float big_p, lf;      // forward: P; reverse: l
+  float mt, st, m, s;   // the state outside K, and of the whole row
+};
+
+__device__ __forceinline__ float entry_prob(const DistillArgs& a, const Teacher& te, const RowFactors& f, int i) {
+  return hw_exp2(fmaf(te.z[i], a.k2, -f.rm)) * f.inv_s;
+}
+// log(p_i / q_i)
+__device__ __forceinline__ double entry_gap(const DistillArgs& a, const Teacher& te, double lse, int i) {
+  return static_cast<double>(te.t[i]) * a.inv_tau - te.row.lse -
+         (static_cast<double>(te.z[i]) * static_cast<double>(a.k2) * 0.69314718055994530942 - lse);
+}
+// The gradient at entry i.
+__device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher& te, const RowFactors& f, int i) {
+  const float q = entry_prob(a, te, f, i);
+  if (a.forward) return f.c * (q * f.big_p - te.p[i]);
+  return q > 0.f ? -f.c * q * (static_cast<float>(entry_gap(a, te, ms_lse(f.m, f.s), i)) + f.lf) : 0.f;
+}
+
+__device__ __forceinline__ bool has_tail(const DistillArgs& a, const RowFactors& f) {
+  return a.tlse != nullptr && f.st * hw_exp2(f.mt - f.rm) * f.inv_s >= 0x1p-126f;
+}
+
+// The row's divergence l, by a whole wave. Its sums run in 64 bits: l may be far below its terms.
+__device__ __forceinline__ double row_loss(const DistillArgs& a, const Teacher& te, const RowFactors& f) {
+  const int lane = threadIdx.x & 63, groups = groups_of(a);
+  const double lse = ms_lse(f.m, f.s);
+  double l = 0.;
+  for (int w = 0; w < groups; ++w) {
+    const int i = lane + kWave * w;
+    if (te.id[i] < 0) continue;
+    const float weight = a.forward ? te.p[i] : -entry_prob(a, te, f, i);
+    if (weight != 0.f) l += weight * entry_gap(a, te, lse, i);
   }
   l = wave_sum64(l);
-  float tail_factor;
+  if (has_tail(a, f)) {
+    const double gap = te.row.log_pt - (ms_lse(f.mt, f.st) - lse);   // log(p_T / q_T)
+    l += a.forward ? te.row.pt * gap : -(f.st * hw_exp2(f.mt - f.rm) * f.inv_s) * gap;
+  }
+  if (lane == 0 && !(__builtin_isfinite(lse) && l == l)) raise_error(a.err, kErrNonFinite);
+  return l;
+}
+
+// mt, st: the state outside K. The forward gradient does without the loss, the reverse one holds it
+// (loss: l, formed here if reverse).
+// weight: the row's scale times its weight.
+__device__ __forceinline__ RowFactors row_factors(const DistillArgs& a, float weight, const Teacher& te, float mt,
+                                                  float st, double& loss) {
+  const int groups = groups_of(a);
+  RowFactors f;
+  f.mt = mt;
+  f.st = st;
+  f.m = fmaxf(mt, entries_max(te, groups));
+  f.rm = ms_ref(f.m);
+  const float ft = st == 0.f ? 0.f : hw_exp2(mt - f.rm);
+  f.s = st == 0.f ? 0.f : st * ft;
+  for (int w = 0; w < groups; ++w) f.s += te.sk[w] == 0.f ? 0.f : te.sk[w] * hw_exp2(te.mk[w] - f.rm);
+  f.inv_s = 1.f / f.s;
+  f.c = static_cast<float>(static_cast<double>(weight) * a.inv_tau);
+  f.ref = ms_ref(mt);
+  f.big_p = f.lf = 0.f;
+  const bool tail = has_tail(a, f);
   if (a.forward) {
-    l += pt > 0.f ? pt * tail_gap : 0.;
-    const float big_p = static_cast<float>(te.row.sum_p + pt);
-    tail_factor = st == 0.f ? 0.f : c * (big_p * ft * inv_s - pt / st);
-#pragma unroll
-    for (int e = 0; e < NS; ++e)
-      if (kWave * e < a.k) o.g[lane + kWave * e] = c * (q[e] * big_p - te.p[lane + kWave * e]);
+    const float pt = tail ? te.row.pt : 0.f;
+    f.big_p = static_cast<float>(te.row.sum_p + pt);
+    f.tail = st == 0.f ? 0.f : f.c * (f.big_p * ft * f.inv_s - pt / st);
   } else {
-    l -= tail ? qt * tail_gap : 0.;
-    const float lf = static_cast<float>(l);
-    tail_factor = st == 0.f ? 0.f : -c * (ft * inv_s) * (static_cast<float>(tail_gap) + lf);
-#pragma unroll
-    for (int e = 0; e < NS; ++e)
-      if (kWave * e < a.k) o.g[lane + kWave * e] = q[e] > 0.f ? -c * q[e] * (static_cast<float>(gap[e]) + lf) : 0.f;
+    loss = row_loss(a, te, f);
+    f.lf = static_cast<float>(loss);
+    const double gap = tail ? te.row.log_pt - (ms_lse(mt, st) - ms_lse(f.m, f.s)) : 0.;
+    f.tail = st == 0.f ? 0.f : -f.c * (ft * f.inv_s) * (static_cast<float>(gap) + f.lf);
   }
-  if (lane == 0) {
-    o.tail = tail_factor;
-    o.ref = ms_ref(mt);
-  }
-  if (lane == 0 && !(__builtin_isfinite(lse) && l == l))
-    raise_error(a.err, kErrNonFinite);
-  return r.w * static_cast<float>(l);
+  return f;
 }
 
 // ---------------------------------------------------------------------------
@@ -533,23 +553,38 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
       }
       if (ek >= 0) xe = TI::load1(xrow, ek);
     }
+    const int groups = groups_of(a);
+    if (tid == 0) te.row = a.teacher[row];
+    for (int w = tid >> 6; w < groups; w += static_cast<int>(blockDim.x) >> 6) {
+      const Entry e = load_entry(a, row, w);
+      const float z = e.id >= 0 ? a.part_z[row * a.k + (tid & 63) + kWave * w] : kNegInf;
+      put_entry(te, w, e);
+      put_student(a, te, w, z);
+    }
+    __syncthreads();
     if (tid < 64) {
-      Entries<NS> e;
-      float z[NS];
-      load_entries(a, row, e);
-#pragma unroll
-      for (int s = 0; s < NS; ++s) z[s] = e.id[s] >= 0 ? a.part_z[row * a.k + tid + kWave * s] : kNegInf;
       float mt, st;
       bool twice;
       merge_tail(a, row, mt, st, twice);
-      put_entries(a, row, te, e);
-      put_student(a, te, z);
       if (tid == 0 && twice) {
         te.row.state = kBad;
         if (part == 0) raise_error(a.err, kErrTeacherTwice);
       }
       float token = 0.f;
-      if (te.row.state == kUsed) token = row_terms<NS>(a, r, te, mt, st, terms);
+      if (te.row.state == kUsed) {
+        double l = 0.;
+        const RowFactors f = row_factors(a, a.seq_scale[r.seq] * r.w, te, mt, st, l);
+        for (int w = 0; w < groups; ++w) {
+          const int i = tid + kWave * w;
+          terms.g[i] = te.id[i] >= 0 ? entry_grad(a, te, f, i) : 0.f;
+        }
+        terms.tail = f.tail;
+        terms.ref = f.ref;
+        if (part == 0) {
+          if (a.forward) l = row_loss(a, te, f);
+          token = r.w * static_cast<float>(l);
+        }
+      }
       if (part == 0 && tid == 0 && a.token_loss) a.token_loss[r.tix] = token;
     }
     __syncthreads();
@@ -570,7 +605,7 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
       ref = terms.ref;
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        const int id = te.id[(tid & 63) + kWave * s];
+        const int id = kWave * s < a.k ? te.id[(tid & 63) + kWave * s] : -1;
         if (id >= 0) g[s] = terms.g[(tid & 63) + kWave * s];
         place[s] = id >= 0 && id - sp.head < end * EPV ? entry_place<TI, kSplit, BLOCK, U>(id - sp.head, v0) : -1;
         if (place[s] >= 0 && ((place[s] >> 10) & 15) != (tid >> 6)) place[s] = -1;
@@ -641,11 +676,15 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
 
 
 // ---------------------------------------------------------------------------
-// A row to a workgroup, kept in registers from its one read to its gradient's write.
-// Persistent: while a row's gradient is stored, each chunk's registers take the next row's
-// load, so the CU reads and writes at once; the next row's entries come the same way (ids and
-// probabilities at the top of this row, the student's logits there after its merge, their
-// sum after its stores, all by the first wave, through the other half of te).
+// A row to a workgroup, kept in registers from its one read to its gradient's write, by a
+// persistent grid. A wave's loads and stores complete in order here, so a value loaded after a
+// row's stores can be had only when they have gone out to memory, several microseconds later:
+// nothing a row needs is loaded then but its chunks. Its entries come two rows ahead, the student's
+// logits there and its teacher's record one row ahead, each with that row's chunks, and go to LDS
+// before that row's stores. The sums need no maximum of their own: they are taken against
+// the largest of the entries' logits, which is the row's largest or near it, and formed again
+// against the true maximum where they leave f32's range (a tail that is masked, or 2^100 above
+// what the teacher named).
 // Requirements (checked on the host): the row's interior fits BLOCK * NCH vectors; dlogits
 // rows split like the logits rows, or hold f32 for 16-bit logits (dword-aligned stores).
 // ---------------------------------------------------------------------------
@@ -653,244 +692,428 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
 // counter, for the reasons given at grpo_resident_kernel.
 template <int BLOCK, int NCH>
 constexpr bool kDealt = BLOCK * NCH <= 2048;
+#ifndef D_SP
+#define D_SP kBufNTSystem
+#endif
 
-template <typename TI, typename TO, int BLOCK, int NCH, int NS>
-__global__ void __launch_bounds__(BLOCK) distill_row_kernel(DistillArgs a) {
+__device__ __forceinline__ float uniform(float v) { return read_lane(v, 0); }
+
+// A wave's entries lie in lane-held lists: entry list[l] of the row with its place, lane l of
+// group 0 in registers, of further groups (over 64 entries in one wave's part of the row: ids
+// that lie close together) in LDS.
+struct Owned {
+  int place;         // of group 0's entry; -1
+  int n;
+  uint32_t chunks;   // bit k: chunk k holds one of them
+};
+
+template <typename TI, typename TO, int BLOCK, int NCH, int FULL>
+__global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
   constexpr int EPV = 16 / TI::kBytes, NW = BLOCK / 64;
   constexpr bool kSplit = TI::kBytes == 2 && TO::kBytes == 4, kStatic = kDealt<BLOCK, NCH>;
   constexpr uint32_t kOutVec = EPV * TO::kBytes;
-  __shared__ Teacher te[2];
-  __shared__ RowTerms terms;
-  __shared__ float4 merge[NW];
+  static_assert(NW >= kMaxSlots, "a wave per group of entries");
+  __shared__ Teacher te4[4];                   // of the row before (its loss is formed under this row's loads), this one, the next two
+  __shared__ RowFactors factors[NW];           // each wave its own copy of the same: out of registers under the stores
+  __shared__ uint8_t list[2][NW][kMaxEntries];
+  __shared__ float2 merge[NW];
   __shared__ int s_next[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = groups_of(a);
   const uint32_t voff = tid * 16u, sgrp = split_group<TI, TO, BLOCK>(tid);
   const char* logits = static_cast<const char*>(a.logits);
-  auto span_of = [&](int64_t row) { return row_span<TI>(logits + row * a.vocab * TI::kBytes, a.vocab); };
-  auto buffer_of = [&](const RowSpan& sp, bool on) {   // off: loads return 0 without an access
-    return row_rsrc(sp.vec, on ? static_cast<uint32_t>(sp.nv) * 16u : 0u);
+  auto row_of = [&](int64_t row) { return logits + row * a.vocab * TI::kBytes; };
+  // kSplit: half h of chunk k of this lane holds values of a row of nv vectors. (The chunk goes to
+  // the uniform side: k * BLOCK + tid would be a register kept for each.)
+  auto held = [&](int nv, int k, int h) {
+    return k < FULL || (kSplit ? static_cast<int>(sgrp) < 2 * nv - k * 2 * BLOCK - 64 * h : tid < nv - k * BLOCK);
   };
-  int64_t stride0 = 0;                                 // static: the current stride's first row
+  int64_t stride0 = 0;                                 // static: the last stride dealt
   uint32_t at = blockIdx.x;
-  auto deal = [&]() -> int64_t {                       // static: the row after this one
+  auto deal = [&]() -> int64_t {
     stride0 += gridDim.x;
     at += static_cast<uint32_t>(a.turn);
     if (at >= gridDim.x) at -= gridDim.x;
     return stride0 + at;
   };
-  int64_t row = blockIdx.x, next = kStatic ? deal() : static_cast<int64_t>(blockIdx.x) + gridDim.x;
-  DistillRow r = distill_row(a, row);
-  RowSpan sp = span_of(row);
-  u32x4 xv[NCH];
-  float xe = 0.f;
-  {
-    const __amdgpu_buffer_rsrc_t buf = buffer_of(sp, r.w != 0.f);
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) xv[k] = load_chunk<TI, TO, BLOCK>(buf, k, voff, sgrp);
-    if (r.w != 0.f) {
-      const int ek = edge_index<TI>(sp, tid);
-      if (ek >= 0) xe = TI::load1(logits + row * a.vocab * TI::kBytes, ek);
-      if (wave == 0) {
-        Entries<NS> e;
-        float z[NS];
-        load_entries(a, row, e);
-#pragma unroll
-        for (int s = 0; s < NS; ++s)
-          z[s] = e.id[s] >= 0 ? TI::load1(logits + row * a.vocab * TI::kBytes, e.id[s]) : kNegInf;
-        put_entries(a, row, te[0], e);
-        put_student(a, te[0], z);
-      }
+  const int64_t grid = gridDim.x;
+  int64_t row = blockIdx.x, next = kStatic ? deal() : blockIdx.x + grid, after = kStatic ? deal() : blockIdx.x + 2 * grid;
+  // Loads that are used a row or more later stay raw till then (LateRow, LateEntry, Late): a conversion,
+  // or a load that only some lanes make, would wait for them where they are issued.
+  struct LateRow {
+    int64_t tix;
+    int32_t seq;
+    uint32_t w;
+    bool tok;
+  };
+  auto load_row = [&](int64_t i) {
+    LateRow r;
+    const int64_t at = i < a.nrows ? i : row;
+    const int64_t s = static_cast<uint32_t>(at) / static_cast<uint32_t>(a.logit_stride), t = at - s * a.logit_stride;
+    r.seq = static_cast<int32_t>(s);
+    r.tok = i < a.nrows && t < a.rows;
+    r.tix = s * a.tok_stride + a.tok_offset + (t < a.rows ? t : 0);
+    r.w = __float_as_uint(1.f);
+    if (a.mask != nullptr && r.tok)
+      r.w = a.mask_u8 ? static_cast<const uint8_t*>(a.mask)[r.tix] : static_cast<const uint32_t*>(a.mask)[r.tix];
+    return r;
+  };
+  auto finish_row = [&](const LateRow& l) {
+    DistillRow r;
+    r.row = 0;
+    r.tix = l.tix;
+    r.seq = l.seq;
+    r.tok = l.tok;
+    const float w = a.mask != nullptr && a.mask_u8 ? (l.w ? 1.f : 0.f) : __uint_as_float(l.w);
+    r.w = uniform(l.tok ? w : 0.f);
+    return r;
+  };
+  auto place_of = [&](int id, const RowSpan& sp) {     // -1 outside the interior
+    return id >= 0 && id - sp.head < sp.nv * EPV ? entry_place<TI, kSplit, BLOCK, NCH>(id - sp.head, 0) : -1;
+  };
+  // This wave's entries of a row, into its list h.
+  auto own = [&](const Teacher& te, const RowSpan& sp, int h) {
+    int n = 0;
+    for (int w = 0; w < groups; ++w) {
+      const int p = place_of(te.id[lane + kWave * w], sp);
+      const bool mine = p >= 0 && ((p >> 10) & 15) == wave;
+      const uint64_t who = __ballot(mine);
+      const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32),
+                                                   __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
+      if (mine) list[h][wave][n + before] = static_cast<uint8_t>(lane + kWave * w);
+      n += __popcll(who);
     }
+    __builtin_amdgcn_wave_barrier();
+    Owned o;
+    o.n = n;
+    o.place = lane < n ? place_of(te.id[list[h][wave][lane]], sp) : -1;
+    o.chunks = n > kWave ? ~0u : 0u;
+    for (int e = 0; e < min(n, kWave); ++e) o.chunks |= 1u << (__builtin_amdgcn_readlane(o.place, e) >> 16);
+    return o;
+  };
+  // f(place, lane of the list, list group) for each of the wave's entries in chunk k.
+  auto each_in_chunk = [&](const Teacher& te, const RowSpan& sp, const Owned& o, int h, int k, auto f) {
+    if ((o.chunks >> k & 1) == 0) return;
+    uint64_t in = __ballot(o.place >= 0 && (o.place >> 16) == k);
+    int place = o.place;
+    for (int w = 0;;) {
+      while (in) {
+        const int src = __builtin_ctzll(in);
+        in &= in - 1;
+        f(__builtin_amdgcn_readlane(place, src), src, w);
+      }
+      if (++w * kWave >= o.n) break;
+      place = kWave * w + lane < o.n ? place_of(te.id[list[h][wave][kWave * w + lane]], sp) : -1;
+      in = __ballot(place >= 0 && (place >> 16) == k);
+    }
+  };
+  // Adds chunk k's terms outside the entries to s, against ref; the entries' elements become -inf.
+  auto sum_chunk = [&](u32x4& x, const Teacher& te, const RowSpan& sp, const Owned& o, int h, int k, float ref, float& s) {
+    each_in_chunk(te, sp, o, h, k, [&](int p, int, int) { mask_element<TI>(x, ((p >> 4) & 63) == lane, p & 15); });
+    uint32_t u[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      u[q] = x[q];
+      asm volatile("" : "+v"(u[q]));   // unpacked here and again for the gradient, not kept between
+    }
+    if constexpr (kSplit) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q)
+        if (held(sp.nv, k, q)) {
+#pragma unroll
+          for (int j = 4 * q; j < 4 * q + 4; ++j) s += hw_exp2(fmaf(TI::unpack(u, j), a.k2, -ref));
+        }
+    } else if (held(sp.nv, k, 0)) {
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) s += hw_exp2(fmaf(TI::unpack(u, j), a.k2, -ref));
+    }
+    asm volatile("" : "+v"(s));   // here, not after the last chunk's entries
+  };
+  // Whether the wave's list has an id twice (equal ids have one place, so one wave has both).
+  auto used_twice = [&](const Teacher& te, int h, int n) {
+    bool twice = false;
+    const int mine = lane < n ? te.id[list[h][wave][lane]] : -1;
+    for (int o = 0; o < min(n, kWave); ++o)
+      twice |= lane < n && o != lane && __builtin_amdgcn_readlane(mine, o) == mine;
+    for (int w = 1; kWave * w < n; ++w) {   // further groups against all before
+      const int later = kWave * w + lane < n ? te.id[list[h][wave][kWave * w + lane]] : -1;
+      for (int o = 0; o < min(n, kWave * w + kWave); ++o)
+        twice |= kWave * w + lane < n && o < kWave * w + lane && te.id[list[h][wave][o]] == later;
+    }
+    return __any(twice);
+  };
+  // The same for the row's head and tail; this lane's element x of them becomes -inf where an entry
+  // has it, or where there is none.
+  auto mask_row_edges = [&](const Teacher& te, const RowSpan& sp, float& x) {
+    const int ek = edge_index<TI>(sp, tid);
+    int n = 0;
+    if (ek >= 0)
+      for (int i = 0; i < a.k; ++i) n += te.id[i] == ek;
+    if (ek < 0 || n > 0) x = kNegInf;
+    return __any(n > 1);
+  };
+
+  auto raw_logit = [&](int64_t i, int e) -> uint32_t {
+    if constexpr (TI::kBytes == 2) return reinterpret_cast<const uint16_t*>(row_of(i))[e];
+    else return reinterpret_cast<const uint32_t*>(row_of(i))[e];
+  };
+  // A row ahead; lane l holds word l % 8 of the teacher's record.
+  struct Late {
+    uint32_t z, xe, record;
+    float scale;
+  };
+  auto load_ahead = [&](int64_t i, int32_t seq, const RowSpan& sp, const Teacher& te) {
+    Late h{0u, 0u, 0u, 0.f};
+    if (i >= a.nrows) return h;
+    h.scale = a.seq_scale[seq];
+    if (wave < groups) {
+      h.z = raw_logit(i, max(te.id[lane + kWave * wave], 0));
+      h.record = reinterpret_cast<const uint32_t*>(a.teacher + i)[lane & 7];
+    }
+    if (wave == 0) h.xe = raw_logit(i, max(edge_index<TI>(sp, tid), 0));
+    return h;
+  };
+  auto put_ahead = [&](Teacher& te, const Late& h) {
+    if (wave >= groups) return;
+    put_student(a, te, wave, te.id[lane + kWave * wave] >= 0 ? TI::unpack(&h.z, 0) : kNegInf);
+    if (wave == 0 && lane < 8) reinterpret_cast<uint32_t*>(&te.row)[lane] = h.record;
+  };
+  struct LateEntry {
+    uint32_t id, id_high;
+    float t, p;
+  };
+  auto entries_ahead = [&](int64_t i) {
+    LateEntry e{0u, 0u, kNegInf, 0.f};
+    if (wave < groups && i < a.nrows) {
+      const int64_t at = i * a.k + min(lane + kWave * wave, a.k - 1);
+      if (a.ids_i64) {
+        const u32x2 v = static_cast<const u32x2*>(a.tids)[at];
+        e.id = v[0];
+        e.id_high = v[1];
+      } else {
+        e.id = static_cast<const uint32_t*>(a.tids)[at];
+      }
+      e.t = a.tlogits[at];
+      e.p = a.teacher_p[at];
+    }
+    return e;
+  };
+  auto put_entries = [&](Teacher& te, int64_t i, const LateEntry& l) {
+    if (wave >= groups) return;
+    const int64_t id = a.ids_i64 ? static_cast<int64_t>(static_cast<uint64_t>(l.id_high) << 32 | l.id)
+                                 : static_cast<int64_t>(static_cast<int32_t>(l.id));
+    const bool is = i < a.nrows && lane + kWave * wave < a.k;
+    put_entry(te, wave, Entry{is ? used_id(a, id, l.t) : -1, l.t, l.p});
+  };
+  static_assert(sizeof(TeacherRow) == 32, "eight words");
+
+  DistillRow r = finish_row(load_row(row)), rn = finish_row(load_row(next));
+  RowSpan sp = row_span<TI>(row_of(row), a.vocab);
+  float xe, scale;
+  {
+    put_entries(te4[0], row, entries_ahead(row));
+    put_entries(te4[1], next, entries_ahead(next));
+    const Late h = load_ahead(row, r.seq, sp, te4[0]);    // (a wave reads its own group only)
+    put_ahead(te4[0], h);
+    xe = TI::unpack(&h.xe, 0);
+    scale = uniform(h.scale);
   }
   __syncthreads();
+  Owned mine{-1, 0, 0u};                               // this wave's entries of the row
+  bool twice = false;
+  if (r.w != 0.f) {
+    mine = own(te4[0], sp, 0);
+    twice = used_twice(te4[0], 0, mine.n);
+  }
+  int64_t owed = -1;                                   // the token whose loss is to be formed, and its weight
+  float owed_w = 0.f;
+  auto pay = [&](const Teacher& te) {                  // by wave NW - 1
+    const float l = static_cast<float>(row_loss(a, te, factors[wave]));
+    if (lane == 0) a.token_loss[owed] = owed_w * l;
+  };
   for (int i = 0;; ++i) {
-    const Teacher& t = te[i & 1];
+    const int h = i & 1;
+    Teacher& te = te4[i & 3];
+    Teacher& tn = te4[(i + 1) & 3];
     const int64_t row_elem = row * a.vocab;
-    // What the next row needs first.
+    const float weight = r.w;
     const bool more = next < a.nrows;
-    DistillRow rn = distill_row(a, more ? next : row);
-    const bool want = more && rn.w != 0.f;
-    Teacher& tn = te[(i + 1) & 1];
-    Entries<NS> en;
-    if (wave == 0 && want) load_entries(a, next, en);
-    int claimed = INT32_MAX;
-    if (!kStatic && tid == 0 && a.nrows > 2 * static_cast<int64_t>(gridDim.x))
-      claimed = atomicAdd(a.next_row, 1) + 2 * static_cast<int>(gridDim.x);
-
-    const int nv = sp.nv;
-    // kSplit: half h of chunk k of this lane holds row values (past the row end it read 0).
-    auto held = [&](int k, int h) {
-      return kSplit ? static_cast<int64_t>(k) * 2 * BLOCK + 64 * h + sgrp < 2 * static_cast<int64_t>(nv)
-                    : k * BLOCK + tid < nv;
-    };
-    bool live = r.w != 0.f && t.row.state == kUsed;
-    float token = 0.f;
-    if (live) {
-      bool twice;
-      const int ek = edge_index<TI>(sp, tid);
-      float x1 = ek >= 0 ? xe : kNegInf;
-      {
-        int id[NS], place[NS];
+    const int ek = wave == 0 ? edge_index<TI>(sp, tid) : -1;
+    const RowSpan spn = row_span<TI>(row_of(more ? next : row), a.vocab);
+    const __amdgpu_buffer_rsrc_t drow = row_rsrc(static_cast<char*>(a.dlogits) + (row_elem + sp.head) * TO::kBytes,
+                                                 static_cast<uint32_t>(sp.nv) * kOutVec);
+    u32x4 xv[NCH];
+    if (weight != 0.f) {
+      const __amdgpu_buffer_rsrc_t buf = row_rsrc(sp.vec, static_cast<uint32_t>(sp.nv) * 16u);
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          id[s] = t.id[lane + kWave * s];
-          place[s] = id[s] >= 0 && id[s] - sp.head < nv * EPV ? entry_place<TI, kSplit, BLOCK, NCH>(id[s] - sp.head, 0) : -1;
-        }
-        twice = mask_entries<TI>(xv, id, place);
-        if (wave == 0) twice |= mask_edges<TI>(sp, x1, id);
+      for (int k = 0; k < NCH; ++k) xv[k] = load_chunk<TI, TO, BLOCK>(buf, k, voff, sgrp);
+    }
+    // Ahead: the next row's student and teacher, the entries and position of the one after it, a
+    // claim. Then, while all that is under way, the next row's list and the last row's loss.
+    const Late ah = load_ahead(next, rn.seq, spn, tn);
+    const LateEntry en = entries_ahead(after);
+    const LateRow ra = load_row(after);
+    int claimed = 0;
+    if (!kStatic && tid == 0 && a.nrows > 3 * grid) claimed = atomicAdd(a.next_row, 1);
+    Owned mine_n{-1, 0, 0u};
+    bool twice_n = false;
+    if (rn.w != 0.f) {
+      mine_n = own(tn, spn, 1 - h);
+      twice_n = used_twice(tn, 1 - h, mine_n.n);
+    }
+    if (wave == NW - 1 && owed >= 0) pay(te4[(i + 3) & 3]);
+    owed = -1;
+    float g = 0.f, tail = 0.f, gref = 0.f;             // the gradient at this lane's entry; elsewhere
+    double loss = 0.;
+    bool live = false;
+    if (weight != 0.f) {
+      const float ref = uniform(ms_ref(entries_max(te, groups)));
+      float s = 0.f;
+      if (wave == 0) {
+        float x1 = xe;
+        twice |= mask_row_edges(te, sp, x1);
+        s += hw_exp2(fmaf(x1, a.k2, -ref));
       }
-      float mx = x1;
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
-        if constexpr (kSplit) {
-          const uint32_t* w = reinterpret_cast<const uint32_t*>(&xv[k]);
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (held(k, h)) {
-#pragma unroll
-              for (int j = 4 * h; j < 4 * h + 4; ++j) mx = fmaxf(mx, TI::unpack(w, j));
-            }
-        } else if (held(k, 0)) {
-          mx = vec_max<TI>(mx, xv[k]);
-        }
+        __builtin_amdgcn_sched_barrier(0);
+        sum_chunk(xv[k], te, sp, mine, h, k, ref, s);
       }
-      float m = mx * a.k2;
-      const float ref = ms_ref(m);
-      float s = hw_exp2(fmaf(x1, a.k2, -ref));
       __builtin_amdgcn_sched_barrier(0);
+      // The workgroup's sum, in a fixed order.
+      s = lanes_sum<64>(s);
+      if (lane == 0) merge[wave] = make_float2(s, twice ? 1.f : 0.f);
+      __syncthreads();
+      const float2 w = merge[lane & (NW - 1)];
+      float m = ref, st = lanes_sum<NW>(w.x);
+      const bool any_twice = __any(w.y != 0.f);
+      live = te.row.state == kUsed && !any_twice;
+      if (live && !(st > 0x1p-100f && st < __builtin_inff())) {
+        // Out of range: the true maximum (the entries' elements are -inf by now), then the sum.
+        float x1 = kNegInf;
+        if (wave == 0) {
+          x1 = xe;
+          mask_row_edges(te, sp, x1);
+        }
+        float mx = x1;
+#pragma unroll
+        for (int k = 0; k < NCH; ++k)
+#pragma unroll
+          for (int j = 0; j < EPV; ++j)
+            if (held(sp.nv, k, kSplit ? j / 4 : 0)) mx = fmaxf(mx, TI::unpack(reinterpret_cast<const uint32_t*>(&xv[k]), j));
+        float mm = mx * a.k2;
+        const float mref = ms_ref(mm);
+        float ss = hw_exp2(fmaf(x1, a.k2, -mref));
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < NCH; ++k) {
+          uint32_t u[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            u[q] = xv[k][q];
+            asm volatile("" : "+v"(u[q]));
+          }
+#pragma unroll
+          for (int j = 0; j < EPV; ++j)
+            if (held(sp.nv, k, kSplit ? j / 4 : 0)) ss += hw_exp2(fmaf(TI::unpack(u, j), a.k2, -mref));
+          asm volatile("" : "+v"(ss));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        lanes_merge<64>(mm, ss);
+        __syncthreads();   // every wave has read the first sums
+        if (lane == 0) merge[wave] = make_float2(mm, ss);
+        __syncthreads();
+        const float2 v = merge[lane & (NW - 1)];
+        m = v.x;
+        st = v.y;
+        lanes_merge<NW>(m, st);
+      }
+      if (live) {
+        const RowFactors f = row_factors(a, scale * weight, te, m, st, loss);
+        if (lane == 0) factors[wave] = f;
+        tail = uniform(f.tail);
+        gref = uniform(f.ref);
+        if (mine.place >= 0) g = entry_grad(a, te, f, list[h][wave][lane]);
+      } else if (tid == 0 && any_twice && te.row.state == kUsed) {
+        raise_error(a.err, kErrTeacherTwice);
+      }
+    }
+    put_ahead(tn, ah);
+    put_entries(te4[(i + 2) & 3], after, en);
+    if (!kStatic && tid == 0) s_next[h] = a.nrows > 3 * grid ? claimed + 3 * static_cast<int>(grid) : INT32_MAX;
+    const float xen = TI::unpack(&ah.xe, 0), scale_n = uniform(ah.scale);
+    const DistillRow raf = finish_row(ra);
+    __builtin_amdgcn_sched_barrier(0);
+    // Vectors past the row end sit past the descriptor: their stores are dropped.
+    if (live) {
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
         uint32_t u[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           u[q] = xv[k][q];
-          asm volatile("" : "+v"(u[q]));   // else the unpacked maxima stay live
+          asm volatile("" : "+v"(u[q]));
         }
-        if constexpr (kSplit) {
+        float out[EPV];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (held(k, h)) {
-#pragma unroll
-              for (int j = 4 * h; j < 4 * h + 4; ++j) s += hw_exp2(fmaf(TI::unpack(u, j), a.k2, -ref));
-            }
-        } else if (held(k, 0)) {
-#pragma unroll
-          for (int j = 0; j < EPV; ++j) s += hw_exp2(fmaf(TI::unpack(u, j), a.k2, -ref));
-        }
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      lanes_merge<64>(m, s);
-      if (lane == 0) merge[wave] = make_float4(m, s, twice ? 1.f : 0.f, 0.f);
-      __syncthreads();
-      const float4 w = merge[lane & (NW - 1)];
-      live = !__any(w.z != 0.f);
-      if (wave == 0) {
-        m = w.x;
-        s = w.y;
-        lanes_merge<NW>(m, s);
-        if (live) token = row_terms<NS>(a, r, t, m, s, terms);
-        else if (lane == 0) raise_error(a.err, kErrTeacherTwice);
-      }
-      __syncthreads();
-    }
-    if (wave == 0 && want) put_entries(a, next, tn, en);
-    if (!live) {
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) xv[k] = u32x4{0u, 0u, 0u, 0u};
-    }
-    // This wave's entries and their gradients.
-    const float tail = live ? terms.tail : 0.f, ref = live ? terms.ref : 0.f;
-    int place[NS];
-    float g[NS];
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      place[s] = -1;
-      g[s] = 0.f;
-      if (live) {
-        const int id = t.id[lane + kWave * s];
-        if (id >= 0 && id - sp.head < nv * EPV) place[s] = entry_place<TI, kSplit, BLOCK, NCH>(id - sp.head, 0);
-        if (place[s] >= 0 && ((place[s] >> 10) & 15) != wave) place[s] = -1;
-        if (place[s] >= 0) g[s] = terms.g[lane + kWave * s];
-      }
-    }
-    if (tid == 0 && r.tok) a.token_loss[r.tix] = token;
-    const char* nrow = logits + (more ? next : row) * a.vocab * TI::kBytes;
-    const RowSpan spn = span_of(more ? next : row);
-    float en_z[NS];
-    if (wave == 0 && want) {
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int id = tn.id[lane + kWave * s];
-        en_z[s] = id >= 0 ? TI::load1(nrow, id) : kNegInf;
-      }
-    }
-    const __amdgpu_buffer_rsrc_t nbuf = buffer_of(spn, want);
-    const __amdgpu_buffer_rsrc_t drow = row_rsrc(static_cast<char*>(a.dlogits) + (row_elem + sp.head) * TO::kBytes,
-                                                 static_cast<uint32_t>(nv) * kOutVec);
-#pragma unroll
-    for (int k = 0; k < NCH; ++k) {
-      uint32_t u[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        u[q] = xv[k][q];
-        asm volatile("" : "+v"(u[q]));   // else the sum pass's unpacked values stay live
-      }
-      float out[EPV];
-#pragma unroll
-      for (int j = 0; j < EPV; ++j) out[j] = tail * hw_exp2(fmaf(TI::unpack(u, j), a.k2, -ref));
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        uint64_t mine = __ballot(place[s] >= 0 && (place[s] >> 16) == k);
-        while (mine) {
-          const int src = __builtin_ctzll(mine);
-          mine &= mine - 1;
-          const int p = __builtin_amdgcn_readlane(place[s], src);
-          const float ge = read_lane(g[s], src);
+        for (int j = 0; j < EPV; ++j) out[j] = tail * hw_exp2(fmaf(TI::unpack(u, j), a.k2, -gref));
+        each_in_chunk(te, sp, mine, h, k, [&](int p, int src, int w) {
+          const float ge = w == 0 ? read_lane(g, src) : entry_grad(a, te, factors[wave], list[h][wave][kWave * w + src]);
           const bool here = ((p >> 4) & 63) == lane;
 #pragma unroll
           for (int j = 0; j < EPV; ++j)
             if (here && j == (p & 15)) out[j] = ge;
+        });
+        if constexpr (kSplit) {
+          const float (&o0)[4] = reinterpret_cast<const float (&)[4]>(out[0]);
+          const float (&o1)[4] = reinterpret_cast<const float (&)[4]>(out[4]);
+          buf_store_vals<TO, 4, true, D_SP>(drow, fresh_off(sgrp * 16u, k * 2 * BLOCK * 16u), o0);
+          buf_store_vals<TO, 4, true, D_SP>(drow, fresh_off(sgrp * 16u, k * 2 * BLOCK * 16u + 1024u), o1);
+        } else {
+          buf_store_vals<TO, EPV, true, D_SP>(drow, fresh_off(tid * kOutVec, k * BLOCK * kOutVec), out);
         }
       }
-      // Vectors past the row end sit past the descriptor: their stores are dropped.
-      if constexpr (kSplit) {
-        const float (&o0)[4] = reinterpret_cast<const float (&)[4]>(out[0]);
-        const float (&o1)[4] = reinterpret_cast<const float (&)[4]>(out[4]);
-        buf_store_vals<TO, 4, true, kBufNTSystem>(drow, fresh_off(sgrp * 16u, k * 2 * BLOCK * 16u), o0);
-        buf_store_vals<TO, 4, true, kBufNTSystem>(drow, fresh_off(sgrp * 16u, k * 2 * BLOCK * 16u + 1024u), o1);
-      } else {
-        buf_store_vals<TO, EPV, true, kBufNTSystem>(drow, fresh_off(tid * kOutVec, k * BLOCK * kOutVec), out);
+    } else {
+      const u32x4 zero = {0u, 0u, 0u, 0u};   // 0 bits are 0 in every output type
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        if constexpr (kSplit) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) buf_st16<true, D_SP>(drow, zero, (k * 2 * BLOCK + 64 * q + sgrp) * 16u);
+        } else {
+#pragma unroll
+          for (uint32_t q = 0; q < kOutVec; q += 16) buf_st16<true, D_SP>(drow, zero, (k * BLOCK + tid) * kOutVec + q);
+        }
       }
-      xv[k] = load_chunk<TI, TO, BLOCK>(nbuf, k, voff, sgrp);
     }
     if (wave == 0) {
-      const int ek = edge_index<TI>(sp, tid);
-      float oe = live && ek >= 0 ? tail * hw_exp2(fmaf(xe, a.k2, -ref)) : 0.f;
-#pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int edge = live ? edge_thread<TI>(sp, t.id[lane + kWave * s]) : -1;
-        const float ge = edge >= 0 ? terms.g[lane + kWave * s] : 0.f;
-        uint64_t mine = __ballot(edge >= 0);
-        while (mine) {
-          const int src = __builtin_ctzll(mine);
-          mine &= mine - 1;
-          if (tid == __builtin_amdgcn_readlane(edge, src)) oe = read_lane(ge, src);
-        }
+      if (ek >= 0) {
+        float oe = live ? tail * hw_exp2(fmaf(xe, a.k2, -gref)) : 0.f;
+        if (live)
+          for (int e = 0; e < a.k; ++e)
+            if (te.id[e] == ek) oe = entry_grad(a, te, factors[0], e);
+        store1<TO>(a.dlogits, row_elem + ek, oe);
       }
-      if (ek >= 0) store1<TO>(a.dlogits, row_elem + ek, oe);
-      if (want) {
-        const int en_k = edge_index<TI>(spn, tid);
-        if (en_k >= 0) xe = TI::load1(nrow, en_k);
-        put_student(a, tn, en_z);
-      }
+      if (tid == 0 && r.tok && !(live && a.forward)) a.token_loss[r.tix] = live ? weight * static_cast<float>(loss) : 0.f;
     }
-    if (!kStatic && tid == 0) s_next[i & 1] = claimed;
-    __syncthreads();
-    if (!more) break;
+    if (live && a.forward) {
+      owed = r.tix;
+      owed_w = weight;
+    }
+    if (!more) {
+      if (wave == NW - 1 && owed >= 0) pay(te);
+      break;
+    }
+    __syncthreads();   // what was put ahead is there
     row = next;
     r = rn;
+    rn = raf;
     sp = spn;
-    next = kStatic ? deal() : static_cast<int64_t>(__builtin_amdgcn_readfirstlane(s_next[i & 1]));
+    xe = xen;
+    scale = scale_n;
+    mine = mine_n;
+    twice = twice_n;
+    next = after;
+    after = kStatic ? deal() : static_cast<int64_t>(__builtin_amdgcn_readfirstlane(s_next[h]));
   }
 }
 
@@ -926,7 +1149,7 @@ hipError_t launch_parts(DistillArgs a, hipStream_t st) {
   return hipSuccess;
 }
 
-template <typename TI, typename TO, int BLOCK, int NCH, int NS>
+template <typename TI, typename TO, int BLOCK, int NCH, int FULL>
 hipError_t launch_row(DistillArgs a, hipStream_t st) {
   static std::atomic<int> cached{0};   // workgroups that the device holds at once
   int slots = cached.load(std::memory_order_relaxed);
@@ -936,7 +1159,7 @@ hipError_t launch_row(DistillArgs a, hipStream_t st) {
     if (e == hipSuccess) e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev);
     if (e == hipSuccess)
       e = hipOccupancyMaxActiveBlocksPerMultiprocessor(
-          &occ, reinterpret_cast<const void*>(&distill_row_kernel<TI, TO, BLOCK, NCH, NS>), BLOCK, 0);
+          &occ, reinterpret_cast<const void*>(&distill_row_kernel<TI, TO, BLOCK, NCH, FULL>), BLOCK, 0);
     if (e != hipSuccess) return e;
     slots = cus * (occ > 0 ? occ : 1);
     cached.store(slots, std::memory_order_relaxed);
@@ -944,30 +1167,35 @@ hipError_t launch_row(DistillArgs a, hipStream_t st) {
   const int64_t grid = a.nrows < slots ? a.nrows : slots;
   distill_prepare_kernel<kPrepBlock><<<dim3(static_cast<unsigned>(prepare_blocks(a))), dim3(kPrepBlock), 0, st>>>(a);
   if (kDealt<BLOCK, NCH>) a.turn = resident_turn(grid, a.logit_stride, a.mask != nullptr);
-  distill_row_kernel<TI, TO, BLOCK, NCH, NS><<<dim3(static_cast<unsigned>(grid)), dim3(BLOCK), 0, st>>>(a);
+  distill_row_kernel<TI, TO, BLOCK, NCH, FULL><<<dim3(static_cast<unsigned>(grid)), dim3(BLOCK), 0, st>>>(a);
   return hipGetLastError();
 }
 
-template <typename TI, typename TO, int NS>
+template <typename TI, typename TO>
 hipError_t launch_rows_of(const DistillArgs& a, int64_t nv, hipStream_t st) {
-  if (nv <= 256) return launch_row<TI, TO, 256, 1, NS>(a, st);
-  if (nv <= 512) return launch_row<TI, TO, 256, 2, NS>(a, st);
-  if (nv <= 1024) return launch_row<TI, TO, 256, 4, NS>(a, st);
-  if (nv <= 2048) return launch_row<TI, TO, 256, 8, NS>(a, st);
-  if (nv <= 4096) return launch_row<TI, TO, 1024, 4, NS>(a, st);
-  if (nv <= 8192) return launch_row<TI, TO, 1024, 8, NS>(a, st);
-  if (nv <= 12288) return launch_row<TI, TO, 1024, 12, NS>(a, st);
-  if (nv <= 16384) return launch_row<TI, TO, 1024, 16, NS>(a, st);
-  if (nv <= kDistillRowVecs) return launch_row<TI, TO, 1024, 19, NS>(a, st);
+  // FULL: chunks that every row of the configuration fills (its interior has nv - 1 vectors at least).
+  if (nv <= 256) return launch_row<TI, TO, 256, 1, 0>(a, st);
+  if (nv <= 512) return launch_row<TI, TO, 256, 2, 1>(a, st);
+  if (nv <= 1024) return launch_row<TI, TO, 256, 4, 2>(a, st);
+  if (nv <= 2048) return launch_row<TI, TO, 256, 8, 4>(a, st);
+#ifdef D_512
+  if (nv <= 4096) return launch_row<TI, TO, 512, 8, 4>(a, st);
+  if (nv <= 6656) return launch_row<TI, TO, 512, 13, 8>(a, st);
+  if (nv <= 8192) return launch_row<TI, TO, 512, 16, 13>(a, st);
+#else
+  if (nv <= 4096) return launch_row<TI, TO, 1024, 4, 2>(a, st);
+  if (nv <= 8192) return launch_row<TI, TO, 1024, 8, 4>(a, st);
+#endif
+  if (nv <= 12288) return launch_row<TI, TO, 1024, 12, 8>(a, st);
+  if (nv <= 16384) return launch_row<TI, TO, 1024, 16, 12>(a, st);
+  if (nv <= kDistillRowVecs) return launch_row<TI, TO, 1024, 19, 16>(a, st);
   return hipErrorInvalidValue;
 }
 
 template <typename TI, typename TO>
 hipError_t launch_pair(const DistillArgs& a, hipStream_t st) {
-  const bool few = a.k <= kWave;
-  if (a.parts > 0) return few ? launch_parts<TI, TO, 1>(a, st) : launch_parts<TI, TO, kMaxSlots>(a, st);
-  const int64_t nv = a.vocab * TI::kBytes / 16;
-  return few ? launch_rows_of<TI, TO, 1>(a, nv, st) : launch_rows_of<TI, TO, kMaxSlots>(a, nv, st);
+  if (a.parts > 0) return a.k <= kWave ? launch_parts<TI, TO, 1>(a, st) : launch_parts<TI, TO, kMaxSlots>(a, st);
+  return launch_rows_of<TI, TO>(a, a.vocab * TI::kBytes / 16, st);
 }
 
 }  // namespace pcp
