@@ -33,15 +33,19 @@ constexpr int kWave = 64;
 // (k <= 64) and for 4.
 constexpr int kMaxSlots = kMaxEntries / kWave;
 
-// What a row's teacher comes to, whatever the student.
+// What the preparation makes of a row, 12 words.
 struct TeacherRow {
   double sum_p;     // of the entries
   double log_pt;    // of the tail's class, if there is one
   double lse;       // the entries' probabilities are exp(t / tau - lse)
   float pt;
+  float mk, sk;     // the student's log-sum-exp state at the entries, base 2
+  float w;          // the row's weight
   int32_t state;    // kUnused, kUsed; kBad: an id out of range
+  int32_t pad;
 };
 constexpr int kUnused = 0, kUsed = 1, kBad = 2;
+constexpr int kRowWords = sizeof(TeacherRow) / 4;
 
 struct DistillArgs {
   const void* logits;
@@ -54,9 +58,10 @@ struct DistillArgs {
   void* dlogits;
   float* token_loss;
   float4* part;             // [nrows, parts]: (m_T, s_T, an id is used twice, -)
-  float* part_z;            // [nrows, k] the entries' logits (dlogits may replace them)
-  TeacherRow* teacher;      // [nrows], by the preparation, and
-  float* teacher_p;         // [nrows, k]
+  TeacherRow* teacher;      // [nrows], by the preparation, and per entry, [nrows, k]:
+  int* entry_ids;           // used_id,
+  float* entry_p;           // its probability,
+  float* entry_z;           // the student's logit (dlogits may replace it)
   int* err;
   int* next_row;            // rows handed out past the first grid (zeroed earlier on the stream)
   int64_t nrows, vocab, rows, logit_stride, tok_stride, tok_offset;
@@ -230,46 +235,64 @@ __device__ __forceinline__ void prepare_sequence(const DistillArgs& a, int64_t s
   }
 }
 
-// Row `row`'s teacher, by one wave.
-__device__ __forceinline__ void prepare_teacher(const DistillArgs& a, int64_t row) {
-  if (distill_row(a, row).w == 0.f) return;
+// Row `row`, by one wave.
+template <typename TI>
+__device__ __forceinline__ void prepare_row(const DistillArgs& a, int64_t row) {
   const int lane = threadIdx.x & 63;
-  int id[kMaxSlots];
-  float t[kMaxSlots], tmax = kNegInf;
-  bool out = false, any = false;
-#pragma unroll
-  for (int s = 0; s < kMaxSlots; ++s) {
-    id[s] = -1;
-    if (kWave * s < a.k) id[s] = entry_id(a, row, lane + kWave * s, t[s]);
-    out |= id[s] == -2;
-    any |= id[s] >= 0;
-    if (id[s] >= 0) tmax = fmaxf(tmax, t[s]);
-  }
   TeacherRow o;
-  if (a.tlse) {
-    o.lse = static_cast<double>(a.tlse[row]);
-  } else {
-    const double m = static_cast<double>(ms_ref(lanes_max<64>(tmax))) * a.inv_tau;
-    double sum = 0.;
+  o.sum_p = o.log_pt = o.lse = 0.;
+  o.pt = o.sk = 0.f;
+  o.mk = kNegInf;
+  o.w = distill_row(a, row).w;
+  o.state = kUnused;
+  o.pad = 0;
+  if (o.w != 0.f) {
+    const char* xrow = static_cast<const char*>(a.logits) + row * a.vocab * TI::kBytes;
+    int id[kMaxSlots];
+    float t[kMaxSlots], z[kMaxSlots], tmax = kNegInf, zmax = kNegInf;
+    bool out = false, any = false;
 #pragma unroll
-    for (int s = 0; s < kMaxSlots; ++s)
-      if (id[s] >= 0) sum += exp(static_cast<double>(t[s]) * a.inv_tau - m);
-    o.lse = m + log(wave_sum64(sum));
-  }
-  double sum_p = 0.;
+    for (int s = 0; s < kMaxSlots; ++s) {
+      id[s] = -1;
+      z[s] = kNegInf;
+      if (kWave * s < a.k) id[s] = entry_id(a, row, lane + kWave * s, t[s]);
+      if (id[s] >= 0) z[s] = TI::load1(xrow, id[s]);
+      out |= id[s] == -2;
+      any |= id[s] >= 0;
+      if (id[s] >= 0) tmax = fmaxf(tmax, t[s]);
+      zmax = fmaxf(zmax, z[s]);
+    }
+    if (a.tlse) {
+      o.lse = static_cast<double>(a.tlse[row]);
+    } else {
+      const double m = static_cast<double>(ms_ref(lanes_max<64>(tmax))) * a.inv_tau;
+      double sum = 0.;
 #pragma unroll
-  for (int s = 0; s < kMaxSlots; ++s) {
-    const int i = lane + kWave * s;
-    if (i >= a.k) continue;
-    const double p = id[s] >= 0 ? exp(static_cast<double>(t[s]) * a.inv_tau - o.lse) : 0.;
-    sum_p += p;
-    a.teacher_p[row * a.k + i] = static_cast<float>(p);
+      for (int s = 0; s < kMaxSlots; ++s)
+        if (id[s] >= 0) sum += exp(static_cast<double>(t[s]) * a.inv_tau - m);
+      o.lse = m + log(wave_sum64(sum));
+    }
+    o.mk = lanes_max<64>(zmax) * a.k2;
+    float sk = 0.f;
+    double sum_p = 0.;
+#pragma unroll
+    for (int s = 0; s < kMaxSlots; ++s) {
+      const int i = lane + kWave * s;
+      if (i >= a.k) continue;
+      const double p = id[s] >= 0 ? exp(static_cast<double>(t[s]) * a.inv_tau - o.lse) : 0.;
+      sum_p += p;
+      if (id[s] >= 0) sk += hw_exp2(fmaf(z[s], a.k2, -ms_ref(o.mk)));
+      a.entry_ids[row * a.k + i] = id[s];
+      a.entry_p[row * a.k + i] = static_cast<float>(p);
+      a.entry_z[row * a.k + i] = z[s];
+    }
+    o.sk = lanes_sum<64>(sk);
+    o.sum_p = wave_sum64(sum_p);
+    const double pt = fmax(1. - o.sum_p, PCP_DISTILL_TAIL_FLOOR);
+    o.log_pt = log(pt);
+    o.pt = static_cast<float>(pt);
+    o.state = __any(out) ? kBad : __any(any) ? kUsed : kUnused;
   }
-  o.sum_p = wave_sum64(sum_p);
-  const double pt = fmax(1. - o.sum_p, PCP_DISTILL_TAIL_FLOOR);
-  o.log_pt = log(pt);
-  o.pt = static_cast<float>(pt);
-  o.state = __any(out) ? kBad : __any(any) ? kUsed : kUnused;
   if (lane != 0) return;
   a.teacher[row] = o;
   if (o.state == kBad) raise_error(a.err, kErrTokenRange);
@@ -278,35 +301,33 @@ __device__ __forceinline__ void prepare_teacher(const DistillArgs& a, int64_t ro
 }
 
 // Workgroup `block` of the preparation: a sequence, or a row per wave.
+template <typename TI>
 __device__ __forceinline__ void prepare(const DistillArgs& a, int64_t block, float* lds) {
   if (block < a.n_seq) {
     prepare_sequence(a, block, lds);
     return;
   }
   const int64_t row = (block - a.n_seq) * (kPrepBlock / 64) + (threadIdx.x >> 6);
-  if (row < a.nrows) prepare_teacher(a, row);
+  if (row < a.nrows) prepare_row<TI>(a, row);
 }
 inline int64_t prepare_blocks(const DistillArgs& a) {
   return a.n_seq + (a.nrows + kPrepBlock / 64 - 1) / (kPrepBlock / 64);
 }
 
-// A kernel template like the others, so that every type's file may hold it.
-template <int BLOCK>
-__global__ void __launch_bounds__(BLOCK) distill_prepare_kernel(DistillArgs a) {
-  __shared__ float lds[BLOCK / 64];
-  prepare(a, blockIdx.x, lds);
+template <typename TI>
+__global__ void __launch_bounds__(kPrepBlock) distill_prepare_kernel(DistillArgs a) {
+  __shared__ float lds[kPrepBlock / 64];
+  prepare<TI>(a, blockIdx.x, lds);
 }
 
 // ---- a row's terms -----------------------------------------------------------------------
-// A row's teacher and the student's logits there, in LDS for the whole workgroup. Entries go by
-// groups of 64, group w staged by wave w.
+// A row's record and entries in LDS, for the whole workgroup.
 struct Teacher {
   TeacherRow row;
   int id[kMaxEntries];
   float t[kMaxEntries];
   float p[kMaxEntries];
-  float z[kMaxEntries];                   // the student's logits, and
-  float mk[kMaxSlots], sk[kMaxSlots];     // per group their log-sum-exp state, base 2
+  float z[kMaxEntries];
 };
 
 // What a row's gradient needs: tail * 2^(x k2 - ref) outside K, g[] at the entries.
@@ -315,42 +336,33 @@ struct RowTerms {
   float g[kMaxEntries];
 };
 
-// A group's entries to LDS in steps: the loads, the stores, the student's part.
-struct Entry {
+// A row on its way to LDS: lane l's entry of group w by wave w, and word l of the record. The loads
+// are the same for every lane and their values are only looked at when they go to LDS.
+struct LateRow {
   int id;
-  float t, p;
+  float t, p, z;
+  uint32_t word;
 };
-__device__ __forceinline__ Entry load_entry(const DistillArgs& a, int64_t row, int group) {
-  const int i = static_cast<int>(threadIdx.x & 63) + kWave * group;
-  Entry e;
-  e.id = entry_id(a, row, i, e.t);
-  e.p = i < a.k ? a.teacher_p[row * a.k + i] : 0.f;
-  return e;
+__device__ __forceinline__ LateRow load_late(const DistillArgs& a, int64_t row, int group) {
+  const int lane = threadIdx.x & 63;
+  const int64_t at = row * a.k + min(lane + kWave * group, a.k - 1);
+  LateRow l;
+  l.id = a.entry_ids[at];
+  l.t = a.tlogits[at];
+  l.p = a.entry_p[at];
+  l.z = a.entry_z[at];
+  l.word = reinterpret_cast<const uint32_t*>(a.teacher + row)[min(lane, kRowWords - 1)];
+  return l;
 }
-__device__ __forceinline__ void put_entry(Teacher& te, int group, const Entry& e) {
-  const int i = static_cast<int>(threadIdx.x & 63) + kWave * group;
-  te.id[i] = e.id;
-  te.t[i] = e.t;
-  te.p[i] = e.p;
-}
-__device__ __forceinline__ void put_student(const DistillArgs& a, Teacher& te, int group, float z) {
+__device__ __forceinline__ void put_late(const DistillArgs& a, Teacher& te, int group, const LateRow& l) {
   const int lane = threadIdx.x & 63, i = lane + kWave * group;
-  const bool used = te.id[i] >= 0;
-  te.z[i] = z;
-  const float mk = lanes_max<64>(used ? z : kNegInf) * a.k2;
-  const float sk = lanes_sum<64>(used ? hw_exp2(fmaf(z, a.k2, -ms_ref(mk))) : 0.f);
-  if (lane == 0) {
-    te.mk[group] = mk;
-    te.sk[group] = sk;
-  }
+  te.id[i] = i < a.k ? l.id : -1;
+  te.t[i] = l.t;
+  te.p[i] = l.p;
+  te.z[i] = l.z;
+  if (group == 0 && lane < kRowWords) reinterpret_cast<uint32_t*>(&te.row)[lane] = l.word;
 }
 __device__ __forceinline__ int groups_of(const DistillArgs& a) { return (a.k + kWave - 1) / kWave; }
-// The largest of the entries' scaled logits.
-__device__ __forceinline__ float entries_max(const Teacher& te, int groups) {
-  float m = te.mk[0];
-  for (int w = 1; w < groups; ++w) m = fmaxf(m, te.mk[w]);
-  return m;
-}
 
 // A row's factors, the same in every lane of any wave that forms them.
 struct RowFactors {
@@ -404,15 +416,14 @@ __device__ __forceinline__ double row_loss(const DistillArgs& a, const Teacher& 
 // weight: the row's scale times its weight.
 __device__ __forceinline__ RowFactors row_factors(const DistillArgs& a, float weight, const Teacher& te, float mt,
                                                   float st, double& loss) {
-  const int groups = groups_of(a);
   RowFactors f;
   f.mt = mt;
   f.st = st;
-  f.m = fmaxf(mt, entries_max(te, groups));
+  f.m = fmaxf(mt, te.row.mk);
   f.rm = ms_ref(f.m);
   const float ft = st == 0.f ? 0.f : hw_exp2(mt - f.rm);
   f.s = st == 0.f ? 0.f : st * ft;
-  for (int w = 0; w < groups; ++w) f.s += te.sk[w] == 0.f ? 0.f : te.sk[w] * hw_exp2(te.mk[w] - f.rm);
+  f.s += te.row.sk == 0.f ? 0.f : te.row.sk * hw_exp2(te.row.mk - f.rm);
   f.inv_s = 1.f / f.s;
   f.c = static_cast<float>(static_cast<double>(weight) * a.inv_tau);
   f.ref = ms_ref(mt);
@@ -447,7 +458,7 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_kernel(DistillArgs a,
   const int tid = threadIdx.x, part = blockIdx.x;
   static_assert(kPartBlock == kPrepBlock, "the preparation's workgroup");
   if (blockIdx.y >= static_cast<unsigned>(n)) {   // past the rows: the preparation
-    if (part == 0) prepare(a, blockIdx.y - n, lds);
+    if (part == 0) prepare<TI>(a, blockIdx.y - n, lds);
     return;
   }
   const int64_t row = a.row0 + blockIdx.y;
@@ -469,7 +480,6 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_kernel(DistillArgs a,
     const int i = (tid & 63) + kWave * s;
     id[s] = entry_id(a, row, i, t);
     place[s] = id[s] >= 0 && id[s] - sp.head < end * EPV ? entry_place<TI, false, BLOCK, U>(id[s] - sp.head, v0) : -1;
-    if (part == 0 && tid < 64 && i < a.k) a.part_z[row * a.k + i] = id[s] >= 0 ? TI::load1(xrow, id[s]) : 0.f;
   }
   bool twice = mask_entries<TI>(x, id, place);
   float xe = kNegInf;
@@ -554,13 +564,7 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
       if (ek >= 0) xe = TI::load1(xrow, ek);
     }
     const int groups = groups_of(a);
-    if (tid == 0) te.row = a.teacher[row];
-    for (int w = tid >> 6; w < groups; w += static_cast<int>(blockDim.x) >> 6) {
-      const Entry e = load_entry(a, row, w);
-      const float z = e.id >= 0 ? a.part_z[row * a.k + (tid & 63) + kWave * w] : kNegInf;
-      put_entry(te, w, e);
-      put_student(a, te, w, z);
-    }
+    for (int w = tid >> 6; w < groups; w += static_cast<int>(blockDim.x) >> 6) put_late(a, te, w, load_late(a, row, w));
     __syncthreads();
     if (tid < 64) {
       float mt, st;
@@ -674,17 +678,22 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
   }
 }
 
-
 // ---------------------------------------------------------------------------
 // A row to a workgroup, kept in registers from its one read to its gradient's write, by a
 // persistent grid. A wave's loads and stores complete in order here, so a value loaded after a
 // row's stores can be had only when they have gone out to memory, several microseconds later:
-// nothing a row needs is loaded then but its chunks. Its entries come two rows ahead, the student's
-// logits there and its teacher's record one row ahead, each with that row's chunks, and go to LDS
-// before that row's stores. The sums need no maximum of their own: they are taken against
-// the largest of the entries' logits, which is the row's largest or near it, and formed again
-// against the true maximum where they leave f32's range (a tail that is masked, or 2^100 above
-// what the teacher named).
+// nothing is loaded then but the row's chunks. Its record and entries, which the preparation
+// has made, come with the row before's chunks and go to LDS before its stores. The sums need no
+// maximum of their own: they are taken against the largest of the entries' logits, which is the
+// row's largest or near it, and formed again against the true maximum where they leave f32's
+// range (a tail that is masked, or 2^100 above what the teacher named).
+// Bound by memory and, nearly as much, by the two exponentials per element (the second instead
+// of a second unpacked copy: 19 chunks of 16-bit logits fill the registers of 4 waves a SIMD).
+// 8 sequences of 512 rows of 151,936 in bf16, part of them masked: 385 us; with the entries and
+// the 64-bit arithmetic in the row's own workgroup 496, with them loaded after the row before's
+// stores 441. 512-thread workgroups, two to a CU, up to 8192 vectors: 16 sequences of 256 rows
+// of 50,257 take 158 us (one of 1024 threads: 170). kBufNT stores against kBufNTSystem: 385
+// and 390.
 // Requirements (checked on the host): the row's interior fits BLOCK * NCH vectors; dlogits
 // rows split like the logits rows, or hold f32 for 16-bit logits (dword-aligned stores).
 // ---------------------------------------------------------------------------
@@ -692,9 +701,6 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
 // counter, for the reasons given at grpo_resident_kernel.
 template <int BLOCK, int NCH>
 constexpr bool kDealt = BLOCK * NCH <= 2048;
-#ifndef D_SP
-#define D_SP kBufNTSystem
-#endif
 
 __device__ __forceinline__ float uniform(float v) { return read_lane(v, 0); }
 
@@ -713,9 +719,9 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
   constexpr bool kSplit = TI::kBytes == 2 && TO::kBytes == 4, kStatic = kDealt<BLOCK, NCH>;
   constexpr uint32_t kOutVec = EPV * TO::kBytes;
   static_assert(NW >= kMaxSlots, "a wave per group of entries");
-  __shared__ Teacher te4[4];                   // of the row before (its loss is formed under this row's loads), this one, the next two
+  __shared__ Teacher te3[3];                   // of the row before (its loss is formed under this row's loads), this one, the next
   __shared__ RowFactors factors[NW];           // each wave its own copy of the same: out of registers under the stores
-  __shared__ uint8_t list[2][NW][kMaxEntries];
+  __shared__ uint8_t list[NW][kMaxEntries];
   __shared__ float2 merge[NW];
   __shared__ int s_next[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = groups_of(a);
@@ -736,42 +742,12 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     return stride0 + at;
   };
   const int64_t grid = gridDim.x;
-  int64_t row = blockIdx.x, next = kStatic ? deal() : blockIdx.x + grid, after = kStatic ? deal() : blockIdx.x + 2 * grid;
-  // Loads that are used a row or more later stay raw till then (LateRow, LateEntry, Late): a conversion,
-  // or a load that only some lanes make, would wait for them where they are issued.
-  struct LateRow {
-    int64_t tix;
-    int32_t seq;
-    uint32_t w;
-    bool tok;
-  };
-  auto load_row = [&](int64_t i) {
-    LateRow r;
-    const int64_t at = i < a.nrows ? i : row;
-    const int64_t s = static_cast<uint32_t>(at) / static_cast<uint32_t>(a.logit_stride), t = at - s * a.logit_stride;
-    r.seq = static_cast<int32_t>(s);
-    r.tok = i < a.nrows && t < a.rows;
-    r.tix = s * a.tok_stride + a.tok_offset + (t < a.rows ? t : 0);
-    r.w = __float_as_uint(1.f);
-    if (a.mask != nullptr && r.tok)
-      r.w = a.mask_u8 ? static_cast<const uint8_t*>(a.mask)[r.tix] : static_cast<const uint32_t*>(a.mask)[r.tix];
-    return r;
-  };
-  auto finish_row = [&](const LateRow& l) {
-    DistillRow r;
-    r.row = 0;
-    r.tix = l.tix;
-    r.seq = l.seq;
-    r.tok = l.tok;
-    const float w = a.mask != nullptr && a.mask_u8 ? (l.w ? 1.f : 0.f) : __uint_as_float(l.w);
-    r.w = uniform(l.tok ? w : 0.f);
-    return r;
-  };
+  int64_t row = blockIdx.x, next = kStatic ? deal() : blockIdx.x + grid;
   auto place_of = [&](int id, const RowSpan& sp) {     // -1 outside the interior
     return id >= 0 && id - sp.head < sp.nv * EPV ? entry_place<TI, kSplit, BLOCK, NCH>(id - sp.head, 0) : -1;
   };
-  // This wave's entries of a row, into its list h.
-  auto own = [&](const Teacher& te, const RowSpan& sp, int h) {
+  // This wave's entries of a row, into its list.
+  auto own = [&](const Teacher& te, const RowSpan& sp) {
     int n = 0;
     for (int w = 0; w < groups; ++w) {
       const int p = place_of(te.id[lane + kWave * w], sp);
@@ -779,19 +755,19 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
       const uint64_t who = __ballot(mine);
       const int before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(who >> 32),
                                                    __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(who), 0));
-      if (mine) list[h][wave][n + before] = static_cast<uint8_t>(lane + kWave * w);
+      if (mine) list[wave][n + before] = static_cast<uint8_t>(lane + kWave * w);
       n += __popcll(who);
     }
     __builtin_amdgcn_wave_barrier();
     Owned o;
     o.n = n;
-    o.place = lane < n ? place_of(te.id[list[h][wave][lane]], sp) : -1;
+    o.place = lane < n ? place_of(te.id[list[wave][lane]], sp) : -1;
     o.chunks = n > kWave ? ~0u : 0u;
     for (int e = 0; e < min(n, kWave); ++e) o.chunks |= 1u << (__builtin_amdgcn_readlane(o.place, e) >> 16);
     return o;
   };
   // f(place, lane of the list, list group) for each of the wave's entries in chunk k.
-  auto each_in_chunk = [&](const Teacher& te, const RowSpan& sp, const Owned& o, int h, int k, auto f) {
+  auto each_in_chunk = [&](const Teacher& te, const RowSpan& sp, const Owned& o, int k, auto f) {
     if ((o.chunks >> k & 1) == 0) return;
     uint64_t in = __ballot(o.place >= 0 && (o.place >> 16) == k);
     int place = o.place;
@@ -802,13 +778,13 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
         f(__builtin_amdgcn_readlane(place, src), src, w);
       }
       if (++w * kWave >= o.n) break;
-      place = kWave * w + lane < o.n ? place_of(te.id[list[h][wave][kWave * w + lane]], sp) : -1;
+      place = kWave * w + lane < o.n ? place_of(te.id[list[wave][kWave * w + lane]], sp) : -1;
       in = __ballot(place >= 0 && (place >> 16) == k);
     }
   };
   // Adds chunk k's terms outside the entries to s, against ref; the entries' elements become -inf.
-  auto sum_chunk = [&](u32x4& x, const Teacher& te, const RowSpan& sp, const Owned& o, int h, int k, float ref, float& s) {
-    each_in_chunk(te, sp, o, h, k, [&](int p, int, int) { mask_element<TI>(x, ((p >> 4) & 63) == lane, p & 15); });
+  auto sum_chunk = [&](u32x4& x, const Teacher& te, const RowSpan& sp, const Owned& o, int k, float ref, float& s) {
+    each_in_chunk(te, sp, o, k, [&](int p, int, int) { mask_element<TI>(x, ((p >> 4) & 63) == lane, p & 15); });
     uint32_t u[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -829,15 +805,15 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     asm volatile("" : "+v"(s));   // here, not after the last chunk's entries
   };
   // Whether the wave's list has an id twice (equal ids have one place, so one wave has both).
-  auto used_twice = [&](const Teacher& te, int h, int n) {
+  auto used_twice = [&](const Teacher& te, int n) {
     bool twice = false;
-    const int mine = lane < n ? te.id[list[h][wave][lane]] : -1;
+    const int mine = lane < n ? te.id[list[wave][lane]] : -1;
     for (int o = 0; o < min(n, kWave); ++o)
       twice |= lane < n && o != lane && __builtin_amdgcn_readlane(mine, o) == mine;
     for (int w = 1; kWave * w < n; ++w) {   // further groups against all before
-      const int later = kWave * w + lane < n ? te.id[list[h][wave][kWave * w + lane]] : -1;
+      const int later = kWave * w + lane < n ? te.id[list[wave][kWave * w + lane]] : -1;
       for (int o = 0; o < min(n, kWave * w + kWave); ++o)
-        twice |= kWave * w + lane < n && o < kWave * w + lane && te.id[list[h][wave][o]] == later;
+        twice |= kWave * w + lane < n && o < kWave * w + lane && te.id[list[wave][o]] == later;
     }
     return __any(twice);
   };
@@ -852,133 +828,67 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     return __any(n > 1);
   };
 
-  auto raw_logit = [&](int64_t i, int e) -> uint32_t {
-    if constexpr (TI::kBytes == 2) return reinterpret_cast<const uint16_t*>(row_of(i))[e];
-    else return reinterpret_cast<const uint32_t*>(row_of(i))[e];
+  // The token of row i, -1 for a pad row.
+  auto token_of = [&](int64_t i) -> int64_t {
+    const int64_t s = static_cast<uint32_t>(i) / static_cast<uint32_t>(a.logit_stride), t = i - s * a.logit_stride;
+    return t < a.rows ? s * a.tok_stride + a.tok_offset + t : -1;
   };
-  // A row ahead; lane l holds word l % 8 of the teacher's record.
-  struct Late {
-    uint32_t z, xe, record;
-    float scale;
-  };
-  auto load_ahead = [&](int64_t i, int32_t seq, const RowSpan& sp, const Teacher& te) {
-    Late h{0u, 0u, 0u, 0.f};
-    if (i >= a.nrows) return h;
-    h.scale = a.seq_scale[seq];
-    if (wave < groups) {
-      h.z = raw_logit(i, max(te.id[lane + kWave * wave], 0));
-      h.record = reinterpret_cast<const uint32_t*>(a.teacher + i)[lane & 7];
-    }
-    if (wave == 0) h.xe = raw_logit(i, max(edge_index<TI>(sp, tid), 0));
-    return h;
-  };
-  auto put_ahead = [&](Teacher& te, const Late& h) {
-    if (wave >= groups) return;
-    put_student(a, te, wave, te.id[lane + kWave * wave] >= 0 ? TI::unpack(&h.z, 0) : kNegInf);
-    if (wave == 0 && lane < 8) reinterpret_cast<uint32_t*>(&te.row)[lane] = h.record;
-  };
-  struct LateEntry {
-    uint32_t id, id_high;
-    float t, p;
-  };
-  auto entries_ahead = [&](int64_t i) {
-    LateEntry e{0u, 0u, kNegInf, 0.f};
-    if (wave < groups && i < a.nrows) {
-      const int64_t at = i * a.k + min(lane + kWave * wave, a.k - 1);
-      if (a.ids_i64) {
-        const u32x2 v = static_cast<const u32x2*>(a.tids)[at];
-        e.id = v[0];
-        e.id_high = v[1];
-      } else {
-        e.id = static_cast<const uint32_t*>(a.tids)[at];
-      }
-      e.t = a.tlogits[at];
-      e.p = a.teacher_p[at];
-    }
-    return e;
-  };
-  auto put_entries = [&](Teacher& te, int64_t i, const LateEntry& l) {
-    if (wave >= groups) return;
-    const int64_t id = a.ids_i64 ? static_cast<int64_t>(static_cast<uint64_t>(l.id_high) << 32 | l.id)
-                                 : static_cast<int64_t>(static_cast<int32_t>(l.id));
-    const bool is = i < a.nrows && lane + kWave * wave < a.k;
-    put_entry(te, wave, Entry{is ? used_id(a, id, l.t) : -1, l.t, l.p});
-  };
-  static_assert(sizeof(TeacherRow) == 32, "eight words");
-
-  DistillRow r = finish_row(load_row(row)), rn = finish_row(load_row(next));
-  RowSpan sp = row_span<TI>(row_of(row), a.vocab);
-  float xe, scale;
-  {
-    put_entries(te4[0], row, entries_ahead(row));
-    put_entries(te4[1], next, entries_ahead(next));
-    const Late h = load_ahead(row, r.seq, sp, te4[0]);    // (a wave reads its own group only)
-    put_ahead(te4[0], h);
-    xe = TI::unpack(&h.xe, 0);
-    scale = uniform(h.scale);
-  }
-  __syncthreads();
-  Owned mine{-1, 0, 0u};                               // this wave's entries of the row
-  bool twice = false;
-  if (r.w != 0.f) {
-    mine = own(te4[0], sp, 0);
-    twice = used_twice(te4[0], 0, mine.n);
-  }
-  int64_t owed = -1;                                   // the token whose loss is to be formed, and its weight
-  float owed_w = 0.f;
-  auto pay = [&](const Teacher& te) {                  // by wave NW - 1
+  auto scale_of = [&](int64_t i) { return a.seq_scale[static_cast<uint32_t>(i) / static_cast<uint32_t>(a.logit_stride)]; };
+  auto pay = [&](const Teacher& te, int64_t owed) {    // by wave NW - 1: token `owed`'s loss
     const float l = static_cast<float>(row_loss(a, te, factors[wave]));
-    if (lane == 0) a.token_loss[owed] = owed_w * l;
+    if (lane == 0) a.token_loss[owed] = te.row.w * l;
   };
+
+  if (wave < groups) put_late(a, te3[0], wave, load_late(a, row, wave));
+  float scale = uniform(scale_of(row));
+  int64_t owed = -1;
+  int c = 0;                                           // te3[c]: this row's
+  __syncthreads();
   for (int i = 0;; ++i) {
-    const int h = i & 1;
-    Teacher& te = te4[i & 3];
-    Teacher& tn = te4[(i + 1) & 3];
-    const int64_t row_elem = row * a.vocab;
-    const float weight = r.w;
+    const int cn = c == 2 ? 0 : c + 1, cp = c == 0 ? 2 : c - 1;
+    const Teacher& te = te3[c];
+    const float weight = uniform(te.row.w);
+    const int64_t row_elem = row * a.vocab, token = token_of(row);
     const bool more = next < a.nrows;
+    const RowSpan sp = row_span<TI>(row_of(row), a.vocab);
     const int ek = wave == 0 ? edge_index<TI>(sp, tid) : -1;
-    const RowSpan spn = row_span<TI>(row_of(more ? next : row), a.vocab);
     const __amdgpu_buffer_rsrc_t drow = row_rsrc(static_cast<char*>(a.dlogits) + (row_elem + sp.head) * TO::kBytes,
                                                  static_cast<uint32_t>(sp.nv) * kOutVec);
     u32x4 xv[NCH];
+    float xe = 0.f;
     if (weight != 0.f) {
       const __amdgpu_buffer_rsrc_t buf = row_rsrc(sp.vec, static_cast<uint32_t>(sp.nv) * 16u);
 #pragma unroll
       for (int k = 0; k < NCH; ++k) xv[k] = load_chunk<TI, TO, BLOCK>(buf, k, voff, sgrp);
     }
-    // Ahead: the next row's student and teacher, the entries and position of the one after it, a
-    // claim. Then, while all that is under way, the next row's list and the last row's loss.
-    const Late ah = load_ahead(next, rn.seq, spn, tn);
-    const LateEntry en = entries_ahead(after);
-    const LateRow ra = load_row(after);
+    // Ahead: the next row, and a claim for the one after it.
+    const LateRow late = load_late(a, more ? next : row, min(wave, groups - 1));
+    const float late_scale = scale_of(more ? next : row);
     int claimed = 0;
-    if (!kStatic && tid == 0 && a.nrows > 3 * grid) claimed = atomicAdd(a.next_row, 1);
-    Owned mine_n{-1, 0, 0u};
-    bool twice_n = false;
-    if (rn.w != 0.f) {
-      mine_n = own(tn, spn, 1 - h);
-      twice_n = used_twice(tn, 1 - h, mine_n.n);
-    }
-    if (wave == NW - 1 && owed >= 0) pay(te4[(i + 3) & 3]);
+    if (!kStatic && tid == 0 && a.nrows > 2 * grid) claimed = atomicAdd(a.next_row, 1);
+    if (wave == NW - 1 && owed >= 0) pay(te3[cp], owed);
     owed = -1;
+    Owned mine{-1, 0, 0u};                             // this wave's entries
     float g = 0.f, tail = 0.f, gref = 0.f;             // the gradient at this lane's entry; elsewhere
     double loss = 0.;
     bool live = false;
     if (weight != 0.f) {
-      const float ref = uniform(ms_ref(entries_max(te, groups)));
+      mine = own(te, sp);
+      bool twice = used_twice(te, mine.n);
+      const float ref = uniform(ms_ref(te.row.mk));
       float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < NCH; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        sum_chunk(xv[k], te, sp, mine, k, ref, s);
+      }
+      __builtin_amdgcn_sched_barrier(0);
       if (wave == 0) {
+        if (ek >= 0) xe = TI::load1(row_of(row), ek);
         float x1 = xe;
         twice |= mask_row_edges(te, sp, x1);
         s += hw_exp2(fmaf(x1, a.k2, -ref));
       }
-#pragma unroll
-      for (int k = 0; k < NCH; ++k) {
-        __builtin_amdgcn_sched_barrier(0);
-        sum_chunk(xv[k], te, sp, mine, h, k, ref, s);
-      }
-      __builtin_amdgcn_sched_barrier(0);
       // The workgroup's sum, in a fixed order.
       s = lanes_sum<64>(s);
       if (lane == 0) merge[wave] = make_float2(s, twice ? 1.f : 0.f);
@@ -1032,16 +942,14 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
         if (lane == 0) factors[wave] = f;
         tail = uniform(f.tail);
         gref = uniform(f.ref);
-        if (mine.place >= 0) g = entry_grad(a, te, f, list[h][wave][lane]);
+        if (mine.place >= 0) g = entry_grad(a, te, f, list[wave][lane]);
       } else if (tid == 0 && any_twice && te.row.state == kUsed) {
         raise_error(a.err, kErrTeacherTwice);
       }
     }
-    put_ahead(tn, ah);
-    put_entries(te4[(i + 2) & 3], after, en);
-    if (!kStatic && tid == 0) s_next[h] = a.nrows > 3 * grid ? claimed + 3 * static_cast<int>(grid) : INT32_MAX;
-    const float xen = TI::unpack(&ah.xe, 0), scale_n = uniform(ah.scale);
-    const DistillRow raf = finish_row(ra);
+    if (wave < groups) put_late(a, te3[cn], wave, late);
+    if (!kStatic && tid == 0) s_next[i & 1] = a.nrows > 2 * grid ? claimed + 2 * static_cast<int>(grid) : INT32_MAX;
+    const float scale_n = uniform(late_scale);
     __builtin_amdgcn_sched_barrier(0);
     // Vectors past the row end sit past the descriptor: their stores are dropped.
     if (live) {
@@ -1056,8 +964,8 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
         float out[EPV];
 #pragma unroll
         for (int j = 0; j < EPV; ++j) out[j] = tail * hw_exp2(fmaf(TI::unpack(u, j), a.k2, -gref));
-        each_in_chunk(te, sp, mine, h, k, [&](int p, int src, int w) {
-          const float ge = w == 0 ? read_lane(g, src) : entry_grad(a, te, factors[wave], list[h][wave][kWave * w + src]);
+        each_in_chunk(te, sp, mine, k, [&](int p, int src, int w) {
+          const float ge = w == 0 ? read_lane(g, src) : entry_grad(a, te, factors[wave], list[wave][kWave * w + src]);
           const bool here = ((p >> 4) & 63) == lane;
 #pragma unroll
           for (int j = 0; j < EPV; ++j)
@@ -1066,10 +974,10 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
         if constexpr (kSplit) {
           const float (&o0)[4] = reinterpret_cast<const float (&)[4]>(out[0]);
           const float (&o1)[4] = reinterpret_cast<const float (&)[4]>(out[4]);
-          buf_store_vals<TO, 4, true, D_SP>(drow, fresh_off(sgrp * 16u, k * 2 * BLOCK * 16u), o0);
-          buf_store_vals<TO, 4, true, D_SP>(drow, fresh_off(sgrp * 16u, k * 2 * BLOCK * 16u + 1024u), o1);
+          buf_store_vals<TO, 4, true>(drow, fresh_off(sgrp * 16u, k * 2 * BLOCK * 16u), o0);
+          buf_store_vals<TO, 4, true>(drow, fresh_off(sgrp * 16u, k * 2 * BLOCK * 16u + 1024u), o1);
         } else {
-          buf_store_vals<TO, EPV, true, D_SP>(drow, fresh_off(tid * kOutVec, k * BLOCK * kOutVec), out);
+          buf_store_vals<TO, EPV, true>(drow, fresh_off(tid * kOutVec, k * BLOCK * kOutVec), out);
         }
       }
     } else {
@@ -1078,10 +986,10 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
       for (int k = 0; k < NCH; ++k) {
         if constexpr (kSplit) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) buf_st16<true, D_SP>(drow, zero, (k * 2 * BLOCK + 64 * q + sgrp) * 16u);
+          for (int q = 0; q < 2; ++q) buf_st16<true>(drow, zero, (k * 2 * BLOCK + 64 * q + sgrp) * 16u);
         } else {
 #pragma unroll
-          for (uint32_t q = 0; q < kOutVec; q += 16) buf_st16<true, D_SP>(drow, zero, (k * BLOCK + tid) * kOutVec + q);
+          for (uint32_t q = 0; q < kOutVec; q += 16) buf_st16<true>(drow, zero, (k * BLOCK + tid) * kOutVec + q);
         }
       }
     }
@@ -1093,27 +1001,19 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
             if (te.id[e] == ek) oe = entry_grad(a, te, factors[0], e);
         store1<TO>(a.dlogits, row_elem + ek, oe);
       }
-      if (tid == 0 && r.tok && !(live && a.forward)) a.token_loss[r.tix] = live ? weight * static_cast<float>(loss) : 0.f;
+      if (tid == 0 && token >= 0 && !(live && a.forward))
+        a.token_loss[token] = live ? weight * static_cast<float>(loss) : 0.f;
     }
-    if (live && a.forward) {
-      owed = r.tix;
-      owed_w = weight;
-    }
+    if (live && a.forward) owed = token;
     if (!more) {
-      if (wave == NW - 1 && owed >= 0) pay(te);
+      if (wave == NW - 1 && owed >= 0) pay(te, owed);
       break;
     }
     __syncthreads();   // what was put ahead is there
     row = next;
-    r = rn;
-    rn = raf;
-    sp = spn;
-    xe = xen;
     scale = scale_n;
-    mine = mine_n;
-    twice = twice_n;
-    next = after;
-    after = kStatic ? deal() : static_cast<int64_t>(__builtin_amdgcn_readfirstlane(s_next[h]));
+    next = kStatic ? deal() : static_cast<int64_t>(__builtin_amdgcn_readfirstlane(s_next[i & 1]));
+    c = cn;
   }
 }
 
@@ -1128,7 +1028,7 @@ hipError_t launch_parts(DistillArgs a, hipStream_t st) {
   // The preparation goes with the first kernel where its workgroups fit that grid.
   const int64_t prep = prepare_blocks(a);
   const bool with = a.nrows + prep <= kRows;
-  if (!with) distill_prepare_kernel<kPrepBlock><<<dim3(static_cast<unsigned>(prep)), dim3(kPrepBlock), 0, st>>>(a);
+  if (!with) distill_prepare_kernel<TI><<<dim3(static_cast<unsigned>(prep)), dim3(kPrepBlock), 0, st>>>(a);
   for (int64_t r0 = 0; r0 < a.nrows; r0 += kRows) {
     a.row0 = r0;
     const unsigned n = static_cast<unsigned>(a.nrows - r0 < kRows ? a.nrows - r0 : kRows);
@@ -1165,7 +1065,7 @@ hipError_t launch_row(DistillArgs a, hipStream_t st) {
     cached.store(slots, std::memory_order_relaxed);
   }
   const int64_t grid = a.nrows < slots ? a.nrows : slots;
-  distill_prepare_kernel<kPrepBlock><<<dim3(static_cast<unsigned>(prepare_blocks(a))), dim3(kPrepBlock), 0, st>>>(a);
+  distill_prepare_kernel<TI><<<dim3(static_cast<unsigned>(prepare_blocks(a))), dim3(kPrepBlock), 0, st>>>(a);
   if (kDealt<BLOCK, NCH>) a.turn = resident_turn(grid, a.logit_stride, a.mask != nullptr);
   distill_row_kernel<TI, TO, BLOCK, NCH, FULL><<<dim3(static_cast<unsigned>(grid)), dim3(BLOCK), 0, st>>>(a);
   return hipGetLastError();
@@ -1178,14 +1078,9 @@ hipError_t launch_rows_of(const DistillArgs& a, int64_t nv, hipStream_t st) {
   if (nv <= 512) return launch_row<TI, TO, 256, 2, 1>(a, st);
   if (nv <= 1024) return launch_row<TI, TO, 256, 4, 2>(a, st);
   if (nv <= 2048) return launch_row<TI, TO, 256, 8, 4>(a, st);
-#ifdef D_512
   if (nv <= 4096) return launch_row<TI, TO, 512, 8, 4>(a, st);
   if (nv <= 6656) return launch_row<TI, TO, 512, 13, 8>(a, st);
   if (nv <= 8192) return launch_row<TI, TO, 512, 16, 13>(a, st);
-#else
-  if (nv <= 4096) return launch_row<TI, TO, 1024, 4, 2>(a, st);
-  if (nv <= 8192) return launch_row<TI, TO, 1024, 8, 4>(a, st);
-#endif
   if (nv <= 12288) return launch_row<TI, TO, 1024, 12, 8>(a, st);
   if (nv <= 16384) return launch_row<TI, TO, 1024, 16, 12>(a, st);
   if (nv <= kDistillRowVecs) return launch_row<TI, TO, 1024, 19, 16>(a, st);
