@@ -54,6 +54,7 @@ struct pcp_ctx {
   size_t lm_dbuf_bytes = 0;
   pcp::OptionalRoom lm_pieces;    // LM-head products' K pieces
   int* sample_ticket = nullptr;   // the sampler's per-row tickets (zero between launches)
+  unsigned* verify_done = nullptr;   // the draft verification's tickets (zero between launches)
   pcp::HostStager* stager = nullptr;  // pinned staging ring of the host-bytes path
   hipStream_t xs[3] = {};         // host-bytes path: upload, compute and download streams
 };

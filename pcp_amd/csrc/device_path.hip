@@ -515,6 +515,7 @@ void pcp_destroy(pcp_ctx* ctx) {
     if (ctx->lm_dbuf) (void)hipFree(ctx->lm_dbuf);
     if (ctx->lm_pieces.buf) (void)hipFree(ctx->lm_pieces.buf);
     if (ctx->sample_ticket) (void)hipFree(ctx->sample_ticket);
+    if (ctx->verify_done) (void)hipFree(ctx->verify_done);
     destroy_stager(ctx);
     for (hipStream_t x : ctx->xs)
       if (x) (void)hipStreamDestroy(x);

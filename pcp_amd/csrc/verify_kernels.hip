@@ -2,12 +2,21 @@
 //
 // Whether a token is accepted and which one follows are comparisons of sums over the
 // vocabulary with given numbers, so everything is formed in 64 bits: a row's terms are
-// e = 2^((x - max) k), k = log2(e) / temperature, by a polynomial (exp2_64), and f64 multiply-adds run at the rate of f32 ones on this chip.
-//   rows:     every target and draft row in parts, (max, sum e) of each
-//   decide:   one workgroup per sequence merges its rows' parts and finds the first refusal
+// e = 2^((x - max) k), k = log2(e) / temperature.
+//   rows:     token i's target and draft row in parts, (max, sum e) of each
+//   decide:   merges a sequence's parts and decides its tokens
 //   residual: sums of max(p - q, 0) over the parts of the row where the sequence ends
 //   pick:     the part, then the element, where the running sum passes the draw
-// Greedy calls take the first two only, with (first maximum) in place of (max, sum).
+// A large call takes the first tokens' rows, decides them, and leaves out the rows of sequences
+// that have ended there. Greedy calls: the rows' first maxima in parts, then one workgroup per
+// sequence.
+//
+// Bound by f64 arithmetic in the rows (16 operations an element) and, with few rows, by the
+// chain of dependent loads from a decision to a token. 64 sequences of 8 drafted tokens over 151,936 bf16 logits:
+// rows 82, decide 2 x 4.7, residual 20, pick 12 us (rows in one launch 109; with the 11-point
+// polynomial alone 150). One sequence of 4: rows 4.7, decide 3.5, residual with pick 14.
+// Deciding in each token's last workgroup, by a ticket, instead of in launches between: the
+// tickets cost 28 us for 4,368 workgroups, 50 for 12,000.
 
 #include <hip/hip_runtime.h>
 
@@ -25,13 +34,25 @@ namespace {
 constexpr int kBlock = 256;
 constexpr int kU = 4;                       // 16-byte vectors per lane of a part
 constexpr int kPartVecs = kBlock * kU;      // 16 KB
-constexpr int kMaxRows = 2 * PCP_VERIFY_MAX_DRAFT + 1;
+// The same of the residual's parts: U vectors per lane, 1 where the last workgroup picks along.
+constexpr int end_vecs(int U) { return kBlock * U; }
+constexpr int kNW = kBlock / 64;
 
+// A part of a row.
 struct RowState {
   double sum;   // greedy: unused
   float max;
-  int32_t at;   // greedy: the first maximum's index; sampling: NaN seen
+  int32_t at;   // greedy: the first maximum's index; sampling: its log-sum-exp is not finite
 };
+
+// Token i of a sequence, and its rows.
+struct Decision {
+  double sum_p, sum_q;   // sum e of the target row, of the draft row
+  float max_p, max_q;
+  float logp;            // of the drafted token
+  int32_t flags;
+};
+constexpr int kAccepted = 1, kInRange = 2, kBadP = 4, kBadQ = 8;
 
 // Where a sequence ends: the row its last token comes from.
 struct SeqEnd {
@@ -40,8 +61,6 @@ struct SeqEnd {
   double lse_p;              // natural units, of logits / temperature
   int32_t j;                 // accepted tokens
   int32_t without;           // a lookup's refused token (r is 0 there), or -1
-  int32_t bad;               // the target row's sum is not finite
-  int32_t pad;
 };
 
 struct VerifyArgs {
@@ -53,15 +72,19 @@ struct VerifyArgs {
   int64_t* tokens;
   int32_t* accepted;
   float* logp;
-  RowState* part;             // [S, 2n + 1, parts]
-  double* seg;                // [S, parts + 2]: residual sums of head, parts, tail
-  SeqEnd* end;                // [S]
+  RowState* part;             // [S, n + 1, 2, parts]; greedy [S, n + 1, parts]
+  Decision* decision;         // [S, n + 1]
+  double* seg;                // [S, end_parts + 2]: residual sums of head, parts, tail
+  int* ended;                 // [S]: one of the first tokens was refused
+  unsigned* done;             // [S]: workgroups done with a sequence's residual; zero between calls
   int* err;
   int64_t vocab, tstride, dstride;   // elements
   double k;                   // log2(e) / temperature
   double inv_t;
-  int32_t n, n_rows;          // drafted tokens, rows per sequence (n + 1, or 2n + 1 with a draft model)
-  int32_t parts, greedy;
+  int32_t n;
+  int32_t parts, end_parts;   // of kPartVecs, end_vecs vectors
+  int32_t greedy;
+  int32_t from;               // the first token of this launch
 };
 
 // 2^y for y <= 0, to the rounding of 64 bits (0 below 2^-1075, NaN kept): 2^n times a polynomial
@@ -83,6 +106,33 @@ __device__ __forceinline__ double exp2_64(double y) {
   p = fma(p, f, 1.0);
   return __builtin_amdgcn_ldexp(p, static_cast<int>(n));
 }
+
+// The same for many terms: 2^y with y = Y / 128 as 2^(j/128), from a table in LDS, times a
+// polynomial in Y - rint(Y) through 5 Chebyshev points (relative error 8e-17) and the exponent
+// set in the table's value. 16 operations an element instead of 27; y >= -1000 here, so that no term
+// is subnormal: what lies below adds nothing to a sum that holds a 1.
+constexpr int kTable = 128;
+__device__ __forceinline__ void fill_table(double* table) {
+  if (threadIdx.x < kTable) table[threadIdx.x] = exp2_64(threadIdx.x * (1. / kTable));
+}
+struct Exp2 {
+  double head;   // 2^(j/128 + e)
+  double poly;
+  __device__ __forceinline__ Exp2(double Y, const double* table) {
+    constexpr double kMagic = 6755399441055744.;   // 1.5 2^52: the sum's low word is rint(Y)
+    const double t = Y + kMagic, f = Y - (t - kMagic);
+    const uint64_t b = __builtin_bit_cast(uint64_t, t);
+    const int n = static_cast<int>(static_cast<uint32_t>(b));
+    const uint64_t h = __builtin_bit_cast(uint64_t, table[n & (kTable - 1)]);
+    const uint32_t hi = static_cast<uint32_t>(h >> 32) + (static_cast<uint32_t>(n & ~(kTable - 1)) << 13);
+    head = __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | static_cast<uint32_t>(h));
+    double p = 3.583033772988275e-11;
+    p = fma(p, f, 2.6466433571126926e-08);
+    p = fma(p, f, 1.4662262387638751e-05);
+    p = fma(p, f, 0.0054152123481238145);
+    poly = fma(p, f, 1.);
+  }
+};
 
 template <typename TI>
 __device__ __forceinline__ const char* target_row(const VerifyArgs& a, int64_t s, int i) {
@@ -118,19 +168,16 @@ __device__ __forceinline__ void better32(float& v, int& i, float v2, int i2) {
   }
 }
 
-// ---- rows ------------------------------------------------------------------------------
-template <typename TI, bool GREEDY>
-__global__ void __launch_bounds__(kBlock) verify_rows_kernel(VerifyArgs a) {
+// ---- greedy ----------------------------------------------------------------------------
+template <typename TI>
+__global__ void __launch_bounds__(kBlock) verify_first_max_kernel(VerifyArgs a) {
   constexpr int EPV = 16 / TI::kBytes, U = kU, BLOCK = kBlock;
-  __shared__ double lds64[BLOCK / 64];
-  __shared__ float wmax[BLOCK / 64];
-  __shared__ int wat[BLOCK / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x, i = blockIdx.y;
-  const int64_t s = blockIdx.z;
-  const int len = draft_len(a, s);
-  const bool is_target = i <= a.n;
-  if (is_target ? i > len : i - a.n - 1 >= len) return;   // rows of tokens that were not drafted
-  const char* row = is_target ? target_row<TI>(a, s, i) : draft_row<TI>(a, s, i - a.n - 1);
+  __shared__ float wmax[kNW];
+  __shared__ int wat[kNW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x, i = blockIdx.z;
+  const int64_t s = blockIdx.y;
+  if (i > draft_len(a, s)) return;   // rows of tokens that were not drafted
+  const char* row = target_row<TI>(a, s, i);
   const RowSpan sp = row_span<TI>(row, a.vocab);
   const int v0 = part * kPartVecs;
   const __amdgpu_buffer_rsrc_t buf = row_rsrc(sp.vec, static_cast<uint32_t>(sp.nv) * 16u);
@@ -139,203 +186,213 @@ __global__ void __launch_bounds__(kBlock) verify_rows_kernel(VerifyArgs a) {
   for (int q = 0; q < U; ++q) x[q] = buf_ld16<false>(buf, static_cast<uint32_t>(v0 + q * BLOCK + tid) * 16u);
   const int ek = part == 0 ? edge_index<TI>(sp, tid) : -1;
   const float xe = ek >= 0 ? TI::load1(row, ek) : kNegInf;
-  auto held = [&](int q) { return v0 + q * BLOCK + tid < sp.nv; };
-  RowState* out = a.part + ((s * a.n_rows + i) * a.parts + part);
-  if constexpr (GREEDY) {
-    float best = kNegInf;
-    int at = INT32_MAX;
-    if (xe > kNegInf) {
-      best = xe;
-      at = ek;
-    }
+  float best = kNegInf;
+  int at = INT32_MAX;
+  if (xe > kNegInf) {
+    best = xe;
+    at = ek;
+  }
 #pragma unroll
-    for (int q = 0; q < U; ++q)
-      if (held(q))
+  for (int q = 0; q < U; ++q)
+    if (v0 + q * BLOCK + tid < sp.nv)
 #pragma unroll
-        for (int j = 0; j < EPV; ++j) {
-          const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j);
-          const int e = sp.head + (v0 + q * BLOCK + tid) * EPV + j;
-          if (v > kNegInf) better32(best, at, v, e);
-        }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) better32(best, at, __shfl_xor(best, o), __shfl_xor(at, o));
-    if (lane == 0) {
-      wmax[wave] = best;
-      wat[wave] = at;
-    }
-    __syncthreads();
-    if (tid == 0) {
-      for (int w = 1; w < BLOCK / 64; ++w) better32(best, at, wmax[w], wat[w]);
-      *out = RowState{0., best, at};
-    }
-  } else {
-    float m = xe;
-    bool nan = !(xe == xe);
-#pragma unroll
-    for (int q = 0; q < U; ++q)
-      if (held(q)) {
-        m = vec_max<TI>(m, x[q]);
-#pragma unroll
-        for (int j = 0; j < EPV; ++j) {
-          const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j);
-          nan |= !(v == v);
-        }
+      for (int j = 0; j < EPV; ++j) {
+        const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j);
+        const int e = sp.head + (v0 + q * BLOCK + tid) * EPV + j;
+        if (v > kNegInf) better32(best, at, v, e);
       }
-    m = lanes_max<64>(m);
-    if (lane == 0) wmax[wave] = m;
-    __syncthreads();
 #pragma unroll
-    for (int w = 0; w < BLOCK / 64; ++w) m = fmaxf(m, wmax[w]);
-    const double ref = -static_cast<double>(ms_ref(m)) * a.k;
-    double sum = exp2_64(fma(static_cast<double>(xe), a.k, ref));   // 0 for threads without one
-#pragma unroll
-    for (int q = 0; q < U; ++q)
-      if (held(q))
-#pragma unroll
-        for (int j = 0; j < EPV; ++j)
-          sum += exp2_64(fma(static_cast<double>(TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j)), a.k, ref));
-    sum = block_sum64<BLOCK>(sum, lds64);
-    const int any_nan = __syncthreads_or(nan);
-    if (tid == 0) *out = RowState{sum, m, any_nan};
+  for (int o = 32; o > 0; o >>= 1) better32(best, at, __shfl_xor(best, o), __shfl_xor(at, o));
+  if (lane == 0) {
+    wmax[wave] = best;
+    wat[wave] = at;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kNW; ++w) better32(best, at, wmax[w], wat[w]);
+    a.part[(s * (a.n + 1) + i) * a.parts + part] = RowState{0., best, at};
   }
 }
 
-// ---- decide ----------------------------------------------------------------------------
-constexpr int kDecideBlock = 512;
+constexpr int kGreedyBlock = 512;
 
-template <typename TI, bool GREEDY>
-__global__ void __launch_bounds__(kDecideBlock) verify_decide_kernel(VerifyArgs a) {
-  __shared__ double row_sum[kMaxRows];
-  __shared__ float row_max[kMaxRows];
-  __shared__ int row_at[kMaxRows];
+__global__ void __launch_bounds__(kGreedyBlock) verify_greedy_kernel(VerifyArgs a) {
+  __shared__ int row_at[PCP_VERIFY_MAX_DRAFT + 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t s = blockIdx.x;
   const int len = draft_len(a, s);
-  for (int i = wave; i < a.n_rows; i += kDecideBlock / 64) {
-    if (i <= a.n ? i > len : i - a.n - 1 >= len) continue;
-    const RowState* p = a.part + (s * a.n_rows + i) * a.parts;
+  for (int i = wave; i <= len; i += kGreedyBlock / 64) {
+    const RowState* p = a.part + (s * (a.n + 1) + i) * a.parts;
     float m = kNegInf;
-    if constexpr (GREEDY) {
-      int at = INT32_MAX;
-      for (int q = lane; q < a.parts; q += 64) better32(m, at, p[q].max, p[q].at);
+    int at = INT32_MAX;
+    for (int q = lane; q < a.parts; q += 64) better32(m, at, p[q].max, p[q].at);
 #pragma unroll
-      for (int o = 32; o > 0; o >>= 1) better32(m, at, __shfl_xor(m, o), __shfl_xor(at, o));
-      if (lane == 0) row_at[i] = at == INT32_MAX ? 0 : at;
-    } else {
-      int nan = 0;
-      for (int q = lane; q < a.parts; q += 64) {
-        m = fmaxf(m, p[q].max);
-        nan |= p[q].at;
-      }
-      m = lanes_max<64>(m);
-      double sum = 0.;
-      for (int q = lane; q < a.parts; q += 64)
-        if (p[q].max > kNegInf) sum += p[q].sum * exp2_64((static_cast<double>(p[q].max) - static_cast<double>(m)) * a.k);
-      sum = wave_sum64(sum);
-      if (lane == 0) {
-        row_sum[i] = sum;
-        row_max[i] = m;
-        row_at[i] = __builtin_isfinite(m) && __builtin_isfinite(sum);
-      }
-      const bool any = __any(nan != 0);
-      if (lane == 0 && any) row_at[i] = 0;
-    }
+    for (int o = 32; o > 0; o >>= 1) better32(m, at, __shfl_xor(m, o), __shfl_xor(at, o));
+    if (lane == 0) row_at[i] = at == INT32_MAX ? 0 : at;
   }
   __syncthreads();
   if (wave != 0) return;
   if (lane == 0 && a.lens && (a.lens[s] < 0 || a.lens[s] > a.n)) raise_error(a.err, kErrDraftLen);
   // Lane i decides token i (n <= 64).
   const int64_t d = lane < len ? a.ids[s * a.n + lane] : 0;
-  const bool in = d >= 0 && d < a.vocab;
-  bool ok = false, bad_p = false, bad_q = false;
-  float lp = 0.f;
-  if (lane < len) {
-    if constexpr (GREEDY) {
-      ok = d == row_at[lane];
-    } else {
-      bad_p = !row_at[lane];
-      bad_q = a.draft && !row_at[a.n + 1 + lane];
-      if (in && !bad_p && !bad_q) {
-        const double y = fma(static_cast<double>(TI::load1(target_row<TI>(a, s, lane), d)), a.k,
-                             -static_cast<double>(row_max[lane]) * a.k);
-        const double p = exp2_64(y) / row_sum[lane];
-        double q = 1.;
-        if (a.draft) {
-          const int r = a.n + 1 + lane;
-          q = exp2_64(fma(static_cast<double>(TI::load1(draft_row<TI>(a, s, lane), d)), a.k,
-                          -static_cast<double>(row_max[r]) * a.k)) / row_sum[r];
-        }
-        ok = static_cast<double>(a.uniforms[s * (a.n + 1) + lane]) * q < p;
-        lp = static_cast<float>(y * 0.69314718055994530942 - log(row_sum[lane]));
-      }
-    }
-  }
-  const uint64_t no = ~__ballot(ok);
+  const uint64_t no = ~__ballot(lane < len && d == row_at[lane]);
   const int j = min(no ? __builtin_ctzll(no) : 64, len);
-  if (lane == j && lane < len && !in) raise_error(a.err, kErrTokenRange);
+  if (lane == j && lane < len && !(d >= 0 && d < a.vocab)) raise_error(a.err, kErrTokenRange);
   if (lane == 0) a.accepted[s] = j;
-  int64_t* tok = a.tokens + s * (a.n + 1);
-  float* logp = a.logp ? a.logp + s * (a.n + 1) : nullptr;
   // Entries 0 .. n (65 at most): the accepted tokens, the one after, then the pad.
   for (int i = lane; i <= a.n; i += 64) {
-    if (i < j) {
-      tok[i] = d;
-      if (logp) logp[i] = lp;
-    } else if (i > j) {
-      tok[i] = PCP_IGNORE_INDEX;
-      if (logp) logp[i] = 0.f;
-    } else if (GREEDY) {
-      tok[i] = row_at[j];
-      if (logp) logp[i] = 0.f;
-    }
-  }
-  if constexpr (!GREEDY) {
-    const bool refused = j < len;
-    const bool q_bad = refused && __builtin_amdgcn_readlane(bad_q, j);
-    const bool out = refused && !__builtin_amdgcn_readlane(in, j);
-    if (lane == 0) {
-      SeqEnd e;
-      e.j = j;
-      e.bad = !row_at[j];
-      e.max_p = ms_ref(row_max[j]);
-      e.scale_p = 1. / row_sum[j];
-      e.lse_p = e.max_p * a.inv_t + log(row_sum[j]);
-      const bool model = refused && a.draft && !q_bad && !out;
-      const int r = a.n + 1 + j;
-      e.max_q = model ? row_max[r] : 0.;
-      e.scale_q = model ? 1. / row_sum[r] : 0.;
-      e.without = refused && !a.draft && !out ? static_cast<int32_t>(a.ids[s * a.n + j]) : -1;
-      e.pad = 0;
-      a.end[s] = e;
-      if (e.bad || q_bad) raise_error(a.err, kErrNonFinite);
-    }
+    a.tokens[s * (a.n + 1) + i] = i < j ? d : i == j ? row_at[j] : PCP_IGNORE_INDEX;
+    if (a.logp) a.logp[s * (a.n + 1) + i] = 0.f;
   }
 }
 
-// ---- residual --------------------------------------------------------------------------
+// ---- rows ------------------------------------------------------------------------------
+template <typename TI>
+__global__ void __launch_bounds__(kBlock) verify_rows_kernel(VerifyArgs a, int rows) {
+  constexpr int EPV = 16 / TI::kBytes, U = kU, BLOCK = kBlock;
+  __shared__ double table[kTable];
+  __shared__ double lds[kNW];
+  __shared__ float wmax[kNW];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = blockIdx.x;
+  const bool is_draft = static_cast<int>(blockIdx.z) >= rows;   // rows target rows, then their draft rows
+  const int i = a.from + blockIdx.z - (is_draft ? rows : 0);
+  const int64_t s = blockIdx.y, token = s * (a.n + 1) + i;
+  if (i + is_draft > draft_len(a, s)) return;   // rows of tokens that were not drafted
+  if (a.from > 0 && a.ended[s]) return;
+  const int v0 = part * kPartVecs;
+  const char* row = is_draft ? draft_row<TI>(a, s, i) : target_row<TI>(a, s, i);
+  const RowSpan sp = row_span<TI>(row, a.vocab);
+  const __amdgpu_buffer_rsrc_t buf = row_rsrc(sp.vec, static_cast<uint32_t>(sp.nv) * 16u);
+  u32x4 x[U];
+#pragma unroll
+  for (int q = 0; q < U; ++q) x[q] = buf_ld16<false>(buf, static_cast<uint32_t>(v0 + q * BLOCK + tid) * 16u);
+  const int ek = part == 0 ? edge_index<TI>(sp, tid) : -1;
+  const float xe = ek >= 0 ? TI::load1(row, ek) : kNegInf;
+  auto held = [&](int q) { return v0 + q * BLOCK + tid < sp.nv; };
+  fill_table(table);
+  float m = xe;   // maximum: NaN where either is
+#pragma unroll
+  for (int q = 0; q < U; ++q)
+    if (held(q))
+#pragma unroll
+      for (int j = 0; j < EPV; ++j)
+        m = __builtin_elementwise_maximum(m, TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j));
+  bool nan = __any(m != m);
+  m = lanes_max<64>(m);
+  if (lane == 0) wmax[wave] = nan ? __builtin_nanf("") : m;
+  __syncthreads();
+  nan = false;
+#pragma unroll
+  for (int w = 0; w < kNW; ++w) {
+    m = fmaxf(m, wmax[w]);
+    nan |= wmax[w] != wmax[w];
+  }
+  const double k = a.k * kTable, ref = -static_cast<double>(ms_ref(m)) * k;
+  auto term = [&](float v, double sum) {
+    const Exp2 e(fmax(fma(static_cast<double>(v), k, ref), -1000. * kTable), table);
+    return fma(e.head, e.poly, sum);
+  };
+  double sum = ek >= 0 ? term(xe, 0.) : 0.;
+#pragma unroll
+  for (int q = 0; q < U; ++q)
+    if (held(q))
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) sum = term(TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j), sum);
+  sum = block_sum64<BLOCK>(sum, lds);
+  if (tid == 0) a.part[(token * 2 + is_draft) * a.parts + part] = RowState{sum, m, nan};
+}
+
+// ---- decide ----------------------------------------------------------------------------
+constexpr int kDecideBlock = 512;
+
+// The tokens from a.from to before `to`.
+template <typename TI>
+__global__ void __launch_bounds__(kDecideBlock) verify_decide_kernel(VerifyArgs a, int to) {
+  __shared__ RowState whole[2 * (PCP_VERIFY_MAX_DRAFT + 1)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t s = blockIdx.x;
+  const int len = draft_len(a, s), n = min(to, len + 1) - a.from;
+  if (a.from > 0 && a.ended[s]) return;
+  for (int i = wave; i < 2 * n; i += kDecideBlock / 64) {
+    if ((i & 1) && !(a.draft && a.from + (i >> 1) < len)) continue;
+    const RowState* p = a.part + ((s * (a.n + 1) + a.from) * 2 + i) * a.parts;
+    float mm = kNegInf;
+    int bad = 0;
+    for (int q = lane; q < a.parts; q += 64) {
+      mm = fmaxf(mm, p[q].max);
+      bad |= p[q].at;
+    }
+    mm = lanes_max<64>(mm);
+    double sum = 0.;
+    for (int q = lane; q < a.parts; q += 64)
+      if (p[q].max > kNegInf) sum += p[q].sum * exp2_64((static_cast<double>(p[q].max) - static_cast<double>(mm)) * a.k);
+    sum = wave_sum64(sum);
+    bad = __any(bad != 0) || !(__builtin_isfinite(mm) && __builtin_isfinite(sum));
+    if (lane == 0) whole[i] = RowState{sum, mm, bad};
+  }
+  __syncthreads();
+  bool refused = false;
+  if (tid < n) {   // at most 65
+    const int i = a.from + tid;
+    const int64_t token = s * (a.n + 1) + i;
+    const bool drafted = i < len, model = drafted && a.draft;
+    const RowState p = whole[2 * tid], q = model ? whole[2 * tid + 1] : RowState{1., 0.f, 0};
+    const int64_t d = drafted ? a.ids[s * a.n + i] : 0;
+    const bool in = d >= 0 && d < a.vocab;
+    Decision o{p.sum, q.sum, p.max, q.max, 0.f, (in ? kInRange : 0) | (p.at ? kBadP : 0) | (q.at ? kBadQ : 0)};
+    if (drafted && in && !p.at && !q.at) {
+      const double y = fma(static_cast<double>(TI::load1(target_row<TI>(a, s, i), d)), a.k,
+                           -static_cast<double>(p.max) * a.k);
+      double qd = 1.;
+      if (model)
+        qd = exp2_64(fma(static_cast<double>(TI::load1(draft_row<TI>(a, s, i), d)), a.k,
+                         -static_cast<double>(q.max) * a.k)) / q.sum;
+      if (static_cast<double>(a.uniforms[token]) * qd < exp2_64(y) / p.sum) o.flags |= kAccepted;
+      o.logp = static_cast<float>(y * 0.69314718055994530942 - log(p.sum));
+    }
+    a.decision[token] = o;
+    refused = drafted && !(o.flags & kAccepted);
+  }
+  if (to <= a.n) {
+    const int any = __syncthreads_or(refused);
+    if (tid == 0) a.ended[s] = any;
+  }
+}
+
+// ---- the sequence's end ----------------------------------------------------------------
 // r of one element: max(p - q, 0), p alone where scale_q is 0.
 struct Residual {
   double k, ref_p, ref_q, scale_p, scale_q;
   int without;
   bool plain;   // p alone: nothing of p lies above q
+  const double* table;
+  __device__ __forceinline__ double prob(float x, double ref, double scale) const {
+    // Below 2^-1000, where Exp2 ends, by the slower form, for the elements that have it.
+    const double Y = fma(static_cast<double>(x), k, ref);
+    const Exp2 e(fmax(Y, -1000. * kTable), table);
+    double v = e.head * e.poly;
+    if (__builtin_expect(Y < -1000. * kTable, 0)) v = exp2_64(Y * (1. / kTable));
+    return v * scale;
+  }
   __device__ __forceinline__ double operator()(float x, float y, int id) const {
-    const double p = exp2_64(fma(static_cast<double>(x), k, ref_p)) * scale_p;
+    const double p = prob(x, ref_p, scale_p);
     if (plain) return p;
-    if (scale_q != 0.) return fmax(p - exp2_64(fma(static_cast<double>(y), k, ref_q)) * scale_q, 0.);
+    if (scale_q != 0.) return fmax(p - prob(y, ref_q, scale_q), 0.);
     return id == without ? 0. : p;
   }
 };
 
-__device__ __forceinline__ Residual residual(const VerifyArgs& a, const SeqEnd& e, bool plain) {
-  return Residual{a.k, -e.max_p * a.k, -e.max_q * a.k, e.scale_p, e.scale_q, e.without, plain};
+__device__ __forceinline__ Residual residual(const VerifyArgs& a, const SeqEnd& e, bool plain, const double* table) {
+  const double k = a.k * kTable;
+  return Residual{k, -e.max_p * k, -e.max_q * k, e.scale_p, e.scale_q, e.without, plain, table};
 }
 
 // The elements of a part: both rows' values, in element order per (chunk, lane, element). The
 // draft row may start at another offset of its 16 bytes, so it is read element by element there.
-template <typename TI, typename F>
+template <typename TI, int U, typename F>
 __device__ __forceinline__ void part_elements(const VerifyArgs& a, const SeqEnd& e, int64_t s, const RowSpan& sp, int v0,
                                               F f) {
-  constexpr int EPV = 16 / TI::kBytes, U = kU, BLOCK = kBlock;
+  constexpr int EPV = 16 / TI::kBytes, BLOCK = kBlock;
   const int tid = threadIdx.x;
   const bool model = e.scale_q != 0.;
   const __amdgpu_buffer_rsrc_t buf = row_rsrc(sp.vec, static_cast<uint32_t>(sp.nv) * 16u);
@@ -363,67 +420,26 @@ __device__ __forceinline__ void part_elements(const VerifyArgs& a, const SeqEnd&
   }
 }
 
-template <typename TI>
-__global__ void __launch_bounds__(kBlock) verify_residual_kernel(VerifyArgs a) {
-  __shared__ double lds[kBlock / 64];
-  const int tid = threadIdx.x, part = blockIdx.x;
-  const int64_t s = blockIdx.y;
-  const SeqEnd e = a.end[s];
-  if (e.bad) return;
-  const char* row = target_row<TI>(a, s, e.j);
-  const RowSpan sp = row_span<TI>(row, a.vocab);
-  const Residual r = residual(a, e, false);
-  double* seg = a.seg + s * (a.parts + 2);
-  if (part == 0 && tid < 64) {
-    const int ek = edge_index<TI>(sp, tid);
-    double v = 0.;
-    if (ek >= 0) v = r(TI::load1(row, ek), e.scale_q != 0. ? TI::load1(draft_row<TI>(a, s, e.j), ek) : 0.f, ek);
-    const double head = wave_sum64(tid < sp.head ? v : 0.), tail = wave_sum64(tid >= sp.head ? v : 0.);
-    if (tid == 0) {
-      seg[0] = head;
-      seg[a.parts + 1] = tail;
-    }
-  }
-  double sum = 0.;
-  part_elements<TI>(a, e, s, sp, part * kPartVecs, [&](int, int, bool held, float x, float y, int id) {
-    if (held) sum += r(x, y, id);
-  });
-  sum = block_sum64<kBlock>(sum, lds);
-  if (tid == 0) seg[1 + part] = sum;
-}
-
-// ---- pick ------------------------------------------------------------------------------
-template <typename TI>
-__global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
-  constexpr int EPV = 16 / TI::kBytes, U = kU, NW = kBlock / 64;
-  __shared__ double chunk_sum[U][NW];
+// The token after the accepted ones, by the whole workgroup.
+template <typename TI, int U>
+__device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e, int64_t s, const char* row,
+                                           const RowSpan& sp, const double* table) {
+  constexpr int EPV = 16 / TI::kBytes;
+  __shared__ double chunk_sum[U][kNW];
   __shared__ int first;       // the smallest element whose running sum passes
   __shared__ int last;        // the largest element with r > 0, where rounding leaves none
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t s = blockIdx.x;
-  const SeqEnd e = a.end[s];
-  int64_t* tok = a.tokens + s * (a.n + 1) + e.j;
-  float* logp = a.logp ? a.logp + s * (a.n + 1) + e.j : nullptr;
-  if (e.bad) {
-    if (tid == 0) {
-      *tok = a.vocab - 1;
-      if (logp) *logp = 0.f;
-    }
-    return;
-  }
-  const char* row = target_row<TI>(a, s, e.j);
   const char* drow = e.scale_q != 0. ? draft_row<TI>(a, s, e.j) : nullptr;
-  const RowSpan sp = row_span<TI>(row, a.vocab);
   const double u = static_cast<double>(a.uniforms[s * (a.n + 1) + a.n]);
-  const double* seg = a.seg + s * (a.parts + 2);
-  const int segs = a.parts + 2;
+  const int segs = a.end_parts + 2;
+  const double* seg = a.seg + s * segs;
   // Each wave: the total, then the first segment whose running sum passes u * total.
   double total = 0.;
   for (int b = 0; b < segs; b += 64) total += wave_sum64(b + lane < segs ? seg[b + lane] : 0.);
   // Nothing of p above q (equal rows): the token comes from p, whose sums are not in seg; the
   // whole row is then one segment, scanned part by part.
   const bool plain = !(total > 0.);
-  const Residual r = residual(a, e, plain);
+  const Residual r = residual(a, e, plain, table);
   const double t = u * (plain ? 1. : total);
   int hit = -1, last_seg = -1;
   double before = 0.;
@@ -451,7 +467,7 @@ __global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
       last = -1;
     }
     __syncthreads();
-    if (g == 0 || g == a.parts + 1) {   // the head or the tail: at most 7 elements, each thread alone
+    if (g == 0 || g == a.end_parts + 1) {   // the head or the tail: at most 7 elements, each thread alone
       const int n0 = g == 0 ? 0 : sp.head + sp.nv * EPV, n1 = g == 0 ? sp.head : static_cast<int>(a.vocab);
       for (int i = n0; i < n1; ++i) {
         const double v = r(TI::load1(row, i), drow ? TI::load1(drow, i) : 0.f, i);
@@ -466,7 +482,7 @@ __global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
       double mine[U][EPV];
 #pragma unroll
       for (int q = 0; q < U; ++q) part_sum[q] = 0.;
-      part_elements<TI>(a, e, s, sp, (g - 1) * kPartVecs, [&](int q, int j, bool held, float x, float y, int id) {
+      part_elements<TI, U>(a, e, s, sp, (g - 1) * end_vecs(U), [&](int q, int j, bool held, float x, float y, int id) {
         mine[q][j] = held ? r(x, y, id) : 0.;
         part_sum[q] += mine[q][j];
       });
@@ -482,7 +498,7 @@ __global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
 #pragma unroll
       for (int q = 0; q < U; ++q) {
         double b = base;
-        for (int w = 0; w < NW; ++w) {
+        for (int w = 0; w < kNW; ++w) {
           if (w < wave) b += chunk_sum[q][w];
           base += chunk_sum[q][w];
         }
@@ -490,7 +506,7 @@ __global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
 #pragma unroll
         for (int j = 0; j < EPV; ++j) {
           c += mine[q][j];
-          const int id = sp.head + ((g - 1) * kPartVecs + q * kBlock + tid) * EPV + j;
+          const int id = sp.head + ((g - 1) * end_vecs(U) + q * kBlock + tid) * EPV + j;
           if (mine[q][j] > 0.) {
             most = max(most, id);
             if (c > t) seen = min(seen, id);
@@ -521,23 +537,142 @@ __global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
   }
   if (tid == 0) {
     if (pick < 0) pick = static_cast<int>(a.vocab) - 1;
-    *tok = pick;
-    if (logp) *logp = static_cast<float>(static_cast<double>(TI::load1(row, pick)) * a.inv_t - e.lse_p);
+    const int64_t at = s * (a.n + 1) + e.j;
+    a.tokens[at] = pick;
+    if (a.logp) a.logp[at] = static_cast<float>(static_cast<double>(TI::load1(row, pick)) * a.inv_t - e.lse_p);
   }
 }
 
+// The end of sequence s, by each wave: false where the row of its last token is bad.
+__device__ __forceinline__ bool seq_end(const VerifyArgs& a, int64_t s, SeqEnd& e) {
+  const int lane = threadIdx.x & 63, len = draft_len(a, s);
+  const Decision* dec = a.decision + s * (a.n + 1);
+  // Lane i has token i (n <= 64). What lies after a refusal may be of another call.
+  const uint64_t no = ~__ballot(lane < len && (dec[min(lane, len)].flags & kAccepted));
+  const int j = min(no ? __builtin_ctzll(no) : 64, len);
+  const Decision at = dec[j];
+  const bool refused = j < len, in = at.flags & kInRange;
+  const bool model = refused && a.draft && in && !(at.flags & kBadQ);
+  e.j = j;
+  e.max_p = at.max_p;
+  e.scale_p = 1. / at.sum_p;
+  e.lse_p = e.max_p * a.inv_t + log(at.sum_p);
+  e.max_q = model ? at.max_q : 0.;
+  e.scale_q = model ? 1. / at.sum_q : 0.;
+  e.without = refused && !a.draft && in ? static_cast<int32_t>(a.ids[s * a.n + j]) : -1;
+  return !(at.flags & kBadP);
+}
+
+// The workgroup's count is full: this call comes from its last, and the count is 0 again.
+__device__ __forceinline__ bool last_of(unsigned* count, int n) {
+  return atomicInc(count, static_cast<unsigned>(n - 1)) == static_cast<unsigned>(n - 1);
+}
+
+// PICK: the sequence's last workgroup picks the token.
+template <typename TI, int U, bool PICK>
+__global__ void __launch_bounds__(kBlock) verify_residual_kernel(VerifyArgs a) {
+  __shared__ double table[kTable];
+  __shared__ double lds[kNW];
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 63, part = blockIdx.x;
+  const int64_t s = blockIdx.y;
+  fill_table(table);
+  SeqEnd e;
+  const bool good = seq_end(a, s, e);
+  if (part == 0 && tid < 64) {
+    const Decision* dec = a.decision + s * (a.n + 1);
+    int64_t* tok = a.tokens + s * (a.n + 1);
+    float* logp = a.logp ? a.logp + s * (a.n + 1) : nullptr;
+    // Entries 0 .. n (65 at most): the accepted tokens, the one after (V - 1 where its row is
+    // bad; else pick_token's), then the pad.
+    for (int i = lane; i <= a.n; i += 64)
+      if (i != e.j || !good) {
+        tok[i] = i < e.j ? a.ids[s * a.n + i] : i == e.j ? a.vocab - 1 : PCP_IGNORE_INDEX;
+        if (logp) logp[i] = i < e.j ? dec[i].logp : 0.f;
+      }
+    if (lane == 0) {
+      const bool refused = e.j < draft_len(a, s);
+      a.accepted[s] = e.j;
+      if (a.lens && (a.lens[s] < 0 || a.lens[s] > a.n)) raise_error(a.err, kErrDraftLen);
+      if (refused && !(dec[e.j].flags & kInRange)) raise_error(a.err, kErrTokenRange);
+      if (!good || (refused && (dec[e.j].flags & kBadQ))) raise_error(a.err, kErrNonFinite);
+    }
+  }
+  if (!good) return;
+  const char* row = target_row<TI>(a, s, e.j);
+  const RowSpan sp = row_span<TI>(row, a.vocab);
+  const Residual r = residual(a, e, false, table);
+  double* seg = a.seg + s * (a.end_parts + 2);
+  __syncthreads();   // the table
+  if (part == 0 && tid < 64) {
+    const int ek = edge_index<TI>(sp, tid);
+    double v = 0.;
+    if (ek >= 0) v = r(TI::load1(row, ek), e.scale_q != 0. ? TI::load1(draft_row<TI>(a, s, e.j), ek) : 0.f, ek);
+    const double head = wave_sum64(tid < sp.head ? v : 0.), tail = wave_sum64(tid >= sp.head ? v : 0.);
+    if (tid == 0) {
+      store_coherent(seg, head);
+      store_coherent(seg + a.end_parts + 1, tail);
+    }
+  }
+  double sum = 0.;
+  part_elements<TI, U>(a, e, s, sp, part * end_vecs(U), [&](int, int, bool held, float x, float y, int id) {
+    if (held) sum += r(x, y, id);
+  });
+  sum = block_sum64<kBlock>(sum, lds);
+  if (tid == 0) store_coherent(seg + 1 + part, sum);
+  if constexpr (PICK) {
+    if (tid == 0) {
+      wait_stores();
+      last = last_of(a.done + s, a.end_parts);
+    }
+    __syncthreads();
+    if (!last) return;
+    acquire_coherent();
+    pick_token<TI, U>(a, e, s, row, sp, table);
+  }
+}
+
+template <typename TI, int U>
+__global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
+  __shared__ double table[kTable];
+  fill_table(table);
+  SeqEnd e;
+  if (!seq_end(a, blockIdx.x, e)) return;
+  const char* row = target_row<TI>(a, blockIdx.x, e.j);
+  __syncthreads();   // the table
+  pick_token<TI, U>(a, e, blockIdx.x, row, row_span<TI>(row, a.vocab), table);
+}
+
+// The residual's last workgroup picks along for few sequences: 14 us for one, against 6.8 + 11 and
+// the gap between two launches; for 64 its tickets made 44 of 20 + 12.
+constexpr int64_t kPickAlongMaxSeqs = 4;
+// Rows in two launches from this many workgroups (16 KB each) on: 20,672 took 82 us and a decide
+// of 4.7 instead of 109 where about a third of the sequences went past their first half; 4,368
+// take 13 in one launch, where the second pair of launches would cost more than it leaves out.
+constexpr int64_t kSplitWorkgroups = 8192;
+
 template <typename TI>
-hipError_t launch_verify(const VerifyArgs& a, int64_t n_seq, hipStream_t st) {
-  const unsigned parts = static_cast<unsigned>(a.parts), ns = static_cast<unsigned>(n_seq);
-  const dim3 rows(parts, static_cast<unsigned>(a.n_rows), ns), b(kBlock);
+hipError_t launch_verify(VerifyArgs a, int64_t n_seq, hipStream_t st) {
+  const unsigned ns = static_cast<unsigned>(n_seq), parts = static_cast<unsigned>(a.parts);
+  const dim3 b(kBlock), seqs(ns);
   if (a.greedy) {
-    verify_rows_kernel<TI, true><<<rows, b, 0, st>>>(a);
-    verify_decide_kernel<TI, true><<<dim3(ns), dim3(kDecideBlock), 0, st>>>(a);
+    verify_first_max_kernel<TI><<<dim3(parts, ns, static_cast<unsigned>(a.n + 1)), b, 0, st>>>(a);
+    verify_greedy_kernel<<<seqs, dim3(kGreedyBlock), 0, st>>>(a);
+    return hipGetLastError();
+  }
+  const int first = n_seq * (a.draft ? 2 * a.n + 1 : a.n + 1) * a.parts > kSplitWorkgroups ? (a.n + 1) / 2 : 0;
+  for (int from = 0, to = first ? first : a.n + 1; from <= a.n; from = to, to = a.n + 1) {
+    a.from = from;
+    const unsigned rows = static_cast<unsigned>(to - from);
+    verify_rows_kernel<TI><<<dim3(parts, ns, a.draft ? 2 * rows : rows), b, 0, st>>>(a, static_cast<int>(rows));
+    verify_decide_kernel<TI><<<seqs, dim3(kDecideBlock), 0, st>>>(a, to);
+  }
+  const dim3 ends(static_cast<unsigned>(a.end_parts), ns);
+  if (n_seq <= kPickAlongMaxSeqs) {
+    verify_residual_kernel<TI, 1, true><<<ends, b, 0, st>>>(a);
   } else {
-    verify_rows_kernel<TI, false><<<rows, b, 0, st>>>(a);
-    verify_decide_kernel<TI, false><<<dim3(ns), dim3(kDecideBlock), 0, st>>>(a);
-    verify_residual_kernel<TI><<<dim3(parts, ns), b, 0, st>>>(a);
-    verify_pick_kernel<TI><<<dim3(ns), b, 0, st>>>(a);
+    verify_residual_kernel<TI, 2, false><<<ends, b, 0, st>>>(a);
+    verify_pick_kernel<TI, 2><<<seqs, b, 0, st>>>(a);
   }
   return hipGetLastError();
 }
@@ -546,6 +681,29 @@ inline bool misaligned(const void* p, int size) {
   return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(size - 1)) != 0;
 }
 inline size_t round256(size_t b) { return (b + 255) & ~static_cast<size_t>(255); }
+
+// The counts that verify_residual_kernel leaves at zero.
+int ensure_verify_done(pcp_ctx* ctx, hipStream_t st) {
+  if (ctx->verify_done) return PCP_OK;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(st, &status) != hipSuccess) (void)hipGetLastError();
+  else if (status != hipStreamCaptureStatusNone)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "the stream is being captured and the context's counters would have to be "
+                                          "made: make one uncaptured call of the same sizes first");
+  hipError_t e = hipMalloc(&ctx->verify_done, sizeof(unsigned) * kPickAlongMaxSeqs);
+  if (e != hipSuccess) {
+    ctx->verify_done = nullptr;
+    (void)hipGetLastError();
+    return fail(ctx, PCP_ERR_OOM, "hipMalloc of the verification's counters failed");
+  }
+  if ((e = hipMemset(ctx->verify_done, 0, sizeof(unsigned) * kPickAlongMaxSeqs)) != hipSuccess ||
+      (e = hipDeviceSynchronize()) != hipSuccess) {
+    (void)hipFree(ctx->verify_done);
+    ctx->verify_done = nullptr;
+    return hip_fail(ctx, e, "zeroing the verification's counters");
+  }
+  return PCP_OK;
+}
 
 int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   if (!a) return fail(ctx, PCP_ERR_INVALID_ARG, "args is NULL");
@@ -593,11 +751,13 @@ int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   const bool model = !greedy && a->draft_logits && a->n_draft > 0;
   const int64_t nv = a->vocab * size / 16;
   const int64_t parts = nv > 0 ? (nv + kPartVecs - 1) / kPartVecs : 1;
-  const int64_t n_rows = a->n_draft + 1 + (model ? a->n_draft : 0);
-  const size_t S = static_cast<size_t>(a->n_seq);
-  const size_t o_seg = round256(sizeof(RowState) * S * n_rows * parts);
-  const size_t o_end = o_seg + round256(sizeof(double) * S * (parts + 2));
-  const int rc = ensure_scratch_on(ctx, o_end + sizeof(SeqEnd) * S, st);
+  const int64_t ev = end_vecs(a->n_seq <= kPickAlongMaxSeqs ? 1 : 2), end_parts = nv > 0 ? (nv + ev - 1) / ev : 1;
+  const size_t S = static_cast<size_t>(a->n_seq), tokens = S * static_cast<size_t>(a->n_draft + 1);
+  const size_t o_dec = round256(sizeof(RowState) * tokens * (greedy ? 1 : 2) * parts);
+  const size_t o_seg = o_dec + (greedy ? 0 : round256(sizeof(Decision) * tokens));
+  const size_t o_ended = o_seg + (greedy ? 0 : round256(sizeof(double) * S * (end_parts + 2)));
+  int rc = ensure_scratch_on(ctx, o_ended + (greedy ? 0 : sizeof(int) * S), st);
+  if (rc == PCP_OK && !greedy && a->n_seq <= kPickAlongMaxSeqs) rc = ensure_verify_done(ctx, st);
   if (rc != PCP_OK) return rc;
   char* sp = static_cast<char*>(ctx->scratch);
 
@@ -612,8 +772,10 @@ int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   v.accepted = a->accepted;
   v.logp = a->logp;
   v.part = reinterpret_cast<RowState*>(sp);
+  v.decision = reinterpret_cast<Decision*>(sp + o_dec);
   v.seg = reinterpret_cast<double*>(sp + o_seg);
-  v.end = reinterpret_cast<SeqEnd*>(sp + o_end);
+  v.ended = reinterpret_cast<int*>(sp + o_ended);
+  v.done = ctx->verify_done;
   v.err = ctx->d_page->err;
   v.vocab = a->vocab;
   v.tstride = ts;
@@ -621,8 +783,8 @@ int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   v.inv_t = greedy ? 1. : 1. / static_cast<double>(a->temperature);
   v.k = 1.4426950408889634074 * v.inv_t;
   v.n = static_cast<int32_t>(a->n_draft);
-  v.n_rows = static_cast<int32_t>(n_rows);
   v.parts = static_cast<int32_t>(parts);
+  v.end_parts = static_cast<int32_t>(end_parts);
   v.greedy = greedy;
   const bool timed = prof_begin(ctx, st);
   const hipError_t e = a->logits_dtype == PCP_F32    ? launch_verify<F32T>(v, a->n_seq, st)

@@ -71,6 +71,20 @@ def test_verify(dtype, S, n, V, temperature, lookup):
     check(out, xd, yd, d, lens, u, np.float64(np.float32(temperature)))
 
 
+@pytest.mark.parametrize("lookup", [False, True])
+@pytest.mark.parametrize("S,n,V", [(700, 6, 64), (90, 64, 33), (4200, 1, 40), (8300, 0, 16)])
+def test_verify_many_rows(S, n, V, lookup):
+    """Calls whose rows go in two launches, the second without the sequences that have ended."""
+    rng = np.random.default_rng(S)
+    x, y, d, u = make(rng, S, n, V, near=0.3)
+    xd, yd = dev_as(x, "bf16"), None if lookup else dev_as(y, "bf16")
+    lens = rng.integers(0, n + 1, S).astype(np.int32)
+    for _ in range(2):
+        out = step.verify_drafts(xd, torch.from_numpy(d).to(DEV), yd, uniforms=torch.from_numpy(u).to(DEV),
+                                 draft_lens=torch.from_numpy(lens).to(DEV))
+        check(out, xd, yd, d, lens, u, np.float64(1.0))
+
+
 @pytest.mark.parametrize("xo,yo", [(1, 0), (0, 1), (3, 5)])
 @pytest.mark.parametrize("dtype,V", [("bf16", 1000), ("f32", 4097), ("f16", 20001), ("bf16", 5)])
 def test_verify_rows_off_16_bytes(xo, yo, dtype, V):
