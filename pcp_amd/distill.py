@@ -37,6 +37,8 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0, ids_dt
         raise PcpError(-1, "logits of more than two dimensions must be contiguous")
     V = logits.shape[-1]
     R = logits.numel() // V if V else 0
+    if logits.dim() == 2 and R > 1 and logits.stride(0) < V:
+        raise PcpError(-1, "logits rows overlap: expand them with .contiguous()")
     k = int(k)
     ctx = ctx or default_context(logits.device.index or 0)
     a = TopLogitsArgs()

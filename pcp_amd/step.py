@@ -181,6 +181,7 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
         raise PcpError(-1, "uniforms must be f32 [S, n + 1]")
     if draft_lens is not None and (draft_lens.dtype != torch.int32 or draft_lens.shape != (S,)):
         raise PcpError(-1, "draft_lens must be int32 [S]")
+    target_stride, draft_stride = _row_stride(target_logits), _row_stride(draft_logits) if draft_logits is not None else V
     ctx = ctx or default_context(target_logits.device.index or 0)
     a = VerifyArgs()
     lib().pcp_verify_args_init(ctypes.byref(a))
@@ -195,8 +196,7 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
                 or o.accepted.numel() != S or o.logp.dtype != torch.float32 or o.logp.numel() != S * n1):
             raise PcpError(-1, "outputs do not fit the call: tokens int64 and logp f32 [S, n + 1], accepted int32 [S]")
         a.n_seq, a.n_draft, a.vocab = S, n, V
-        a.target_row_stride = _row_stride(target_logits)
-        a.draft_row_stride = _row_stride(draft_logits) if draft_logits is not None else V
+        a.target_row_stride, a.draft_row_stride = target_stride, draft_stride
         a.logits_dtype, a.temperature = dtype_code(target_logits), temperature
         a.target_logits = target_logits.data_ptr()
         a.draft_logits = draft_logits.data_ptr() if draft_logits is not None and n else None
@@ -215,4 +215,7 @@ def _row_stride(t: torch.Tensor) -> int:
         raise PcpError(-1, "logits rows must be contiguous")
     if m > 1 and S > 1 and t.stride(0) != m * t.stride(1):
         raise PcpError(-1, "logits rows must be evenly spaced over the sequences")
-    return t.stride(1) if m > 1 else (t.stride(0) if S > 1 else V)
+    stride = t.stride(1) if m > 1 else (t.stride(0) if S > 1 else V)
+    if stride < V and S * m > 1:
+        raise PcpError(-1, "logits rows overlap: expand them with .contiguous()")
+    return max(stride, V)

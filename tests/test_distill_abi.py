@@ -225,3 +225,22 @@ def test_references_on_small_rows():
     for u0, want in ((0.4, ([1, 1], 1)), (0.6, ([0, -100], 0))):   # p/q of token 1 is 0.5
         tok, acc, _ = verify_ref(x, y, np.array([[1]]), [1], np.array([[u0, 0.5]]), 1.0, 3)
         assert tok[0].tolist() == want[0] and acc[0] == want[1]
+
+
+def test_rows_that_overlap_are_refused():
+    """Expanded rows lie 0 elements apart, which the C entry takes for "vocab apart"."""
+    import torch
+
+    from pcp_amd import distill, step
+    from pcp_amd._lib import PcpError
+    with pytest.raises(PcpError, match="overlap"):
+        distill.top_logits(torch.zeros(1, 16).expand(4, 16), 2)
+    ids = torch.zeros(2, 3, dtype=torch.int64)
+    with pytest.raises(PcpError, match="overlap"):
+        step.verify_drafts(torch.zeros(1, 1, 16).expand(2, 4, 16), ids, temperature=0.0)
+    with pytest.raises(PcpError, match="overlap"):
+        step.verify_drafts(torch.zeros(2, 4, 16), ids, torch.zeros(1, 1, 16).expand(2, 3, 16))
+    with pytest.raises(PcpError, match="overlap"):
+        step.verify_drafts(torch.zeros(1, 1, 16).expand(2, 1, 16), ids[:, :0], temperature=0.0)
+    assert step._row_stride(torch.zeros(2, 4, 16)[:, :, :10]) == 16
+    assert step._row_stride(torch.zeros(2, 0, 16)) == 16
