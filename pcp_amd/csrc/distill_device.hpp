@@ -3,8 +3,9 @@
 //
 // With x a row's logits, k2 = log2(e) / tau, K the used teacher ids and T the rest of the
 // vocabulary, the rows' sums are kept apart: (m_T, s_T) over T while the row streams past
-// (the entries' own elements are replaced by -inf where they sit in registers), and
-// (m_K, s_K) from the k gathered logits. The tail's mass Q_T = s_T 2^(m_T - lse) is then a
+// (the entries' own elements are replaced by -inf where they sit in registers), and s_K from
+// the k gathered logits. Per element in f32; what a row has once (s_K, the merge of its waves'
+// sums, log-sum-exp, the divergence) in f64, since the divergence may be far below its terms. The tail's mass Q_T = s_T 2^(m_T - lse) is then a
 // sum of its own and keeps its relative precision where the teacher's entries hold nearly
 // everything (1 - sum q_i would lose it all). Outside K the gradient is one factor of
 // 2^(x k2 - m_T):
@@ -33,19 +34,24 @@ constexpr int kWave = 64;
 // (k <= 64) and for 4.
 constexpr int kMaxSlots = kMaxEntries / kWave;
 
-// What the preparation makes of a row, 12 words.
+// What the preparation makes of a row. The student's sums are relative to its largest logit at
+// an entry, zref; the kernels form theirs at f32's k2 and references, and adj takes those to zref:
+// 2^(mk - zref k2), which the rounding of mk = zref k2 keeps near 1.
 struct TeacherRow {
   double sum_p;     // of the entries
   double log_pt;    // of the tail's class, if there is one
   double lse;       // the entries' probabilities are exp(t / tau - lse)
+  double sk;        // sum exp((z - zref) / tau) over the entries
+  double adj;
   float pt;
-  float mk, sk;     // the student's log-sum-exp state at the entries, base 2
+  float zref, mk;   // (zref 0 and mk -inf where every entry's logit is -inf)
   float w;          // the row's weight
   int32_t state;    // kUnused, kUsed; kBad: an id out of range
   int32_t pad;
 };
 constexpr int kUnused = 0, kUsed = 1, kBad = 2;
 constexpr int kRowWords = sizeof(TeacherRow) / 4;
+constexpr double kLn2F64 = 0.69314718055994530942;
 
 struct DistillArgs {
   const void* logits;
@@ -60,7 +66,7 @@ struct DistillArgs {
   float4* part;             // [nrows, parts]: (m_T, s_T, an id is used twice, -)
   TeacherRow* teacher;      // [nrows], by the preparation, and per entry, [nrows, k]:
   int* entry_ids;           // used_id,
-  float* entry_p;           // its probability,
+  double* entry_w;          // forward: its probability; reverse: exp((z - zref) / tau),
   float* entry_z;           // the student's logit (dlogits may replace it)
   int* err;
   int* next_row;            // rows handed out past the first grid (zeroed earlier on the stream)
@@ -240,8 +246,9 @@ template <typename TI>
 __device__ __forceinline__ void prepare_row(const DistillArgs& a, int64_t row) {
   const int lane = threadIdx.x & 63;
   TeacherRow o;
-  o.sum_p = o.log_pt = o.lse = 0.;
-  o.pt = o.sk = 0.f;
+  o.sum_p = o.log_pt = o.lse = o.sk = 0.;
+  o.adj = 1.;
+  o.pt = o.zref = 0.f;
   o.mk = kNegInf;
   o.w = distill_row(a, row).w;
   o.state = kUnused;
@@ -272,21 +279,27 @@ __device__ __forceinline__ void prepare_row(const DistillArgs& a, int64_t row) {
         if (id[s] >= 0) sum += exp(static_cast<double>(t[s]) * a.inv_tau - m);
       o.lse = m + log(wave_sum64(sum));
     }
-    o.mk = lanes_max<64>(zmax) * a.k2;
-    float sk = 0.f;
-    double sum_p = 0.;
+    zmax = lanes_max<64>(zmax);
+    o.mk = zmax * a.k2;
+    o.zref = ms_ref(zmax);
+    o.adj = exp((static_cast<double>(ms_ref(o.mk)) - static_cast<double>(o.zref) * a.k2) * kLn2F64);
+    double sum_p = 0., sk = 0.;
 #pragma unroll
     for (int s = 0; s < kMaxSlots; ++s) {
       const int i = lane + kWave * s;
       if (i >= a.k) continue;
-      const double p = id[s] >= 0 ? exp(static_cast<double>(t[s]) * a.inv_tau - o.lse) : 0.;
+      double p = 0., e = 0.;
+      if (id[s] >= 0) {
+        p = exp(static_cast<double>(t[s]) * a.inv_tau - o.lse);
+        e = exp((static_cast<double>(z[s]) - o.zref) * a.inv_tau);
+      }
       sum_p += p;
-      if (id[s] >= 0) sk += hw_exp2(fmaf(z[s], a.k2, -ms_ref(o.mk)));
+      sk += e;
       a.entry_ids[row * a.k + i] = id[s];
-      a.entry_p[row * a.k + i] = static_cast<float>(p);
+      a.entry_w[row * a.k + i] = a.forward ? p : e;
       a.entry_z[row * a.k + i] = z[s];
     }
-    o.sk = lanes_sum<64>(sk);
+    o.sk = wave_sum64(sk);
     o.sum_p = wave_sum64(sum_p);
     const double pt = fmax(1. - o.sum_p, PCP_DISTILL_TAIL_FLOOR);
     o.log_pt = log(pt);
@@ -326,8 +339,11 @@ struct Teacher {
   TeacherRow row;
   int id[kMaxEntries];
   float t[kMaxEntries];
-  float p[kMaxEntries];
   float z[kMaxEntries];
+  uint32_t w_lo[kMaxEntries], w_hi[kMaxEntries];   // all five arrays at one offset per lane
+  __device__ __forceinline__ double w(int i) const {
+    return __builtin_bit_cast(double, static_cast<uint64_t>(w_hi[i]) << 32 | w_lo[i]);
+  }
 };
 
 // What a row's gradient needs: tail * 2^(x k2 - ref) outside K, g[] at the entries.
@@ -340,25 +356,33 @@ struct RowTerms {
 // are the same for every lane and their values are only looked at when they go to LDS.
 struct LateRow {
   int id;
-  float t, p, z;
+  float t, z;
+  double w;
   uint32_t word;
 };
+// Through buffer descriptors, which need no address in registers from row to row and give 0 past
+// the row's k entries. group: the same in the whole wave.
 __device__ __forceinline__ LateRow load_late(const DistillArgs& a, int64_t row, int group) {
   const int lane = threadIdx.x & 63;
-  const int64_t at = row * a.k + min(lane + kWave * group, a.k - 1);
+  const int64_t base = row * a.k + kWave * group;
+  const uint32_t n = static_cast<uint32_t>(a.k - kWave * group), off = lane * 4u;
+  auto word = [&](const void* p, uint32_t bytes) {
+    return static_cast<uint32_t>(__builtin_amdgcn_raw_buffer_load_b32(row_rsrc(p, bytes), off, 0, 0));
+  };
   LateRow l;
-  l.id = a.entry_ids[at];
-  l.t = a.tlogits[at];
-  l.p = a.entry_p[at];
-  l.z = a.entry_z[at];
-  l.word = reinterpret_cast<const uint32_t*>(a.teacher + row)[min(lane, kRowWords - 1)];
+  l.id = static_cast<int>(word(a.entry_ids + base, n * 4u));
+  l.t = __uint_as_float(word(a.tlogits + base, n * 4u));
+  l.z = __uint_as_float(word(a.entry_z + base, n * 4u));
+  l.w = __builtin_bit_cast(double, __builtin_amdgcn_raw_buffer_load_b64(row_rsrc(a.entry_w + base, n * 8u), lane * 8u, 0, 0));
+  l.word = word(a.teacher + row, sizeof(TeacherRow));
   return l;
 }
 __device__ __forceinline__ void put_late(const DistillArgs& a, Teacher& te, int group, const LateRow& l) {
   const int lane = threadIdx.x & 63, i = lane + kWave * group;
   te.id[i] = i < a.k ? l.id : -1;
   te.t[i] = l.t;
-  te.p[i] = l.p;
+  te.w_lo[i] = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, l.w));
+  te.w_hi[i] = static_cast<uint32_t>(__builtin_bit_cast(uint64_t, l.w) >> 32);
   te.z[i] = l.z;
   if (group == 0 && lane < kRowWords) reinterpret_cast<uint32_t*>(&te.row)[lane] = l.word;
 }
@@ -369,45 +393,71 @@ struct RowFactors {
   float tail, ref;      // the gradient outside K: tail * 2^(x k2 - ref)
   float c, rm, inv_s;   // the coefficient; q_i = 2^(z k2 - rm) inv_s
   float big_p, lf;      // forward: P; reverse: l
-  float mt, st, m, s;   // the state outside K, and of the whole row
+  float ek;             // 2^(mk - rm)
+  double s;             // the whole row's sum over 2^(rm - mk) exp(zref / tau)
+  double qt, log_qt;    // the tail's mass; 0: no tail
+  double lse;           // of the student's row; with log_qt only after set_logs
 };
+
+// log(s) to 1e-12, by atanh's series. Its constants are set where they are used: over the row
+// kernel's loop the compiler would keep them all in registers.
+__device__ __forceinline__ double log64(double s) {
+  if (s == 0.) return -__builtin_inf();
+  int k = __builtin_amdgcn_frexp_exp(s);
+  double m = __builtin_amdgcn_frexp_mant(s);
+  if (m < 0.70710678118654752) {
+    m *= 2.;
+    --k;
+  }
+  const double t = (m - 1.) / (m + 1.), u = t * t;
+  double p = 0.;
+#pragma unroll
+  for (int i = 17; i >= 1; i -= 2) {
+    double c = 1. / i;
+    asm volatile("" : "+s"(c));
+    p = fma(p, u, c);
+  }
+  double ln2 = kLn2F64;
+  asm volatile("" : "+s"(ln2));
+  return fma(2. * t, p, k * ln2);
+}
 
 __device__ __forceinline__ float entry_prob(const DistillArgs& a, const Teacher& te, const RowFactors& f, int i) {
   return hw_exp2(fmaf(te.z[i], a.k2, -f.rm)) * f.inv_s;
 }
 // log(p_i / q_i)
-__device__ __forceinline__ double entry_gap(const DistillArgs& a, const Teacher& te, double lse, int i) {
-  return static_cast<double>(te.t[i]) * a.inv_tau - te.row.lse -
-         (static_cast<double>(te.z[i]) * static_cast<double>(a.k2) * 0.69314718055994530942 - lse);
+__device__ __forceinline__ double entry_gap(const DistillArgs& a, const Teacher& te, const RowFactors& f, int i) {
+  return (static_cast<double>(te.t[i]) - te.z[i]) * a.inv_tau - (te.row.lse - f.lse);
 }
 // The gradient at entry i.
 __device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher& te, const RowFactors& f, int i) {
   const float q = entry_prob(a, te, f, i);
-  if (a.forward) return f.c * (q * f.big_p - te.p[i]);
-  return q > 0.f ? -f.c * q * (static_cast<float>(entry_gap(a, te, ms_lse(f.m, f.s), i)) + f.lf) : 0.f;
+  if (a.forward) return f.c * (q * f.big_p - static_cast<float>(te.w(i)));
+  return q > 0.f ? -f.c * q * (static_cast<float>(entry_gap(a, te, f, i)) + f.lf) : 0.f;
 }
 
-__device__ __forceinline__ bool has_tail(const DistillArgs& a, const RowFactors& f) {
-  return a.tlse != nullptr && f.st * hw_exp2(f.mt - f.rm) * f.inv_s >= 0x1p-126f;
+__device__ __forceinline__ void set_logs(const DistillArgs& a, const Teacher& te, RowFactors& f) {
+  f.lse = static_cast<double>(te.row.zref) * a.inv_tau + static_cast<double>(f.rm - ms_ref(te.row.mk)) * kLn2F64 + log64(f.s);
+  f.log_qt = f.qt > 0. ? log64(f.qt) : 0.;
 }
 
-// The row's divergence l, by a whole wave. Its sums run in 64 bits: l may be far below its terms.
+// The row's divergence l, by a whole wave, after set_logs. Formed in 64 bits: l may be far below
+// its terms.
 __device__ __forceinline__ double row_loss(const DistillArgs& a, const Teacher& te, const RowFactors& f) {
   const int lane = threadIdx.x & 63, groups = groups_of(a);
-  const double lse = ms_lse(f.m, f.s);
   double l = 0.;
   for (int w = 0; w < groups; ++w) {
     const int i = lane + kWave * w;
     if (te.id[i] < 0) continue;
-    const float weight = a.forward ? te.p[i] : -entry_prob(a, te, f, i);
-    if (weight != 0.f) l += weight * entry_gap(a, te, lse, i);
+    const double weight = a.forward ? te.w(i) : -te.w(i) * f.ek / f.s;
+    if (weight != 0.) l += weight * entry_gap(a, te, f, i);
   }
   l = wave_sum64(l);
-  if (has_tail(a, f)) {
-    const double gap = te.row.log_pt - (ms_lse(f.mt, f.st) - lse);   // log(p_T / q_T)
-    l += a.forward ? te.row.pt * gap : -(f.st * hw_exp2(f.mt - f.rm) * f.inv_s) * gap;
+  if (f.qt > 0.) {
+    const double gap = te.row.log_pt - f.log_qt;   // log(p_T / q_T)
+    l += a.forward ? te.row.pt * gap : -f.qt * gap;
   }
-  if (lane == 0 && !(__builtin_isfinite(lse) && l == l)) raise_error(a.err, kErrNonFinite);
+  if (lane == 0 && !(__builtin_isfinite(f.lse) && l == l)) raise_error(a.err, kErrNonFinite);
   return l;
 }
 
@@ -415,29 +465,30 @@ __device__ __forceinline__ double row_loss(const DistillArgs& a, const Teacher& 
 // (loss: l, formed here if reverse).
 // weight: the row's scale times its weight.
 __device__ __forceinline__ RowFactors row_factors(const DistillArgs& a, float weight, const Teacher& te, float mt,
-                                                  float st, double& loss) {
+                                                  double st, double& loss) {
   RowFactors f;
-  f.mt = mt;
-  f.st = st;
-  f.m = fmaxf(mt, te.row.mk);
-  f.rm = ms_ref(f.m);
-  const float ft = st == 0.f ? 0.f : hw_exp2(mt - f.rm);
-  f.s = st == 0.f ? 0.f : st * ft;
-  f.s += te.row.sk == 0.f ? 0.f : te.row.sk * hw_exp2(te.row.mk - f.rm);
-  f.inv_s = 1.f / f.s;
+  f.rm = ms_ref(fmaxf(mt, te.row.mk));
+  f.ek = te.row.sk == 0. ? 0.f : hw_exp2(te.row.mk - f.rm);
+  const double ft = st == 0. ? 0. : hw_exp2(mt - f.rm) * te.row.adj;
+  f.s = te.row.sk * f.ek + st * ft;
+  const double inv = 1. / f.s;
+  f.inv_s = static_cast<float>(te.row.adj * inv);
+  f.qt = st * ft * inv;
+  f.qt = a.tlse != nullptr && f.qt >= 0x1p-126 ? f.qt : 0.;
   f.c = static_cast<float>(static_cast<double>(weight) * a.inv_tau);
   f.ref = ms_ref(mt);
   f.big_p = f.lf = 0.f;
-  const bool tail = has_tail(a, f);
+  f.lse = f.log_qt = 0.;
   if (a.forward) {
-    const float pt = tail ? te.row.pt : 0.f;
+    const double pt = f.qt > 0. ? te.row.pt : 0.;
     f.big_p = static_cast<float>(te.row.sum_p + pt);
-    f.tail = st == 0.f ? 0.f : f.c * (f.big_p * ft * f.inv_s - pt / st);
+    f.tail = st == 0. ? 0.f : f.c * static_cast<float>((te.row.sum_p + pt) * (ft * inv) - pt / st);
   } else {
+    set_logs(a, te, f);
     loss = row_loss(a, te, f);
     f.lf = static_cast<float>(loss);
-    const double gap = tail ? te.row.log_pt - (ms_lse(mt, st) - ms_lse(f.m, f.s)) : 0.;
-    f.tail = st == 0.f ? 0.f : -f.c * (ft * f.inv_s) * (static_cast<float>(gap) + f.lf);
+    const double gap = f.qt > 0. ? te.row.log_pt - f.log_qt : 0.;
+    f.tail = st == 0. ? 0.f : -f.c * static_cast<float>(ft * inv * (gap + loss));
   }
   return f;
 }
@@ -564,7 +615,8 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
       if (ek >= 0) xe = TI::load1(xrow, ek);
     }
     const int groups = groups_of(a);
-    for (int w = tid >> 6; w < groups; w += static_cast<int>(blockDim.x) >> 6) put_late(a, te, w, load_late(a, row, w));
+    for (int w = __builtin_amdgcn_readfirstlane(tid >> 6); w < groups; w += static_cast<int>(blockDim.x) >> 6)
+      put_late(a, te, w, load_late(a, row, w));
     __syncthreads();
     if (tid < 64) {
       float mt, st;
@@ -577,7 +629,7 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
       float token = 0.f;
       if (te.row.state == kUsed) {
         double l = 0.;
-        const RowFactors f = row_factors(a, a.seq_scale[r.seq] * r.w, te, mt, st, l);
+        RowFactors f = row_factors(a, a.seq_scale[r.seq] * r.w, te, mt, st, l);
         for (int w = 0; w < groups; ++w) {
           const int i = tid + kWave * w;
           terms.g[i] = te.id[i] >= 0 ? entry_grad(a, te, f, i) : 0.f;
@@ -585,7 +637,10 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
         terms.tail = f.tail;
         terms.ref = f.ref;
         if (part == 0) {
-          if (a.forward) l = row_loss(a, te, f);
+          if (a.forward) {
+            set_logs(a, te, f);
+            l = row_loss(a, te, f);
+          }
           token = r.w * static_cast<float>(l);
         }
       }
@@ -689,11 +744,13 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
 // range (a tail that is masked, or 2^100 above what the teacher named).
 // Bound by memory and, nearly as much, by the two exponentials per element (the second instead
 // of a second unpacked copy: 19 chunks of 16-bit logits fill the registers of 4 waves a SIMD).
-// 8 sequences of 512 rows of 151,936 in bf16, part of them masked: 385 us; with the entries and
+// 8 sequences of 512 rows of 151,936 in bf16, part of them masked: 381 us; with the entries and
 // the 64-bit arithmetic in the row's own workgroup 496, with them loaded after the row before's
-// stores 441. 512-thread workgroups, two to a CU, up to 8192 vectors: 16 sequences of 256 rows
-// of 50,257 take 158 us (one of 1024 threads: 170). kBufNT stores against kBufNTSystem: 385
-// and 390.
+// stores 441, with a few registers of the loop spilled to scratch memory 391 (a reload waits for
+// the stores too: hence the buffer descriptors, 32-bit compares and wave-uniform indexes here).
+// 512-thread workgroups, two to a CU, up to 8192 vectors: 16 sequences of 256 rows
+// of 50,257 take 158 us (one of 1024 threads: 170). kBufNT stores against kBufNTSystem: 5 us
+// less.
 // Requirements (checked on the host): the row's interior fits BLOCK * NCH vectors; dlogits
 // rows split like the logits rows, or hold f32 for 16-bit logits (dword-aligned stores).
 // ---------------------------------------------------------------------------
@@ -724,7 +781,7 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
   __shared__ uint8_t list[NW][kMaxEntries];
   __shared__ float2 merge[NW];
   __shared__ int s_next[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = groups_of(a);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), groups = groups_of(a);
   const uint32_t voff = tid * 16u, sgrp = split_group<TI, TO, BLOCK>(tid);
   const char* logits = static_cast<const char*>(a.logits);
   auto row_of = [&](int64_t row) { return logits + row * a.vocab * TI::kBytes; };
@@ -830,12 +887,15 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
 
   // The token of row i, -1 for a pad row.
   auto token_of = [&](int64_t i) -> int64_t {
-    const int64_t s = static_cast<uint32_t>(i) / static_cast<uint32_t>(a.logit_stride), t = i - s * a.logit_stride;
-    return t < a.rows ? s * a.tok_stride + a.tok_offset + t : -1;
+    const uint32_t s = static_cast<uint32_t>(i) / static_cast<uint32_t>(a.logit_stride);
+    const uint32_t t = static_cast<uint32_t>(i) - s * static_cast<uint32_t>(a.logit_stride);   // 64 bits: a vector compare
+    return t < static_cast<uint32_t>(a.rows) ? s * a.tok_stride + a.tok_offset + t : -1;
   };
   auto scale_of = [&](int64_t i) { return a.seq_scale[static_cast<uint32_t>(i) / static_cast<uint32_t>(a.logit_stride)]; };
   auto pay = [&](const Teacher& te, int64_t owed) {    // by wave NW - 1: token `owed`'s loss
-    const float l = static_cast<float>(row_loss(a, te, factors[wave]));
+    RowFactors f = factors[wave];
+    set_logs(a, te, f);
+    const float l = static_cast<float>(row_loss(a, te, f));
     if (lane == 0) a.token_loss[owed] = te.row.w * l;
   };
 
@@ -854,6 +914,10 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     const int ek = wave == 0 ? edge_index<TI>(sp, tid) : -1;
     const __amdgpu_buffer_rsrc_t drow = row_rsrc(static_cast<char*>(a.dlogits) + (row_elem + sp.head) * TO::kBytes,
                                                  static_cast<uint32_t>(sp.nv) * kOutVec);
+    // (Under the loads its 64-bit arithmetic would need registers that they fill.)
+    if (wave == NW - 1 && owed >= 0) pay(te3[cp], owed);
+    owed = -1;
+    __builtin_amdgcn_sched_barrier(0);
     u32x4 xv[NCH];
     float xe = 0.f;
     if (weight != 0.f) {
@@ -866,8 +930,6 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     const float late_scale = scale_of(more ? next : row);
     int claimed = 0;
     if (!kStatic && tid == 0 && a.nrows > 2 * grid) claimed = atomicAdd(a.next_row, 1);
-    if (wave == NW - 1 && owed >= 0) pay(te3[cp], owed);
-    owed = -1;
     Owned mine{-1, 0, 0u};                             // this wave's entries
     float g = 0.f, tail = 0.f, gref = 0.f;             // the gradient at this lane's entry; elsewhere
     double loss = 0.;
@@ -892,12 +954,20 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
       // The workgroup's sum, in a fixed order.
       s = lanes_sum<64>(s);
       if (lane == 0) merge[wave] = make_float2(s, twice ? 1.f : 0.f);
+    }
+    // What was loaded ahead goes out of registers before the row's factors need theirs.
+    if (wave < groups) put_late(a, te3[cn], wave, late);
+    if (!kStatic && tid == 0) s_next[i & 1] = a.nrows > 2 * grid ? claimed + 2 * static_cast<int>(grid) : INT32_MAX;
+    const float scale_n = uniform(late_scale);
+    __builtin_amdgcn_sched_barrier(0);
+    if (weight != 0.f) {
       __syncthreads();
       const float2 w = merge[lane & (NW - 1)];
-      float m = ref, st = lanes_sum<NW>(w.x);
+      float m = uniform(ms_ref(te.row.mk));
+      double st = wave_sum64(lane < NW ? static_cast<double>(w.x) : 0.);
       const bool any_twice = __any(w.y != 0.f);
       live = te.row.state == kUsed && !any_twice;
-      if (live && !(st > 0x1p-100f && st < __builtin_inff())) {
+      if (live && !(st > 0x1p-100 && st < __builtin_inf())) {
         // Out of range: the true maximum (the entries' elements are -inf by now), then the sum.
         float x1 = kNegInf;
         if (wave == 0) {
@@ -934,8 +1004,9 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
         __syncthreads();
         const float2 v = merge[lane & (NW - 1)];
         m = v.x;
-        st = v.y;
-        lanes_merge<NW>(m, st);
+        float st1 = v.y;
+        lanes_merge<NW>(m, st1);
+        st = st1;
       }
       if (live) {
         const RowFactors f = row_factors(a, scale * weight, te, m, st, loss);
@@ -947,9 +1018,6 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
         raise_error(a.err, kErrTeacherTwice);
       }
     }
-    if (wave < groups) put_late(a, te3[cn], wave, late);
-    if (!kStatic && tid == 0) s_next[i & 1] = a.nrows > 2 * grid ? claimed + 2 * static_cast<int>(grid) : INT32_MAX;
-    const float scale_n = uniform(late_scale);
     __builtin_amdgcn_sched_barrier(0);
     // Vectors past the row end sit past the descriptor: their stores are dropped.
     if (live) {
