@@ -740,8 +740,8 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
 // nothing is loaded then but the row's chunks. Its record and entries, which the preparation
 // has made, come with the row before's chunks and go to LDS before its stores. The sums need no
 // maximum of their own: they are taken against the largest of the entries' logits, which is the
-// row's largest or near it, and formed again against the true maximum where they leave f32's
-// range (a tail that is masked, or 2^100 above what the teacher named).
+// row's largest or near it, and formed again against the true maximum where they are 2^60 off (a
+// tail that is masked, or far above what the teacher named).
 // Bound by memory and, nearly as much, by the two exponentials per element (the second instead
 // of a second unpacked copy: 19 chunks of 16-bit logits fill the registers of 4 waves a SIMD).
 // 8 sequences of 512 rows of 151,936 in bf16, part of them masked: 381 us; with the entries and
@@ -967,8 +967,9 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
       double st = wave_sum64(lane < NW ? static_cast<double>(w.x) : 0.);
       const bool any_twice = __any(w.y != 0.f);
       live = te.row.state == kUsed && !any_twice;
-      if (live && !(st > 0x1p-100 && st < __builtin_inf())) {
-        // Out of range: the true maximum (the entries' elements are -inf by now), then the sum.
+      if (live && !(st > 0x1p-60 && st < 0x1p60)) {
+        // Too far from the entries: elements next to the tail's largest could leave f32's range. The
+        // true maximum (the entries' elements are -inf by now), then the sum.
         float x1 = kNegInf;
         if (wave == 0) {
           x1 = xe;

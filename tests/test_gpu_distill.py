@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from distill_ref import IGNORE, distill_ref, half_step, lse_ref, top_ref
+from distill_ref import IGNORE, REL, distill_ref, half_step, lse_ref, row_ref, top_ref
 from pcp_amd import distill, grpo
 from pcp_amd._lib import PcpError
 
@@ -501,3 +501,113 @@ def test_a_student_learns_its_teachers_distribution():
     own = distill.top_logits(student, k)
     zero = distill.distill_fwd_bwd(student, own.ids, own.values, own.lse)
     assert abs(float(zero.loss)) <= 4e-5
+
+
+MANY = [("bf16", "bf16", 60, 6000, 7), ("f32", "f32", 1021, 2500, 64), ("f16", "f16", 5003, 2100, 20),
+        ("bf16", "f32", 16001, 900, 256), ("f32", "f32", 20002, 820, 70), ("bf16", "bf16", 33003, 900, 256),
+        ("f16", "f32", 60000, 800, 64), ("bf16", "bf16", 98003, 790, 130), ("f16", "f16", 130001, 780, 256),
+        ("f32", "f32", 77001, 780, 33), ("bf16", "f32", 151936, 790, 64), ("bf16", "bf16", 155600, 1100, 256)]
+
+
+@pytest.mark.parametrize("dtype,out,V,N,k", MANY)
+@pytest.mark.parametrize("mode", ["forward", "renormalised", "reverse"])
+def test_distill_more_rows_than_workgroups(dtype, out, V, N, k, mode):
+    """Rows that follow each other in one workgroup, up to the widest that it keeps: trained ones
+    between ones without weight, without entries and with bad entries; entries side by side; tails
+    far above and below the entries; the gradient over the logits where types allow."""
+    rng = np.random.default_rng(V)
+    S, T = 2, N // 2
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.randn((S, T, V), device=DEV, generator=g).mul_(3).to(DT[dtype])
+    weight = rng.random((S, T)).astype(np.float32) + 0.25
+    live = sorted(rng.choice(N, 40, replace=False))
+    weight[rng.random((S, T)) < 0.5] = 0
+    weight.reshape(-1)[live] = 1.5
+    ids, val = np.full((S, T, k), IGNORE, np.int32), np.zeros((S, T, k), np.float32)
+    lse = np.full((S, T), 40.0, np.float32)
+    some = min(k, V)
+    for n in range(N):
+        first = int(rng.integers(0, V - some + 1))
+        ids.reshape(N, k)[n, :some] = np.arange(first, first + some)
+        val.reshape(N, k)[n, :some] = rng.standard_normal(some) + 30
+    twice = [n for n in range(N) if n not in live][:2]
+    bad = [n for n in range(N) if n not in live][2:4]
+    weight.reshape(-1)[twice + bad] = 1
+    if some > 1:
+        ids.reshape(N, k)[twice, 1] = ids.reshape(N, k)[twice, 0]
+    ids.reshape(N, k)[bad, 0] = V
+    rows, oracle = x.view(N, V), {}
+    for j, n in enumerate(live):
+        r = rows[n].float().cpu().numpy()
+        at = ids.reshape(N, k)[n]
+        if j % 4 == 1:                                        # anywhere in the row
+            at[:some] = rng.choice(V, some, replace=False)
+        if j % 4 == 2:
+            at[rng.random(k) < 0.7] = IGNORE                  # few entries, or none
+        used = at[at != IGNORE]
+        if len(used) and j % 8 in (2, 6):
+            r[used] -= 180 if j % 8 == 2 else -180            # a tail beyond 2^100 on either side
+        if j == 8:
+            r[:] = -np.inf
+            r[used] = 1.0
+        rows[n] = torch.from_numpy(r).to(DT[dtype])
+        t = rows[n].float().cpu().numpy() + rng.standard_normal(V).astype(np.float32)
+        val.reshape(N, k)[n][at != IGNORE] = t[used]
+        lse.reshape(-1)[n] = lse_ref(t[None].astype(np.float64))[0]
+    forward, tail = mode != "reverse", mode != "renormalised"
+    for n in live:
+        oracle[n] = row_ref(host64(rows[n]), ids.reshape(N, k)[n], val.reshape(N, k)[n].astype(np.float64),
+                            float(lse.reshape(-1)[n]) if tail else None, 1.0, forward)
+    ctx = grpo.Context(0)
+    args = (torch.from_numpy(ids).to(DEV), torch.from_numpy(val).to(DEV),
+            torch.from_numpy(lse).to(DEV) if tail else None, torch.from_numpy(weight).to(DEV))
+    o = distill.distill_fwd_bwd(x, *args, divergence="forward" if forward else "reverse", dlogits_dtype=DT[out],
+                                sync=False, ctx=ctx)
+    with pytest.raises(PcpError):
+        ctx.sync()
+    tok, dz = host64(o.token_loss).reshape(-1), o.dlogits.view(N, V)
+    L = np.maximum(weight.astype(np.float64).sum(1), 1.0)
+    for n in live:
+        if oracle[n] is None:
+            assert tok[n] == 0 and not dz[n].any()
+            continue
+        l, grad, mag, lb = oracle[n]
+        w = float(weight.reshape(-1)[n])
+        assert abs(tok[n] - w * l) <= w * lb + 2.0 ** -24 * abs(w * l), n
+        c = w / (S * L[n // T])
+        bar = c * REL * mag
+        # The length is summed in f32: its relative error, 2^-24 log2(T) at most, moves c. A term
+        # 2^(x k2 - m) below 2^-126 is 0, with m within 2^60 V of the tail's largest (V <= 2^24): at
+        # most 2^-42 of the largest gradient; and so is a result below 2^-126.
+        flushed = 2.0 ** -42 * np.abs(c * grad).max() + 2.0 ** -126
+        worst = (np.abs(host64(dz[n]) - c * grad) - bar - half_step(out, c * grad) - 2.0 ** -8 * bar
+                 - 1e-6 * c * np.abs(grad) - flushed)
+        assert worst.max() <= 0, (n, worst.argmax(), worst.max())
+    dead = torch.from_numpy((weight.reshape(-1) == 0)).to(DEV)
+    dead[bad] = True
+    if some > 1:
+        dead[twice] = True
+    for n in dead.nonzero()[:, 0].tolist():
+        assert tok[n] == 0
+    assert not dz[dead].any()
+    if DT[dtype] == DT[out]:                                  # the same bits over the logits themselves
+        distill.distill_fwd_bwd(x, *args, divergence="forward" if forward else "reverse", dlogits=x, sync=False, ctx=ctx)
+        with pytest.raises(PcpError):
+            ctx.sync()
+        assert torch.equal(x, o.dlogits)
+
+
+def test_distill_two_contexts_at_once():
+    """Calls on two streams, each with its own context, give what each gives alone."""
+    cases = [make_case(np.random.default_rng(s), 2, 30, 9001, 40) for s in (21, 22)]
+    want = [run_distill(c, "bf16", "bf16")[1] for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    ctxs = [grpo.Context(0) for _ in cases]
+    outs = [[run_distill(c, "bf16", "bf16", stream=s, ctx=x, sync=False)[1] for c, s, x in zip(cases, streams, ctxs)]
+            for _ in range(3)]
+    for x in ctxs:
+        x.sync()
+    torch.cuda.synchronize()
+    for again in outs:
+        for o, w in zip(again, want):
+            assert torch.equal(o.dlogits, w.dlogits) and torch.equal(o.token_loss, w.token_loss)
