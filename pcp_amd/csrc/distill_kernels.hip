@@ -32,7 +32,16 @@ inline bool misaligned(const void* p, int size) {
   return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(size - 1)) != 0;
 }
 
-constexpr int64_t kPartMinVecs = 4096, kPartMaxRows = 768;
+// Rows in parts where they are wide and few: parts | a row to a workgroup, us, forward divergence
+// with k = 64, by rows:
+//   bf16 151,936   16  18 | 32   64 19 | 34   128 29 | 35   256 51 | 42   512 94 | 74   1024 170 | 142
+//   bf16 100,000   16  18 | 29   64 19 | 31   128 23 | 31   256 39 | 35   512 68 | 57   1024 118 | 105
+//   bf16  50,257   16  18 | 27   64 19 | 29   128 21 | 30   256 27 | 31   512 45 | 37   1024  72 |  66
+//   bf16  33,000   16  19 | 24   64 20 | 25   128 21 | 27   256 24 | 27   512 34 | 33   1024  56 |  53
+//   bf16  16,000   16  24 | 24   64 24 | 26   128 25 | 27   256 25 | 27   512 28 | 30   1024  41 |  37
+//   f32   50,257   16  17 | 25   64 18 | 27   128 22 | 28   256 38 | 35   512 63 | 59   1024 113 | 105
+constexpr int64_t kPartMinVecs = 4096, kPartMaxRows = 320;
+constexpr int64_t kPartWideVecs = 12000, kPartMaxRowsWide = 192;
 
 int distill(pcp_ctx* ctx, const pcp_distill_args* a) {
   if (!a) return fail(ctx, PCP_ERR_INVALID_ARG, "args is NULL");
@@ -98,7 +107,8 @@ int distill(pcp_ctx* ctx, const pcp_distill_args* a) {
   const bool together = a->dlogits && (a->dlogits_dtype != a->logits_dtype ||
                                        ((reinterpret_cast<uintptr_t>(a->logits) ^
                                          reinterpret_cast<uintptr_t>(a->dlogits)) & 15u) == 0) &&
-                        nv <= kDistillRowVecs && (nv < kPartMinVecs || nrows > kPartMaxRows);
+                        nv <= kDistillRowVecs &&
+                        (nv < kPartMinVecs || nrows > (nv < kPartWideVecs ? kPartMaxRows : kPartMaxRowsWide));
   const int64_t parts = together ? 0 : nv > 0 ? (nv + kPartBlock * kPartU - 1) / (kPartBlock * kPartU) : 1;
   // Scratch: seq_len | seq_scale | seq_val | loss, counters | token_loss | rows' records |
   // entries' ids, logits, weights | parts.

@@ -498,10 +498,15 @@ int top_logits(pcp_ctx* ctx, const pcp_top_logits_args* a) {
   if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
   hipStream_t st = static_cast<hipStream_t>(a->stream);
 
-  // Workgroups per row: at least a batch each, and no more than it takes to fill the chip.
+  // Workgroups per row: at least a batch each, and no more than it takes to fill the chip, 2048; from
+  // 512 rows on 1024, since fewer and longer parts leave fewer candidates to merge. Rows of 151,936
+  // bf16, k = 64, us for 256 | 512 | 1024 | 2048 workgroups in all:
+  //   32 rows 22 | 18 | 18 | 18   128 35 | 30 | 27 | 24   256 49 | 40 | 38 | 34   512 55 | 57 | 53 | 61
+  //   1024 rows 79 | 78 | 79 | 89
   const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
   const int64_t batches = nv > 0 ? (nv + kBlock * kU - 1) / (kBlock * kU) : 1;
-  int64_t parts = (2048 + a->n_rows - 1) / a->n_rows;
+  const int64_t fill = a->n_rows < 512 ? 2048 : 1024;
+  int64_t parts = (fill + a->n_rows - 1) / a->n_rows;
   if (parts > batches) parts = batches;
   if (parts > 64) parts = 64;   // one wave merges their sums
   const int64_t per_batches = (batches + parts - 1) / parts;
