@@ -44,7 +44,7 @@ struct TeacherRow {
   double sk;        // sum exp((z - zref) / tau) over the entries
   double adj;
   float pt;
-  float zref, mk;   // (zref 0 and mk -inf where every entry's logit is -inf)
+  float zref, mk;   // (zref 0 and mk -inf where every entry is masked)
   float w;          // the row's weight
   int32_t state;    // kUnused, kUsed; kBad: an id out of range
   int32_t pad;
@@ -281,7 +281,7 @@ __device__ __forceinline__ void prepare_row(const DistillArgs& a, int64_t row) {
     }
     zmax = lanes_max<64>(zmax);
     o.mk = zmax * a.k2;
-    o.zref = ms_ref(zmax);
+    o.zref = o.mk == kNegInf ? 0.f : zmax;   // (-inf too where zmax is a type's lowest value)
     o.adj = exp((static_cast<double>(ms_ref(o.mk)) - static_cast<double>(o.zref) * a.k2) * kLn2F64);
     double sum_p = 0., sk = 0.;
 #pragma unroll

@@ -317,6 +317,36 @@ def test_distill_masked_vocabulary(mode, dtype):
     check_distill(xd, o, small, dtype, tail=True, rows=3, off=0, forward=mode == "forward")
 
 
+@pytest.mark.parametrize("mode", ["forward", "reverse"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("N,V", [(3, 700), (3, 40000), (900, 40000)])
+def test_distill_entries_that_the_student_masks(mode, dtype, N, V):
+    """Every entry's logit -inf, or the type's lowest value, with the rest ordinary: the student
+    gives the entries nothing. (Forward, the loss is infinite or next to it; its gradient is not.)"""
+    rng = np.random.default_rng(V + N)
+    case = make_case(rng, 1, 3, V, 20, cut=False, mask="ones")
+    x, ids, val, lse, m = case
+    for r in range(3):
+        x[0, r, ids[0, r]] = (-np.inf, float(torch.finfo(DT[dtype]).min), -np.inf)[r]
+    x[0, 2] += 200 if dtype == "f32" else 0
+    xs = torch.zeros((1, N, V), dtype=DT[dtype], device=DEV)
+    xs[0, -3:] = to_dev(x[0], dtype)
+
+    def all_rows(t, fill):
+        out = torch.full((1, N) + t.shape[2:], fill, dtype=torch.from_numpy(t).dtype)
+        out[0, -3:] = torch.from_numpy(t[0])
+        return out.to(DEV)
+
+    out = distill.distill_fwd_bwd(xs, all_rows(ids, IGNORE), all_rows(val, 0.0), all_rows(lse, 0.0), all_rows(m, 0.0),
+                                  divergence=mode, sync=False, ctx=grpo.Context(0))
+    want, bars = distill_ref(host64(xs[:, -3:]), ids, val, lse, m, rows=3, off=0, forward=mode == "forward")
+    d = host64(out.dlogits[:, -3:])
+    assert (np.abs(d - want[2]) <= bars[2] + half_step(dtype, want[2]) + 2.0 ** -8 * bars[2] + 2.0 ** -126).all()
+    if mode == "reverse":
+        tok = host64(out.token_loss)[:, -3:]
+        assert (np.abs(tok - want[1]) <= bars[1] + 2.0 ** -24 * np.abs(want[1])).all()
+
+
 @pytest.mark.parametrize("mode", ["forward", "renormalised", "reverse"])
 def test_distill_gradient_against_differences(mode):
     """Central differences of the kernel's own token losses, one logit of one row each:
