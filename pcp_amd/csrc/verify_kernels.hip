@@ -12,9 +12,10 @@
 // sequence.
 //
 // Bound by f64 arithmetic in the rows (16 operations an element) and, with few rows, by the
-// chain of dependent loads from a decision to a token. 64 sequences of 8 drafted tokens over 151,936 bf16 logits:
-// rows 82, decide 2 x 4.7, residual 20, pick 12 us (rows in one launch 109; with the 11-point
-// polynomial alone 150). One sequence of 4: rows 4.7, decide 3.5, residual with pick 14.
+// chain of dependent loads from a decision to a token. 64 sequences of 8 drafted tokens over
+// 151,936 bf16 logits: rows 82, decide 2 x 4.8, residual 18, pick 11 us (rows in one launch 109;
+// with the 11-point polynomial alone 150). One sequence of 4: rows 4.5, decide 3.9, residual
+// with pick 12.5.
 // Deciding in each token's last workgroup, by a ticket, instead of in launches between: the
 // tickets cost 28 us for 4,368 workgroups, 50 for 12,000.
 
@@ -108,32 +109,38 @@ __device__ __forceinline__ double exp2_64(double y) {
 }
 
 // The same for many terms: 2^y with y = Y / 128 as 2^(j/128), from a table in LDS, times a
-// polynomial in Y - rint(Y) through 5 Chebyshev points (relative error 8e-17) and the exponent
-// set in the table's value. 16 operations an element instead of 27 (with 16 to 64 entries and a
-// longer polynomial the rows take 3 to 7 us more of 82: the lookups hide under the arithmetic); y >= -1000 here, so that no term
-// is subnormal: what lies below adds nothing to a sum that holds a 1.
+// polynomial in Y - rint(Y) through 5 Chebyshev points (relative error 8e-17), times 2^e: 16
+// operations an element instead of 27. (With 16 to 64 entries and a longer polynomial the rows
+// take 3 to 7 us more of 82: the lookups hide under the arithmetic.)
 constexpr int kTable = 128;
 __device__ __forceinline__ void fill_table(double* table) {
   if (threadIdx.x < kTable) table[threadIdx.x] = exp2_64(threadIdx.x * (1. / kTable));
 }
 struct Exp2 {
-  double head;   // 2^(j/128 + e)
-  double poly;
+  double head, poly;   // 2^(j/128), 2^(f/128)
+  int n;
   __device__ __forceinline__ Exp2(double Y, const double* table) {
     constexpr double kMagic = 6755399441055744.;   // 1.5 2^52: the sum's low word is rint(Y)
     const double t = Y + kMagic, f = Y - (t - kMagic);
-    const uint64_t b = __builtin_bit_cast(uint64_t, t);
-    const int n = static_cast<int>(static_cast<uint32_t>(b));
-    const uint64_t h = __builtin_bit_cast(uint64_t, table[n & (kTable - 1)]);
-    const uint32_t hi = static_cast<uint32_t>(h >> 32) + (static_cast<uint32_t>(n & ~(kTable - 1)) << 13);
-    head = __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | static_cast<uint32_t>(h));
+    n = static_cast<int>(static_cast<uint32_t>(__builtin_bit_cast(uint64_t, t)));
+    head = table[n & (kTable - 1)];
     double p = 3.583033772988275e-11;
     p = fma(p, f, 2.6466433571126926e-08);
     p = fma(p, f, 1.4662262387638751e-05);
     p = fma(p, f, 0.0054152123481238145);
     poly = fma(p, f, 1.);
   }
+  // sum + 2^y, y >= -1000: the exponent goes into the table's value. (What lies below adds nothing
+  // to a sum that holds a 1.)
+  __device__ __forceinline__ double add_to(double sum) const {
+    const uint64_t h = __builtin_bit_cast(uint64_t, head);
+    const uint32_t hi = static_cast<uint32_t>(h >> 32) + (static_cast<uint32_t>(n & ~(kTable - 1)) << 13);
+    return fma(__builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | static_cast<uint32_t>(h)), poly, sum);
+  }
+  // 2^y, subnormal or 0 from -1022 down.
+  __device__ __forceinline__ double value() const { return __builtin_amdgcn_ldexp(head * poly, n >> 7); }
 };
+static_assert(kTable == 1 << 7, "");
 
 template <typename TI>
 __device__ __forceinline__ const char* target_row(const VerifyArgs& a, int64_t s, int i) {
@@ -290,8 +297,7 @@ __global__ void __launch_bounds__(kBlock) verify_rows_kernel(VerifyArgs a, int r
   }
   const double k = a.k * kTable, ref = -static_cast<double>(ms_ref(m)) * k;
   auto term = [&](float v, double sum) {
-    const Exp2 e(fmax(fma(static_cast<double>(v), k, ref), -1000. * kTable), table);
-    return fma(e.head, e.poly, sum);
+    return Exp2(fmax(fma(static_cast<double>(v), k, ref), -1000. * kTable), table).add_to(sum);
   };
   double sum = ek >= 0 ? term(xe, 0.) : 0.;
 #pragma unroll
@@ -368,11 +374,8 @@ struct Residual {
   bool plain;   // p alone: nothing of p lies above q
   const double* table;
   __device__ __forceinline__ double prob(float x, double ref, double scale) const {
-    // Below 2^-1000, where Exp2 ends, by the slower form, for the elements that have it.
-    const double Y = fma(static_cast<double>(x), k, ref);
-    const Exp2 e(fmax(Y, -1000. * kTable), table);
-    double v = e.head * e.poly;
-    if (__builtin_expect(Y < -1000. * kTable, 0)) v = exp2_64(Y * (1. / kTable));
+    // Exactly 0 from 2^-1100 down; an element that has any mass can be drawn.
+    const double v = Exp2(fmax(fma(static_cast<double>(x), k, ref), -1100. * kTable), table).value();
     return v * scale;
   }
   __device__ __forceinline__ double operator()(float x, float y, int id) const {
@@ -521,20 +524,16 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e,
     __syncthreads();
     return first != INT32_MAX;
   };
+  // The segment where the sum passes (rounding past the last one: its last element); plain, one
+  // after the other.
   int pick = -1;
-  if (!plain) {
-    double run = before;
-    const int g = hit >= 0 ? hit : last_seg;   // rounding past the last segment: its last element
-    pick = scan(g, run) ? first : last;
-  } else {
-    double run = 0.;
-    for (int g = 0; g < segs; ++g) {
-      const bool found = scan(g, run);
-      if (last >= 0) pick = found ? first : last;
-      const bool stop = found;
-      __syncthreads();   // first / last read before the next segment resets them
-      if (stop) break;
-    }
+  double run = before;
+  const int end = plain ? segs : hit >= 0 ? hit + 1 : last_seg + 1;
+  for (int g = plain ? 0 : end - 1; g < end; ++g) {
+    const bool found = scan(g, run);
+    if (last >= 0) pick = found ? first : last;
+    __syncthreads();   // first / last read before the next segment resets them
+    if (found) break;
   }
   if (tid == 0) {
     if (pick < 0) pick = static_cast<int>(a.vocab) - 1;
@@ -546,12 +545,21 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e,
 
 // The end of sequence s, by each wave: false where the row of its last token is bad.
 __device__ __forceinline__ bool seq_end(const VerifyArgs& a, int64_t s, SeqEnd& e) {
-  const int lane = threadIdx.x & 63, len = draft_len(a, s);
+  const int lane = threadIdx.x & 63;
   const Decision* dec = a.decision + s * (a.n + 1);
-  // Lane i has token i (n <= 64). What lies after a refusal may be of another call.
-  const uint64_t no = ~__ballot(lane < len && (dec[min(lane, len)].flags & kAccepted));
+  // Lane i has token i, in one load beside the length's (n <= 64). What lies after a refusal may be of
+  // another call.
+  const Decision mine = dec[min(lane, a.n)];
+  const int len = draft_len(a, s);
+  const uint64_t no = ~__ballot(lane < len && (mine.flags & kAccepted));
   const int j = min(no ? __builtin_ctzll(no) : 64, len);
-  const Decision at = dec[j];
+  Decision at;
+  if (j < 64) {
+    at = Decision{read_lane64(mine.sum_p, j), read_lane64(mine.sum_q, j), read_lane(mine.max_p, j), read_lane(mine.max_q, j),
+                  0.f, __builtin_amdgcn_readlane(mine.flags, j)};
+  } else {
+    at = dec[j];
+  }
   const bool refused = j < len, in = at.flags & kInRange;
   const bool model = refused && a.draft && in && !(at.flags & kBadQ);
   e.j = j;
@@ -644,8 +652,8 @@ __global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
   pick_token<TI, U>(a, e, blockIdx.x, row, row_span<TI>(row, a.vocab), table);
 }
 
-// The residual's last workgroup picks along for few sequences: 14 us for one, against 6.8 + 11 and
-// the gap between two launches; for 64 its tickets made 44 of 20 + 12.
+// The residual's last workgroup picks along for few sequences: 12.5 us for one, against 6.8 + 10
+// and the gap between two launches; for 64 its tickets made 44 of 20 + 12.
 constexpr int64_t kPickAlongMaxSeqs = 4;
 // Rows in two launches from this many workgroups (16 KB each) on: 20,672 took 82 us and a decide
 // of 4.7 instead of 109 where about a third of the sequences went past their first half; 4,368
