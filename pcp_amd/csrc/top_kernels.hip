@@ -504,15 +504,15 @@ int top_logits(pcp_ctx* ctx, const pcp_top_logits_args* a) {
   if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
   hipStream_t st = static_cast<hipStream_t>(a->stream);
 
-  // Workgroups per row: at least a batch each, and no more than it takes to fill the chip, 2048; from
-  // 512 rows on 1024, since fewer and longer parts leave fewer candidates to merge. Rows of 151,936
-  // bf16, k = 64, us for 256 | 512 | 1024 | 2048 workgroups in all:
-  //   32 rows 22 | 18 | 18 | 18   128 35 | 30 | 27 | 24   256 49 | 40 | 38 | 34   512 55 | 57 | 53 | 61
-  //   1024 rows 79 | 78 | 79 | 89
+  // Workgroups per row: one from 512 rows on, which need no merge then; below, no more than it takes
+  // to fill the chip (2048), at least a batch each. us for 2048 | 1024 workgroups in all | one per row:
+  //   bf16 151,936, k 64    128 rows 24 | 27 | -    256 34 | 38 | 49   512 61 | 53 | 56   1024  89 | 78 | 78
+  //   f16  151,936, k 256   128      37 | 37 | -    256 46 | 51 | 61   512 78 | 67 | 70   1024 109 | 99 | 99
+  //   f32   50,257, k 20    128      16 | 17 | -    256 22 | 21 | 27   512 32 | 32 | 31   1024  53 | 43 | 43
+  //   bf16  50,257, k 64    128      16 | 16 | -    256 21 | 21 | 23   512 30 | 30 | 26   1024  49 | 35 | 35
   const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
   const int64_t batches = nv > 0 ? (nv + kBlock * kU - 1) / (kBlock * kU) : 1;
-  const int64_t fill = a->n_rows < 512 ? 2048 : 1024;
-  int64_t parts = (fill + a->n_rows - 1) / a->n_rows;
+  int64_t parts = a->n_rows < 512 ? (2048 + a->n_rows - 1) / a->n_rows : 1;
   if (parts > batches) parts = batches;
   if (parts > 64) parts = 64;   // one wave merges their sums
   const int64_t per_batches = (batches + parts - 1) / parts;
