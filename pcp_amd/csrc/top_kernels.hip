@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kBlock, 6) top_part_kernel(TopArgs a) {
 #pragma unroll
     for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
     auto held = [&](int q) { return base + q * BLOCK + tid < end; };
-    uint64_t near[U];   // the lanes whose vector may hold an element that passes
+    bool near[U];   // this lane's vector may hold an element that passes
     bool fresh = round >= 0 || base == v0 || __any(m == kNegInf);
     if (!fresh) {
       // Terms against the lane's maximum so far, and the vectors compared by their largest term:
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kBlock, 6) top_part_kernel(TopArgs a) {
 #pragma unroll
           for (int j = 0; j < EPV; j += 2) ve = max3(ve, e[j], e[j + 1]);
         }
-        near[q] = __ballot(held(q) && ve >= floor);
+        near[q] = held(q) && ve >= floor;
         most = fmaxf(most, ve);
       }
       fresh = __any(most > 0x1p40f);
@@ -334,30 +334,42 @@ __global__ void __launch_bounds__(kBlock, 6) top_part_kernel(TopArgs a) {
         if (base == v0) c.least_x = reached_by(sh, vm, a.k);
       }
 #pragma unroll
-      for (int q = 0; q < U; ++q) near[q] = __ballot(held(q) && (vm[q] >= c.least_x || c.least_x == kNegInf));
+      for (int q = 0; q < U; ++q) near[q] = held(q) && (vm[q] >= c.least_x || c.least_x == kNegInf);
     }
     // While nothing is ruled out NaN is taken too, which ranks below all.
     const bool all = c.least_x == kNegInf;
+    // Each lane takes its own vectors one after the other: about a dozen of a wave's 512 pass, so
+    // that two turns serve all.
+    uint32_t left_q = 0;
 #pragma unroll
-    for (int q = 0; q < U; ++q) {
-      if (near[q] == 0) continue;
+    for (int q = 0; q < U; ++q) left_q |= near[q] ? 1u << q : 0u;
+    if (round >= 0) left_q &= 1u << (round / (EPV / 4));
+    while (__any(left_q != 0)) {
+      const int mine = __builtin_ctz(left_q | 1u << U);
+      u32x4 w = x[0];
+#pragma unroll
+      for (int q = 1; q < U; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = mine == q ? x[q][i] : w[i];
       // Bit EPV - 1 - j: element j passes. Few lanes have any, fewer have two.
       uint32_t bits = 0;
 #pragma unroll
       for (int j = 0; j < EPV; ++j) {
-        const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j);
+        const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&w), j);
         bits = 2 * bits + ((v >= c.least_x || all) ? 1u : 0u);
       }
-      if (!held(q)) bits = 0;
-      if (round >= 0) bits &= round / (EPV / 4) == q ? 0xf0u >> (EPV == 4 ? 4 : 4 * (round % 2)) : 0u;
+      if (left_q == 0) bits = 0;
+      left_q &= left_q - 1;
+      if (round >= 0) bits &= 0xf0u >> (EPV == 4 ? 4 : 4 * (round % 2));
+      const uint32_t first = static_cast<uint32_t>(sp.head + (base + mine * BLOCK + tid) * EPV);
       while (__any(bits != 0)) {
         const int j = EPV - 32 + __builtin_clz(bits | 1u);   // the first that is left
-        uint32_t w = x[q][0];
+        uint32_t u = w[0];
         const int word = TI::kBytes == 4 ? j : j >> 1;
 #pragma unroll
-        for (int i = 1; i < 4; ++i) w = word == i ? x[q][i] : w;
-        if constexpr (TI::kBytes == 2) w >>= 16 * (j & 1);
-        const uint64_t k = element_key(TI::unpack(&w, 0), static_cast<uint32_t>(sp.head + (base + q * BLOCK + tid) * EPV + j));
+        for (int i = 1; i < 4; ++i) u = word == i ? w[i] : u;
+        if constexpr (TI::kBytes == 2) u >>= 16 * (j & 1);
+        const uint64_t k = element_key(TI::unpack(&u, 0), first + j);
         c.add(bits != 0 && k > c.least, k);
         bits &= ~((1u << (EPV - 1)) >> j);
       }
