@@ -12,10 +12,11 @@
 // with one part is ranked and written by its workgroup; else each part leaves its
 // candidates and a second kernel merges them.
 //
-// Bound by the exponentials and the comparisons with many rows (4096 rows of 151,936 bf16, k = 64:
-// 238 us, 5.2 TB/s; 474 with thresholds from sorted lists and a pass of its own for the vectors'
-// maxima), by latency with few: one such row takes 8.7 us in 10 parts and 6.5 to merge them. The
-// merge of many long lists costs most: 192 rows, k = 256, 27 + 17 us.
+// Bound by the exponentials and HBM with many rows (4096 rows of 151,936 bf16, k = 64: 202 us,
+// 6.2 TB/s; 231 while every lane looked at each vector that passed in any, 474 with thresholds from sorted
+// lists and a pass of its own for the vectors' maxima), by latency with few: one such row takes
+// 7.0 us in 10 parts and 6.5 to merge them. The merge of many long lists costs most: 192 rows,
+// k = 256, 25 + 17 us.
 
 #include <hip/hip_runtime.h>
 
@@ -247,9 +248,9 @@ __device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, float m
   if (!__builtin_isfinite(lse)) raise_error(a.err, kErrNonFinite);
 }
 
-// 6 waves a SIMD: with the 85 registers that it would take, and 5, f32 rows run 4% longer.
+// 5 waves a SIMD: at 6 a register is spilled, and 2048 f32 rows of 50,257 take 74 us instead of 69.
 template <typename TI>
-__global__ void __launch_bounds__(kBlock, 6) top_part_kernel(TopArgs a) {
+__global__ void __launch_bounds__(kBlock, 5) top_part_kernel(TopArgs a) {
   constexpr int EPV = 16 / TI::kBytes, U = kU, BLOCK = kBlock;
   __shared__ __align__(16) Shared sh;
   __shared__ __align__(16) float lds[4 * (BLOCK / 64)];
@@ -518,10 +519,10 @@ int top_logits(pcp_ctx* ctx, const pcp_top_logits_args* a) {
 
   // Workgroups per row: one from 512 rows on, which need no merge then; below, no more than it takes
   // to fill the chip (2048), at least a batch each. us for 2048 | 1024 workgroups in all | one per row:
-  //   bf16 151,936, k 64    128 rows 24 | 27 | -    256 34 | 38 | 49   512 61 | 53 | 56   1024  89 | 78 | 78
-  //   f16  151,936, k 256   128      37 | 37 | -    256 46 | 51 | 61   512 78 | 67 | 70   1024 109 | 99 | 99
-  //   f32   50,257, k 20    128      16 | 17 | -    256 22 | 21 | 27   512 32 | 32 | 31   1024  53 | 43 | 43
-  //   bf16  50,257, k 64    128      16 | 16 | -    256 21 | 21 | 23   512 30 | 30 | 26   1024  49 | 35 | 35
+  //   bf16 151,936, k 64    128 rows 21 | 23 | 34   256 29 | 32 | 36   400 39 | 40 | 42   512 49 | 42 | 42   1024 69 | 60 | 59
+  //   f16  151,936, k 256   128      37 | 34 | 56   256 41 | 44 | 49   400 54 | 55 | 56   512 66 | 57 | 56   1024 89 | 76 | 76
+  //   f32   50,257, k 20    128      16 | 16 | 21   256 21 | 20 | 22   400 26 | 24 | 24   512 29 | 29 | 25   1024 50 | 41 | 40
+  //   bf16  50,257, k 64    128      16 | 15 | 17   256 20 | 19 | 18   400 24 | 25 | 21   512 26 | 26 | 21   1024 40 | 28 | 29
   const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
   const int64_t batches = nv > 0 ? (nv + kBlock * kU - 1) / (kBlock * kU) : 1;
   int64_t parts = a->n_rows < 512 ? (2048 + a->n_rows - 1) / a->n_rows : 1;
