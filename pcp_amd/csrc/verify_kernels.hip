@@ -195,20 +195,20 @@ __global__ void __launch_bounds__(kBlock) verify_first_max_kernel(VerifyArgs a) 
   const int ek = part == 0 ? edge_index<TI>(sp, tid) : -1;
   const float xe = ek >= 0 ? TI::load1(row, ek) : kNegInf;
   float best = kNegInf;
-  int at = INT32_MAX;
-  if (xe > kNegInf) {
-    best = xe;
-    at = ek;
-  }
+  int slot = -1;   // a lane's elements come by rising index: the first of equals stays
 #pragma unroll
   for (int q = 0; q < U; ++q)
     if (v0 + q * BLOCK + tid < sp.nv)
 #pragma unroll
       for (int j = 0; j < EPV; ++j) {
         const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j);
-        const int e = sp.head + (v0 + q * BLOCK + tid) * EPV + j;
-        if (v > kNegInf) better32(best, at, v, e);
+        if (v > best) {
+          best = v;
+          slot = q * EPV + j;
+        }
       }
+  int at = slot < 0 ? INT32_MAX : sp.head + (v0 + slot / EPV * BLOCK + tid) * EPV + slot % EPV;
+  if (xe > kNegInf) better32(best, at, xe, ek);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) better32(best, at, __shfl_xor(best, o), __shfl_xor(at, o));
   if (lane == 0) {
