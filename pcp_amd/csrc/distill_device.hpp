@@ -75,6 +75,7 @@ struct DistillArgs {
   double inv_tau;
   int64_t n_seq;
   int* done;                // the loss reduction's ticket
+  float* loss;              // formed by the last workgroup to finish, or nullptr: by loss_reduce_kernel
   float loss_norm;          // loss_norm / weight
   float k2;                 // log2(e) / tau
   int32_t k, ids_i64, mask_u8, forward;
@@ -493,6 +494,33 @@ __device__ __forceinline__ RowFactors row_factors(const DistillArgs& a, float we
   return f;
 }
 
+// The loss from the token losses, which are stored through to the coherent level: by the last of
+// `n` workgroups to come here, each after its last one; in a fixed order.
+template <int BLOCK>
+__device__ __forceinline__ void finish_loss(const DistillArgs& a, int n) {
+  __shared__ double sums[BLOCK / 64];
+  __shared__ int last;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  wait_stores();     // this wave's token losses ...
+  __syncthreads();   // ... and every wave's, before the ticket
+  if (tid == 0) last = atomicAdd(a.done, 1) == n - 1;
+  __syncthreads();
+  if (!last) return;
+  acquire_coherent();
+  double sum = 0.;
+  for (int64_t s = wave; s < a.n_seq; s += BLOCK / 64) {
+    const float* t = a.token_loss + s * a.tok_stride + a.tok_offset;
+    double l = 0.;
+    for (int64_t i = lane; i < a.rows; i += 64) l += t[i];
+    sum += wave_sum64(l) / a.seq_len[s];
+  }
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  if (tid != 0) return;
+  for (int w = 1; w < BLOCK / 64; ++w) sum += sums[w];
+  *a.loss = static_cast<float>(sum / a.loss_norm);
+}
+
 // ---------------------------------------------------------------------------
 // Rows in parts: workgroups of 256 lanes take `per` vectors of a row each. The first kernel
 // leaves each part's (m_T, s_T); in the second every workgroup of a row merges them for
@@ -644,12 +672,12 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
           token = r.w * static_cast<float>(l);
         }
       }
-      if (part == 0 && tid == 0 && a.token_loss) a.token_loss[r.tix] = token;
+      if (part == 0 && tid == 0) store_coherent(a.token_loss + r.tix, token);
     }
     __syncthreads();
     live = te.row.state == kUsed;
-  } else if (part == 0 && tid == 0 && r.tok && a.token_loss) {
-    a.token_loss[r.tix] = 0.f;
+  } else if (part == 0 && tid == 0 && r.tok) {
+    store_coherent(a.token_loss + r.tix, 0.f);
   }
   float g[NS], tail = 0.f, ref = 0.f;
   int place[NS], edge[NS];
@@ -731,6 +759,7 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
       if (ek >= 0) store1<TO>(a.dlogits, row_elem + ek, o);
     }
   }
+  if (part == 0 && a.loss) finish_loss<GRAD ? BLOCK : 64>(a, static_cast<int>(a.nrows));
 }
 
 // ---------------------------------------------------------------------------
@@ -896,7 +925,7 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     RowFactors f = factors[wave];
     set_logs(a, te, f);
     const float l = static_cast<float>(row_loss(a, te, f));
-    if (lane == 0) a.token_loss[owed] = te.row.w * l;
+    if (lane == 0) store_coherent(a.token_loss + owed, te.row.w * l);
   };
 
   if (wave < groups) put_late(a, te3[0], wave, load_late(a, row, wave));
@@ -1071,7 +1100,7 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
         store1<TO>(a.dlogits, row_elem + ek, oe);
       }
       if (tid == 0 && token >= 0 && !(live && a.forward))
-        a.token_loss[token] = live ? weight * static_cast<float>(loss) : 0.f;
+        store_coherent(a.token_loss + token, live ? weight * static_cast<float>(loss) : 0.f);
     }
     if (live && a.forward) owed = token;
     if (!more) {
@@ -1084,6 +1113,7 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     next = kStatic ? deal() : static_cast<int64_t>(__builtin_amdgcn_readfirstlane(s_next[i & 1]));
     c = cn;
   }
+  if (a.loss) finish_loss<BLOCK>(a, static_cast<int>(gridDim.x));
 }
 
 // ---------------------------------------------------------------------------

@@ -42,6 +42,12 @@ inline bool misaligned(const void* p, int size) {
 //   f32   50,257   16  17 | 25   64 18 | 27   128 22 | 28   256 38 | 35   512 63 | 59   1024 113 | 105
 constexpr int64_t kPartMinVecs = 4096, kPartMaxRows = 320;
 constexpr int64_t kPartWideVecs = 12000, kPartMaxRowsWide = 192;
+// The loss by the last workgroup to finish, where few take tickets; else by a kernel of its own.
+// us per call, along | by its own kernel, by rows:
+//   bf16 151,936   4  13 | 16   64 17 | 20   128 26 | 28   256 41 | 42   320 62 | 62   512 73 | 71   1024 144 | 142
+//   bf16  50,257   4  14 | 17   64 15 | 18   128 18 | 20   256 23 | 26   320 27 | 29   512 35 | 35   1024  64 |  63
+//   f32    1,024   4  17 | 18   64 18 | 20   128 19 | 20   256 19 | 21   320 20 | 21   512 23 | 23   1024  32 |  27
+constexpr int64_t kAlongMaxRows = 320;
 
 int distill(pcp_ctx* ctx, const pcp_distill_args* a) {
   if (!a) return fail(ctx, PCP_ERR_INVALID_ARG, "args is NULL");
@@ -166,11 +172,14 @@ int distill(pcp_ctx* ctx, const pcp_distill_args* a) {
   d.forward = a->divergence == PCP_DIVERGENCE_FORWARD;
   d.parts = static_cast<int32_t>(parts);
   d.per = parts ? static_cast<int32_t>((nv + parts - 1) / parts) : 0;
+  const bool along = nrows <= kAlongMaxRows;
+  if (along) d.loss = a->loss ? a->loss : s_loss;
 
   const bool timed = prof_begin(ctx, st);
   hipError_t e = launch_distill(d, a->logits_dtype, a->dlogits ? a->dlogits_dtype : a->logits_dtype, st);
   prof_end(ctx, st, timed);
   if (e != hipSuccess) return hip_fail(ctx, e, "distillation launch");
+  if (along) return finish_call(ctx, a->flags, st);
   const LossReduceArgs la{s_tl, a->rows, tstride, a->tok_offset, s_len, nullptr, 0, s_val, a->n_seq, norm, s_done,
                           a->loss ? a->loss : s_loss};
   if ((e = launch_loss_reduce_fused(la, st)) != hipSuccess) return hip_fail(ctx, e, "loss reduction launch");
