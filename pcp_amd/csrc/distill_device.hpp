@@ -4,11 +4,11 @@
 // With x a row's logits, k2 = log2(e) / tau, K the used teacher ids and T the rest of the
 // vocabulary, the rows' sums are kept apart: (m_T, s_T) over T while the row streams past
 // (the entries' own elements are replaced by -inf where they sit in registers), and s_K from
-// the k gathered logits. Per element in f32; what a row has once (s_K, the merge of its waves'
-// sums, log-sum-exp, the divergence) in f64, since the divergence may be far below its terms. The tail's mass Q_T = s_T 2^(m_T - lse) is then a
-// sum of its own and keeps its relative precision where the teacher's entries hold nearly
-// everything (1 - sum q_i would lose it all). Outside K the gradient is one factor of
-// 2^(x k2 - m_T):
+// the k gathered logits. The tail's mass Q_T = s_T 2^(m_T - lse) is then a sum of its own and
+// keeps its relative precision where the teacher's entries hold nearly everything (1 - sum q_i
+// would lose it all). Per element the arithmetic is f32; what a row has once (s_K, the merge of
+// its waves' sums, log-sum-exp, the divergence) f64, since the divergence may be far below its
+// terms. Outside K the gradient is one factor of 2^(x k2 - m_T):
 //   forward:  c (P 2^(m_T - lse) - p_T / s_T),   reverse:  c 2^(m_T - lse) (log(Q_T/p_T) - l),
 // with c = weight m / (loss_norm L tau) and P = sum p_i + p_T; on K each entry has its own
 // value, which takes the element's place before its vector is stored.
@@ -84,7 +84,7 @@ struct DistillArgs {
 };
 
 struct DistillRow {
-  int64_t row, tix;
+  int64_t tix;
   float w;
   int32_t seq;
   bool tok;
@@ -92,7 +92,6 @@ struct DistillRow {
 
 __device__ __forceinline__ DistillRow distill_row(const DistillArgs& a, int64_t row) {
   DistillRow r;
-  r.row = row;
   const int64_t s = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.logit_stride);
   const int64_t t = row - s * a.logit_stride;
   r.seq = static_cast<int32_t>(s);
@@ -374,7 +373,8 @@ __device__ __forceinline__ LateRow load_late(const DistillArgs& a, int64_t row, 
   l.id = static_cast<int>(word(a.entry_ids + base, n * 4u));
   l.t = __uint_as_float(word(a.tlogits + base, n * 4u));
   l.z = __uint_as_float(word(a.entry_z + base, n * 4u));
-  l.w = __builtin_bit_cast(double, __builtin_amdgcn_raw_buffer_load_b64(row_rsrc(a.entry_w + base, n * 8u), lane * 8u, 0, 0));
+  l.w = __builtin_bit_cast(double, __builtin_amdgcn_raw_buffer_load_b64(row_rsrc(a.entry_w + base, n * 8u),
+                                                                         lane * 8u, 0, 0));
   l.word = word(a.teacher + row, sizeof(TeacherRow));
   return l;
 }
@@ -438,7 +438,8 @@ __device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher&
 }
 
 __device__ __forceinline__ void set_logs(const DistillArgs& a, const Teacher& te, RowFactors& f) {
-  f.lse = static_cast<double>(te.row.zref) * a.inv_tau + static_cast<double>(f.rm - ms_ref(te.row.mk)) * kLn2F64 + log64(f.s);
+  f.lse = static_cast<double>(te.row.zref) * a.inv_tau + static_cast<double>(f.rm - ms_ref(te.row.mk)) * kLn2F64 +
+          log64(f.s);
   f.log_qt = f.qt > 0. ? log64(f.qt) : 0.;
 }
 
@@ -805,7 +806,7 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
   constexpr bool kSplit = TI::kBytes == 2 && TO::kBytes == 4, kStatic = kDealt<BLOCK, NCH>;
   constexpr uint32_t kOutVec = EPV * TO::kBytes;
   static_assert(NW >= kMaxSlots, "a wave per group of entries");
-  __shared__ Teacher te3[3];                   // of the row before (its loss is formed under this row's loads), this one, the next
+  __shared__ Teacher te3[3];                   // of the row before (its loss comes with this row), this one, the next
   __shared__ RowFactors factors[NW];           // each wave its own copy of the same: out of registers under the stores
   __shared__ uint8_t list[NW][kMaxEntries];
   __shared__ float2 merge[NW];

@@ -555,8 +555,8 @@ __device__ __forceinline__ bool seq_end(const VerifyArgs& a, int64_t s, SeqEnd& 
   const int j = min(no ? __builtin_ctzll(no) : 64, len);
   Decision at;
   if (j < 64) {
-    at = Decision{read_lane64(mine.sum_p, j), read_lane64(mine.sum_q, j), read_lane(mine.max_p, j), read_lane(mine.max_q, j),
-                  0.f, __builtin_amdgcn_readlane(mine.flags, j)};
+    at = Decision{read_lane64(mine.sum_p, j), read_lane64(mine.sum_q, j), read_lane(mine.max_p, j),
+                  read_lane(mine.max_q, j), 0.f, __builtin_amdgcn_readlane(mine.flags, j)};
   } else {
     at = dec[j];
   }
