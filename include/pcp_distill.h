@@ -34,7 +34,8 @@ extern "C" {
 /* The k largest logits of each row with their ids, by falling logit, equal logits by
  * rising id, and the row's log-sum-exp  lse = log sum_v exp(logit_v / temperature).
  * -0 counts as 0 and is handed on as 0. NaN ranks below every number; a row whose
- * log-sum-exp is not finite (a NaN or +Inf logit, or nothing above -Inf) is reported as
+ * log-sum-exp is not finite as an f32 (a NaN or +Inf logit, nothing above -Inf, or a
+ * largest logit that leaves f32's range divided by the temperature) is reported as
  * PCP_ERR_NONFINITE after the call, with its outputs written. Entries may be -Inf where
  * fewer than k logits are larger. */
 typedef struct pcp_top_logits_args {

@@ -353,6 +353,62 @@ __device__ __forceinline__ void lanes_merge(float& m, float& s) {
   m = M;
 }
 
+// ---------------------------------------------------------------------------
+// Sums of 2^((x - mx) k) at a scale k = log2(e) / temperature, mx the largest logit of those
+// summed, itself and not times k: a mask such as -1e30 is as far from its rounded product with
+// k as 2^75, so that terms against the product would be inf or 0 where they are 1. mx is -inf
+// and s 0 where there is none; NaN stays in s as above.
+// ---------------------------------------------------------------------------
+// The terms as 2^(fma(x, k, -ref)), one instruction, times term_adj(). |mx k| < 2^31: ref is the
+// rounded product, at most 2^6 off, which f32's range takes. From there on two f32 logits
+// that differ at all lie 2^128 apart, whatever k is within a factor of two: k becomes the power of
+// two that takes mx to [2^31, 2^32), and the product is exact.
+struct TermScale {
+  float k, ref;
+};
+__device__ __forceinline__ TermScale term_scale(float mx, float k) {
+  TermScale t{k, ms_ref(mx) * k};
+  if (!(fabsf(t.ref) < 0x1p31f)) {
+    t.k = __builtin_amdgcn_ldexpf(1.f, min(32 - __builtin_amdgcn_frexp_expf(mx), 127));
+    t.ref = mx * t.k;
+  }
+  return t;
+}
+// The rounding of ref, exactly; 2 to its negative.
+__device__ __forceinline__ float term_residue(float mx, const TermScale& t) { return fmaf(ms_ref(mx), t.k, -t.ref); }
+__device__ __forceinline__ float term_adj(float mx, const TermScale& t) { return hw_exp2(-term_residue(mx, t)); }
+
+// A sum relative to m, relative to M >= m.
+template <typename T>
+__device__ __forceinline__ T rescale_at(T s, float m, float M, float k) {
+  return s == T(0) ? T(0) : s * hw_exp2((m - ms_ref(M)) * k);
+}
+// The merge of the first N lanes' sums, on every lane, in a fixed order.
+template <int N>
+__device__ __forceinline__ void lanes_merge_at(float& mx, float& s, float k) {
+  const float M = lanes_max<N>(mx);
+  s = lanes_sum<N>(rescale_at(s, mx, M, k));
+  mx = M;
+}
+// The same over the workgroup, on every thread; lds: one entry per wave.
+template <int BLOCK>
+__device__ __forceinline__ void block_merge_at(float& mx, float& s, float k, float2* lds) {
+  constexpr int NW = BLOCK / 64;
+  lanes_merge_at<64>(mx, s, k);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (lane == 0) lds[wave] = make_float2(mx, s);
+  __syncthreads();
+  const float2 w = lds[lane & (NW - 1)];
+  mx = w.x;
+  s = w.y;
+  lanes_merge_at<NW>(mx, s, k);
+}
+// A part of a row as its workgroup leaves it: its sum, and a count or a flag.
+struct alignas(16) PartSum {
+  float mx, s;
+  int32_t n, pad;
+};
+
 // Reduce two (m, s) pairs over the workgroup. `lds` holds 4 floats per wave, 16-byte
 // aligned. Returns the same values on every thread. The rows' merge is a serial chain
 // during which the workgroup has no load in flight: six butterfly steps through

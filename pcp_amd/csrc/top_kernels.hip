@@ -49,8 +49,9 @@ struct TopArgs {
   void* ids;
   float* lse;
   uint64_t* part_key;     // [n_rows, parts, part_cap]
-  float4* part_ms;        // [n_rows, parts]: (m, s, candidates left, -)
+  PartSum* part_sum;      // [n_rows, parts]: n the candidates left
   int* err;
+  double inv_tau;
   float k2;               // log2(e) / temperature
   int32_t k, ids_i64, parts, per, part_cap;
 };
@@ -242,9 +243,10 @@ __device__ __forceinline__ void write_entries(const TopArgs& a, int64_t row, Sha
   }
 }
 
-__device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, float m, float s) {
-  const double lse = ms_lse(m, s);
-  if (a.lse) a.lse[row] = static_cast<float>(lse);
+// From the row's sum against its largest logit, which may leave f32's range divided by the temperature.
+__device__ __forceinline__ void write_lse(const TopArgs& a, int64_t row, float mx, float s) {
+  const float lse = static_cast<float>(static_cast<double>(mx) * a.inv_tau + ms_lse(0.f, s));
+  if (a.lse) a.lse[row] = lse;
   if (!__builtin_isfinite(lse)) raise_error(a.err, kErrNonFinite);
 }
 
@@ -253,7 +255,7 @@ template <typename TI>
 __global__ void __launch_bounds__(kBlock, 5) top_part_kernel(TopArgs a) {
   constexpr int EPV = 16 / TI::kBytes, U = kU, BLOCK = kBlock;
   __shared__ __align__(16) Shared sh;
-  __shared__ __align__(16) float lds[4 * (BLOCK / 64)];
+  __shared__ float2 wave_sum[kWaves];
   const int tid = threadIdx.x, part = blockIdx.x;
   const int64_t row = a.row0 + blockIdx.y;
   const char* xrow = static_cast<const char*>(a.logits) + row * a.row_stride * TI::kBytes;
@@ -262,15 +264,19 @@ __global__ void __launch_bounds__(kBlock, 5) top_part_kernel(TopArgs a) {
   const __amdgpu_buffer_rsrc_t xbuf = row_rsrc(sp.vec, static_cast<uint32_t>(max(end, 0)) * 16u);
   Candidates c{sh, 0, kNegInf};
   if (tid == 0) sh.count = 0;
-  float m = kNegInf, s = 0.f;
+  // The lane's largest logit and its sum against it: a batch's in f32, the batches' in f64 (a lane has
+  // up to 65,536 elements of a row).
+  float mx = kNegInf, adj = 1.f;
+  double s = 0.;
+  TermScale ts{a.k2, 0.f};
   __syncthreads();
   if (part == 0 && tid < 64) {   // the elements outside the interior
     const int ek = edge_index<TI>(sp, tid);
     float xe = kNegInf;
     if (ek >= 0) {
       xe = TI::load1(xrow, ek);
-      m = fmaxf(m, xe * a.k2);
-      s = hw_exp2(fmaf(xe, a.k2, -ms_ref(m)));
+      mx = fmaxf(mx, xe);
+      s = hw_exp2((xe - ms_ref(mx)) * a.k2);
     }
     c.add(ek >= 0, element_key(xe, static_cast<uint32_t>(ek)));
   }
@@ -286,13 +292,13 @@ __global__ void __launch_bounds__(kBlock, 5) top_part_kernel(TopArgs a) {
     for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
     auto held = [&](int q) { return base + q * BLOCK + tid < end; };
     bool near[U];   // this lane's vector may hold an element that passes
-    bool fresh = round >= 0 || base == v0 || __any(m == kNegInf);
+    bool fresh = round >= 0 || base == v0 || __any(mx == kNegInf);
     if (!fresh) {
       // Terms against the lane's maximum so far, and the vectors compared by their largest term:
       // no pass for a new maximum unless one has risen far above.
-      const float cut = hw_exp2(fmaf(c.least_x, a.k2, -m)) * (1.f - 0x1p-16f);
+      const float cut = hw_exp2(fmaf(c.least_x, ts.k, -ts.ref)) * (1.f - 0x1p-16f);
       const float floor = cut > 0x1p-100f ? cut : 0.f;   // rounding above, underflow below
-      float acc = s, most = 0.f;
+      float acc = 0.f, most = 0.f;
 #pragma unroll
       for (int q = 0; q < U; ++q) {
         float e[EPV], ve = 0.f;
@@ -300,7 +306,7 @@ __global__ void __launch_bounds__(kBlock, 5) top_part_kernel(TopArgs a) {
           const uint32_t* w = reinterpret_cast<const uint32_t*>(&x[q]);
 #pragma unroll
           for (int j = 0; j < EPV; ++j) {
-            e[j] = hw_exp2(fmaf(TI::unpack(w, j), a.k2, -m));
+            e[j] = hw_exp2(fmaf(TI::unpack(w, j), ts.k, -ts.ref));
             acc += e[j];
           }
 #pragma unroll
@@ -310,7 +316,7 @@ __global__ void __launch_bounds__(kBlock, 5) top_part_kernel(TopArgs a) {
         most = fmaxf(most, ve);
       }
       fresh = __any(most > 0x1p40f);
-      if (!fresh) s = acc;
+      if (!fresh) s += static_cast<double>(acc * adj);
     }
     if (fresh) {
       float vm[U], bx = kNegInf;
@@ -320,17 +326,19 @@ __global__ void __launch_bounds__(kBlock, 5) top_part_kernel(TopArgs a) {
         bx = fmaxf(bx, vm[q]);
       }
       if (round < 0) {
-        const float nm = fmaxf(m, bx * a.k2), ref = ms_ref(nm);
-        float acc = ms_rescale(s, m, nm);
+        const float nm = fmaxf(mx, bx);
+        ts = term_scale(nm, a.k2);
+        adj = term_adj(nm, ts);
+        float acc = 0.f;
 #pragma unroll
         for (int q = 0; q < U; ++q)
           if (held(q)) {
             const uint32_t* w = reinterpret_cast<const uint32_t*>(&x[q]);
 #pragma unroll
-            for (int j = 0; j < EPV; ++j) acc += hw_exp2(fmaf(TI::unpack(w, j), a.k2, -ref));
+            for (int j = 0; j < EPV; ++j) acc += hw_exp2(fmaf(TI::unpack(w, j), ts.k, -ts.ref));
           }
-        m = nm;
-        s = acc;
+        s = rescale_at(s, mx, nm, a.k2) + static_cast<double>(acc * adj);
+        mx = nm;
         // k vectors of the first batch reach this, each with one element at least.
         if (base == v0) c.least_x = reached_by(sh, vm, a.k);
       }
@@ -392,15 +400,15 @@ __global__ void __launch_bounds__(kBlock, 5) top_part_kernel(TopArgs a) {
   }
   __syncthreads();
   n = sh.count;
-  float m2 = kNegInf, s2 = 0.f;
-  block_merge2<BLOCK>(m, s, m2, s2, lds);
+  float sum = static_cast<float>(s);
+  block_merge_at<BLOCK>(mx, sum, a.k2, wave_sum);
   if (a.parts == 1) {
     write_entries(a, row, sh, n);
-    if (tid == 0) write_lse(a, row, m, s);
+    if (tid == 0) write_lse(a, row, mx, sum);
   } else {
     uint64_t* out = a.part_key + (row * a.parts + part) * a.part_cap;
     for (int i = tid; i < n; i += BLOCK) out[i] = sh.key[i];
-    if (tid == 0) a.part_ms[row * a.parts + part] = make_float4(m, s, __int_as_float(n), 0.f);
+    if (tid == 0) a.part_sum[row * a.parts + part] = PartSum{mx, sum, n, 0};
   }
 }
 
@@ -415,7 +423,7 @@ __global__ void __launch_bounds__(kBlock) top_merge_kernel(TopArgs a) {
   const int tid = threadIdx.x;
   const int64_t row = a.row0 + blockIdx.x;
   const uint64_t* in = a.part_key + row * a.parts * a.part_cap;
-  const float4* ms = a.part_ms + row * a.parts;
+  const PartSum* sums = a.part_sum + row * a.parts;
   const int total = a.parts * a.part_cap;
   Candidates c{sh, 0, kNegInf};
   if (tid == 0) sh.count = 0;
@@ -427,7 +435,7 @@ __global__ void __launch_bounds__(kBlock) top_merge_kernel(TopArgs a) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       const int at = base + i * kBlock + tid, p = at / a.part_cap;
-      const bool is = at < total && at - p * a.part_cap < __float_as_int(ms[p].z);
+      const bool is = at < total && at - p * a.part_cap < sums[p].n;
       k[i] = is ? in[at] : 0;   // no key is 0
     }
 #pragma unroll
@@ -455,13 +463,13 @@ __global__ void __launch_bounds__(kBlock) top_merge_kernel(TopArgs a) {
   }
   write_entries(a, row, sh, n);
   if (tid < 64) {
-    float m = kNegInf, s = 0.f;
+    float mx = kNegInf, s = 0.f;
     if (tid < a.parts) {
-      m = ms[tid].x;
-      s = ms[tid].y;
+      mx = sums[tid].mx;
+      s = sums[tid].s;
     }
-    lanes_merge<64>(m, s);
-    if (tid == 0) write_lse(a, row, m, s);
+    lanes_merge_at<64>(mx, s, a.k2);
+    if (tid == 0) write_lse(a, row, mx, s);
   }
 }
 
@@ -532,8 +540,8 @@ int top_logits(pcp_ctx* ctx, const pcp_top_logits_args* a) {
   parts = (batches + per_batches - 1) / per_batches;
   const int64_t part_cap = a->k + 64;
   const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(a->n_rows) * parts * part_cap : 0;
-  const size_t ms = parts > 1 ? sizeof(float4) * static_cast<size_t>(a->n_rows) * parts + 16 : 0;
-  const int rc = ensure_scratch_on(ctx, keys + ms, st);
+  const size_t sums = parts > 1 ? sizeof(PartSum) * static_cast<size_t>(a->n_rows) * parts + 16 : 0;
+  const int rc = ensure_scratch_on(ctx, keys + sums, st);
   if (rc != PCP_OK) return rc;
 
   TopArgs t;
@@ -546,8 +554,9 @@ int top_logits(pcp_ctx* ctx, const pcp_top_logits_args* a) {
   t.ids = a->ids;
   t.lse = a->lse;
   t.part_key = static_cast<uint64_t*>(ctx->scratch);
-  t.part_ms = reinterpret_cast<float4*>(static_cast<char*>(ctx->scratch) + ((keys + 15) & ~static_cast<size_t>(15)));
+  t.part_sum = reinterpret_cast<PartSum*>(static_cast<char*>(ctx->scratch) + ((keys + 15) & ~static_cast<size_t>(15)));
   t.err = ctx->d_page->err;
+  t.inv_tau = 1. / static_cast<double>(a->temperature);
   t.k2 = k2;
   t.k = a->k;
   t.ids_i64 = a->ids_dtype == PCP_I64;

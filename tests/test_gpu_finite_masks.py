@@ -1,0 +1,132 @@
+"""Finite masks of any size (-1e9 .. a type's lowest value) at several temperatures: top logits,
+distillation and draft verification against their definitions in 64 bits (tests/distill_ref.py,
+which also derives the distillation's bars).
+
+A finite mask differs from -inf in that a lane, a part or a row may hold nothing else: sums are
+then against the mask itself, whose product with log2(e) / temperature is rounded by far more
+than the whole range of an exponential.
+"""
+import numpy as np
+import pytest
+import torch
+
+from distill_ref import lse_ref, top_ref
+from pcp_amd import distill
+from pcp_amd._lib import PcpError
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda:0")
+DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+MASKS = {"f32": [-1e9, -1e10, -1e20, -1e30, "lowest"], "bf16": [-1e9, -1e10, -1e20, -1e30, "lowest"],
+         "f16": [-3e4, "lowest"]}
+CASES = [(d, m) for d in MASKS for m in MASKS[d]]
+TEMPERATURES = [0.7, 1.0, 1.5, 2.0, 3.0, 4.0]
+PATTERNS = ["run", "scattered", "tail", "alone"]
+
+
+def mask_value(dtype, mask):
+    return float(torch.finfo(DT[dtype]).min) if mask == "lowest" else float(torch.tensor(mask).to(DT[dtype]))
+
+
+def to_dev(x, dtype, offset=0):
+    t = torch.from_numpy(np.ascontiguousarray(x, dtype=np.float32)).to(DT[dtype])
+    buf = torch.empty(t.numel() + offset, dtype=t.dtype, device=DEV)
+    v = buf[offset:].view(t.shape)
+    v.copy_(t)
+    return v
+
+
+def host64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def where_masked(rng, pattern, R, V):
+    """[R, V] of booleans: a run through the middle, most of the row, the row's end, all but one token."""
+    m = np.zeros((R, V), bool)
+    if pattern == "run":
+        m[:, V // 5:4 * V // 5] = True
+    elif pattern == "scattered":
+        m[:] = rng.random((R, V)) < 0.97
+        m[:, rng.integers(0, V, 3)] = False
+    elif pattern == "tail":
+        m[:, V - V // 3:] = True
+    else:
+        m[:] = True
+        m[np.arange(R), rng.integers(0, V, R)] = False
+    return m
+
+
+# ---- top logits ------------------------------------------------------------------------
+
+
+def lse_bar(z):
+    """Bar of an f32 log-sum-exp of z = x / temperature [R, V]. A lane adds up to 64 terms in f32
+    (63 roundings of 2^-24), its batches in f64, rounded once; the trees over lanes, waves and
+    parts add 6 + 2 + 6. A term 2^y, y below the largest by |y|, has the roundings of
+    the exponent, of k and of the two of each rescaling: 5 * 2^-24 |y| ln 2; v_exp_f32 once for the
+    term and once for each rescaling (lane, wave, part, the reference's residue), 5 * 2^-23; the
+    batch's product 2^-24, log2f 2^-23. Then half a step of the result."""
+    z = z.astype(np.float64)
+    lse = lse_ref(z)
+    q = np.exp(z - lse[:, None])
+    far = (q * np.minimum(z.max(1)[:, None] - z, 1e4)).sum(1)     # |y| ln 2; q is 0 beyond
+    return 2.0 ** -24 * (63 + 1 + 14 + 10 + 1 + 2 + 5 * far) * 1.01 + 2.0 ** -24 * np.abs(lse)
+
+
+def check_top(x, k, temperature, out):
+    v, i, lse = top_ref(host64(x), k, float(np.float32(temperature)))
+    assert np.array_equal(out.ids.cpu().numpy(), i)
+    assert np.array_equal(host64(out.values), v)
+    off = np.abs(host64(out.lse) - lse)
+    assert (off <= lse_bar(host64(x) / float(np.float32(temperature)))).all(), off.max()
+
+
+@pytest.mark.parametrize("dtype,mask", CASES)
+@pytest.mark.parametrize("pattern", PATTERNS)
+@pytest.mark.parametrize("R,V,k", [(3, 40000, 30), (700, 21000, 5), (2, 300, 7)])
+def test_top_logits(dtype, mask, pattern, R, V, k):
+    rng = np.random.default_rng(V)
+    x = rng.standard_normal((R, V)).astype(np.float32) * 3
+    x[where_masked(rng, pattern, R, V)] = mask_value(dtype, mask)
+    for offset in (0, 3):
+        xd = to_dev(x, dtype, offset)
+        for t in TEMPERATURES:
+            check_top(xd if R < 100 else xd[:4], k, t, distill.top_logits(xd, k, temperature=t) if R < 100 else
+                      first_rows(distill.top_logits(xd, k, temperature=t), 4))
+
+
+def first_rows(out, n):
+    return distill.TopLogits(out.values[:n], out.ids[:n], out.lse[:n])
+
+
+@pytest.mark.parametrize("dtype,mask", CASES)
+@pytest.mark.parametrize("R,V", [(2, 40000), (600, 20000)])
+def test_top_logits_of_rows_with_nothing_else(dtype, mask, R, V):
+    """Every logit the mask: a uniform distribution, whose log-sum-exp is reported only where it
+    leaves f32's range."""
+    low = mask_value(dtype, mask)
+    x = torch.full((R, V), low, dtype=DT[dtype], device=DEV)
+    for t in TEMPERATURES:
+        if low / t < -float(torch.finfo(torch.float32).max):
+            with pytest.raises(PcpError):
+                distill.top_logits(x, 9, temperature=t)
+            continue
+        out = distill.top_logits(x, 9, temperature=t)
+        assert torch.equal(out.ids.cpu(), torch.arange(9, dtype=torch.int32).expand(R, 9))
+        assert bool((out.values == low).all())
+        want = low / float(np.float32(t)) + np.log(V)
+        assert (np.abs(host64(out.lse) - want) <= 2.0 ** -23 * abs(want)).all()
+
+
+@pytest.mark.parametrize("dtype,R,V", [("bf16", 2, 151936), ("f32", 5, 50257), ("f16", 600, 32000), ("bf16", 520, 1 << 24)])
+def test_log_sum_exp_to_its_rounding(dtype, R, V):
+    """Ordinary rows, up to the largest vocabulary in one workgroup, to the bar that the sums
+    leave (the rest of the probability, 1 - sum p, is taken from this number)."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.empty((R, V), dtype=DT[dtype], device=DEV).normal_(0, 3, generator=g)
+    for t in (1.0, 0.6):
+        out = distill.top_logits(x, 4, temperature=t)
+        for r in (0, R // 2, R - 1):
+            z = (x[r].double() / float(np.float32(t)))[None].cpu().numpy()
+            assert abs(float(out.lse[r]) - lse_ref(z)[0]) <= lse_bar(z)[0]
