@@ -77,7 +77,7 @@ typedef enum pcp_divergence {
  *   with teacher_lse:  p_i = exp(t_i / tau - lse), and the other tokens form one class of
  *     probabilities  p_T = max(1 - sum p_i, PCP_DISTILL_TAIL_FLOOR),  q_T = sum_{v not in K} q_v
  *     (no such class where q_T is below 2^-126: every logit outside K masked, by -Inf or by
- *     a type's lowest value, or K holding every token);
+ *     a finite value far below the others, or K holding every token);
  *   without:           p = softmax(t / tau) over K, no such class.
  *   forward:  l = sum_i p_i log(p_i / q_i) + p_T log(p_T / q_T)
  *   reverse:  l = sum_i q_i log(q_i / p_i) + q_T log(q_T / p_T)

@@ -4,12 +4,12 @@
 // With x a row's logits, k2 = log2(e) / tau, K the used teacher ids and T the rest of the
 // vocabulary, the rows' sums are kept apart: (m_T, s_T) over T while the row streams past
 // (the entries' own elements are replaced by -inf where they sit in registers), and s_K from
-// the k gathered logits. The tail's mass Q_T = s_T 2^(m_T - lse) is then a sum of its own and
-// keeps its relative precision where the teacher's entries hold nearly everything (1 - sum q_i
-// would lose it all). Per element the arithmetic is f32; what a row has once (s_K, the merge of
+// the k gathered logits. Maxima are logits and sums relative to them (see term_scale). The tail's
+// mass Q_T = s_T 2^((m_T - R) k2) / s is then a sum of its own and keeps its relative precision
+// where the teacher's entries hold nearly everything (1 - sum q_i would lose it all). Per element the arithmetic is f32; what a row has once (s_K, the merge of
 // its waves' sums, log-sum-exp, the divergence) f64, since the divergence may be far below its
-// terms. Outside K the gradient is one factor of 2^(x k2 - m_T):
-//   forward:  c (P 2^(m_T - lse) - p_T / s_T),   reverse:  c 2^(m_T - lse) (log(Q_T/p_T) - l),
+// terms. Outside K the gradient is one factor of 2^((x - m_T) k2):
+//   forward:  c (P Q_T - p_T) / s_T,   reverse:  c (Q_T / s_T) (log(Q_T/p_T) - l),
 // with c = weight m / (loss_norm L tau) and P = sum p_i + p_T; on K each entry has its own
 // value, which takes the element's place before its vector is stored.
 #pragma once
@@ -34,21 +34,26 @@ constexpr int kWave = 64;
 // (k <= 64) and for 4.
 constexpr int kMaxSlots = kMaxEntries / kWave;
 
-// What the preparation makes of a row. The student's sums are relative to its largest logit at
-// an entry, zref; the kernels form theirs at f32's k2 and references, and adj takes those to zref:
-// 2^(mk - zref k2), which the rounding of mk = zref k2 keeps near 1.
+// What the preparation makes of a row. zref is the student's largest logit at an entry (0 and sk 0
+// where all are -inf); the row kernel takes its first sums against it.
 struct TeacherRow {
   double sum_p;     // of the entries
   double log_pt;    // of the tail's class, if there is one
-  double lse;       // the entries' probabilities are exp(t / tau - lse)
+  double lse;       // the entries' probabilities are exp((t - tref) / tau - lse) (see log_base)
   double sk;        // sum exp((z - zref) / tau) over the entries
-  double adj;
+  double adj;       // term_adj of zref and at, in 64 bits
   float pt;
-  float zref, mk;   // (zref 0 and mk -inf where every entry is masked)
+  float zref;
+  TermScale at;     // term_scale of zref
+  float tref;
   float w;          // the row's weight
   int32_t state;    // kUnused, kUsed; kBad: an id out of range
   int32_t pad;
 };
+// What log-probabilities of a row with largest logit m are taken relative to: 0, where (x - 0) / tau and
+// a log-sum-exp in 64 bits lose nothing; else m, since a row of huge logits (each -1e30, say) has
+// its log-probabilities in the last bits of neither.
+__device__ __forceinline__ float log_base(float m) { return fabsf(m) < 0x1p16f ? 0.f : m; }
 constexpr int kUnused = 0, kUsed = 1, kBad = 2;
 constexpr int kRowWords = sizeof(TeacherRow) / 4;
 constexpr double kLn2F64 = 0.69314718055994530942;
@@ -63,7 +68,7 @@ struct DistillArgs {
   float* seq_scale;         // [n_seq]: weight / (loss_norm * seq_len), by the preparation
   void* dlogits;
   float* token_loss;
-  float4* part;             // [nrows, parts]: (m_T, s_T, an id is used twice, -)
+  PartSum* part;            // [nrows, parts]: m_T, s_T, n: an id is used twice
   TeacherRow* teacher;      // [nrows], by the preparation, and per entry, [nrows, k]:
   int* entry_ids;           // used_id,
   double* entry_w;          // forward: its probability; reverse: exp((z - zref) / tau),
@@ -248,8 +253,8 @@ __device__ __forceinline__ void prepare_row(const DistillArgs& a, int64_t row) {
   TeacherRow o;
   o.sum_p = o.log_pt = o.lse = o.sk = 0.;
   o.adj = 1.;
-  o.pt = o.zref = 0.f;
-  o.mk = kNegInf;
+  o.pt = o.zref = o.tref = 0.f;
+  o.at = TermScale{a.k2, 0.f};
   o.w = distill_row(a, row).w;
   o.state = kUnused;
   o.pad = 0;
@@ -272,17 +277,17 @@ __device__ __forceinline__ void prepare_row(const DistillArgs& a, int64_t row) {
     if (a.tlse) {
       o.lse = static_cast<double>(a.tlse[row]);
     } else {
-      const double m = static_cast<double>(ms_ref(lanes_max<64>(tmax))) * a.inv_tau;
+      const float m = ms_ref(lanes_max<64>(tmax));
       double sum = 0.;
 #pragma unroll
       for (int s = 0; s < kMaxSlots; ++s)
-        if (id[s] >= 0) sum += exp(static_cast<double>(t[s]) * a.inv_tau - m);
-      o.lse = m + log(wave_sum64(sum));
+        if (id[s] >= 0) sum += exp((static_cast<double>(t[s]) - m) * a.inv_tau);
+      o.tref = log_base(m);
+      o.lse = static_cast<double>(m - o.tref) * a.inv_tau + log(wave_sum64(sum));
     }
-    zmax = lanes_max<64>(zmax);
-    o.mk = zmax * a.k2;
-    o.zref = o.mk == kNegInf ? 0.f : zmax;   // (-inf too where zmax is a type's lowest value)
-    o.adj = exp((static_cast<double>(ms_ref(o.mk)) - static_cast<double>(o.zref) * a.k2) * kLn2F64);
+    o.zref = ms_ref(lanes_max<64>(zmax));
+    o.at = term_scale(o.zref, a.k2);
+    o.adj = exp(-term_residue(o.zref, o.at) * kLn2F64);
     double sum_p = 0., sk = 0.;
 #pragma unroll
     for (int s = 0; s < kMaxSlots; ++s) {
@@ -290,7 +295,7 @@ __device__ __forceinline__ void prepare_row(const DistillArgs& a, int64_t row) {
       if (i >= a.k) continue;
       double p = 0., e = 0.;
       if (id[s] >= 0) {
-        p = exp(static_cast<double>(t[s]) * a.inv_tau - o.lse);
+        p = exp((static_cast<double>(t[s]) - o.tref) * a.inv_tau - o.lse);
         e = exp((static_cast<double>(z[s]) - o.zref) * a.inv_tau);
       }
       sum_p += p;
@@ -346,9 +351,10 @@ struct Teacher {
   }
 };
 
-// What a row's gradient needs: tail * 2^(x k2 - ref) outside K, g[] at the entries.
+// What a row's gradient needs: tail * 2^(x at.k - at.ref) outside K, g[] at the entries.
 struct RowTerms {
-  float tail, ref;
+  float tail;
+  TermScale at;
   float g[kMaxEntries];
 };
 
@@ -391,13 +397,15 @@ __device__ __forceinline__ int groups_of(const DistillArgs& a) { return (a.k + k
 
 // A row's factors, the same in every lane of any wave that forms them.
 struct RowFactors {
-  float tail, ref;      // the gradient outside K: tail * 2^(x k2 - ref)
-  float c, rm, inv_s;   // the coefficient; q_i = 2^(z k2 - rm) inv_s
+  float tail;           // the gradient outside K: tail * 2^(x at.k - at.ref)
+  TermScale at;
+  float c, r, inv_s;    // the coefficient; q_i = 2^((z - r) k2) inv_s
   float big_p, lf;      // forward: P; reverse: l
-  float ek;             // 2^(mk - rm)
-  double s;             // the whole row's sum over 2^(rm - mk) exp(zref / tau)
+  float ek;             // 2^((zref - r) k2)
+  double s;             // the whole row's sum over exp(r / tau)
   double qt, log_qt;    // the tail's mass; 0: no tail
-  double lse;           // of the student's row; with log_qt only after set_logs
+  double lse;           // log q_i = (z - zbase) / tau - lse; these and log_qt only after set_logs
+  float zbase;
 };
 
 // log(s) to 1e-12, by atanh's series. Its constants are set where they are used: over the row
@@ -423,12 +431,18 @@ __device__ __forceinline__ double log64(double s) {
   return fma(2. * t, p, k * ln2);
 }
 
+// A value that is the same in every lane, in a scalar register (two vector registers fewer where the
+// widest rows leave none).
+__device__ __forceinline__ float first_lane(float v) {
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v)));
+}
 __device__ __forceinline__ float entry_prob(const DistillArgs& a, const Teacher& te, const RowFactors& f, int i) {
-  return hw_exp2(fmaf(te.z[i], a.k2, -f.rm)) * f.inv_s;
+  return hw_exp2((te.z[i] - f.r) * a.k2) * f.inv_s;
 }
 // log(p_i / q_i)
 __device__ __forceinline__ double entry_gap(const DistillArgs& a, const Teacher& te, const RowFactors& f, int i) {
-  return (static_cast<double>(te.t[i]) - te.z[i]) * a.inv_tau - (te.row.lse - f.lse);
+  return (static_cast<double>(te.t[i] - first_lane(te.row.tref)) - (te.z[i] - first_lane(f.zbase))) * a.inv_tau -
+         (te.row.lse - f.lse);
 }
 // The gradient at entry i.
 __device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher& te, const RowFactors& f, int i) {
@@ -437,9 +451,9 @@ __device__ __forceinline__ float entry_grad(const DistillArgs& a, const Teacher&
   return q > 0.f ? -f.c * q * (static_cast<float>(entry_gap(a, te, f, i)) + f.lf) : 0.f;
 }
 
-__device__ __forceinline__ void set_logs(const DistillArgs& a, const Teacher& te, RowFactors& f) {
-  f.lse = static_cast<double>(te.row.zref) * a.inv_tau + static_cast<double>(f.rm - ms_ref(te.row.mk)) * kLn2F64 +
-          log64(f.s);
+__device__ __forceinline__ void set_logs(const DistillArgs& a, RowFactors& f) {
+  f.zbase = log_base(f.r);
+  f.lse = static_cast<double>(f.r - f.zbase) * a.inv_tau + log64(f.s);
   f.log_qt = f.qt > 0. ? log64(f.qt) : 0.;
 }
 
@@ -463,35 +477,37 @@ __device__ __forceinline__ double row_loss(const DistillArgs& a, const Teacher& 
   return l;
 }
 
-// mt, st: the state outside K. The forward gradient does without the loss, the reverse one holds it
-// (loss: l, formed here if reverse).
+// st: the sum outside K, relative to mt, its largest logit or the row's zref. The forward gradient does
+// without the loss, the reverse one holds it (loss: l, formed here if reverse).
 // weight: the row's scale times its weight.
 __device__ __forceinline__ RowFactors row_factors(const DistillArgs& a, float weight, const Teacher& te, float mt,
                                                   double st, double& loss) {
   RowFactors f;
-  f.rm = ms_ref(fmaxf(mt, te.row.mk));
-  f.ek = te.row.sk == 0. ? 0.f : hw_exp2(te.row.mk - f.rm);
-  const double ft = st == 0. ? 0. : hw_exp2(mt - f.rm) * te.row.adj;
+  f.r = ms_ref(te.row.sk == 0. ? mt : fmaxf(mt, te.row.zref));
+  f.ek = te.row.sk == 0. ? 0.f : hw_exp2((te.row.zref - f.r) * a.k2);
+  const double ft = st == 0. ? 0. : hw_exp2((mt - f.r) * a.k2);
   f.s = te.row.sk * f.ek + st * ft;
   const double inv = 1. / f.s;
-  f.inv_s = static_cast<float>(te.row.adj * inv);
+  f.inv_s = static_cast<float>(inv);
   f.qt = st * ft * inv;
   f.qt = a.tlse != nullptr && f.qt >= 0x1p-126 ? f.qt : 0.;
   f.c = static_cast<float>(static_cast<double>(weight) * a.inv_tau);
-  f.ref = ms_ref(mt);
   f.big_p = f.lf = 0.f;
   f.lse = f.log_qt = 0.;
+  f.zbase = 0.f;
   if (a.forward) {
     const double pt = f.qt > 0. ? te.row.pt : 0.;
     f.big_p = static_cast<float>(te.row.sum_p + pt);
     f.tail = st == 0. ? 0.f : f.c * static_cast<float>((te.row.sum_p + pt) * (ft * inv) - pt / st);
   } else {
-    set_logs(a, te, f);
+    set_logs(a, f);
     loss = row_loss(a, te, f);
     f.lf = static_cast<float>(loss);
     const double gap = f.qt > 0. ? te.row.log_pt - f.log_qt : 0.;
     f.tail = st == 0. ? 0.f : -f.c * static_cast<float>(ft * inv * (gap + loss));
   }
+  f.at = term_scale(mt, a.k2);
+  f.tail *= term_adj(mt, f.at);
   return f;
 }
 
@@ -533,12 +549,12 @@ constexpr int kPartU = 8;
 template <typename TI, int NS>
 __global__ void __launch_bounds__(kPartBlock) distill_part_kernel(DistillArgs a, int n) {
   constexpr int EPV = 16 / TI::kBytes, U = kPartU, BLOCK = kPartBlock;
-  __shared__ __align__(16) float lds[4 * (BLOCK / 64)];
+  __shared__ float2 lds[BLOCK / 64];
   __shared__ int any_twice;
   const int tid = threadIdx.x, part = blockIdx.x;
   static_assert(kPartBlock == kPrepBlock, "the preparation's workgroup");
   if (blockIdx.y >= static_cast<unsigned>(n)) {   // past the rows: the preparation
-    if (part == 0) prepare<TI>(a, blockIdx.y - n, lds);
+    if (part == 0) prepare<TI>(a, blockIdx.y - n, &lds[0].x);
     return;
   }
   const int64_t row = a.row0 + blockIdx.y;
@@ -572,20 +588,20 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_kernel(DistillArgs a,
 #pragma unroll
   for (int q = 0; q < U; ++q)
     if (v0 + q * BLOCK + tid < end) bx = vec_max<TI>(bx, x[q]);
-  float m = bx * a.k2, s = 0.f, m0 = kNegInf, s0 = 0.f;
-  const float ref = ms_ref(m);
-  s = hw_exp2(fmaf(xe, a.k2, -ref));
+  const TermScale ts = term_scale(bx, a.k2);
+  float s = hw_exp2(fmaf(xe, ts.k, -ts.ref));
 #pragma unroll
   for (int q = 0; q < U; ++q)
     if (v0 + q * BLOCK + tid < end) {
       const uint32_t* w = reinterpret_cast<const uint32_t*>(&x[q]);
 #pragma unroll
-      for (int j = 0; j < EPV; ++j) s += hw_exp2(fmaf(TI::unpack(w, j), a.k2, -ref));
+      for (int j = 0; j < EPV; ++j) s += hw_exp2(fmaf(TI::unpack(w, j), ts.k, -ts.ref));
     }
+  s *= term_adj(bx, ts);
   __syncthreads();
   if (twice && (tid & 63) == 0) any_twice = 1;
-  block_merge2<BLOCK>(m, s, m0, s0, lds);
-  if (tid == 0) a.part[row * a.parts + part] = make_float4(m, s, any_twice ? 1.f : 0.f, 0.f);
+  block_merge_at<BLOCK>(bx, s, a.k2, lds);
+  if (tid == 0) a.part[row * a.parts + part] = PartSum{bx, s, any_twice, 0};
 }
 
 // The row's state outside K from its parts, and whether an id is used twice.
@@ -595,13 +611,13 @@ __device__ __forceinline__ void merge_tail(const DistillArgs& a, int64_t row, fl
   s = 0.f;
   bool t = false;
   for (int p = lane; p < a.parts; p += 64) {
-    const float4 v = a.part[row * a.parts + p];
-    const float M = fmaxf(m, v.x);
-    s = ms_rescale(s, m, M) + ms_rescale(v.y, v.x, M);
+    const PartSum v = a.part[row * a.parts + p];
+    const float M = fmaxf(m, v.mx);
+    s = rescale_at(s, m, M, a.k2) + rescale_at(v.s, v.mx, M, a.k2);
     m = M;
-    t |= v.z != 0.f;
+    t |= v.n != 0;
   }
-  lanes_merge<64>(m, s);
+  lanes_merge_at<64>(m, s, a.k2);
   twice = __any(t);
 }
 
@@ -664,10 +680,10 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
           terms.g[i] = te.id[i] >= 0 ? entry_grad(a, te, f, i) : 0.f;
         }
         terms.tail = f.tail;
-        terms.ref = f.ref;
+        terms.at = f.at;
         if (part == 0) {
           if (a.forward) {
-            set_logs(a, te, f);
+            set_logs(a, f);
             l = row_loss(a, te, f);
           }
           token = r.w * static_cast<float>(l);
@@ -680,7 +696,8 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
   } else if (part == 0 && tid == 0 && r.tok) {
     store_coherent(a.token_loss + r.tix, 0.f);
   }
-  float g[NS], tail = 0.f, ref = 0.f;
+  float g[NS], tail = 0.f;
+  TermScale ts{0.f, 0.f};
   int place[NS], edge[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
@@ -690,7 +707,7 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
   if (live) {
     if constexpr (GRAD) {
       tail = terms.tail;
-      ref = terms.ref;
+      ts = terms.at;
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         const int id = kWave * s < a.k ? te.id[(tid & 63) + kWave * s] : -1;
@@ -708,7 +725,7 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
       if (live) {
         const uint32_t* w = reinterpret_cast<const uint32_t*>(&x[q]);
 #pragma unroll
-        for (int j = 0; j < EPV; ++j) o[j] = tail * hw_exp2(fmaf(TI::unpack(w, j), a.k2, -ref));
+        for (int j = 0; j < EPV; ++j) o[j] = tail * hw_exp2(fmaf(TI::unpack(w, j), ts.k, -ts.ref));
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
           uint64_t at = __ballot(place[s] >= 0 && (place[s] >> 16) == q);
@@ -743,7 +760,7 @@ __global__ void __launch_bounds__(kPartBlock) distill_part_grad_kernel(DistillAr
       }
     }
     if (part == 0 && tid < 64) {
-      float o = live && ek >= 0 ? tail * hw_exp2(fmaf(xe, a.k2, -ref)) : 0.f;
+      float o = live && ek >= 0 ? tail * hw_exp2(fmaf(xe, ts.k, -ts.ref)) : 0.f;
       if (live) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -869,8 +886,9 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
       in = __ballot(place >= 0 && (place >> 16) == k);
     }
   };
-  // Adds chunk k's terms outside the entries to s, against ref; the entries' elements become -inf.
-  auto sum_chunk = [&](u32x4& x, const Teacher& te, const RowSpan& sp, const Owned& o, int k, float ref, float& s) {
+  // Adds chunk k's terms outside the entries to s, at ts; the entries' elements become -inf.
+  auto sum_chunk = [&](u32x4& x, const Teacher& te, const RowSpan& sp, const Owned& o, int k, const TermScale& ts,
+                       float& s) {
     each_in_chunk(te, sp, o, k, [&](int p, int, int) { mask_element<TI>(x, ((p >> 4) & 63) == lane, p & 15); });
     uint32_t u[4];
 #pragma unroll
@@ -883,11 +901,11 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
       for (int q = 0; q < 2; ++q)
         if (held(sp.nv, k, q)) {
 #pragma unroll
-          for (int j = 4 * q; j < 4 * q + 4; ++j) s += hw_exp2(fmaf(TI::unpack(u, j), a.k2, -ref));
+          for (int j = 4 * q; j < 4 * q + 4; ++j) s += hw_exp2(fmaf(TI::unpack(u, j), ts.k, -ts.ref));
         }
     } else if (held(sp.nv, k, 0)) {
 #pragma unroll
-      for (int j = 0; j < EPV; ++j) s += hw_exp2(fmaf(TI::unpack(u, j), a.k2, -ref));
+      for (int j = 0; j < EPV; ++j) s += hw_exp2(fmaf(TI::unpack(u, j), ts.k, -ts.ref));
     }
     asm volatile("" : "+v"(s));   // here, not after the last chunk's entries
   };
@@ -924,7 +942,7 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
   auto scale_of = [&](int64_t i) { return a.seq_scale[static_cast<uint32_t>(i) / static_cast<uint32_t>(a.logit_stride)]; };
   auto pay = [&](const Teacher& te, int64_t owed) {    // by wave NW - 1: token `owed`'s loss
     RowFactors f = factors[wave];
-    set_logs(a, te, f);
+    set_logs(a, f);
     const float l = static_cast<float>(row_loss(a, te, f));
     if (lane == 0) store_coherent(a.token_loss + owed, te.row.w * l);
   };
@@ -961,25 +979,26 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     int claimed = 0;
     if (!kStatic && tid == 0 && a.nrows > 2 * grid) claimed = atomicAdd(a.next_row, 1);
     Owned mine{-1, 0, 0u};                             // this wave's entries
-    float g = 0.f, tail = 0.f, gref = 0.f;             // the gradient at this lane's entry; elsewhere
+    float g = 0.f, tail = 0.f;                         // the gradient at this lane's entry; elsewhere
+    TermScale gs{0.f, 0.f};
     double loss = 0.;
     bool live = false;
     if (weight != 0.f) {
       mine = own(te, sp);
       bool twice = used_twice(te, mine.n);
-      const float ref = uniform(ms_ref(te.row.mk));
+      const TermScale ts{uniform(te.row.at.k), uniform(te.row.at.ref)};
       float s = 0.f;
 #pragma unroll
       for (int k = 0; k < NCH; ++k) {
         __builtin_amdgcn_sched_barrier(0);
-        sum_chunk(xv[k], te, sp, mine, k, ref, s);
+        sum_chunk(xv[k], te, sp, mine, k, ts, s);
       }
       __builtin_amdgcn_sched_barrier(0);
       if (wave == 0) {
         if (ek >= 0) xe = TI::load1(row_of(row), ek);
         float x1 = xe;
         twice |= mask_row_edges(te, sp, x1);
-        s += hw_exp2(fmaf(x1, a.k2, -ref));
+        s += hw_exp2(fmaf(x1, ts.k, -ts.ref));
       }
       // The workgroup's sum, in a fixed order.
       s = lanes_sum<64>(s);
@@ -993,11 +1012,12 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     if (weight != 0.f) {
       __syncthreads();
       const float2 w = merge[lane & (NW - 1)];
-      float m = uniform(ms_ref(te.row.mk));
-      double st = wave_sum64(lane < NW ? static_cast<double>(w.x) : 0.);
+      float m = uniform(te.row.zref);
+      const double first = wave_sum64(lane < NW ? static_cast<double>(w.x) : 0.);
+      double st = first * te.row.adj;
       const bool any_twice = __any(w.y != 0.f);
       live = te.row.state == kUsed && !any_twice;
-      if (live && !(st > 0x1p-60 && st < 0x1p60)) {
+      if (live && !(first > 0x1p-60 && first < 0x1p60)) {
         // Too far from the entries: elements next to the tail's largest could leave f32's range. The
         // true maximum (the entries' elements are -inf by now), then the sum.
         float x1 = kNegInf;
@@ -1011,9 +1031,8 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
 #pragma unroll
           for (int j = 0; j < EPV; ++j)
             if (held(sp.nv, k, kSplit ? j / 4 : 0)) mx = fmaxf(mx, TI::unpack(reinterpret_cast<const uint32_t*>(&xv[k]), j));
-        float mm = mx * a.k2;
-        const float mref = ms_ref(mm);
-        float ss = hw_exp2(fmaf(x1, a.k2, -mref));
+        const TermScale own_ts = term_scale(mx, a.k2);
+        float ss = hw_exp2(fmaf(x1, own_ts.k, -own_ts.ref));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int k = 0; k < NCH; ++k) {
@@ -1025,25 +1044,26 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
           }
 #pragma unroll
           for (int j = 0; j < EPV; ++j)
-            if (held(sp.nv, k, kSplit ? j / 4 : 0)) ss += hw_exp2(fmaf(TI::unpack(u, j), a.k2, -mref));
+            if (held(sp.nv, k, kSplit ? j / 4 : 0)) ss += hw_exp2(fmaf(TI::unpack(u, j), own_ts.k, -own_ts.ref));
           asm volatile("" : "+v"(ss));
         }
         __builtin_amdgcn_sched_barrier(0);
-        lanes_merge<64>(mm, ss);
+        ss *= term_adj(mx, own_ts);
+        lanes_merge_at<64>(mx, ss, a.k2);
         __syncthreads();   // every wave has read the first sums
-        if (lane == 0) merge[wave] = make_float2(mm, ss);
+        if (lane == 0) merge[wave] = make_float2(mx, ss);
         __syncthreads();
         const float2 v = merge[lane & (NW - 1)];
         m = v.x;
         float st1 = v.y;
-        lanes_merge<NW>(m, st1);
+        lanes_merge_at<NW>(m, st1, a.k2);
         st = st1;
       }
       if (live) {
         const RowFactors f = row_factors(a, scale * weight, te, m, st, loss);
         if (lane == 0) factors[wave] = f;
         tail = uniform(f.tail);
-        gref = uniform(f.ref);
+        gs = TermScale{uniform(f.at.k), uniform(f.at.ref)};
         if (mine.place >= 0) g = entry_grad(a, te, f, list[wave][lane]);
       } else if (tid == 0 && any_twice && te.row.state == kUsed) {
         raise_error(a.err, kErrTeacherTwice);
@@ -1062,7 +1082,7 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
         }
         float out[EPV];
 #pragma unroll
-        for (int j = 0; j < EPV; ++j) out[j] = tail * hw_exp2(fmaf(TI::unpack(u, j), a.k2, -gref));
+        for (int j = 0; j < EPV; ++j) out[j] = tail * hw_exp2(fmaf(TI::unpack(u, j), gs.k, -gs.ref));
         each_in_chunk(te, sp, mine, k, [&](int p, int src, int w) {
           const float ge = w == 0 ? read_lane(g, src) : entry_grad(a, te, factors[wave], list[wave][kWave * w + src]);
           const bool here = ((p >> 4) & 63) == lane;
@@ -1094,7 +1114,7 @@ __global__ void __launch_bounds__(BLOCK, 4) distill_row_kernel(DistillArgs a) {
     }
     if (wave == 0) {
       if (ek >= 0) {
-        float oe = live ? tail * hw_exp2(fmaf(xe, a.k2, -gref)) : 0.f;
+        float oe = live ? tail * hw_exp2(fmaf(xe, gs.k, -gs.ref)) : 0.f;
         if (live)
           for (int e = 0; e < a.k; ++e)
             if (te.id[e] == ek) oe = entry_grad(a, te, factors[0], e);

@@ -120,7 +120,7 @@ int distill(pcp_ctx* ctx, const pcp_distill_args* a) {
   // entries' ids, logits, weights | parts.
   const size_t sv = round256(sizeof(float) * static_cast<size_t>(a->n_seq));
   const size_t tl = a->token_loss ? 0 : round256(sizeof(float) * static_cast<size_t>(a->n_seq * tstride));
-  const size_t pb = round256(sizeof(float4) * static_cast<size_t>(nrows) * static_cast<size_t>(parts));
+  const size_t pb = round256(sizeof(PartSum) * static_cast<size_t>(nrows) * static_cast<size_t>(parts));
   const size_t tb = round256(sizeof(TeacherRow) * static_cast<size_t>(nrows));
   const size_t eb = round256(sizeof(float) * static_cast<size_t>(nrows) * static_cast<size_t>(a->k));
   const int rc = ensure_scratch_on(ctx, 3 * sv + 512 + tl + tb + 4 * eb + pb, st);
@@ -155,7 +155,7 @@ int distill(pcp_ctx* ctx, const pcp_distill_args* a) {
   d.entry_ids = reinterpret_cast<int*>(work + tb);
   d.entry_z = reinterpret_cast<float*>(work + tb + eb);
   d.entry_w = reinterpret_cast<double*>(work + tb + 2 * eb);
-  d.part = reinterpret_cast<float4*>(work + tb + 4 * eb);
+  d.part = reinterpret_cast<PartSum*>(work + tb + 4 * eb);
   d.err = ctx->d_page->err;
   d.next_row = s_next;
   d.nrows = nrows;

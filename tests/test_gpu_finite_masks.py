@@ -10,8 +10,8 @@ import numpy as np
 import pytest
 import torch
 
-from distill_ref import lse_ref, top_ref
-from pcp_amd import distill
+from distill_ref import IGNORE, REL, half_step, lse_ref, row_ref, top_ref
+from pcp_amd import distill, grpo
 from pcp_amd._lib import PcpError
 
 pytestmark = pytest.mark.gpu
@@ -130,3 +130,90 @@ def test_log_sum_exp_to_its_rounding(dtype, R, V):
         for r in (0, R // 2, R - 1):
             z = (x[r].double() / float(np.float32(t)))[None].cpu().numpy()
             assert abs(float(out.lse[r]) - lse_ref(z)[0]) <= lse_bar(z)[0]
+
+
+# ---- distillation ----------------------------------------------------------------------
+
+
+def masked_rows(rng, V, k, low, huge_teacher):
+    """Student rows [8, V] with teacher ids and logits [8, k]: a masked run outside the entries; nothing
+    else outside them; all entries masked; all but one; the whole row; the entries and most of the
+    rest; all but one entry; an ordinary row (or one whose teacher has the mask at every entry)."""
+    R = 8
+    x = rng.standard_normal((R, V)).astype(np.float32) * 3
+    ids = np.stack([rng.choice(V, k, replace=False) for _ in range(R)]).astype(np.int32)
+    t = (np.take_along_axis(x, ids, 1) + rng.standard_normal((R, k))).astype(np.float32)
+    lse = np.zeros(R, np.float32)
+    for r in range(R):
+        lse[r] = lse_ref(t[r].astype(np.float64)[None])[0] + rng.random() * 0.2
+    outside = np.ones((R, V), bool)
+    np.put_along_axis(outside, ids, False, 1)
+    run = np.zeros(V, bool)
+    run[V // 5:4 * V // 5] = True
+    x[0, outside[0] & run] = low
+    x[1, outside[1]] = low
+    x[2, ids[2]] = low
+    x[3, ids[3, 1:]] = low
+    x[3, outside[3] & run] = low
+    x[4] = low
+    x[5, ids[5]] = low
+    x[5, outside[5] & (rng.random(V) < 0.99)] = low
+    x[5, np.flatnonzero(outside[5])[:2]] = 1.0
+    x[6] = low
+    x[6, ids[6, 0]] = 0.5
+    if huge_teacher:
+        t[7] = low
+    return x, ids, t, lse
+
+
+@pytest.mark.parametrize("dtype,mask", CASES)
+@pytest.mark.parametrize("mode", ["forward", "renormalised", "reverse"])
+@pytest.mark.parametrize("N,V", [(8, 701), (8, 40000), (900, 40000)])
+def test_distill(dtype, mask, mode, N, V):
+    """Rows in parts and rows kept by a workgroup, against the definition of each row shifted by
+    its largest logit (in 64 bits -1e30 + log q would lose the second)."""
+    rng = np.random.default_rng(V + N)
+    k = 20
+    x, ids, t, lse = masked_rows(rng, V, k, mask_value(dtype, mask), mode == "renormalised")
+    xs = torch.zeros((1, N, V), dtype=DT[dtype], device=DEV)
+    xs[0, -8:] = to_dev(x, dtype)
+
+    def all_rows(a, fill):
+        out = torch.full((1, N) + a.shape[1:], fill, dtype=torch.from_numpy(a).dtype)
+        out[0, -8:] = torch.from_numpy(a)
+        return out.to(DEV)
+
+    weight = torch.zeros((1, N), device=DEV)
+    weight[0, -8:] = 1.0
+    args = (all_rows(ids, IGNORE), all_rows(t, 0.0), None if mode == "renormalised" else all_rows(lse, 0.0), weight)
+    kw = dict(divergence="reverse" if mode == "reverse" else "forward", sync=False)
+    x64 = host64(xs[0, -8:])
+    ctx = grpo.Context(0)
+    for tau in (0.7, 1.0, 1.5, 2.0, 4.0):
+        out = distill.distill_fwd_bwd(xs, *args, temperature=tau, ctx=ctx, **kw)
+        alone = distill.distill_fwd_bwd(xs, *args, temperature=tau, ctx=ctx, want_dlogits=False, **kw)
+        wide = None
+        if dtype != "f32":
+            wide = distill.distill_fwd_bwd(xs, *args, temperature=tau, ctx=ctx, dlogits_dtype=torch.float32, **kw)
+        ctx.sync()
+        tau64 = float(np.float32(tau))
+        for r in range(8):
+            t64 = t[r].astype(np.float64)
+            l, grad, mag, lb = row_ref(x64[r] - x64[r].max(), ids[r], t64 - t64.max() if mode == "renormalised" else t64,
+                                       None if mode == "renormalised" else float(lse[r]), tau64, mode != "reverse")
+            for o in (out, alone):
+                got = float(o.token_loss[0, N - 8 + r])
+                if abs(l) < 3.3e38:
+                    assert abs(got - l) <= lb + 2.0 ** -24 * abs(l), (tau, r, got, l)
+                else:
+                    assert not np.isnan(got) and got > 3e38
+            c = 1.0 / (8 * tau64)
+            bar = c * REL * mag
+            flushed = 2.0 ** -42 * np.abs(c * grad).max() + 2.0 ** -126
+            for o, kind in ((out, dtype), (wide, "f32")):
+                if o is None:
+                    continue
+                off = np.abs(host64(o.dlogits[0, N - 8 + r]) - c * grad)
+                worst = off - bar - half_step(kind, c * grad) - 2.0 ** -8 * bar - flushed
+                assert worst.max() <= 0, (tau, r, kind, worst.argmax(), off[worst.argmax()])
+        assert not out.dlogits[0, :-8].any()
