@@ -21,6 +21,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
@@ -58,8 +59,8 @@ constexpr int kAccepted = 1, kInRange = 2, kBadP = 4, kBadQ = 8;
 // Where a sequence ends: the row its last token comes from.
 struct SeqEnd {
   double scale_p, scale_q;   // 1 / sum e of the target row, of the draft row (0: q is 0)
-  double max_p, max_q;
-  double lse_p;              // natural units, of logits / temperature
+  float max_p, max_q;
+  double log_p;              // log of the target row's sum e
   int32_t j;                 // accepted tokens
   int32_t without;           // a lookup's refused token (r is 0 there), or -1
 };
@@ -82,6 +83,7 @@ struct VerifyArgs {
   int64_t vocab, tstride, dstride;   // elements
   double k;                   // log2(e) / temperature
   double inv_t;
+  float plain;                // see scale64
   int32_t n;
   int32_t parts, end_parts;   // of kPartVecs, end_vecs vectors
   int32_t greedy;
@@ -141,6 +143,26 @@ struct Exp2 {
   __device__ __forceinline__ double value() const { return __builtin_amdgcn_ldexp(head * poly, n >> 7); }
 };
 static_assert(kTable == 1 << 7, "");
+
+// Terms 2^((x - max) k) of Exp2 as 2^(fma(x, k', -ref) / 128), one instruction. Up to |max| =
+// a.plain ref is the rounded product with k' = 128 k, below 2^42 and so off by at most 2^-12 (a row
+// all at a mask such as -1e30 would otherwise have a product off by 2^50, and anything for a term);
+// adj() takes its rounding out of a sum. From there on two f32 logits that differ at all lie 2^2048
+// apart: k' is the power of two that takes max to [2^42, 2^43), and the product exact.
+struct Scale64 {
+  double k, ref;
+};
+__device__ __forceinline__ Scale64 scale64(const VerifyArgs& a, float max) {
+  const float m = ms_ref(max);
+  Scale64 t{a.k * kTable, 0.};
+  if (!(fabsf(m) < a.plain))   // also +inf
+    t.k = __builtin_amdgcn_ldexp(1., 43 - __builtin_amdgcn_frexp_expf(m));
+  t.ref = m * t.k;
+  return t;
+}
+__device__ __forceinline__ double adj(float max, const Scale64& t) {
+  return fma(fma(static_cast<double>(ms_ref(max)), t.k, -t.ref), -0.69314718055994530942 / kTable, 1.);
+}
 
 template <typename TI>
 __device__ __forceinline__ const char* target_row(const VerifyArgs& a, int64_t s, int i) {
@@ -295,9 +317,9 @@ __global__ void __launch_bounds__(kBlock) verify_rows_kernel(VerifyArgs a, int r
     m = fmaxf(m, wmax[w]);
     nan |= wmax[w] != wmax[w];
   }
-  const double k = a.k * kTable, ref = -static_cast<double>(ms_ref(m)) * k;
+  const Scale64 at = scale64(a, m);
   auto term = [&](float v, double sum) {
-    return Exp2(fmax(fma(static_cast<double>(v), k, ref), -1000. * kTable), table).add_to(sum);
+    return Exp2(fmax(fma(static_cast<double>(v), at.k, -at.ref), -1000. * kTable), table).add_to(sum);
   };
   double sum = ek >= 0 ? term(xe, 0.) : 0.;
 #pragma unroll
@@ -306,7 +328,7 @@ __global__ void __launch_bounds__(kBlock) verify_rows_kernel(VerifyArgs a, int r
 #pragma unroll
       for (int j = 0; j < EPV; ++j) sum = term(TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j), sum);
   sum = block_sum64<BLOCK>(sum, lds);
-  if (tid == 0) a.part[(token * 2 + is_draft) * a.parts + part] = RowState{sum, m, nan};
+  if (tid == 0) a.part[(token * 2 + is_draft) * a.parts + part] = RowState{sum * adj(m, at), m, nan};
 }
 
 // ---- decide ----------------------------------------------------------------------------
@@ -348,12 +370,9 @@ __global__ void __launch_bounds__(kDecideBlock) verify_decide_kernel(VerifyArgs 
     const bool in = d >= 0 && d < a.vocab;
     Decision o{p.sum, q.sum, p.max, q.max, 0.f, (in ? kInRange : 0) | (p.at ? kBadP : 0) | (q.at ? kBadQ : 0)};
     if (drafted && in && !p.at && !q.at) {
-      const double y = fma(static_cast<double>(TI::load1(target_row<TI>(a, s, i), d)), a.k,
-                           -static_cast<double>(p.max) * a.k);
+      const double y = (static_cast<double>(TI::load1(target_row<TI>(a, s, i), d)) - p.max) * a.k;
       double qd = 1.;
-      if (model)
-        qd = exp2_64(fma(static_cast<double>(TI::load1(draft_row<TI>(a, s, i), d)), a.k,
-                         -static_cast<double>(q.max) * a.k)) / q.sum;
+      if (model) qd = exp2_64((static_cast<double>(TI::load1(draft_row<TI>(a, s, i), d)) - q.max) * a.k) / q.sum;
       if (static_cast<double>(a.uniforms[token]) * qd < exp2_64(y) / p.sum) o.flags |= kAccepted;
       o.logp = static_cast<float>(y * 0.69314718055994530942 - log(p.sum));
     }
@@ -369,26 +388,27 @@ __global__ void __launch_bounds__(kDecideBlock) verify_decide_kernel(VerifyArgs 
 // ---- the sequence's end ----------------------------------------------------------------
 // r of one element: max(p - q, 0), p alone where scale_q is 0.
 struct Residual {
-  double k, ref_p, ref_q, scale_p, scale_q;
+  Scale64 p, q;
+  double scale_p, scale_q;  // 1 / sum e
   int without;
   bool plain;   // p alone: nothing of p lies above q
   const double* table;
-  __device__ __forceinline__ double prob(float x, double ref, double scale) const {
+  __device__ __forceinline__ double prob(float x, const Scale64& at, double scale) const {
     // Exactly 0 from 2^-1100 down; an element that has any mass can be drawn.
-    const double v = Exp2(fmax(fma(static_cast<double>(x), k, ref), -1100. * kTable), table).value();
+    const double v = Exp2(fmax(fma(static_cast<double>(x), at.k, -at.ref), -1100. * kTable), table).value();
     return v * scale;
   }
   __device__ __forceinline__ double operator()(float x, float y, int id) const {
-    const double p = prob(x, ref_p, scale_p);
-    if (plain) return p;
-    if (scale_q != 0.) return fmax(p - prob(y, ref_q, scale_q), 0.);
-    return id == without ? 0. : p;
+    const double v = prob(x, p, scale_p);
+    if (plain) return v;
+    if (scale_q != 0.) return fmax(v - prob(y, q, scale_q), 0.);
+    return id == without ? 0. : v;
   }
 };
 
 __device__ __forceinline__ Residual residual(const VerifyArgs& a, const SeqEnd& e, bool plain, const double* table) {
-  const double k = a.k * kTable;
-  return Residual{k, -e.max_p * k, -e.max_q * k, e.scale_p, e.scale_q, e.without, plain, table};
+  const Scale64 p = scale64(a, e.max_p), q = scale64(a, e.max_q);
+  return Residual{p, q, e.scale_p * adj(e.max_p, p), e.scale_q * adj(e.max_q, q), e.without, plain, table};
 }
 
 // The elements of a part: both rows' values, in element order per (chunk, lane, element). The
@@ -539,7 +559,7 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e,
     if (pick < 0) pick = static_cast<int>(a.vocab) - 1;
     const int64_t at = s * (a.n + 1) + e.j;
     a.tokens[at] = pick;
-    if (a.logp) a.logp[at] = static_cast<float>(static_cast<double>(TI::load1(row, pick)) * a.inv_t - e.lse_p);
+    if (a.logp) a.logp[at] = static_cast<float>((static_cast<double>(TI::load1(row, pick)) - e.max_p) * a.inv_t - e.log_p);
   }
 }
 
@@ -565,8 +585,8 @@ __device__ __forceinline__ bool seq_end(const VerifyArgs& a, int64_t s, SeqEnd& 
   e.j = j;
   e.max_p = at.max_p;
   e.scale_p = 1. / at.sum_p;
-  e.lse_p = e.max_p * a.inv_t + log(at.sum_p);
-  e.max_q = model ? at.max_q : 0.;
+  e.log_p = log(at.sum_p);
+  e.max_q = model ? at.max_q : 0.f;
   e.scale_q = model ? 1. / at.sum_q : 0.;
   e.without = refused && !a.draft && in ? static_cast<int32_t>(a.ids[s * a.n + j]) : -1;
   return !(at.flags & kBadP);
@@ -791,6 +811,8 @@ int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   v.dstride = ds;
   v.inv_t = greedy ? 1. : 1. / static_cast<double>(a->temperature);
   v.k = 1.4426950408889634074 * v.inv_t;
+  const double plain = 0x1p42 / (v.k * kTable);
+  v.plain = plain < static_cast<double>(FLT_MAX) ? static_cast<float>(plain) : HUGE_VALF;
   v.n = static_cast<int32_t>(a->n_draft);
   v.parts = static_cast<int32_t>(parts);
   v.end_parts = static_cast<int32_t>(end_parts);

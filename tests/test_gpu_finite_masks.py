@@ -10,8 +10,8 @@ import numpy as np
 import pytest
 import torch
 
-from distill_ref import IGNORE, REL, half_step, lse_ref, row_ref, top_ref
-from pcp_amd import distill, grpo
+from distill_ref import IGNORE, REL, half_step, lse_ref, row_ref, top_ref, verify_ref
+from pcp_amd import distill, grpo, step
 from pcp_amd._lib import PcpError
 
 pytestmark = pytest.mark.gpu
@@ -217,3 +217,39 @@ def test_distill(dtype, mask, mode, N, V):
                 worst = off - bar - half_step(kind, c * grad) - 2.0 ** -8 * bar - flushed
                 assert worst.max() <= 0, (tau, r, kind, worst.argmax(), off[worst.argmax()])
         assert not out.dlogits[0, :-8].any()
+
+
+# ---- draft verification ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,mask", CASES)
+@pytest.mark.parametrize("pattern", PATTERNS + ["everything"])
+@pytest.mark.parametrize("S", [2, 6])
+@pytest.mark.parametrize("lookup", [False, True])
+def test_verify(dtype, mask, pattern, S, lookup):
+    """Tokens and counts equal to the definition's, log-probs to f32 rounding. The second sequence's
+    target is masked throughout, so that every token is as probable as any other."""
+    rng = np.random.default_rng(S)
+    n, V = 2, 40000
+    low = mask_value(dtype, mask)
+    x = rng.standard_normal((S, n + 1, V)).astype(np.float32) * 3
+    y = x[:, :n] + 0.5 * rng.standard_normal((S, n, V)).astype(np.float32)
+    out_of = np.ones((S, V), bool) if pattern == "everything" else where_masked(rng, pattern, S, V)
+    for s in range(S):
+        x[s, :, out_of[s]] = low
+        y[s, :, out_of[s]] = low
+    x[1] = low
+    d = np.zeros((S, n), np.int64)
+    for s in range(S):
+        for i in range(n):
+            z = y[s, i].astype(np.float64)
+            d[s, i] = np.argmax(np.where(out_of[s] & ~out_of[s].all(), -np.inf, z - z.max()) + rng.gumbel(size=V))
+    xd, yd = to_dev(x, dtype, 1), None if lookup else to_dev(y, dtype)
+    for t in (0.7, 1.0, 1.5, 2.0, 4.0):
+        u = rng.random((S, n + 1)).astype(np.float32)
+        u[0, 0] = 0.0                         # accepted if the token has any probability
+        out = step.verify_drafts(xd, torch.from_numpy(d).to(DEV), yd, temperature=t, uniforms=torch.from_numpy(u).to(DEV))
+        want = verify_ref(host64(xd), None if lookup else host64(yd), d, np.full(S, n), u, float(np.float32(t)), V)
+        assert np.array_equal(out.accepted.cpu().numpy(), want[1]), t
+        assert np.array_equal(out.tokens.cpu().numpy(), want[0]), t
+        assert (np.abs(host64(out.logp) - want[2]) <= 2.0 ** -24 * np.abs(want[2]) + 1e-12).all(), t
