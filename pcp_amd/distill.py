@@ -43,7 +43,8 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0, ids_dt
     ctx = ctx or default_context(logits.device.index or 0)
     a = TopLogitsArgs()
     lib().pcp_top_logits_args_init(ctypes.byref(a))
-    with call_scope(ctx, stream, logits) as handle:
+    given = () if outputs is None else (outputs.values, outputs.ids, outputs.lse)
+    with call_scope(ctx, stream, logits, *given) as handle:
         if outputs is None:
             lead, dev = tuple(logits.shape[:-1]), logits.device
             outputs = TopLogits(torch.empty(lead + (max(k, 0),), dtype=torch.float32, device=dev),
@@ -107,7 +108,8 @@ def distill_fwd_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log
     ctx = ctx or default_context(logits.device.index or 0)
     a = DistillArgs()
     lib().pcp_distill_args_init(ctypes.byref(a))
-    with call_scope(ctx, stream, logits, teacher_ids, teacher_logits, teacher_lse, mask) as handle:
+    given = (dlogits,) if outputs is None else (outputs.loss, outputs.token_loss, outputs.dlogits)
+    with call_scope(ctx, stream, logits, teacher_ids, teacher_logits, teacher_lse, mask, *given) as handle:
         if outputs is None:
             dev = logits.device
             if want_dlogits and dlogits is None:

@@ -185,7 +185,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     ctx = ctx or default_context(target_logits.device.index or 0)
     a = VerifyArgs()
     lib().pcp_verify_args_init(ctypes.byref(a))
-    with call_scope(ctx, stream, target_logits, draft_ids, draft_logits, uniforms, draft_lens) as handle:
+    given = () if outputs is None else (outputs.tokens, outputs.accepted, outputs.logp)
+    with call_scope(ctx, stream, target_logits, draft_ids, draft_logits, uniforms, draft_lens, *given) as handle:
         if outputs is None:
             dev = target_logits.device
             outputs = Verified(torch.empty((S, n1), dtype=torch.int64, device=dev),
