@@ -86,7 +86,11 @@ def distill_fwd_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log
     more class; without, its entries are renormalised. divergence is "forward"
     (sum p log(p/q)) or "reverse" (sum q log(q/p), which needs teacher_lse). An id of
     IGNORE_INDEX leaves an entry unused. mask [S, TS] weights tokens as in
-    ``grpo_loss_fwd_bwd``; without a mask, `tokens` (default LS) is TS."""
+    ``grpo_loss_fwd_bwd``; without a mask, `tokens` (default LS) is TS.
+
+    dlogits is written into `dlogits` or, with ``outputs`` of an earlier call, into theirs (one
+    of the two; dlogits_dtype only says what a new one holds). want_dlogits=False forms the
+    loss alone and leaves ``outputs.dlogits`` as it is."""
     if logits.dim() != 3:
         raise PcpError(-1, "logits must be [S, LS, V]")
     S, LS, V = logits.shape
@@ -103,6 +107,16 @@ def distill_fwd_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log
             divergence = Divergence[divergence]
         except KeyError:
             raise PcpError(-1, f"unknown divergence {divergence!r}") from None
+    if dlogits is not None and not want_dlogits:
+        raise PcpError(-1, "dlogits is given and want_dlogits is False")
+    if outputs is not None and dlogits is not None and dlogits is not outputs.dlogits:
+        raise PcpError(-1, "dlogits is given twice: by itself and in outputs")
+    if want_dlogits and dlogits_dtype is not None:
+        into = dlogits if outputs is None else outputs.dlogits
+        if into is not None and into.dtype != dlogits_dtype:
+            raise PcpError(-2, f"dlogits_dtype is {dlogits_dtype}, the given dlogits are {into.dtype}")
+        if into is None and outputs is not None:
+            raise PcpError(-1, "dlogits_dtype is given and outputs have no dlogits")
     TS = mask.shape[1] if mask is not None else (LS if tokens is None else int(tokens))
     rows = LS if rows is None else int(rows)
     ctx = ctx or default_context(logits.device.index or 0)
@@ -116,7 +130,7 @@ def distill_fwd_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log
                 dlogits = torch.empty((S, LS, V), dtype=dlogits_dtype or logits.dtype, device=dev)
             outputs = DistillOutputs(torch.empty((), dtype=torch.float32, device=dev),
                                      torch.zeros((S, TS), dtype=torch.float32, device=dev),
-                                     dlogits if want_dlogits else None)
+                                     dlogits)
         o = outputs
         if (o.loss.dtype != torch.float32 or o.loss.numel() != 1 or o.token_loss.dtype != torch.float32
                 or o.token_loss.numel() != S * TS or (o.dlogits is not None and o.dlogits.numel() != S * LS * V)):
@@ -129,7 +143,7 @@ def distill_fwd_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log
         a.teacher_lse = _ptr(teacher_lse)
         if mask is not None:
             a.mask, a.mask_dtype = _ptr(mask), dtype_code(mask)
-        if o.dlogits is not None:
+        if o.dlogits is not None and want_dlogits:
             a.dlogits, a.dlogits_dtype = _ptr(o.dlogits), dtype_code(o.dlogits)
         a.token_loss, a.loss = _ptr(o.token_loss), _ptr(o.loss)
         a.temperature, a.weight, a.loss_norm = temperature, weight, loss_norm

@@ -1,0 +1,43 @@
+"""Arguments that contradict each other in the calls of a draft model are refused before any work
+(no GPU needed); those that go together do what each says."""
+import pytest
+import torch
+
+from pcp_amd import distill
+from pcp_amd._lib import PcpError
+
+X = torch.zeros((2, 3, 50))
+IDS, VAL, LSE = torch.zeros((2, 3, 4), dtype=torch.int32), torch.zeros((2, 3, 4)), torch.zeros((2, 3))
+
+
+def outputs(dlogits):
+    return distill.DistillOutputs(torch.empty(()), torch.empty((2, 3)), dlogits)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(dlogits=torch.empty_like(X), want_dlogits=False), -1, "want_dlogits"),
+    (dict(dlogits=torch.empty_like(X), outputs=outputs(torch.empty_like(X))), -1, "twice"),
+    (dict(dlogits=torch.empty_like(X), outputs=outputs(None)), -1, "twice"),
+    (dict(dlogits=torch.empty_like(X), dlogits_dtype=torch.bfloat16), -2, "bfloat16"),
+    (dict(outputs=outputs(torch.empty_like(X)), dlogits_dtype=torch.bfloat16), -2, "bfloat16"),
+    (dict(outputs=outputs(None), dlogits_dtype=torch.float32), -1, "no dlogits"),
+])
+def test_dlogits_given_in_two_ways(kw, code, text):
+    with pytest.raises(PcpError, match=text) as e:
+        distill.distill_fwd_bwd(X, IDS, VAL, LSE, **kw)
+    assert e.value.code == code
+
+
+@pytest.mark.gpu
+def test_loss_alone_into_outputs_that_have_dlogits():
+    dev = torch.device("cuda:0")
+    x = torch.randn((2, 3, 700), device=dev)
+    top = distill.top_logits(torch.randn((2, 3, 700), device=dev), 9)
+    out = distill.distill_fwd_bwd(x, top.ids, top.values, top.lse)
+    want, kept = float(out.loss), out.dlogits.fill_(7.0)
+    out.loss.zero_()
+    again = distill.distill_fwd_bwd(x, top.ids, top.values, top.lse, outputs=out, want_dlogits=False)
+    assert again is out and abs(float(out.loss) - want) <= 4e-5 * (1 + abs(want))
+    assert out.dlogits is kept and bool((kept == 7.0).all())
+    distill.distill_fwd_bwd(x, top.ids, top.values, top.lse, outputs=out, dlogits=kept, dlogits_dtype=torch.float32)
+    assert not bool((kept == 7.0).any())
