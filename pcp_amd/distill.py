@@ -40,6 +40,8 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0, ids_dt
     if logits.dim() == 2 and R > 1 and logits.stride(0) < V:
         raise PcpError(-1, "logits rows overlap: expand them with .contiguous()")
     k = int(k)
+    if not 1 <= k <= min(V, _lib.TOP_LOGITS_MAX):
+        raise PcpError(-1, f"k must be in [1, {min(V, _lib.TOP_LOGITS_MAX)}] (got {k})")
     ctx = ctx or default_context(logits.device.index or 0)
     a = TopLogitsArgs()
     lib().pcp_top_logits_args_init(ctypes.byref(a))
@@ -47,8 +49,8 @@ def top_logits(logits: torch.Tensor, k: int, *, temperature: float = 1.0, ids_dt
     with call_scope(ctx, stream, logits, *given) as handle:
         if outputs is None:
             lead, dev = tuple(logits.shape[:-1]), logits.device
-            outputs = TopLogits(torch.empty(lead + (max(k, 0),), dtype=torch.float32, device=dev),
-                                torch.empty(lead + (max(k, 0),), dtype=ids_dtype, device=dev),
+            outputs = TopLogits(torch.empty(lead + (k,), dtype=torch.float32, device=dev),
+                                torch.empty(lead + (k,), dtype=ids_dtype, device=dev),
                                 torch.empty(lead, dtype=torch.float32, device=dev))
         o = outputs
         if (o.values.dtype != torch.float32 or o.values.numel() != R * k or o.ids.dtype != ids_dtype
@@ -118,7 +120,13 @@ def distill_fwd_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log
         if into is None and outputs is not None:
             raise PcpError(-1, "dlogits_dtype is given and outputs have no dlogits")
     TS = mask.shape[1] if mask is not None else (LS if tokens is None else int(tokens))
-    rows = LS if rows is None else int(rows)
+    rows, tok_offset = LS if rows is None else int(rows), int(tok_offset)
+    # (A mask or token count of no tokens has no pointer and no stride: the C entry would take it for
+    # "no mask" and "one token per row".)
+    if rows < 0 or tok_offset < 0 or tok_offset + rows > TS:
+        raise PcpError(-1, f"{rows} rows from token {tok_offset} on do not fit in {TS} tokens")
+    if not 1 <= teacher_ids.shape[2] <= _lib.TOP_LOGITS_MAX:
+        raise PcpError(-1, f"k must be in [1, {_lib.TOP_LOGITS_MAX}] (got {teacher_ids.shape[2]})")
     ctx = ctx or default_context(logits.device.index or 0)
     a = DistillArgs()
     lib().pcp_distill_args_init(ctypes.byref(a))
@@ -136,7 +144,7 @@ def distill_fwd_bwd(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_log
                 or o.token_loss.numel() != S * TS or (o.dlogits is not None and o.dlogits.numel() != S * LS * V)):
             raise PcpError(-1, "outputs do not fit the call: loss f32 [], token_loss f32 [S, TS], dlogits [S, LS, V]")
         a.n_seq, a.rows, a.vocab = S, rows, V
-        a.logit_seq_stride, a.tok_seq_stride, a.tok_offset = LS, TS, int(tok_offset)
+        a.logit_seq_stride, a.tok_seq_stride, a.tok_offset = LS, TS, tok_offset
         a.k, a.divergence = teacher_ids.shape[2], int(divergence)
         a.logits_dtype, a.ids_dtype = dtype_code(logits), dtype_code(teacher_ids)
         a.logits, a.teacher_ids, a.teacher_logits = _ptr(logits), _ptr(teacher_ids), _ptr(teacher_logits)

@@ -28,6 +28,26 @@ def test_dlogits_given_in_two_ways(kw, code, text):
     assert e.value.code == code
 
 
+@pytest.mark.parametrize("kw", [
+    dict(mask=torch.ones((2, 0))), dict(mask=torch.ones((2, 0), dtype=torch.bool), rows=1), dict(tokens=0),
+    dict(tokens=2), dict(mask=torch.ones((2, 3)), tok_offset=1), dict(rows=-1), dict(tok_offset=-1, rows=2),
+    dict(rows=1 << 40),
+])
+def test_rows_that_no_token_belongs_to(kw):
+    with pytest.raises(PcpError, match="do not fit"):
+        distill.distill_fwd_bwd(X, IDS, VAL, LSE, **kw)
+
+
+@pytest.mark.parametrize("k", [0, -1, 51, 257, (1 << 32) + 5])
+def test_numbers_of_entries(k):
+    with pytest.raises(PcpError, match="k must be"):
+        distill.top_logits(X if k != 257 else torch.zeros((2, 400)), k)
+    with pytest.raises(PcpError, match="k must be"):
+        distill.distill_fwd_bwd(X, IDS[..., :1].expand(2, 3, 257), VAL[..., :1].expand(2, 3, 257), LSE)
+    with pytest.raises(PcpError, match="k must be"):
+        distill.distill_fwd_bwd(X, IDS[..., :0], VAL[..., :0], LSE)
+
+
 @pytest.mark.gpu
 def test_loss_alone_into_outputs_that_have_dlogits():
     dev = torch.device("cuda:0")
