@@ -16,6 +16,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 
@@ -333,9 +334,17 @@ inline int64_t prepare_blocks(const DistillArgs& a) {
 }
 
 template <typename TI>
-__global__ void __launch_bounds__(kPrepBlock) distill_prepare_kernel(DistillArgs a) {
+__global__ void __launch_bounds__(kPrepBlock) distill_prepare_kernel(DistillArgs a, int64_t block0) {
   __shared__ float lds[kPrepBlock / 64];
-  prepare<TI>(a, blockIdx.x, lds);
+  prepare<TI>(a, block0 + blockIdx.x, lds);
+}
+// A grid has fewer than 2^32 threads: calls of some ten million rows and more take several.
+template <typename TI>
+void launch_prepare(const DistillArgs& a, hipStream_t st) {
+  constexpr int64_t kMost = (int64_t{1} << 31) / kPrepBlock;
+  const int64_t blocks = prepare_blocks(a);
+  for (int64_t b = 0; b < blocks; b += kMost)
+    distill_prepare_kernel<TI><<<dim3(static_cast<unsigned>(std::min(blocks - b, kMost))), dim3(kPrepBlock), 0, st>>>(a, b);
 }
 
 // ---- a row's terms -----------------------------------------------------------------------
@@ -1148,7 +1157,7 @@ hipError_t launch_parts(DistillArgs a, hipStream_t st) {
   // The preparation goes with the first kernel where its workgroups fit that grid.
   const int64_t prep = prepare_blocks(a);
   const bool with = a.nrows + prep <= kRows;
-  if (!with) distill_prepare_kernel<TI><<<dim3(static_cast<unsigned>(prep)), dim3(kPrepBlock), 0, st>>>(a);
+  if (!with) launch_prepare<TI>(a, st);
   for (int64_t r0 = 0; r0 < a.nrows; r0 += kRows) {
     a.row0 = r0;
     const unsigned n = static_cast<unsigned>(a.nrows - r0 < kRows ? a.nrows - r0 : kRows);
@@ -1185,7 +1194,7 @@ hipError_t launch_row(DistillArgs a, hipStream_t st) {
     cached.store(slots, std::memory_order_relaxed);
   }
   const int64_t grid = a.nrows < slots ? a.nrows : slots;
-  distill_prepare_kernel<TI><<<dim3(static_cast<unsigned>(prepare_blocks(a))), dim3(kPrepBlock), 0, st>>>(a);
+  launch_prepare<TI>(a, st);
   if (kDealt<BLOCK, NCH>) a.turn = resident_turn(grid, a.logit_stride, a.mask != nullptr);
   distill_row_kernel<TI, TO, BLOCK, NCH, FULL><<<dim3(static_cast<unsigned>(grid)), dim3(BLOCK), 0, st>>>(a);
   return hipGetLastError();
