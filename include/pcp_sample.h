@@ -107,9 +107,13 @@ typedef struct pcp_verify_args {
   float* logp;               /* [S, n + 1], or NULL                                       */
   uint32_t flags;            /* PCP_FLAG_ASYNC                                            */
   void* stream;              /* hipStream_t; NULL => the default stream                   */
+  int64_t target_seq_stride; /* elements between sequences; 0 => n + 1 rows               */
+  int64_t draft_seq_stride;  /* elements between sequences; 0 => n rows                   */
 } pcp_verify_args;
 
-/* Defaults: strides 0, bf16, temperature 1. */
+/* Defaults: strides 0, bf16, temperature 1. Strides may be in either order: rows of one
+ * drafting step after another, [n, S, V], have a row stride of S * V and a sequence stride
+ * of V. */
 void pcp_verify_args_init(pcp_verify_args* a);
 int pcp_verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a);
 

@@ -163,6 +163,7 @@ class VerifyArgs(ctypes.Structure):
         ("draft_lens", ctypes.c_void_p), ("uniforms", ctypes.c_void_p),
         ("tokens", ctypes.c_void_p), ("accepted", ctypes.c_void_p), ("logp", ctypes.c_void_p),
         ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
+        ("target_seq_stride", ctypes.c_int64), ("draft_seq_stride", ctypes.c_int64),
     ]
 
 

@@ -80,7 +80,7 @@ struct VerifyArgs {
   int* ended;                 // [S]: one of the first tokens was refused
   unsigned* done;             // [S]: workgroups done with a sequence's residual; zero between calls
   int* err;
-  int64_t vocab, tstride, dstride;   // elements
+  int64_t vocab, tstride, dstride, tseq, dseq;   // elements: between rows, between sequences
   double k;                   // log2(e) / temperature
   double inv_t;
   float plain;                // see scale64
@@ -166,11 +166,11 @@ __device__ __forceinline__ double adj(float max, const Scale64& t) {
 
 template <typename TI>
 __device__ __forceinline__ const char* target_row(const VerifyArgs& a, int64_t s, int i) {
-  return static_cast<const char*>(a.target) + (s * (a.n + 1) + i) * a.tstride * TI::kBytes;
+  return static_cast<const char*>(a.target) + (s * a.tseq + i * a.tstride) * TI::kBytes;
 }
 template <typename TI>
 __device__ __forceinline__ const char* draft_row(const VerifyArgs& a, int64_t s, int i) {
-  return static_cast<const char*>(a.draft) + (s * a.n + i) * a.dstride * TI::kBytes;
+  return static_cast<const char*>(a.draft) + (s * a.dseq + i * a.dstride) * TI::kBytes;
 }
 
 __device__ __forceinline__ int draft_len(const VerifyArgs& a, int64_t s) {
@@ -748,9 +748,20 @@ int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   const int64_t ts = a->target_row_stride ? a->target_row_stride : a->vocab;
   const int64_t ds = a->draft_row_stride ? a->draft_row_stride : a->vocab;
   if (ts < a->vocab || ds < a->vocab) return fail(ctx, PCP_ERR_INVALID_ARG, "row strides must be >= vocab");
-  int64_t tmp;
-  if (mul_overflows(a->n_seq * (a->n_draft + 1), ts, &tmp) || mul_overflows(tmp, 4, &tmp) ||
-      mul_overflows(a->n_seq * a->n_draft, ds, &tmp) || mul_overflows(tmp, 4, &tmp))
+  int64_t tseq, dseq;
+  if (mul_overflows(a->n_draft + 1, ts, &tseq) || mul_overflows(a->n_draft, ds, &dseq))
+    return fail(ctx, PCP_ERR_OVERFLOW, "logits byte size overflows int64");
+  if (a->target_seq_stride) tseq = a->target_seq_stride;
+  if (a->draft_seq_stride) dseq = a->draft_seq_stride;
+  if (tseq < a->vocab || (dseq < a->vocab && a->n_draft > 0))
+    return fail(ctx, PCP_ERR_INVALID_ARG, "sequence strides must be >= vocab");
+  // The bytes up to the last row's end, from above.
+  auto too_far = [&](int64_t rows, int64_t row, int64_t seq) {
+    int64_t in_seq, all, sum;
+    return mul_overflows(rows, row, &in_seq) || mul_overflows(a->n_seq, seq, &all) ||
+           __builtin_add_overflow(in_seq, all, &sum) || mul_overflows(sum, 4, &sum);
+  };
+  if (too_far(a->n_draft + 1, ts, tseq) || too_far(a->n_draft, ds, dseq))
     return fail(ctx, PCP_ERR_OVERFLOW, "logits byte size overflows int64");
   if (a->logits_dtype != PCP_BF16 && a->logits_dtype != PCP_F16 && a->logits_dtype != PCP_F32)
     return fail(ctx, PCP_ERR_DTYPE, "logits dtype must be bf16, f16 or f32 (got %d)", a->logits_dtype);
@@ -809,6 +820,8 @@ int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   v.vocab = a->vocab;
   v.tstride = ts;
   v.dstride = ds;
+  v.tseq = tseq;
+  v.dseq = dseq;
   v.inv_t = greedy ? 1. : 1. / static_cast<double>(a->temperature);
   v.k = 1.4426950408889634074 * v.inv_t;
   const double plain = 0x1p42 / (v.k * kTable);

@@ -167,8 +167,9 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
     prefix and one more token. draft_logits [S, n, V] is the distribution the tokens were drawn
     from, None for drafts looked up or chosen greedily; uniforms f32 [S, n + 1] in [0, 1), n
     for the tokens and the last for the one after (None when temperature < 1e-6, which is
-    greedy); draft_lens int32 [S] the tokens drafted per sequence (None: n). The rows may lie
-    further apart than V if evenly so. sync=False only enqueues the launches."""
+    greedy); draft_lens int32 [S] the tokens drafted per sequence (None: n). The logits may be views
+    with contiguous rows, such as ``logits[:, -(n + 1):]`` or a stack [n, S, V] of drafting steps,
+    transposed. sync=False only enqueues the launches."""
     if target_logits.dim() != 3 or target_logits.shape[1] < 1:
         raise PcpError(-1, "target_logits must be [S, n + 1, V]")
     S, n1, V = target_logits.shape
@@ -181,7 +182,8 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
         raise PcpError(-1, "uniforms must be f32 [S, n + 1]")
     if draft_lens is not None and (draft_lens.dtype != torch.int32 or draft_lens.shape != (S,)):
         raise PcpError(-1, "draft_lens must be int32 [S]")
-    target_stride, draft_stride = _row_stride(target_logits), _row_stride(draft_logits) if draft_logits is not None else V
+    target_stride, target_seq = _row_stride(target_logits), _seq_stride(target_logits)
+    draft_stride, draft_seq = (V, 0) if draft_logits is None else (_row_stride(draft_logits), _seq_stride(draft_logits))
     ctx = ctx or default_context(target_logits.device.index or 0)
     a = VerifyArgs()
     lib().pcp_verify_args_init(ctypes.byref(a))
@@ -198,6 +200,7 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
             raise PcpError(-1, "outputs do not fit the call: tokens int64 and logp f32 [S, n + 1], accepted int32 [S]")
         a.n_seq, a.n_draft, a.vocab = S, n, V
         a.target_row_stride, a.draft_row_stride = target_stride, draft_stride
+        a.target_seq_stride, a.draft_seq_stride = target_seq, draft_seq
         a.logits_dtype, a.temperature = dtype_code(target_logits), temperature
         a.target_logits = target_logits.data_ptr()
         a.draft_logits = draft_logits.data_ptr() if draft_logits is not None and n else None
@@ -210,13 +213,18 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
 
 
 def _row_stride(t: torch.Tensor) -> int:
-    """Elements between the evenly spaced rows of [S, m, V]."""
+    """Elements between the rows of a sequence of [S, m, V]."""
     S, m, V = t.shape
     if V > 1 and t.stride(2) != 1:
         raise PcpError(-1, "logits rows must be contiguous")
-    if m > 1 and S > 1 and t.stride(0) != m * t.stride(1):
-        raise PcpError(-1, "logits rows must be evenly spaced over the sequences")
-    stride = t.stride(1) if m > 1 else (t.stride(0) if S > 1 else V)
-    if stride < V and S * m > 1:
+    if m > 1 and t.stride(1) < V:
         raise PcpError(-1, "logits rows overlap: expand them with .contiguous()")
-    return max(stride, V)
+    return t.stride(1) if m > 1 else V
+
+
+def _seq_stride(t: torch.Tensor) -> int:
+    """Elements between the sequences of [S, m, V]; 0: m rows (there is one sequence, or no row)."""
+    S, m, V = t.shape
+    if S > 1 and m > 0 and t.stride(0) < V:
+        raise PcpError(-1, "logits rows overlap: expand them with .contiguous()")
+    return t.stride(0) if S > 1 and m > 0 else 0

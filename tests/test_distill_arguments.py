@@ -1,9 +1,11 @@
 """Arguments that contradict each other in the calls of a draft model are refused before any work
 (no GPU needed); those that go together do what each says."""
+import ctypes
+
 import pytest
 import torch
 
-from pcp_amd import distill
+from pcp_amd import _lib, distill, step
 from pcp_amd._lib import PcpError
 
 X = torch.zeros((2, 3, 50))
@@ -46,6 +48,38 @@ def test_numbers_of_entries(k):
         distill.distill_fwd_bwd(X, IDS[..., :1].expand(2, 3, 257), VAL[..., :1].expand(2, 3, 257), LSE)
     with pytest.raises(PcpError, match="k must be"):
         distill.distill_fwd_bwd(X, IDS[..., :0], VAL[..., :0], LSE)
+
+
+@pytest.mark.parametrize("kw,code,text", [
+    (dict(target_seq_stride=99), -1, "sequence strides"),
+    (dict(target_seq_stride=-400), -1, "sequence strides"),
+    (dict(draft_seq_stride=99, draft_logits=0x1000), -1, "sequence strides"),
+    (dict(target_seq_stride=1 << 62), -9, "overflows"),
+    (dict(target_row_stride=1 << 62), -9, "overflows"),
+    (dict(draft_seq_stride=1 << 61), -9, "overflows"),
+    (dict(draft_row_stride=1 << 60), -9, "overflows"),
+    (dict(target_row_stride=200, target_seq_stride=100), -1, "context is NULL"),
+    (dict(n_draft=0, draft_ids=None), -1, "context is NULL"),
+])
+def test_strides_of_the_verification(kw, code, text):
+    L, a = _lib.lib(), _lib.VerifyArgs()
+    L.pcp_verify_args_init(ctypes.byref(a))
+    for k, v in {**dict(n_seq=2, n_draft=3, vocab=100, target_logits=0x1000, draft_ids=0x2000, uniforms=0x3000,
+                        tokens=0x4000, accepted=0x5000), **kw}.items():
+        setattr(a, k, v)
+    assert L.pcp_verify_drafts(None, ctypes.byref(a)) == code
+    assert text in L.pcp_last_error(None).decode()
+
+
+def test_strides_of_views():
+    x = torch.zeros((4, 9, 50))
+    assert (step._row_stride(x[:, -3:]), step._seq_stride(x[:, -3:])) == (50, 450)
+    t = torch.zeros((3, 4, 50)).transpose(0, 1)
+    assert (step._row_stride(t), step._seq_stride(t)) == (200, 50)
+    assert step._seq_stride(x[:1]) == 0 and step._seq_stride(x[:, :0]) == 0
+    for bad in (x.transpose(1, 2), x[..., ::2]):
+        with pytest.raises(PcpError, match="contiguous"):
+            step._row_stride(bad)
 
 
 @pytest.mark.gpu
