@@ -13,8 +13,10 @@
  * can be captured in a HIP graph. A call under capture that would need a larger work
  * buffer fails with PCP_ERR_INVALID_ARG before any work: make one uncaptured call of the
  * same sizes first. Calls on one context share its work buffer and run in stream order;
- * calls (and replayed graphs) that may overlap need separate contexts. The calling
- * thread's current device is the same after a call as before it.
+ * calls (and replayed graphs) that may overlap need separate contexts. A captured call's
+ * work buffer stays where it is when a later call needs a larger one, until
+ * pcp_release_workspace or pcp_destroy, after which its graph must not be replayed. The
+ * calling thread's current device is the same after a call as before it.
  */
 #ifndef PCP_DISTILL_H
 #define PCP_DISTILL_H

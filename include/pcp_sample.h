@@ -87,7 +87,9 @@ int pcp_sample_tokens_async(pcp_ctx* ctx, const void* logits, int dtype, int64_t
  * refuses its token for one from p_j).
  * Calls on one context share its work buffer: calls that may overlap on different
  * streams need separate contexts. Under stream capture the work buffer must have grown
- * by an uncaptured call of the same sizes (PCP_ERR_INVALID_ARG before any work if not).
+ * by an uncaptured call of the same sizes (PCP_ERR_INVALID_ARG before any work if not);
+ * it then stays where it is until pcp_release_workspace or pcp_destroy, after which the
+ * graph must not be replayed.
  */
 typedef struct pcp_verify_args {
   int64_t n_seq;             /* S, 0 .. PCP_SAMPLE_MAX_ROWS                               */

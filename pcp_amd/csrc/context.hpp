@@ -41,6 +41,9 @@ struct pcp_ctx {
   std::atomic<bool> logprob_parts_busy{false};   // this flag
   void* scratch = nullptr;       // per-call work buffers, grown on demand
   size_t scratch_bytes = 0;
+  bool scratch_in_graph = false;      // a call of ensure_scratch_on has been captured with it
+  std::vector<void*> graph_scratch;   // earlier ones that were, kept for the graphs' replays
+  size_t graph_scratch_bytes = 0;
   // Streams holding PCP_FLAG_ASYNC work (a fixed set, so recording one allocates nothing).
   static constexpr int kMaxPending = 32;
   hipStream_t pending[kMaxPending] = {};
@@ -110,7 +113,8 @@ inline int dtype_bytes(int dt) {
 int ensure_scratch(pcp_ctx* ctx, size_t bytes);
 
 // The same for work enqueued on `st`; a stream under capture cannot grow it
-// (PCP_ERR_INVALID_ARG, the capture left as it was).
+// (PCP_ERR_INVALID_ARG, the capture left as it was). What a captured call uses is not freed when
+// the scratch grows, only by pcp_release_workspace and pcp_destroy.
 int ensure_scratch_on(pcp_ctx* ctx, size_t bytes, hipStream_t st);
 
 // Makes a device current for a scope and the caller's current again after it.

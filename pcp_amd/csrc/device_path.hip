@@ -41,7 +41,13 @@ int ensure_scratch(pcp_ctx* ctx, size_t bytes) {
   if (ctx->scratch) {
     hipError_t e = hipDeviceSynchronize();
     if (e != hipSuccess) return hip_fail(ctx, e, "hipDeviceSynchronize");
-    (void)hipFree(ctx->scratch);
+    if (ctx->scratch_in_graph) {
+      ctx->graph_scratch.push_back(ctx->scratch);
+      ctx->graph_scratch_bytes += ctx->scratch_bytes;
+      ctx->scratch_in_graph = false;
+    } else {
+      (void)hipFree(ctx->scratch);
+    }
     ctx->scratch = nullptr;
     ctx->scratch_bytes = 0;
   }
@@ -58,15 +64,26 @@ int ensure_scratch(pcp_ctx* ctx, size_t bytes) {
 }
 
 int ensure_scratch_on(pcp_ctx* ctx, size_t bytes, hipStream_t st) {
-  if (bytes <= ctx->scratch_bytes) return PCP_OK;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(st, &status) != hipSuccess) (void)hipGetLastError();
-  else if (status != hipStreamCaptureStatusNone)
-    return fail(ctx, PCP_ERR_INVALID_ARG,
-                "the stream is being captured and the context's work buffer would have to grow from %zu to %zu bytes: "
-                "make one uncaptured call of the same sizes first",
-                ctx->scratch_bytes, bytes);
+  else if (status != hipStreamCaptureStatusNone) {
+    if (bytes > ctx->scratch_bytes)
+      return fail(ctx, PCP_ERR_INVALID_ARG,
+                  "the stream is being captured and the context's work buffer would have to grow from %zu to %zu bytes: "
+                  "make one uncaptured call of the same sizes first",
+                  ctx->scratch_bytes, bytes);
+    ctx->scratch_in_graph = true;
+    ctx->graph_scratch.reserve(ctx->graph_scratch.size() + 1);   // no allocation where it is kept
+    return PCP_OK;
+  }
   return ensure_scratch(ctx, bytes);
+}
+
+void free_graph_scratch(pcp_ctx* ctx) {
+  for (void* p : ctx->graph_scratch) (void)hipFree(p);
+  ctx->graph_scratch.clear();
+  ctx->graph_scratch_bytes = 0;
+  ctx->scratch_in_graph = false;
 }
 
 int finish_call(pcp_ctx* ctx, uint32_t flags, hipStream_t st) {
@@ -512,6 +529,7 @@ void pcp_destroy(pcp_ctx* ctx) {
     (void)hipDeviceSynchronize();
     release_profile_events(ctx);
     if (ctx->scratch) (void)hipFree(ctx->scratch);
+    free_graph_scratch(ctx);
     if (ctx->lm_dbuf) (void)hipFree(ctx->lm_dbuf);
     if (ctx->lm_pieces.buf) (void)hipFree(ctx->lm_pieces.buf);
     if (ctx->sample_ticket) (void)hipFree(ctx->sample_ticket);
@@ -529,13 +547,14 @@ int pcp_release_workspace(pcp_ctx* ctx) {
   if (!ctx) return fail(nullptr, PCP_ERR_INVALID_ARG, "context is NULL");
   hipError_t e = hipSetDevice(ctx->device);
   if (e != hipSuccess) return hip_fail(ctx, e, "hipSetDevice");
-  if (!ctx->scratch && !ctx->lm_dbuf && !ctx->lm_pieces.buf) {
+  if (!ctx->scratch && ctx->graph_scratch.empty() && !ctx->lm_dbuf && !ctx->lm_pieces.buf) {
     ctx->lm_pieces.reset();
     return PCP_OK;
   }
   // Earlier calls (PCP_FLAG_ASYNC ones included) may still use the buffers.
   if ((e = hipDeviceSynchronize()) != hipSuccess) return hip_fail(ctx, e, "hipDeviceSynchronize");
   if (ctx->scratch) (void)hipFree(ctx->scratch);
+  free_graph_scratch(ctx);
   if (ctx->lm_dbuf) (void)hipFree(ctx->lm_dbuf);
   if (ctx->lm_pieces.buf) (void)hipFree(ctx->lm_pieces.buf);
   ctx->lm_pieces.reset();
@@ -544,7 +563,9 @@ int pcp_release_workspace(pcp_ctx* ctx) {
   return PCP_OK;
 }
 
-size_t pcp_workspace_bytes(const pcp_ctx* ctx) { return ctx ? ctx->scratch_bytes + ctx->lm_dbuf_bytes + ctx->lm_pieces.bytes : 0; }
+size_t pcp_workspace_bytes(const pcp_ctx* ctx) {
+  return ctx ? ctx->scratch_bytes + ctx->graph_scratch_bytes + ctx->lm_dbuf_bytes + ctx->lm_pieces.bytes : 0;
+}
 
 int pcp_get_backend_type(const pcp_ctx* ctx) { return ctx ? ctx->backend : PCP_ERR_INVALID_ARG; }
 
