@@ -105,7 +105,7 @@ class call_scope:
 
     def __init__(self, ctx: Context, stream, *tensors):
         for t in tensors:
-            if t is not None and (not t.is_cuda or t.device.index != ctx.device):
+            if t is not None and t.get_device() != ctx.device:   # -1 on the CPU
                 raise PcpError(-1, f"tensor on {t.device}, context on device {ctx.device}")
         self.inner = None
         current = torch.cuda.current_stream(ctx.device)

@@ -214,17 +214,23 @@ def verify_drafts(target_logits: torch.Tensor, draft_ids: torch.Tensor, draft_lo
 
 def _row_stride(t: torch.Tensor) -> int:
     """Elements between the rows of a sequence of [S, m, V]."""
-    S, m, V = t.shape
-    if V > 1 and t.stride(2) != 1:
+    _, m, V = t.shape
+    _, row, one = t.stride()
+    if one != 1 and V > 1:
         raise PcpError(-1, "logits rows must be contiguous")
-    if m > 1 and t.stride(1) < V:
+    if m <= 1:
+        return V
+    if row < V:
         raise PcpError(-1, "logits rows overlap: expand them with .contiguous()")
-    return t.stride(1) if m > 1 else V
+    return row
 
 
 def _seq_stride(t: torch.Tensor) -> int:
     """Elements between the sequences of [S, m, V]; 0: m rows (there is one sequence, or no row)."""
     S, m, V = t.shape
-    if S > 1 and m > 0 and t.stride(0) < V:
+    if S <= 1 or m < 1:
+        return 0
+    seq = t.stride(0)
+    if seq < V:
         raise PcpError(-1, "logits rows overlap: expand them with .contiguous()")
-    return t.stride(0) if S > 1 and m > 0 else 0
+    return seq
