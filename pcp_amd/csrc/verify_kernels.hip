@@ -21,6 +21,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 #include <cstdint>
@@ -87,6 +88,7 @@ struct VerifyArgs {
   int32_t n;
   int32_t parts, end_parts;   // of kPartVecs, end_vecs vectors
   int32_t greedy;
+  int32_t along;              // the residual's last workgroup picks the token
   int32_t from;               // the first token of this launch
 };
 
@@ -672,13 +674,33 @@ __global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
   pick_token<TI, U>(a, e, blockIdx.x, row, row_span<TI>(row, a.vocab), table);
 }
 
-// The residual's last workgroup picks along for few sequences: 12.5 us for one, against 6.8 + 10
-// and the gap between two launches; for 64 its tickets made 44 of 20 + 12.
-constexpr int64_t kPickAlongMaxSeqs = 4;
-// Rows in two launches from this many workgroups (16 KB each) on: 20,672 took 82 us and a decide
-// of 4.7 instead of 109 where about a third of the sequences went past their first half; 4,368
-// take 13 in one launch, where the second pair of launches would cost more than it leaves out.
-constexpr int64_t kSplitWorkgroups = 8192;
+// The residual's last workgroup picks the token along, by a ticket of each of its workgroups (4 KB of a
+// row), where all sequences have at most so many, fewer where rows are narrow; else a launch of its
+// own does. us for a whole call with 4 drafted tokens, along | by its own launch, by sequences:
+//   bf16 151,936, looked up  1  20 | 23   2  22 | 24   4  25 | 26    6  28 | 27   12  37 | 31   64  94 | 61
+//   bf16 151,936, a model    1  21 | 24   2  24 | 27   4  27 | 28    6  31 | 31   12  42 | 37   64 123 | 93
+//   bf16  50,257, looked up  1  20 | 23   4  21 | 25   8  24 | 26   12  25 | 26   16  28 | 28   32  34 | 32
+//   f32   50,257, a model    1  19 | 21   4  22 | 24   6  24 | 25    8  27 | 27   12  31 | 28   32  45 | 36
+//   bf16  32,000, a model    1  20 | 24   4  21 | 26   8  24 | 27   16  28 | 29   24  32 | 31   32  34 | 32
+//   f32    8,192, looked up  1  17 | 19   4  18 | 20   8  20 | 21   12  21 | 21   16  22 | 22   24  24 | 22
+//   bf16   4,096, a model    1  19 | 22   8  20 | 25  32  22 | 26   64  25 | 27   80  26 | 27  128  31 | 28
+//   bf16   1,000, a model    1  18 | 20   8  20 | 22  32  21 | 22   80  23 | 23  128  25 | 24  160  26 | 25
+constexpr int64_t kPickAlongWorkgroups = 320, kPickAlongNarrow = 96, kNarrowParts = 16;
+static_assert(kPickAlongWorkgroups / kNarrowParts <= kPickAlongNarrow, "a count per sequence");
+// Rows in two launches from this many workgroups (16 KB of a row each) on: what it leaves out depends on
+// how many sequences end in their first half. us for a whole call, two | one, by accepted tokens:
+//   of 8, a model     10,336: 3.7  79 |  81   5.8  86 |  80   7.0  89 |  79   8  89 |  78
+//                     17,408: 3.8 112 | 123   5.5 118 | 121   6.8 123 | 119   8 124 | 115
+//                     20,672: 3.6 121 | 140   5.8 133 | 137   7.3 141 | 135   8 140 | 134
+//   of 4, looked up    6,080: 0    47 |  61   0.9  59 |  61   2.4  66 |  61   4  72 |  61
+//                     12,160: 0    68 | 100   1.0  83 |  99   2.3  97 | 100   4 109 |  99
+// Looked-up tokens are refused more often than a model's.
+constexpr int64_t kSplitWorkgroupsModel = 16384, kSplitWorkgroupsLookup = 8192;
+
+bool picks_along(int64_t n_seq, int64_t nv) {
+  const int64_t parts = std::max<int64_t>((nv + end_vecs(1) - 1) / end_vecs(1), 1);
+  return n_seq * parts <= (parts < kNarrowParts ? kPickAlongNarrow : kPickAlongWorkgroups);
+}
 
 template <typename TI>
 hipError_t launch_verify(VerifyArgs a, int64_t n_seq, hipStream_t st) {
@@ -689,7 +711,9 @@ hipError_t launch_verify(VerifyArgs a, int64_t n_seq, hipStream_t st) {
     verify_greedy_kernel<<<seqs, dim3(kGreedyBlock), 0, st>>>(a);
     return hipGetLastError();
   }
-  const int first = n_seq * (a.draft ? 2 * a.n + 1 : a.n + 1) * a.parts > kSplitWorkgroups ? (a.n + 1) / 2 : 0;
+  const bool split = a.draft ? n_seq * (2 * a.n + 1) * a.parts > kSplitWorkgroupsModel
+                             : n_seq * (a.n + 1) * a.parts > kSplitWorkgroupsLookup;
+  const int first = split ? (a.n + 1) / 2 : 0;
   for (int from = 0, to = first ? first : a.n + 1; from <= a.n; from = to, to = a.n + 1) {
     a.from = from;
     const unsigned rows = static_cast<unsigned>(to - from);
@@ -697,7 +721,7 @@ hipError_t launch_verify(VerifyArgs a, int64_t n_seq, hipStream_t st) {
     verify_decide_kernel<TI><<<seqs, dim3(kDecideBlock), 0, st>>>(a, to);
   }
   const dim3 ends(static_cast<unsigned>(a.end_parts), ns);
-  if (n_seq <= kPickAlongMaxSeqs) {
+  if (a.along) {
     verify_residual_kernel<TI, 1, true><<<ends, b, 0, st>>>(a);
   } else {
     verify_residual_kernel<TI, 2, false><<<ends, b, 0, st>>>(a);
@@ -711,7 +735,7 @@ inline bool misaligned(const void* p, int size) {
 }
 inline size_t round256(size_t b) { return (b + 255) & ~static_cast<size_t>(255); }
 
-// The counts that verify_residual_kernel leaves at zero.
+// The counts that verify_residual_kernel leaves at zero, one per sequence: at most kPickAlongNarrow.
 int ensure_verify_done(pcp_ctx* ctx, hipStream_t st) {
   if (ctx->verify_done) return PCP_OK;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
@@ -719,13 +743,13 @@ int ensure_verify_done(pcp_ctx* ctx, hipStream_t st) {
   else if (status != hipStreamCaptureStatusNone)
     return fail(ctx, PCP_ERR_INVALID_ARG, "the stream is being captured and the context's counters would have to be "
                                           "made: make one uncaptured call of the same sizes first");
-  hipError_t e = hipMalloc(&ctx->verify_done, sizeof(unsigned) * kPickAlongMaxSeqs);
+  hipError_t e = hipMalloc(&ctx->verify_done, sizeof(unsigned) * kPickAlongNarrow);
   if (e != hipSuccess) {
     ctx->verify_done = nullptr;
     (void)hipGetLastError();
     return fail(ctx, PCP_ERR_OOM, "hipMalloc of the verification's counters failed");
   }
-  if ((e = hipMemset(ctx->verify_done, 0, sizeof(unsigned) * kPickAlongMaxSeqs)) != hipSuccess ||
+  if ((e = hipMemset(ctx->verify_done, 0, sizeof(unsigned) * kPickAlongNarrow)) != hipSuccess ||
       (e = hipDeviceSynchronize()) != hipSuccess) {
     (void)hipFree(ctx->verify_done);
     ctx->verify_done = nullptr;
@@ -791,13 +815,14 @@ int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   const bool model = !greedy && a->draft_logits && a->n_draft > 0;
   const int64_t nv = a->vocab * size / 16;
   const int64_t parts = nv > 0 ? (nv + kPartVecs - 1) / kPartVecs : 1;
-  const int64_t ev = end_vecs(a->n_seq <= kPickAlongMaxSeqs ? 1 : 2), end_parts = nv > 0 ? (nv + ev - 1) / ev : 1;
+  const bool along = !greedy && picks_along(a->n_seq, nv);
+  const int64_t ev = end_vecs(along ? 1 : 2), end_parts = nv > 0 ? (nv + ev - 1) / ev : 1;
   const size_t S = static_cast<size_t>(a->n_seq), tokens = S * static_cast<size_t>(a->n_draft + 1);
   const size_t o_dec = round256(sizeof(RowState) * tokens * (greedy ? 1 : 2) * parts);
   const size_t o_seg = o_dec + (greedy ? 0 : round256(sizeof(Decision) * tokens));
   const size_t o_ended = o_seg + (greedy ? 0 : round256(sizeof(double) * S * (end_parts + 2)));
   int rc = ensure_scratch_on(ctx, o_ended + (greedy ? 0 : sizeof(int) * S), st);
-  if (rc == PCP_OK && !greedy && a->n_seq <= kPickAlongMaxSeqs) rc = ensure_verify_done(ctx, st);
+  if (rc == PCP_OK && along) rc = ensure_verify_done(ctx, st);
   if (rc != PCP_OK) return rc;
   char* sp = static_cast<char*>(ctx->scratch);
 
@@ -830,6 +855,7 @@ int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   v.parts = static_cast<int32_t>(parts);
   v.end_parts = static_cast<int32_t>(end_parts);
   v.greedy = greedy;
+  v.along = along;
   const bool timed = prof_begin(ctx, st);
   const hipError_t e = a->logits_dtype == PCP_F32    ? launch_verify<F32T>(v, a->n_seq, st)
                        : a->logits_dtype == PCP_BF16 ? launch_verify<BF16T>(v, a->n_seq, st)

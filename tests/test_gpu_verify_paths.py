@@ -1,6 +1,7 @@
-"""Draft verification by number of sequences: up to four the last workgroup of a sequence's residual
-picks its token, by counters that are zero again after each call. Captured and replayed, with bad
-rows and clean calls after them, and with every one of 64 drafted tokens accepted."""
+"""Draft verification by number of sequences: with few the last workgroup of a sequence's residual
+picks its token, by counters that are zero again after each call; with many the rows go in two
+launches. Captured and replayed, with bad rows and clean calls after them, and with every one of
+64 drafted tokens accepted."""
 import numpy as np
 import pytest
 import torch
@@ -34,11 +35,12 @@ def check(out, x, y, d, u, rows=slice(None)):
     assert (np.abs(lp - want[2]) <= 2.0 ** -24 * np.abs(want[2]) + 1e-12)[rows].all()
 
 
-@pytest.mark.parametrize("S", [1, 2, 4, 5, 6])
+@pytest.mark.parametrize("S,V", [(1, 20000), (2, 20000), (4, 20000), (5, 20000), (6, 20000), (16, 20000), (17, 20000),
+                                 (96, 500), (97, 500), (12, 8000), (13, 8000)])
 @pytest.mark.parametrize("lookup", [False, True])
-def test_captured_and_replayed(S, lookup):
+def test_captured_and_replayed(S, V, lookup):
     rng = np.random.default_rng(S)
-    n, V = 3, 20000
+    n = 3
     ctx, cold = grpo.Context(0), grpo.Context(0)
     x, y, d, u = on_gpu(*make(rng, S, n, V))
     draft = None if lookup else y
@@ -64,11 +66,12 @@ def test_captured_and_replayed(S, lookup):
 
 
 def test_counters_made_under_capture_are_refused():
-    """A context that has run only calls of more than four sequences has no counters yet."""
+    """A context that has run only calls of many sequences has no counters yet."""
     rng = np.random.default_rng(1)
     n, V = 2, 3000
+    many = 40
     ctx, s, g = grpo.Context(0), torch.cuda.Stream(), torch.cuda.CUDAGraph()
-    x, y, d, u = on_gpu(*make(rng, 6, n, V))
+    x, y, d, u = on_gpu(*make(rng, many, n, V))
     out = step.verify_drafts(x, d, y, uniforms=u, ctx=ctx)
     few = step.verify_drafts(x[:2], d[:2], y[:2], uniforms=u[:2])
     s.wait_stream(torch.cuda.current_stream())
@@ -81,7 +84,7 @@ def test_counters_made_under_capture_are_refused():
     assert torch.equal(few.tokens, out.tokens[:2]) and torch.equal(few.logp, out.logp[:2])
 
 
-@pytest.mark.parametrize("S", [1, 4, 6])
+@pytest.mark.parametrize("S", [1, 4, 10, 11])
 @pytest.mark.parametrize("bad_row", ["target", "draft", "after", "token"])
 def test_clean_calls_after_bad_ones(S, bad_row):
     """A bad row ends its sequence before the counters; the calls after it on the same context are right."""
@@ -144,3 +147,14 @@ def test_all_of_64_accepted(S, kind):
         assert (out.tokens[:, n] == IGNORE).all()
     else:
         check(out, x, y if kind == "model" else None, d, u)
+
+
+@pytest.mark.parametrize("lookup", [False, True])
+@pytest.mark.parametrize("S,n,V", [(1300, 6, 64), (130, 64, 33), (5500, 1, 40), (300, 6, 9000), (3, 2, 700)])
+def test_rows_in_two_launches(S, n, V, lookup):
+    """Calls on both sides of the number of rows from which those of ended sequences are left out."""
+    rng = np.random.default_rng(S)
+    x, y, d, u = make(rng, S, n, V)
+    xd, yd, dd, ud = on_gpu(x, y, d, u)
+    for _ in range(2):
+        check(step.verify_drafts(xd, dd, None if lookup else yd, uniforms=ud), x, None if lookup else y, d, u)
