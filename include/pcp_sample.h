@@ -73,7 +73,7 @@ int pcp_sample_tokens_async(pcp_ctx* ctx, const void* logits, int dtype, int64_t
  * maximum of target row i, whose first maximum is the token after; draft_logits and
  * uniforms are not read.
  * Every probability, sum and comparison is formed in 64 bits from the logits, so the
- * choice is the formulas' own up to their 64-bit rounding.
+ * choice is the formulas' own up to about 1e-14 of a probability.
  *
  * tokens[s, :] receives d_0 .. d_{j-1}, the token after them, then PCP_IGNORE_INDEX;
  * accepted[s] = j; logp[s, i] = log p_i(tokens[s, i]) for i <= j (0 when greedy) and 0

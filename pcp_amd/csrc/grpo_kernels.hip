@@ -1286,10 +1286,6 @@ __global__ void __launch_bounds__(kSmallBlock) loss_reduce_kernel(LossReduceArgs
 // ---------------------------------------------------------------------------
 // Host-side launchers
 // ---------------------------------------------------------------------------
-namespace {
-
-}  // namespace
-
 // How far on each stride of rows dealt in grid strides (kResStatic) starts. Where a workgroup
 // would meet three positions of a sequence or fewer over and over (sequences of 128, 256 or 96
 // rows, say), it would get rows that are all live or all dead: it then moves on by the golden
