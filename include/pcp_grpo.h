@@ -85,6 +85,10 @@ typedef enum pcp_status {
  *     rho = exp(logp - old_logp)
  *     l_t = -min(rho*A, clip(rho, 1-eps, 1+eps)*A) + beta*(exp(ref-logp) - (ref-logp) - 1)
  * dlogits[row, v] = c_t * (onehot(id_t)[v] - softmax(row)[v]),  c_t = d loss / d logp_t.
+ *
+ * Logits may be masked by -Inf or by a large finite value: below -1.49e9 (-2^31 ln 2) they
+ * count as -Inf in a row's sum, and a row with nothing above that as one without a finite
+ * log-sum-exp.
  */
 typedef enum pcp_loss_mode {
   PCP_LOSS_REINFORCE = 0,

@@ -265,9 +265,16 @@ __device__ __forceinline__ void ms_merge(float& m, float& s, float m2, float s2)
 // (all elements so far -inf or NaN), so -inf terms give 0 and NaN terms NaN.
 __device__ __forceinline__ float ms_ref(float m) { return (m == kNegInf) ? 0.f : m; }
 
+// The same for terms 2^(fma(x, log2e, -ref)) of a lane that knows m = fl(max(x) * log2e) alone. The fma
+// is exact, so its exponent at the maximum is m's rounding: up to 2^6 below 2^31, where f32 has room for
+// the sum, but 2^9 at -1e10 and 2^75 at -1e30, the masks of a lane that holds nothing else (inf or
+// 0 for a term of 1, and NaN for the row). A largest logit below -2^31 ln 2 (-1.49e9) therefore counts as
+// -inf: its terms against 0 are 0.
+__device__ __forceinline__ float ms_shift(float m) { return (m < -0x1p31f) ? 0.f : m; }
+
 // Rescale a running sum from reference m to reference nm (nm >= m).
 __device__ __forceinline__ float ms_rescale(float s, float m, float nm) {
-  return (s == 0.f) ? 0.f : s * hw_exp2(m - ms_ref(nm));
+  return (s == 0.f) ? 0.f : s * hw_exp2(m - ms_shift(nm));
 }
 
 // log-sum-exp (natural units) of a merged state, to a few 1e-8: m and the exponent of s
@@ -476,7 +483,7 @@ __device__ __forceinline__ void edge_state(const void* p, const RowSpan& sp, int
   if (k < 0) return;
   const float x = TI::load1(p, k) * kLog2e;
   m = fmaxf(m, x);
-  s = hw_exp2(x - ms_ref(m));
+  s = hw_exp2(x - ms_shift(m));   // (contracted to the fma)
 }
 
 template <typename TI, typename TO, int BLOCK>

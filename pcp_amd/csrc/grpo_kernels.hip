@@ -239,7 +239,7 @@ __device__ __forceinline__ int64_t resident_row(const RowArgs& a, const int64_t 
     if constexpr (EDGE) mx = fmaxf(mx, xe);
     pm = mx * kLog2e;
   }
-  const float m2 = ms_ref(pm);   // this lane's shift (kept for the cached terms)
+  const float m2 = ms_shift(pm);   // this lane's shift (kept for the cached terms)
   float ps = 0.f, rm = kNegInf, rs = 0.f;
   if (EDGE && has_ref) edge_state<TI>(rrow, rsp, tid, rm, rs);
   __builtin_amdgcn_sched_barrier(0);
@@ -295,7 +295,7 @@ __device__ __forceinline__ int64_t resident_row(const RowArgs& a, const int64_t 
         }
       }
       const float nm = fmaxf(rm, bm * kLog2e);
-      const float ref = ms_ref(nm);
+      const float ref = ms_shift(nm);
       float acc = ms_rescale(rs, rm, nm);
 #pragma unroll
       for (int q = 0; q < RB; ++q) {
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(BLOCK) grpo_fwd_kernel(RowArgs a) {
     }
     {
       const float nm = fmaxf(pm, bx * kLog2e);
-      const float ref = ms_ref(nm);
+      const float ref = ms_shift(nm);
       float acc = ms_rescale(ps, pm, nm);
 #pragma unroll
       for (int q = 0; q < U; ++q)
@@ -639,7 +639,7 @@ __global__ void __launch_bounds__(BLOCK) grpo_fwd_kernel(RowArgs a) {
     }
     if constexpr (REF) {
       const float nm = fmaxf(rm, br * kLog2e);
-      const float ref = ms_ref(nm);
+      const float ref = ms_shift(nm);
       float acc = ms_rescale(rs, rm, nm);
 #pragma unroll
       for (int q = 0; q < U; ++q)
@@ -859,7 +859,7 @@ __global__ void __launch_bounds__(kPartBlock) grpo_part_kernel(RowArgs a, StepPr
 #pragma unroll
     for (int q = 0; q < U; ++q)
       if (v0 + q * BLOCK + tid < lim) bx = vec_max<TI>(bx, b[q]);
-    const float nm = fmaxf(m, bx * kLog2e), ref = ms_ref(nm);
+    const float nm = fmaxf(m, bx * kLog2e), ref = ms_shift(nm);
     float acc = ms_rescale(s, m, nm);
 #pragma unroll
     for (int q = 0; q < U; ++q)
@@ -1091,7 +1091,7 @@ __global__ void __launch_bounds__(BLOCK) grpo_stream_kernel(RowArgs a) {
     }
     {
       const float nm = fmaxf(pm, bx * kLog2e);
-      const float ref = ms_ref(nm);
+      const float ref = ms_shift(nm);
       float acc = ms_rescale(ps, pm, nm);
 #pragma unroll
       for (int q = 0; q < U; ++q)
@@ -1103,7 +1103,7 @@ __global__ void __launch_bounds__(BLOCK) grpo_stream_kernel(RowArgs a) {
     }
     if (has_ref) {
       const float nm = fmaxf(rm, br * kLog2e);
-      const float ref = ms_ref(nm);
+      const float ref = ms_shift(nm);
       float acc = ms_rescale(rs, rm, nm);
 #pragma unroll
       for (int q = 0; q < U; ++q)
