@@ -6,9 +6,9 @@
 // (the entries' own elements are replaced by -inf where they sit in registers), and s_K from
 // the k gathered logits. Maxima are logits and sums relative to them (see term_scale). The tail's
 // mass Q_T = s_T 2^((m_T - R) k2) / s is then a sum of its own and keeps its relative precision
-// where the teacher's entries hold nearly everything (1 - sum q_i would lose it all). Per element the arithmetic is f32; what a row has once (s_K, the merge of
-// its waves' sums, log-sum-exp, the divergence) f64, since the divergence may be far below its
-// terms. Outside K the gradient is one factor of 2^((x - m_T) k2):
+// where the teacher's entries hold nearly everything (1 - sum q_i would lose it all). Per element
+// the arithmetic is f32; what a row has once (s_K, the merge of its waves' sums, the logarithms,
+// the divergence) f64, since the divergence may be far below its terms. Outside K the gradient is one factor of 2^((x - m_T) k2):
 //   forward:  c (P Q_T - p_T) / s_T,   reverse:  c (Q_T / s_T) (log(Q_T/p_T) - l),
 // with c = weight m / (loss_norm L tau) and P = sum p_i + p_T; on K each entry has its own
 // value, which takes the element's place before its vector is stored.

@@ -15,8 +15,11 @@
 // Bound by the exponentials and HBM with many rows (4096 rows of 151,936 bf16, k = 64: 202 us,
 // 6.2 TB/s; 231 while every lane looked at each vector that passed in any, 474 with thresholds from sorted
 // lists and a pass of its own for the vectors' maxima), by latency with few: one such row takes
-// 7.0 us in 10 parts and 6.5 to merge them. The merge of many long lists costs most: 192 rows,
-// k = 256, 25 + 17 us.
+// 7.9 us in 10 parts and 6.3 to merge them. The merge of many long lists costs most: 192 rows,
+// k = 256, 25 + 17 us. Rows with fewer than k logits above the masks, or of equal values, have no
+// threshold, and every element goes through the candidates' loop: 4096 rows of 151,936 with 40 tokens
+// left 961 us (plain 241 in the same run), 512 rows 213 (42), 64 rows 136 (18), one row 111 (14); so does a
+// part that holds nothing but masks: half of the vocabulary in a run, 64 rows 102, one row 92.
 
 #include <hip/hip_runtime.h>
 
