@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <cstring>
 #include <mutex>
+#include <new>
 
 #include "context.hpp"
 #include "host_transfer.hpp"
@@ -72,8 +73,12 @@ int ensure_scratch_on(pcp_ctx* ctx, size_t bytes, hipStream_t st) {
                   "the stream is being captured and the context's work buffer would have to grow from %zu to %zu bytes: "
                   "make one uncaptured call of the same sizes first",
                   ctx->scratch_bytes, bytes);
+    try {
+      ctx->graph_scratch.reserve(ctx->graph_scratch.size() + 1);   // no allocation where it is kept
+    } catch (const std::bad_alloc&) {
+      return fail(ctx, PCP_ERR_OOM, "no host memory for the list of captured work buffers");
+    }
     ctx->scratch_in_graph = true;
-    ctx->graph_scratch.reserve(ctx->graph_scratch.size() + 1);   // no allocation where it is kept
     return PCP_OK;
   }
   return ensure_scratch(ctx, bytes);
