@@ -253,3 +253,57 @@ def test_verify(dtype, mask, pattern, S, lookup):
         assert np.array_equal(out.accepted.cpu().numpy(), want[1]), t
         assert np.array_equal(out.tokens.cpu().numpy(), want[0]), t
         assert (np.abs(host64(out.logp) - want[2]) <= 2.0 ** -24 * np.abs(want[2]) + 1e-12).all(), t
+
+
+# ---- rows with one large offset ---------------------------------------------------------
+
+OFFSETS = [1e3, -1e4, 1e5, -1e6, 1e7, -3e7, 2e8, -1e9, 1.4e9, -1.6e9, 3e9, -1e10]
+
+
+def with_offset(rng, shape, offset):
+    """f32 logits a few f32 steps (at least a few units) around `offset`: a softmax like any other, whose
+    reference point's product with the scale is rounded by up to 2^6."""
+    step = max(1.0, float(np.spacing(np.float32(abs(offset)))))
+    return (offset + np.round(rng.standard_normal(shape) * 3) * step).astype(np.float32)
+
+
+@pytest.mark.parametrize("offset", OFFSETS)
+def test_rows_far_from_zero(offset):
+    rng = np.random.default_rng(3)
+    for R, V, k in ((3, 40000, 30), (600, 20000, 8)):
+        x = to_dev(with_offset(rng, (R, V), offset), "f32", 1)
+        for t in (0.7, 1.0, 2.0):
+            out = distill.top_logits(x, k, temperature=t)
+            check_top(x[:4], k, t, first_rows(out, 4))
+    for N, V in ((4, 701), (4, 40000), (900, 40000)):
+        x = with_offset(rng, (4, V), offset)
+        ids = np.stack([rng.choice(V, 12, replace=False) for _ in range(4)]).astype(np.int32)
+        t = rng.standard_normal((4, 12)).astype(np.float32) * 2
+        lse = (lse_ref(t.astype(np.float64)) + 0.3).astype(np.float32)
+        xs = torch.zeros((1, N, V), device=DEV)
+        xs[0, -4:] = to_dev(x, "f32")
+        full = lambda a, fill: torch.cat([torch.full((N - 4,) + a.shape[1:], fill, dtype=torch.from_numpy(a).dtype),
+                                          torch.from_numpy(a)])[None].to(DEV)
+        weight = torch.zeros((1, N), device=DEV)
+        weight[0, -4:] = 1.0
+        for forward in (True, False):
+            out = distill.distill_fwd_bwd(xs, full(ids, IGNORE), full(t, 0.0), full(lse, 0.0), weight,
+                                          divergence="forward" if forward else "reverse")
+            x64 = x.astype(np.float64)
+            for r in range(4):
+                l, grad, mag, lb = row_ref(x64[r] - x64[r].max(), ids[r], t[r].astype(np.float64), float(lse[r]), 1.0, forward)
+                assert abs(float(out.token_loss[0, N - 4 + r]) - l) <= lb + 2.0 ** -24 * abs(l)
+                bar = REL * mag / 4
+                off = np.abs(host64(out.dlogits[0, N - 4 + r]) - grad / 4)
+                assert (off <= bar + half_step("f32", grad / 4) + 2.0 ** -42 * np.abs(grad).max() + 2.0 ** -126).all()
+    for S in (2, 30):
+        n, V = 2, 9001
+        x = with_offset(rng, (S, n + 1, V), offset)
+        y = with_offset(rng, (S, n, V), -offset)
+        d = np.argmax(y + rng.gumbel(size=y.shape), -1).astype(np.int64)
+        u = rng.random((S, n + 1)).astype(np.float32)
+        for draft in (None, to_dev(y, "f32")):
+            out = step.verify_drafts(to_dev(x, "f32"), torch.from_numpy(d).to(DEV), draft, uniforms=torch.from_numpy(u).to(DEV))
+            want = verify_ref(x.astype(np.float64), None if draft is None else y.astype(np.float64), d, np.full(S, n), u, 1.0, V)
+            assert np.array_equal(out.accepted.cpu().numpy(), want[1]) and np.array_equal(out.tokens.cpu().numpy(), want[0])
+            assert (np.abs(host64(out.logp) - want[2]) <= 2.0 ** -24 * np.abs(want[2]) + 1e-12).all()
