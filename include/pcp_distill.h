@@ -91,8 +91,8 @@ typedef enum pcp_divergence {
  *
  * Reported after the call (or by pcp_sync): a used id outside [0, V)
  * (PCP_ERR_TOKEN_RANGE) and an id used twice in one row (PCP_ERR_INVALID_ARG), in a row
- * with weight: that row has zero dlogits and loss; a non-finite log-sum-exp or NaN in
- * the teacher's entries or a NaN loss (PCP_ERR_NONFINITE). dlogits may be the logits
+ * with weight: that row has zero dlogits and loss; a non-finite log-sum-exp, NaN in the
+ * teacher's entries, a NaN loss or a weight that is not finite (PCP_ERR_NONFINITE). dlogits may be the logits
  * themselves (their element type, the same address). Rows are summed in a fixed order:
  * the same call gives the same bits, but calls with other row counts may deal a row to
  * other numbers of workgroups, so a row's last bits depend on the call's size.

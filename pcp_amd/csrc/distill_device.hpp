@@ -315,7 +315,7 @@ __device__ __forceinline__ void prepare_row(const DistillArgs& a, int64_t row) {
   if (lane != 0) return;
   a.teacher[row] = o;
   if (o.state == kBad) raise_error(a.err, kErrTokenRange);
-  else if (o.state == kUsed && !(__builtin_isfinite(o.lse) && __builtin_isfinite(o.sum_p)))
+  else if (o.state == kUsed && !(__builtin_isfinite(o.lse) && __builtin_isfinite(o.sum_p) && __builtin_isfinite(o.w)))
     raise_error(a.err, kErrNonFinite);
 }
 

@@ -95,3 +95,19 @@ def test_loss_alone_into_outputs_that_have_dlogits():
     assert out.dlogits is kept and bool((kept == 7.0).all())
     distill.distill_fwd_bwd(x, top.ids, top.values, top.lse, outputs=out, dlogits=kept, dlogits_dtype=torch.float32)
     assert not bool((kept == 7.0).any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,want_dlogits", [(700, True), (40000, True), (40000, False)])
+@pytest.mark.parametrize("weight", [float("nan"), float("inf")])
+def test_weights_that_are_not_finite_are_reported(V, want_dlogits, weight):
+    dev = torch.device("cuda:0")
+    x, t = torch.randn((2, 3, V), device=dev), torch.randn((2, 3, V), device=dev)
+    top, mask = distill.top_logits(t, 9), torch.ones((2, 3), device=dev)
+    distill.distill_fwd_bwd(x, top.ids, top.values, top.lse, mask, want_dlogits=want_dlogits)
+    mask[1, 2] = weight
+    with pytest.raises(PcpError) as e:
+        distill.distill_fwd_bwd(x, top.ids, top.values, top.lse, mask, want_dlogits=want_dlogits)
+    assert e.value.code == -4
+    top.ids[1, 2] = -100                       # a row without entries has no loss, whatever its weight
+    distill.distill_fwd_bwd(x, top.ids, top.values, top.lse, mask, want_dlogits=want_dlogits)
