@@ -696,8 +696,10 @@ static_assert(kPickAlongWorkgroups / kNarrowParts <= kPickAlongNarrow, "a count 
 //                     20,672: 3.6 121 | 140   5.8 133 | 137   7.3 141 | 135   8 140 | 134
 //   of 4, looked up    6,080: 0    47 |  61   0.9  59 |  61   2.4  66 |  61   4  72 |  61
 //                     12,160: 0    68 | 100   1.0  83 |  99   2.3  97 | 100   4 109 |  99
-// Looked-up tokens are refused more often than a model's.
-constexpr int64_t kSplitWorkgroupsModel = 16384, kSplitWorkgroupsLookup = 8192;
+// Drafts that are mostly accepted lose a tenth by it, those that are refused early gain more: 14,079
+// workgroups of a model's draft with about half of the tokens accepted take 100 | 110, and looked-up
+// tokens are refused more often than a model's.
+constexpr int64_t kSplitWorkgroups = 8192;
 
 bool picks_along(int64_t n_seq, int64_t nv) {
   const int64_t parts = std::max<int64_t>((nv + end_vecs(1) - 1) / end_vecs(1), 1);
@@ -713,9 +715,7 @@ hipError_t launch_verify(VerifyArgs a, int64_t n_seq, hipStream_t st) {
     verify_greedy_kernel<<<seqs, dim3(kGreedyBlock), 0, st>>>(a);
     return hipGetLastError();
   }
-  const bool split = a.draft ? n_seq * (2 * a.n + 1) * a.parts > kSplitWorkgroupsModel
-                             : n_seq * (a.n + 1) * a.parts > kSplitWorkgroupsLookup;
-  const int first = split ? (a.n + 1) / 2 : 0;
+  const int first = n_seq * (a.draft ? 2 * a.n + 1 : a.n + 1) * a.parts > kSplitWorkgroups ? (a.n + 1) / 2 : 0;
   for (int from = 0, to = first ? first : a.n + 1; from <= a.n; from = to, to = a.n + 1) {
     a.from = from;
     const unsigned rows = static_cast<unsigned>(to - from);
