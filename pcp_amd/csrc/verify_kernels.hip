@@ -43,14 +43,14 @@ constexpr int kNW = kBlock / 64;
 
 // A part of a row.
 struct RowState {
-  double sum;   // greedy: unused
+  double sum;   // with the terms' ref (see scale64); greedy: unused
   float max;
   int32_t at;   // greedy: the first maximum's index; sampling: its log-sum-exp is not finite
 };
 
 // Token i of a sequence, and its rows.
 struct Decision {
-  double sum_p, sum_q;   // sum e of the target row, of the draft row
+  double sum_p, sum_q;   // sum e of the target row, of the draft row, with the terms' ref (see scale64)
   float max_p, max_q;
   float logp;            // of the drafted token
   int32_t flags;
@@ -61,7 +61,7 @@ constexpr int kAccepted = 1, kInRange = 2, kBadP = 4, kBadQ = 8;
 struct SeqEnd {
   double scale_p, scale_q;   // 1 / sum e of the target row, of the draft row (0: q is 0)
   float max_p, max_q;
-  double log_p;              // log of the target row's sum e
+  double sum_p;
   int32_t j;                 // accepted tokens
   int32_t without;           // a lookup's refused token (r is 0 there), or -1
 };
@@ -83,12 +83,9 @@ struct VerifyArgs {
   int* err;
   int64_t vocab, tstride, dstride, tseq, dseq;   // elements: between rows, between sequences
   double k;                   // log2(e) / temperature
-  double inv_t;
   float plain;                // see scale64
   int32_t n;
   int32_t parts, end_parts;   // of kPartVecs, end_vecs vectors
-  int32_t greedy;
-  int32_t along;              // the residual's last workgroup picks the token
   int32_t from;               // the first token of this launch
 };
 
@@ -156,16 +153,28 @@ static_assert(kTable == 1 << 7, "");
 struct Scale64 {
   double k, ref;
 };
+__device__ __forceinline__ bool is_plain(const VerifyArgs& a, float m) { return fabsf(m) < a.plain; }   // not +inf
+__device__ __forceinline__ Scale64 plain_scale(const VerifyArgs& a, float m) {
+  return Scale64{a.k * kTable, m * (a.k * kTable)};
+}
+__device__ __forceinline__ Scale64 exact_scale(float m) {
+  const double k = __builtin_amdgcn_ldexp(1., 43 - __builtin_amdgcn_frexp_expf(m));
+  return Scale64{k, m * k};
+}
+// max: the same in every lane of a wave, so that this is a branch.
 __device__ __forceinline__ Scale64 scale64(const VerifyArgs& a, float max) {
   const float m = ms_ref(max);
-  Scale64 t{a.k * kTable, 0.};
-  if (!(fabsf(m) < a.plain))   // also +inf
-    t.k = __builtin_amdgcn_ldexp(1., 43 - __builtin_amdgcn_frexp_expf(m));
-  t.ref = m * t.k;
+  Scale64 t = plain_scale(a, m);
+  if (__any(!is_plain(a, m))) t = exact_scale(m);
   return t;
 }
 __device__ __forceinline__ double adj(float max, const Scale64& t) {
   return fma(fma(static_cast<double>(ms_ref(max)), t.k, -t.ref), -0.69314718055994530942 / kTable, 1.);
+}
+
+// The same for a part or a row of the lane's own.
+__device__ __forceinline__ double row_adj(const VerifyArgs& a, float max) {
+  return is_plain(a, max) ? adj(max, plain_scale(a, max)) : 1.;
 }
 
 template <typename TI>
@@ -332,7 +341,7 @@ __global__ void __launch_bounds__(kBlock) verify_rows_kernel(VerifyArgs a, int r
 #pragma unroll
       for (int j = 0; j < EPV; ++j) sum = term(TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j), sum);
   sum = block_sum64<BLOCK>(sum, lds);
-  if (tid == 0) a.part[(token * 2 + is_draft) * a.parts + part] = RowState{sum * adj(m, at), m, nan};
+  if (tid == 0) a.part[(token * 2 + is_draft) * a.parts + part] = RowState{sum, m, nan};
 }
 
 // ---- decide ----------------------------------------------------------------------------
@@ -358,7 +367,9 @@ __global__ void __launch_bounds__(kDecideBlock) verify_decide_kernel(VerifyArgs 
     mm = lanes_max<64>(mm);
     double sum = 0.;
     for (int q = lane; q < a.parts; q += 64)
-      if (p[q].max > kNegInf) sum += p[q].sum * exp2_64((static_cast<double>(p[q].max) - static_cast<double>(mm)) * a.k);
+      if (p[q].max > kNegInf)
+        sum += p[q].sum * row_adj(a, p[q].max) *
+               exp2_64((static_cast<double>(p[q].max) - static_cast<double>(mm)) * a.k);
     sum = wave_sum64(sum);
     bad = __any(bad != 0) || !(__builtin_isfinite(mm) && __builtin_isfinite(sum));
     if (lane == 0) whole[i] = RowState{sum, mm, bad};
@@ -372,7 +383,8 @@ __global__ void __launch_bounds__(kDecideBlock) verify_decide_kernel(VerifyArgs 
     const RowState p = whole[2 * tid], q = model ? whole[2 * tid + 1] : RowState{1., 0.f, 0};
     const int64_t d = drafted ? a.ids[s * a.n + i] : 0;
     const bool in = d >= 0 && d < a.vocab;
-    Decision o{p.sum, q.sum, p.max, q.max, 0.f, (in ? kInRange : 0) | (p.at ? kBadP : 0) | (q.at ? kBadQ : 0)};
+    Decision o{p.sum / row_adj(a, p.max), q.sum / row_adj(a, q.max), p.max, q.max, 0.f,
+               (in ? kInRange : 0) | (p.at ? kBadP : 0) | (q.at ? kBadQ : 0)};
     if (drafted && in && !p.at && !q.at) {
       const double y = (static_cast<double>(TI::load1(target_row<TI>(a, s, i), d)) - p.max) * a.k;
       double qd = 1.;
@@ -411,8 +423,12 @@ struct Residual {
 };
 
 __device__ __forceinline__ Residual residual(const VerifyArgs& a, const SeqEnd& e, bool plain, const double* table) {
-  const Scale64 p = scale64(a, e.max_p), q = scale64(a, e.max_q);
-  return Residual{p, q, e.scale_p * adj(e.max_p, p), e.scale_q * adj(e.max_q, q), e.without, plain, table};
+  Residual r{plain_scale(a, e.max_p), plain_scale(a, e.max_q), e.scale_p, e.scale_q, e.without, plain, table};
+  if (__any(!(is_plain(a, e.max_p) && is_plain(a, e.max_q)))) {   // one branch for both
+    r.p = scale64(a, e.max_p);
+    r.q = scale64(a, e.max_q);
+  }
+  return r;
 }
 
 // The elements of a part: both rows' values, in element order per (chunk, lane, element). The
@@ -469,6 +485,7 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e,
   const bool plain = !(total > 0.);
   const Residual r = residual(a, e, plain, table);
   const double t = u * (plain ? 1. : total);
+  const double log_p = log(e.sum_p * adj(e.max_p, r.p));   // ahead of the scans' loads
   int hit = -1, last_seg = -1;
   double before = 0.;
   if (!plain) {
@@ -563,7 +580,8 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e,
     if (pick < 0) pick = static_cast<int>(a.vocab) - 1;
     const int64_t at = s * (a.n + 1) + e.j;
     a.tokens[at] = pick;
-    if (a.logp) a.logp[at] = static_cast<float>((static_cast<double>(TI::load1(row, pick)) - e.max_p) * a.inv_t - e.log_p);
+    if (a.logp) a.logp[at] = static_cast<float>((static_cast<double>(TI::load1(row, pick)) - e.max_p) * a.k * 0.69314718055994530942 -
+                                             log_p);
   }
 }
 
@@ -586,10 +604,10 @@ __device__ __forceinline__ bool seq_end(const VerifyArgs& a, int64_t s, SeqEnd& 
   }
   const bool refused = j < len, in = at.flags & kInRange;
   const bool model = refused && a.draft && in && !(at.flags & kBadQ);
-  e.j = j;
+  e.j = __builtin_amdgcn_readfirstlane(j);   // (its rows' addresses by scalar products)
   e.max_p = at.max_p;
   e.scale_p = 1. / at.sum_p;
-  e.log_p = log(at.sum_p);
+  e.sum_p = at.sum_p;
   e.max_q = model ? at.max_q : 0.f;
   e.scale_q = model ? 1. / at.sum_q : 0.;
   e.without = refused && !a.draft && in ? static_cast<int32_t>(a.ids[s * a.n + j]) : -1;
@@ -707,10 +725,10 @@ bool picks_along(int64_t n_seq, int64_t nv) {
 }
 
 template <typename TI>
-hipError_t launch_verify(VerifyArgs a, int64_t n_seq, hipStream_t st) {
+hipError_t launch_verify(VerifyArgs a, int64_t n_seq, bool greedy, bool along, hipStream_t st) {
   const unsigned ns = static_cast<unsigned>(n_seq), parts = static_cast<unsigned>(a.parts);
   const dim3 b(kBlock), seqs(ns);
-  if (a.greedy) {
+  if (greedy) {
     verify_first_max_kernel<TI><<<dim3(parts, ns, static_cast<unsigned>(a.n + 1)), b, 0, st>>>(a);
     verify_greedy_kernel<<<seqs, dim3(kGreedyBlock), 0, st>>>(a);
     return hipGetLastError();
@@ -723,7 +741,7 @@ hipError_t launch_verify(VerifyArgs a, int64_t n_seq, hipStream_t st) {
     verify_decide_kernel<TI><<<seqs, dim3(kDecideBlock), 0, st>>>(a, to);
   }
   const dim3 ends(static_cast<unsigned>(a.end_parts), ns);
-  if (a.along) {
+  if (along) {
     verify_residual_kernel<TI, 1, true><<<ends, b, 0, st>>>(a);
   } else {
     verify_residual_kernel<TI, 2, false><<<ends, b, 0, st>>>(a);
@@ -849,19 +867,16 @@ int verify_drafts(pcp_ctx* ctx, const pcp_verify_args* a) {
   v.dstride = ds;
   v.tseq = tseq;
   v.dseq = dseq;
-  v.inv_t = greedy ? 1. : 1. / static_cast<double>(a->temperature);
-  v.k = 1.4426950408889634074 * v.inv_t;
+  v.k = 1.4426950408889634074 * (greedy ? 1. : 1. / static_cast<double>(a->temperature));
   const double plain = 0x1p42 / (v.k * kTable);
   v.plain = plain < static_cast<double>(FLT_MAX) ? static_cast<float>(plain) : HUGE_VALF;
   v.n = static_cast<int32_t>(a->n_draft);
   v.parts = static_cast<int32_t>(parts);
   v.end_parts = static_cast<int32_t>(end_parts);
-  v.greedy = greedy;
-  v.along = along;
   const bool timed = prof_begin(ctx, st);
-  const hipError_t e = a->logits_dtype == PCP_F32    ? launch_verify<F32T>(v, a->n_seq, st)
-                       : a->logits_dtype == PCP_BF16 ? launch_verify<BF16T>(v, a->n_seq, st)
-                                                     : launch_verify<F16T>(v, a->n_seq, st);
+  const hipError_t e = a->logits_dtype == PCP_F32    ? launch_verify<F32T>(v, a->n_seq, greedy, along, st)
+                       : a->logits_dtype == PCP_BF16 ? launch_verify<BF16T>(v, a->n_seq, greedy, along, st)
+                                                     : launch_verify<F16T>(v, a->n_seq, greedy, along, st);
   prof_end(ctx, st, timed);
   if (e != hipSuccess) return hip_fail(ctx, e, "draft verification launch");
   return finish_call(ctx, a->flags, st);
