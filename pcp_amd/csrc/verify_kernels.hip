@@ -66,6 +66,8 @@ struct SeqEnd {
   int32_t without;           // a lookup's refused token (r is 0 there), or -1
 };
 
+// With a kernel's own argument within three cache lines: a fourth, which holds that argument, took the
+// decision's kernel from 4.8 to 5.1 us.
 struct VerifyArgs {
   const void* target;
   const void* draft;          // nullptr: all of q on the drafted token
@@ -88,6 +90,7 @@ struct VerifyArgs {
   int32_t parts, end_parts;   // of kPartVecs, end_vecs vectors
   int32_t from;               // the first token of this launch
 };
+static_assert(sizeof(VerifyArgs) + sizeof(int) <= 192, "");
 
 // 2^y for y <= 0 (0 below 2^-1075, NaN kept): 2^n times a polynomial in y - n that meets 2^f in the
 // 11 Chebyshev points of [-1/2, 1/2]. Relative error 4.0e-16 at most of 40,000 arguments, against 60
@@ -145,36 +148,24 @@ struct Exp2 {
 };
 static_assert(kTable == 1 << 7, "");
 
-// Terms 2^((x - max) k) of Exp2 as 2^(fma(x, k', -ref) / 128), one instruction. Up to |max| =
+// Terms 2^((x - max) k) of Exp2 as 2^(fma(x, k', -ref) / 128), one instruction. Below |max| =
 // a.plain ref is the rounded product with k' = 128 k, below 2^42 and so off by at most 2^-12 (a row
 // all at a mask such as -1e30 would otherwise have a product off by 2^50, and anything for a term);
-// adj() takes its rounding out of a sum. From there on two f32 logits that differ at all lie 2^2048
-// apart: k' is the power of two that takes max to [2^42, 2^43), and the product exact.
+// where sums of different ref meet, adj() takes that out. From there on two f32 logits that differ
+// at all lie 2^2048 apart, whatever k' is from 128 k up: it is the next power of two, and the product
+// exact.
 struct Scale64 {
   double k, ref;
 };
-__device__ __forceinline__ bool is_plain(const VerifyArgs& a, float m) { return fabsf(m) < a.plain; }   // not +inf
-__device__ __forceinline__ Scale64 plain_scale(const VerifyArgs& a, float m) {
-  return Scale64{a.k * kTable, m * (a.k * kTable)};
-}
-__device__ __forceinline__ Scale64 exact_scale(float m) {
-  const double k = __builtin_amdgcn_ldexp(1., 43 - __builtin_amdgcn_frexp_expf(m));
-  return Scale64{k, m * k};
-}
-// max: the same in every lane of a wave, so that this is a branch.
 __device__ __forceinline__ Scale64 scale64(const VerifyArgs& a, float max) {
   const float m = ms_ref(max);
-  Scale64 t = plain_scale(a, m);
-  if (__any(!is_plain(a, m))) t = exact_scale(m);
-  return t;
+  double k = a.k * kTable;
+  if (!(fabsf(m) < a.plain)) k = __builtin_amdgcn_ldexp(1., __builtin_amdgcn_frexp_exp(k));   // also +inf
+  return Scale64{k, m * k};
 }
-__device__ __forceinline__ double adj(float max, const Scale64& t) {
-  return fma(fma(static_cast<double>(ms_ref(max)), t.k, -t.ref), -0.69314718055994530942 / kTable, 1.);
-}
-
-// The same for a part or a row of the lane's own.
-__device__ __forceinline__ double row_adj(const VerifyArgs& a, float max) {
-  return is_plain(a, max) ? adj(max, plain_scale(a, max)) : 1.;
+__device__ __forceinline__ double adj(const VerifyArgs& a, float max) {
+  const double m = max, k = a.k * kTable;
+  return fabsf(max) < a.plain ? fma(fma(m, k, -(m * k)), -0.69314718055994530942 / kTable, 1.) : 1.;
 }
 
 template <typename TI>
@@ -368,7 +359,7 @@ __global__ void __launch_bounds__(kDecideBlock) verify_decide_kernel(VerifyArgs 
     double sum = 0.;
     for (int q = lane; q < a.parts; q += 64)
       if (p[q].max > kNegInf)
-        sum += p[q].sum * row_adj(a, p[q].max) *
+        sum += p[q].sum * adj(a, p[q].max) *
                exp2_64((static_cast<double>(p[q].max) - static_cast<double>(mm)) * a.k);
     sum = wave_sum64(sum);
     bad = __any(bad != 0) || !(__builtin_isfinite(mm) && __builtin_isfinite(sum));
@@ -383,7 +374,7 @@ __global__ void __launch_bounds__(kDecideBlock) verify_decide_kernel(VerifyArgs 
     const RowState p = whole[2 * tid], q = model ? whole[2 * tid + 1] : RowState{1., 0.f, 0};
     const int64_t d = drafted ? a.ids[s * a.n + i] : 0;
     const bool in = d >= 0 && d < a.vocab;
-    Decision o{p.sum / row_adj(a, p.max), q.sum / row_adj(a, q.max), p.max, q.max, 0.f,
+    Decision o{p.sum / adj(a, p.max), q.sum / adj(a, q.max), p.max, q.max, 0.f,
                (in ? kInRange : 0) | (p.at ? kBadP : 0) | (q.at ? kBadQ : 0)};
     if (drafted && in && !p.at && !q.at) {
       const double y = (static_cast<double>(TI::load1(target_row<TI>(a, s, i), d)) - p.max) * a.k;
@@ -423,12 +414,7 @@ struct Residual {
 };
 
 __device__ __forceinline__ Residual residual(const VerifyArgs& a, const SeqEnd& e, bool plain, const double* table) {
-  Residual r{plain_scale(a, e.max_p), plain_scale(a, e.max_q), e.scale_p, e.scale_q, e.without, plain, table};
-  if (__any(!(is_plain(a, e.max_p) && is_plain(a, e.max_q)))) {   // one branch for both
-    r.p = scale64(a, e.max_p);
-    r.q = scale64(a, e.max_q);
-  }
-  return r;
+  return Residual{scale64(a, e.max_p), scale64(a, e.max_q), e.scale_p, e.scale_q, e.without, plain, table};
 }
 
 // The elements of a part: both rows' values, in element order per (chunk, lane, element). The
@@ -485,7 +471,7 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e,
   const bool plain = !(total > 0.);
   const Residual r = residual(a, e, plain, table);
   const double t = u * (plain ? 1. : total);
-  const double log_p = log(e.sum_p * adj(e.max_p, r.p));   // ahead of the scans' loads
+  const double log_p = log(e.sum_p * adj(a, e.max_p));   // ahead of the scans' loads
   int hit = -1, last_seg = -1;
   double before = 0.;
   if (!plain) {
@@ -621,7 +607,7 @@ __device__ __forceinline__ bool last_of(unsigned* count, int n) {
 
 // PICK: the sequence's last workgroup picks the token.
 template <typename TI, int U, bool PICK>
-__global__ void __launch_bounds__(kBlock) verify_residual_kernel(VerifyArgs a) {
+__device__ __forceinline__ void residual_part(const VerifyArgs& a) {
   __shared__ double table[kTable];
   __shared__ double lds[kNW];
   __shared__ int last;
@@ -683,6 +669,18 @@ __global__ void __launch_bounds__(kBlock) verify_residual_kernel(VerifyArgs a) {
   }
 }
 
+// Scalar registers come in sixteens, of 800 a SIMD, and sixteen more of a wave's are the trap handler's: past
+// 80 a CU holds 7 workgroups, not 8, and 1,976 of them take 12.7 us instead of 11.5.
+template <typename TI>
+__global__ void __launch_bounds__(kBlock) __attribute__((amdgpu_num_sgpr(80))) verify_residual_kernel(VerifyArgs a) {
+  residual_part<TI, 2, false>(a);
+}
+// Few workgroups: with the same limit one sequence takes 21.5 us instead of 20.5.
+template <typename TI>
+__global__ void __launch_bounds__(kBlock) verify_residual_pick_kernel(VerifyArgs a) {
+  residual_part<TI, 1, true>(a);
+}
+
 template <typename TI, int U>
 __global__ void __launch_bounds__(kBlock) verify_pick_kernel(VerifyArgs a) {
   __shared__ double table[kTable];
@@ -742,9 +740,9 @@ hipError_t launch_verify(VerifyArgs a, int64_t n_seq, bool greedy, bool along, h
   }
   const dim3 ends(static_cast<unsigned>(a.end_parts), ns);
   if (along) {
-    verify_residual_kernel<TI, 1, true><<<ends, b, 0, st>>>(a);
+    verify_residual_pick_kernel<TI><<<ends, b, 0, st>>>(a);
   } else {
-    verify_residual_kernel<TI, 2, false><<<ends, b, 0, st>>>(a);
+    verify_residual_kernel<TI><<<ends, b, 0, st>>>(a);
     verify_pick_kernel<TI, 2><<<seqs, b, 0, st>>>(a);
   }
   return hipGetLastError();
@@ -755,7 +753,7 @@ inline bool misaligned(const void* p, int size) {
 }
 inline size_t round256(size_t b) { return (b + 255) & ~static_cast<size_t>(255); }
 
-// The counts that verify_residual_kernel leaves at zero, one per sequence: at most kPickAlongNarrow.
+// The counts that verify_residual_pick_kernel leaves at zero, one per sequence: at most kPickAlongNarrow.
 int ensure_verify_done(pcp_ctx* ctx, hipStream_t st) {
   if (ctx->verify_done) return PCP_OK;
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
