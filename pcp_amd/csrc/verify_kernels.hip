@@ -61,7 +61,7 @@ constexpr int kAccepted = 1, kInRange = 2, kBadP = 4, kBadQ = 8;
 struct SeqEnd {
   double scale_p, scale_q;   // 1 / sum e of the target row, of the draft row (0: q is 0)
   float max_p, max_q;
-  double sum_p;
+  double log_p;              // log of the target row's sum
   int32_t j;                 // accepted tokens
   int32_t without;           // a lookup's refused token (r is 0 there), or -1
 };
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kDecideBlock) verify_decide_kernel(VerifyArgs 
     const RowState p = whole[2 * tid], q = model ? whole[2 * tid + 1] : RowState{1., 0.f, 0};
     const int64_t d = drafted ? a.ids[s * a.n + i] : 0;
     const bool in = d >= 0 && d < a.vocab;
-    Decision o{p.sum / adj(a, p.max), q.sum / adj(a, q.max), p.max, q.max, 0.f,
+    Decision o{p.sum * (2. - adj(a, p.max)), q.sum * (2. - adj(a, q.max)), p.max, q.max, 0.f,   // 1 / adj
                (in ? kInRange : 0) | (p.at ? kBadP : 0) | (q.at ? kBadQ : 0)};
     if (drafted && in && !p.at && !q.at) {
       const double y = (static_cast<double>(TI::load1(target_row<TI>(a, s, i), d)) - p.max) * a.k;
@@ -471,7 +471,6 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e,
   const bool plain = !(total > 0.);
   const Residual r = residual(a, e, plain, table);
   const double t = u * (plain ? 1. : total);
-  const double log_p = log(e.sum_p * adj(a, e.max_p));   // ahead of the scans' loads
   int hit = -1, last_seg = -1;
   double before = 0.;
   if (!plain) {
@@ -567,7 +566,7 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e,
     const int64_t at = s * (a.n + 1) + e.j;
     a.tokens[at] = pick;
     if (a.logp) a.logp[at] = static_cast<float>((static_cast<double>(TI::load1(row, pick)) - e.max_p) * a.k * 0.69314718055994530942 -
-                                             log_p);
+                                             e.log_p);
   }
 }
 
@@ -590,10 +589,10 @@ __device__ __forceinline__ bool seq_end(const VerifyArgs& a, int64_t s, SeqEnd& 
   }
   const bool refused = j < len, in = at.flags & kInRange;
   const bool model = refused && a.draft && in && !(at.flags & kBadQ);
-  e.j = __builtin_amdgcn_readfirstlane(j);   // (its rows' addresses by scalar products)
+  e.j = j;
   e.max_p = at.max_p;
   e.scale_p = 1. / at.sum_p;
-  e.sum_p = at.sum_p;
+  e.log_p = log(at.sum_p * adj(a, at.max_p));
   e.max_q = model ? at.max_q : 0.f;
   e.scale_q = model ? 1. / at.sum_q : 0.;
   e.without = refused && !a.draft && in ? static_cast<int32_t>(a.ids[s * a.n + j]) : -1;
