@@ -8,7 +8,8 @@
 // mass Q_T = s_T 2^((m_T - R) k2) / s is then a sum of its own and keeps its relative precision
 // where the teacher's entries hold nearly everything (1 - sum q_i would lose it all). Per element
 // the arithmetic is f32; what a row has once (s_K, the merge of its waves' sums, the logarithms,
-// the divergence) f64, since the divergence may be far below its terms. Outside K the gradient is one factor of 2^((x - m_T) k2):
+// the divergence) f64, since the divergence may be far below its terms. Outside K the gradient is
+// one factor of 2^((x - m_T) k2):
 //   forward:  c (P Q_T - p_T) / s_T,   reverse:  c (Q_T / s_T) (log(Q_T/p_T) - l),
 // with c = weight m / (loss_norm L tau) and P = sum p_i + p_T; on K each entry has its own
 // value, which takes the element's place before its vector is stored.
@@ -344,7 +345,8 @@ void launch_prepare(const DistillArgs& a, hipStream_t st) {
   constexpr int64_t kMost = (int64_t{1} << 31) / kPrepBlock;
   const int64_t blocks = prepare_blocks(a);
   for (int64_t b = 0; b < blocks; b += kMost)
-    distill_prepare_kernel<TI><<<dim3(static_cast<unsigned>(std::min(blocks - b, kMost))), dim3(kPrepBlock), 0, st>>>(a, b);
+    distill_prepare_kernel<TI>
+        <<<dim3(static_cast<unsigned>(std::min(blocks - b, kMost))), dim3(kPrepBlock), 0, st>>>(a, b);
 }
 
 // ---- a row's terms -----------------------------------------------------------------------

@@ -565,8 +565,8 @@ __device__ __forceinline__ void pick_token(const VerifyArgs& a, const SeqEnd& e,
     if (pick < 0) pick = static_cast<int>(a.vocab) - 1;
     const int64_t at = s * (a.n + 1) + e.j;
     a.tokens[at] = pick;
-    if (a.logp) a.logp[at] = static_cast<float>((static_cast<double>(TI::load1(row, pick)) - e.max_p) * a.k * 0.69314718055994530942 -
-                                             e.log_p);
+    const double below = static_cast<double>(TI::load1(row, pick)) - e.max_p;
+    if (a.logp) a.logp[at] = static_cast<float>(below * a.k * 0.69314718055994530942 - e.log_p);
   }
 }
 
