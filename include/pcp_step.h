@@ -63,6 +63,50 @@ int pcp_grad_stats_compute(pcp_ctx* ctx, const float* grad, int64_t n, int accum
 int pcp_grad_stats_compute_many(pcp_ctx* ctx, int n_tensors, const float* const* grads, const int64_t* counts,
                                 int accumulate, pcp_grad_stats* stats, void* stream);
 
+/* ---- gradient norm and clipping -----------------------------------------------------
+ * No counterpart in the reference, which logs the norm (pcp_grad_stats_compute) and never
+ * clips. Over all elements of n_tensors tensors together:
+ *   norm = sqrt(sum g^2) (PCP_NORM_L2) or max |g| (PCP_NORM_MAX)
+ *   coef = max_norm / norm where norm > max_norm, else 1
+ *   out  = coef * g
+ * norm and coef stay on the device: pcp_nesterov_update_many takes coef there, so that a step
+ * waits nowhere. The sum of squares runs in f64 in a fixed order; norm and coef are rounded to
+ * f32 once, out from the f32 product. A norm that is not finite as an f32 (a NaN or infinite
+ * gradient among them) is reported as PCP_ERR_NONFINITE after the call (or by pcp_sync): coef is
+ * NaN then and out holds the gradients as they are. Without elements norm is 0.
+ *
+ * The arrays are host memory, read during the call; what they point to is device memory, at any
+ * element's address. Every out[i] is either grads[i] in the same type (in place) or overlaps
+ * no gradient and no other output. A gradient may stand in the list twice where there is no
+ * output. Synchronous unless PCP_FLAG_ASYNC is set. The call allocates no device memory, and can be
+ * captured in a HIP graph, with the pointers that it was given. */
+typedef enum {
+  PCP_NORM_L2 = 0,
+  PCP_NORM_MAX = 1
+} pcp_norm_type;
+
+/* Most tensors in the lists of pcp_grad_clip and pcp_nesterov_update_many. */
+#define PCP_GRAD_MAX_TENSORS 262144
+
+typedef struct pcp_grad_clip_args {
+  int64_t n_tensors;            /* 0 .. PCP_GRAD_MAX_TENSORS                              */
+  const void* const* grads;     /* [n_tensors]                                            */
+  const int64_t* counts;        /* [n_tensors] elements, 0 allowed (its pointers are unused) */
+  const int32_t* dtypes;        /* [n_tensors] PCP_F32 | PCP_BF16 | PCP_F16; NULL => all f32 */
+  void* const* out;             /* [n_tensors], or NULL: norm and coef alone              */
+  const int32_t* out_dtypes;    /* [n_tensors]; NULL => the gradients' types              */
+  float* norm;                  /* device scalar                                          */
+  float* coef;                  /* device scalar                                          */
+  int32_t norm_type;            /* pcp_norm_type                                          */
+  float max_norm;               /* > 0; infinity: coef is 1                               */
+  uint32_t flags;               /* PCP_FLAG_ASYNC                                         */
+  void* stream;                 /* hipStream_t; NULL => the default stream                */
+} pcp_grad_clip_args;
+
+/* Defaults: f32 types, no outputs, PCP_NORM_L2, max_norm infinite. */
+void pcp_grad_clip_args_init(pcp_grad_clip_args* a);
+int pcp_grad_clip(pcp_ctx* ctx, const pcp_grad_clip_args* a);
+
 /* ---- Nesterov optimizer on HBM (src/optimizers/nesterov.zig) ---------------------- */
 typedef enum {
   /* Host Nesterov used by RLShepherd (nesterov.zig:86-97), strict f32 rounding:
@@ -95,6 +139,37 @@ int pcp_nesterov_update(pcp_nesterov* opt, int index, float* param, const float*
  * No reference counterpart: the reference loops update() over the tensors. */
 int pcp_nesterov_update_flat(pcp_nesterov* opt, float* params, const float* grads, void* param_bf16,
                              void* stream);
+/* The update of n_tensors tensors where they lie, in a few launches: parameters, velocities (f32)
+ * and gradients as lists, the gradients as the backward pass left them and times *coef, rounded
+ * to f32 before it enters the formulas above. No counterpart in the reference, whose parameters
+ * are one flat buffer. A coef that is not finite leaves parameters, velocities and copies as they
+ * are (the step after gradients that pcp_grad_clip has reported is skipped).
+ *
+ * The arrays are host memory, read during the call. params[i], velocities[i] and param_copies[i]
+ * overlap nothing else in the lists. Synchronous unless PCP_FLAG_ASYNC is set. The call allocates
+ * no device memory, and can be captured in a HIP graph, with the pointers that it was given.
+ * pcp_nesterov_velocity gives the place of an optimizer's velocities, so that its tensors can be
+ * updated in this way too and still be serialized. */
+typedef struct pcp_nesterov_many_args {
+  int64_t n_tensors;            /* 0 .. PCP_GRAD_MAX_TENSORS                              */
+  const int64_t* counts;        /* [n_tensors] elements, 0 allowed (its pointers are unused) */
+  float* const* params;         /* [n_tensors] f32 master weights                         */
+  float* const* velocities;     /* [n_tensors]                                            */
+  const void* const* grads;     /* [n_tensors]                                            */
+  const int32_t* dtypes;        /* [n_tensors] of grads: PCP_F32 | PCP_BF16 | PCP_F16; NULL => all f32 */
+  void* const* param_copies;    /* [n_tensors] the updated weights as bf16 (an entry may be NULL), or NULL */
+  const float* coef;            /* device scalar, or NULL: 1                              */
+  float learning_rate, momentum;
+  int32_t mode;                 /* pcp_nesterov_mode                                      */
+  uint32_t flags;               /* PCP_FLAG_ASYNC                                         */
+  void* stream;                 /* hipStream_t; NULL => the default stream                */
+} pcp_nesterov_many_args;
+
+/* Defaults: f32 gradients, learning rate 0.01, momentum 0.9, PCP_NESTEROV_SUTSKEVER. */
+void pcp_nesterov_many_args_init(pcp_nesterov_many_args* a);
+int pcp_nesterov_update_many(pcp_ctx* ctx, const pcp_nesterov_many_args* a);
+/* Device address of tensor `index`'s velocities (counts[index] f32); NULL where there is none. */
+float* pcp_nesterov_velocity(pcp_nesterov* opt, int index);
 /* Total velocity elements and the serialized size in bytes (4 per element). */
 int64_t pcp_nesterov_total(const pcp_nesterov* opt);
 /* ~ serialize (:101-115): the velocities, tensor after tensor, into host memory of

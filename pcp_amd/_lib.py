@@ -49,6 +49,8 @@ FLAG_NO_ZERO_FILL = 0x2
 FLAG_FORCE_STREAMING = 0x4
 FLAG_EXACT_BF16 = 0x8
 TOP_LOGITS_MAX = 256
+SCORE_TOP_MAX = 256
+GRAD_MAX_TENSORS = 262144
 VERIFY_MAX_DRAFT = 64
 NOALLOC_SCRATCH_BYTES = 4 << 20
 IGNORE_INDEX = -100
@@ -167,6 +169,63 @@ class VerifyArgs(ctypes.Structure):
     ]
 
 
+class ScoreArgs(ctypes.Structure):
+    """pcp_score_args (include/pcp_score.h)."""
+    _fields_ = [
+        ("n_seq", ctypes.c_int64), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64), ("seq_stride", ctypes.c_int64),
+        ("tok_seq_stride", ctypes.c_int64), ("tok_offset", ctypes.c_int64),
+        ("k", ctypes.c_int32), ("logits_dtype", ctypes.c_int32), ("ids_dtype", ctypes.c_int32),
+        ("mask_dtype", ctypes.c_int32), ("top_ids_dtype", ctypes.c_int32), ("temperature", ctypes.c_float),
+        ("logits", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+        ("logp", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("row_max", ctypes.c_void_p),
+        ("log_sum", ctypes.c_void_p), ("top_logp", ctypes.c_void_p), ("top_ids", ctypes.c_void_p),
+        ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
+    ]
+
+
+class ScoreBwdArgs(ctypes.Structure):
+    """pcp_score_bwd_args (include/pcp_score.h)."""
+    _fields_ = [
+        ("n_seq", ctypes.c_int64), ("rows", ctypes.c_int64), ("logit_rows", ctypes.c_int64), ("vocab", ctypes.c_int64),
+        ("row_stride", ctypes.c_int64), ("seq_stride", ctypes.c_int64),
+        ("drow_stride", ctypes.c_int64), ("dseq_stride", ctypes.c_int64),
+        ("tok_seq_stride", ctypes.c_int64), ("tok_offset", ctypes.c_int64),
+        ("logits_dtype", ctypes.c_int32), ("dlogits_dtype", ctypes.c_int32), ("ids_dtype", ctypes.c_int32),
+        ("mask_dtype", ctypes.c_int32), ("accumulate", ctypes.c_int32), ("temperature", ctypes.c_float),
+        ("logits", ctypes.c_void_p), ("ids", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+        ("row_max", ctypes.c_void_p), ("log_sum", ctypes.c_void_p), ("entropy", ctypes.c_void_p),
+        ("dlogp", ctypes.c_void_p), ("dentropy", ctypes.c_void_p), ("dlogits", ctypes.c_void_p),
+        ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
+    ]
+
+
+class GradClipArgs(ctypes.Structure):
+    """pcp_grad_clip_args (include/pcp_step.h); the lists as addresses of host arrays."""
+    _fields_ = [
+        ("n_tensors", ctypes.c_int64), ("grads", ctypes.c_void_p), ("counts", ctypes.c_void_p),
+        ("dtypes", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_dtypes", ctypes.c_void_p),
+        ("norm", ctypes.c_void_p), ("coef", ctypes.c_void_p), ("norm_type", ctypes.c_int32), ("max_norm", ctypes.c_float),
+        ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
+    ]
+
+
+class NesterovManyArgs(ctypes.Structure):
+    """pcp_nesterov_many_args (include/pcp_step.h); the lists as addresses of host arrays."""
+    _fields_ = [
+        ("n_tensors", ctypes.c_int64), ("counts", ctypes.c_void_p), ("params", ctypes.c_void_p),
+        ("velocities", ctypes.c_void_p), ("grads", ctypes.c_void_p), ("dtypes", ctypes.c_void_p),
+        ("param_copies", ctypes.c_void_p), ("coef", ctypes.c_void_p),
+        ("learning_rate", ctypes.c_float), ("momentum", ctypes.c_float), ("mode", ctypes.c_int32),
+        ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
+    ]
+
+
+class NormType(enum.IntEnum):
+    l2 = 0      # sqrt(sum g^2)
+    max = 1     # max |g|
+
+
 class Divergence(enum.IntEnum):
     forward = 0   # sum p log(p / q)
     reverse = 1   # sum q log(q / p)
@@ -229,6 +288,15 @@ SIGNATURES = {
     "pcp_top_logits": (_I, [_VP, ctypes.POINTER(TopLogitsArgs)]),
     "pcp_distill_args_init": (None, [ctypes.POINTER(DistillArgs)]),
     "pcp_distill_fwd_bwd": (_I, [_VP, ctypes.POINTER(DistillArgs)]),
+    "pcp_score_args_init": (None, [ctypes.POINTER(ScoreArgs)]),
+    "pcp_score_fwd": (_I, [_VP, ctypes.POINTER(ScoreArgs)]),
+    "pcp_score_bwd_args_init": (None, [ctypes.POINTER(ScoreBwdArgs)]),
+    "pcp_score_bwd": (_I, [_VP, ctypes.POINTER(ScoreBwdArgs)]),
+    "pcp_grad_clip_args_init": (None, [ctypes.POINTER(GradClipArgs)]),
+    "pcp_grad_clip": (_I, [_VP, ctypes.POINTER(GradClipArgs)]),
+    "pcp_nesterov_many_args_init": (None, [ctypes.POINTER(NesterovManyArgs)]),
+    "pcp_nesterov_update_many": (_I, [_VP, ctypes.POINTER(NesterovManyArgs)]),
+    "pcp_nesterov_velocity": (_VP, [_VP, _I]),
     "pcp_prompts_load": (_I, [_VP, ctypes.c_char_p, _VP, _I64, _VP, _I64, ctypes.POINTER(_I64),
                               ctypes.POINTER(_I64)]),
     "pcp_weights_load": (_I, [_VP, ctypes.c_char_p, _I, ctypes.POINTER(_I64), _VP, _VP]),

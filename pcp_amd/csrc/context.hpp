@@ -17,6 +17,10 @@ struct HostStager;
 }
 
 namespace pcp {
+// Rows of token scores that several workgroups may share, and workgroups of a gradient norm.
+constexpr int kScoreTickets = 512;
+constexpr int kNormBlocks = 2048;
+
 // What kernels hand back to the host: one pinned, coherent host page per context, written
 // by the device with plain system-scope stores and read by the host after the stream is
 // synchronised, so no call copies a result back. (An error word in device memory cost
@@ -39,6 +43,9 @@ struct pcp_ctx {
   float4* d_loss_parts = nullptr;     // RowArgs::part of losses (same allocation)
   float4* d_logprob_parts = nullptr;  // and of log-probs: of the synchronous call that holds
   std::atomic<bool> logprob_parts_busy{false};   // this flag
+  unsigned* d_score_done = nullptr;   // the token scores' tickets, kScoreTickets (same allocation; zero between launches)
+  unsigned* d_norm_done = nullptr;    // the gradient norm's ticket (the same)
+  double* d_norm_parts = nullptr;     // and its partial results, kNormBlocks
   void* scratch = nullptr;       // per-call work buffers, grown on demand
   size_t scratch_bytes = 0;
   bool scratch_in_graph = false;      // a call of ensure_scratch_on has been captured with it

@@ -446,7 +446,9 @@ int pcp_init(int backend, int device_ordinal, pcp_ctx** out) {
   // The row counter, and the results of rows in parts: those of the largest call (1.6 MB), for
   // losses and for log-probs. Held from the start, they add nothing to what a call needs.
   void* fixed = nullptr;
-  e = hipMalloc(&fixed, 256 + 2 * kPartScratchBytes);
+  // Behind them the tickets and the partial results of pcp_score_fwd and pcp_grad_clip.
+  constexpr size_t kTicketBytes = sizeof(unsigned) * (kScoreTickets + 64), kNormBytes = sizeof(double) * kNormBlocks;
+  e = hipMalloc(&fixed, 256 + 2 * kPartScratchBytes + kTicketBytes + kNormBytes);
   if (e != hipSuccess) {
     delete c;
     return fail(nullptr, PCP_ERR_OOM, "hipMalloc(row counter): %s", hipGetErrorString(e));
@@ -454,6 +456,10 @@ int pcp_init(int backend, int device_ordinal, pcp_ctx** out) {
   c->d_next_row = static_cast<int*>(fixed);
   c->d_loss_parts = reinterpret_cast<float4*>(static_cast<char*>(fixed) + 256);
   c->d_logprob_parts = c->d_loss_parts + kPartScratchBytes / sizeof(float4);
+  char* const tickets = static_cast<char*>(fixed) + 256 + 2 * kPartScratchBytes;
+  c->d_score_done = reinterpret_cast<unsigned*>(tickets);
+  c->d_norm_done = c->d_score_done + kScoreTickets;
+  c->d_norm_parts = reinterpret_cast<double*>(tickets + kTicketBytes);
   void* page = nullptr;
   void* d_page = nullptr;
   e = hipHostMalloc(&page, sizeof(HostPage), hipHostMallocMapped | hipHostMallocCoherent);
@@ -462,6 +468,7 @@ int pcp_init(int backend, int device_ordinal, pcp_ctx** out) {
     e = hipHostGetDevicePointer(&d_page, page, 0);
   }
   if (e == hipSuccess) e = hipMemset(c->d_next_row, 0, 64);
+  if (e == hipSuccess) e = hipMemset(tickets, 0, kTicketBytes);
   if (e == hipSuccess) e = hipDeviceSynchronize();
   if (e != hipSuccess) {
     if (page) (void)hipHostFree(page);

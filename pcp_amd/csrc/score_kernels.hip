@@ -1,0 +1,651 @@
+// Scores of given tokens (pcp_score.h): log-probs, entropy and the top alternatives of rows of
+// logits, and the gradient of a function of the log-probs and entropies.
+
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <cstring>
+
+#include "context.hpp"
+#include "grpo_device.hpp"
+#include "pcp_score.h"
+#include "top_device.hpp"
+
+namespace pcp {
+namespace {
+
+constexpr double kLn2d = 0.69314718055994530942;
+
+// The token arrays of a call and the rows that they weigh.
+struct TokenArrays {
+  const void* ids;      // nullptr: no row has a token
+  const void* mask;     // nullptr: all ones
+  int64_t rows, tok_stride, tok_offset, vocab;
+  int* err;
+  int32_t ids_i64, mask_u8;
+};
+
+struct ScoreRow {
+  int64_t at;      // index in the token arrays
+  int64_t id;      // -1: no token
+  bool live;
+};
+
+__device__ __forceinline__ ScoreRow score_row(const TokenArrays& a, int64_t s, int64_t t) {
+  ScoreRow r{s * a.tok_stride + a.tok_offset + t, -1, true};
+  if (a.mask != nullptr)
+    r.live = a.mask_u8 ? static_cast<const uint8_t*>(a.mask)[r.at] != 0 : static_cast<const float*>(a.mask)[r.at] != 0.f;
+  if (a.ids != nullptr && r.live) {
+    r.id = a.ids_i64 ? static_cast<const int64_t*>(a.ids)[r.at] : static_cast<const int32_t*>(a.ids)[r.at];
+    if (r.id < 0 || r.id >= a.vocab) {
+      if (r.id != PCP_IGNORE_INDEX && threadIdx.x == 0) raise_error(a.err, kErrTokenRange);
+      r.live = false;
+    }
+  }
+  return r;
+}
+
+// ---- forward ----------------------------------------------------------------------------
+
+// A part of a row as its workgroup leaves it.
+struct alignas(16) ScorePart {
+  double s, t;
+  float mx;
+  int32_t n;
+  int64_t pad;
+};
+
+struct ScoreArgs {
+  TokenArrays tok;
+  const void* logits;
+  int64_t row_stride, seq_stride;
+  int64_t row0;            // of this launch
+  float* logp;
+  float* entropy;
+  float* row_max;
+  float* log_sum;
+  float* top_logp;
+  void* top_ids;
+  uint64_t* part_key;      // [row, parts, part_cap]
+  ScorePart* part;         // [row, parts]
+  unsigned* done;          // [row] parts that are, 0 between launches
+  double inv_tau;
+  float k2;                // log2(e) / temperature
+  int32_t k, top_i64, parts, per, part_cap;
+};
+
+// An exponent this low is a term of 0, whose product with it then is 0 too (and not NaN at -inf).
+constexpr float kLeastExp = -1024.f;
+
+// A sum of terms and one of terms times their exponents (both against m), against M >= m.
+__device__ __forceinline__ void score_rebase(double& s, double& t, float m, float M, float k) {
+  const float d = fmaxf((m - ms_ref(M)) * k, kLeastExp);
+  const double w = hw_exp2(d);
+  t = s == 0. ? 0. : w * (t + d * s);
+  s = s == 0. ? 0. : w * s;
+}
+
+// Of a lane: its largest logit mx, and against it the sum s of the terms 2^d, d = (x - mx) k, and the sum t of
+// 2^d d. The sums of a batch are f32 against the rounded product ref of mx and k, whose residue is
+// taken out once per batch: of terms 2^d it leaves 2^-r s and 2^-r (t - r s).
+struct ScoreSums {
+  static constexpr bool kFresh = true;
+  float k2, mx;
+  double s, t;
+
+  template <typename TI, int U, typename Held>
+  __device__ __forceinline__ void fresh(const u32x4 (&x)[U], Held held, float bx) {
+    const float nm = fmaxf(mx, bx);
+    const TermScale ts = term_scale(nm, k2);
+    float s1 = 0.f, t1 = 0.f;
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+      if (held(q)) {
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&x[q]);
+#pragma unroll
+        for (int j = 0; j < 16 / TI::kBytes; ++j) {
+          const float d = fmaf(TI::unpack(w, j), ts.k, -ts.ref);
+          const float e = hw_exp2(d);
+          s1 += e;
+          t1 = fmaf(e, fmaxf(d, kLeastExp), t1);
+        }
+      }
+    score_rebase(s, t, mx, nm, k2);
+    const float r = term_residue(nm, ts), adj = hw_exp2(-r);
+    s += static_cast<double>(s1 * adj);
+    t += static_cast<double>(fmaf(-r, s1, t1) * adj);
+    mx = nm;
+  }
+  template <typename TI, int U, typename Held>
+  __device__ __forceinline__ bool add(const u32x4 (&)[U], Held, float, bool (&)[U]) { return false; }
+};
+
+// The merge of the first N lanes' sums, on every lane, in a fixed order.
+template <int N>
+__device__ __forceinline__ void score_merge(float& mx, double& s, double& t, float k) {
+  const float M = lanes_max<N>(mx);
+  score_rebase(s, t, mx, M, k);
+  const int lane = threadIdx.x & 63;
+  s = wave_sum64(lane < N ? s : 0.);
+  t = wave_sum64(lane < N ? t : 0.);
+  mx = M;
+}
+
+template <typename TI>
+__device__ __forceinline__ void score_write(const ScoreArgs& a, const ScoreRow& r, const char* xrow, Shared& sh, int n,
+                                            float mx, double s, double t) {
+  const double log_sum = ms_lse(0.f, static_cast<float>(s));
+  if (a.k > 0)
+    rank_entries(sh, n, a.k, [&](int rank, float x, int64_t id) {
+      const int64_t at = r.at * a.k + rank;
+      a.top_logp[at] = static_cast<float>((static_cast<double>(x) - static_cast<double>(mx)) * a.inv_tau - log_sum);
+      if (a.top_i64) static_cast<int64_t*>(a.top_ids)[at] = id;
+      else static_cast<int32_t*>(a.top_ids)[at] = static_cast<int32_t>(id);
+    });
+  if (threadIdx.x != 0) return;
+  if (!__builtin_isfinite(mx) || !__builtin_isfinite(log_sum)) raise_error(a.tok.err, kErrNonFinite);
+  if (a.logp) {
+    const double x = r.id < 0 ? static_cast<double>(mx) : static_cast<double>(TI::load1(xrow, r.id));
+    a.logp[r.at] = r.id < 0 ? 0.f : static_cast<float>((x - static_cast<double>(mx)) * a.inv_tau - log_sum);
+  }
+  if (a.entropy) a.entropy[r.at] = static_cast<float>(log_sum - t / s * kLn2d);
+  if (a.row_max) a.row_max[r.at] = mx;
+  if (a.log_sum) a.log_sum[r.at] = static_cast<float>(log_sum);
+}
+
+__device__ __forceinline__ void score_dead(const ScoreArgs& a, const ScoreRow& r) {
+  for (int i = threadIdx.x; i < a.k; i += kBlock) {
+    const int64_t at = r.at * a.k + i;
+    a.top_logp[at] = 0.f;
+    if (a.top_i64) static_cast<int64_t*>(a.top_ids)[at] = PCP_IGNORE_INDEX;
+    else static_cast<int32_t*>(a.top_ids)[at] = PCP_IGNORE_INDEX;
+  }
+  if (threadIdx.x != 0) return;
+  if (a.logp) a.logp[r.at] = 0.f;
+  if (a.entropy) a.entropy[r.at] = 0.f;
+  if (a.row_max) a.row_max[r.at] = 0.f;
+  if (a.log_sum) a.log_sum[r.at] = 0.f;
+}
+
+template <typename TI, bool TOP>
+__global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
+  constexpr int BLOCK = kBlock, U = kU;
+  __shared__ __align__(16) Shared sh;
+  __shared__ double wave_s[kWaves], wave_t[kWaves];
+  __shared__ float wave_mx[kWaves];
+  __shared__ unsigned turn;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t of = blockIdx.x / static_cast<uint32_t>(a.parts);
+  const int part = static_cast<int>(blockIdx.x - of * static_cast<uint32_t>(a.parts));
+  const int64_t row = a.row0 + of;
+  const int64_t seq = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.tok.rows);
+  const int64_t t = row - seq * a.tok.rows;
+  const ScoreRow r = score_row(a.tok, seq, t);
+  if (!r.live) {
+    if (part == 0) score_dead(a, r);
+    return;
+  }
+  const char* xrow = static_cast<const char*>(a.logits) + (seq * a.seq_stride + t * a.row_stride) * TI::kBytes;
+  const RowSpan sp = row_span<TI>(xrow, a.tok.vocab);
+  const int v0 = part * a.per, end = min(v0 + a.per, sp.nv);
+  const __amdgpu_buffer_rsrc_t xbuf = row_rsrc(sp.vec, static_cast<uint32_t>(max(end, 0)) * 16u);
+  ScoreSums sums{a.k2, kNegInf, 0., 0.};
+  Candidates c{sh, 0, kNegInf};
+  if constexpr (TOP) {
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+  }
+  if (part == 0 && tid < 64) {   // the elements outside the interior
+    const int ek = edge_index<TI>(sp, tid);
+    float xe = kNegInf;
+    if (ek >= 0) {
+      xe = TI::load1(xrow, ek);
+      sums.mx = fmaxf(sums.mx, xe);
+      sums.s = hw_exp2((xe - ms_ref(sums.mx)) * a.k2);
+    }
+    if constexpr (TOP) c.add(ek >= 0, element_key(xe, static_cast<uint32_t>(ek)));
+  }
+  int n = 0;
+  if constexpr (TOP) {
+    scan_part<TI>(sp, xbuf, v0, end, part == 0 ? sp.head + sp.tail : 0, a.k, a.parts == 1 ? a.k + 64 : a.part_cap, sums, c,
+                  sh);
+    __syncthreads();
+    n = sh.count;
+  } else {
+    for (int base = v0; base < end; base += BLOCK * U) {
+      u32x4 x[U];
+      const uint32_t off = static_cast<uint32_t>(base + tid) * 16u;
+#pragma unroll
+      for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
+      auto held = [&](int q) { return base + q * BLOCK + tid < end; };
+      float bx = kNegInf;
+#pragma unroll
+      for (int q = 0; q < U; ++q) bx = held(q) ? vec_max<TI>(bx, x[q]) : bx;
+      sums.template fresh<TI>(x, held, bx);
+    }
+  }
+  float mx = sums.mx;
+  double s = sums.s, tt = sums.t;
+  score_merge<64>(mx, s, tt, a.k2);
+  if (lane == 0) {
+    wave_mx[wave] = mx;
+    wave_s[wave] = s;
+    wave_t[wave] = tt;
+  }
+  __syncthreads();
+  mx = wave_mx[lane & (kWaves - 1)];
+  s = wave_s[lane & (kWaves - 1)];
+  tt = wave_t[lane & (kWaves - 1)];
+  score_merge<kWaves>(mx, s, tt, a.k2);
+  if (a.parts == 1) {
+    score_write<TI>(a, r, xrow, sh, n, mx, s, tt);
+    return;
+  }
+  // The part's candidates and sums for the last of the row's workgroups to finish, which merges them.
+  ScorePart* parts = a.part + static_cast<int64_t>(of) * a.parts;
+  uint64_t* keys = a.part_key + static_cast<int64_t>(of) * a.parts * a.part_cap;
+  if constexpr (TOP)
+    for (int i = tid; i < n; i += BLOCK) store_coherent(keys + static_cast<int64_t>(part) * a.part_cap + i, sh.key[i]);
+  if (tid == 0) {
+    store_coherent(&parts[part].s, s);
+    store_coherent(&parts[part].t, tt);
+    store_coherent(&parts[part].mx, mx);
+    store_coherent(&parts[part].n, n);
+  }
+  wait_stores();
+  __syncthreads();
+  if (tid == 0) turn = __hip_atomic_fetch_add(a.done + of, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (turn + 1 != static_cast<unsigned>(a.parts)) return;
+  acquire_coherent();
+  if (tid == 0) store_coherent(a.done + of, 0u);
+  if constexpr (TOP) n = merge_parts(keys, a.parts, a.part_cap, a.k, [&](int p) { return parts[p].n; }, sh);
+  mx = kNegInf;
+  s = tt = 0.;
+  if (lane < a.parts) {
+    mx = parts[lane].mx;
+    s = parts[lane].s;
+    tt = parts[lane].t;
+  }
+  score_merge<64>(mx, s, tt, a.k2);
+  score_write<TI>(a, r, xrow, sh, n, mx, s, tt);
+}
+
+template <typename TI>
+hipError_t launch_score(ScoreArgs a, int64_t n_rows, hipStream_t st) {
+  constexpr int64_t kRows = 1 << 22;   // of a launch: 2^30 lanes, and rows in parts are fewer
+  for (int64_t r0 = 0; r0 < n_rows; r0 += kRows) {
+    a.row0 = r0;
+    const unsigned grid = static_cast<unsigned>((n_rows - r0 < kRows ? n_rows - r0 : kRows) * a.parts);
+    if (a.k > 0) score_kernel<TI, true><<<grid, kBlock, 0, st>>>(a);
+    else score_kernel<TI, false><<<grid, kBlock, 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+// ---- backward ---------------------------------------------------------------------------
+
+struct ScoreBwdArgs {
+  TokenArrays tok;
+  const void* logits;
+  void* dlogits;
+  int64_t row_stride, seq_stride, drow_stride, dseq_stride, logit_rows;
+  int64_t row0;
+  const float* row_max;
+  const float* log_sum;
+  const float* entropy;
+  const float* dlogp;
+  const float* dentropy;
+  float k2, inv_tau;
+  int32_t blocks;          // workgroups per row
+};
+
+// 16 bytes of dlogits each: the logits of the same elements (16 or 8 bytes) at any element's address.
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+typedef u32x2 u32x2_any __attribute__((aligned(2)));
+
+constexpr int kGradU = 2;    // groups per lane
+
+// A row's gradient is one pass: dz = p (A + B d) with d = (x - m) k2 - log2 sum, p = 2^d, and the token's
+// own term.
+template <typename TI, typename TO, bool ACC>
+__global__ void __launch_bounds__(kBlock) score_grad_kernel(ScoreBwdArgs a) {
+  constexpr int N = 16 / TO::kBytes, U = kGradU;   // elements per group
+  const int tid = threadIdx.x;
+  const uint32_t of = blockIdx.x / static_cast<uint32_t>(a.blocks);
+  const int block = static_cast<int>(blockIdx.x - of * static_cast<uint32_t>(a.blocks));
+  const int64_t row = a.row0 + of;
+  const int64_t seq = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.logit_rows);
+  const int64_t t = row - seq * a.logit_rows;
+  ScoreRow r{0, -1, false};
+  if (t < a.tok.rows) r = score_row(a.tok, seq, t);
+  float gl = 0.f, gh = 0.f;
+  if (r.live) {
+    if (a.dlogp) gl = a.dlogp[r.at];
+    if (a.dentropy) gh = a.dentropy[r.at];
+    r.live = gl != 0.f || gh != 0.f;
+  }
+  if (ACC && !r.live) return;
+  char* drow = static_cast<char*>(a.dlogits) + (seq * a.dseq_stride + t * a.drow_stride) * TO::kBytes;
+  const int V = static_cast<int>(a.tok.vocab);
+  // Group g: elements first + N g on, 16-byte aligned in dlogits; the first and the last may be cut.
+  const int first = -static_cast<int>((reinterpret_cast<uintptr_t>(drow) & 15u) / TO::kBytes);
+  const int e0 = first + (block * (U * kBlock) + tid) * N;
+  if (!r.live) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int e = e0 + u * (kBlock * N);
+      if (e >= 0 && e + N <= V) {
+        __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, reinterpret_cast<u32x4*>(drow + static_cast<int64_t>(e) * TO::kBytes));
+      } else {
+        for (int j = max(-e, 0); j < min(N, V - e); ++j) store1<TO>(drow, e + j, 0.f);
+      }
+    }
+    return;
+  }
+  const char* xrow = static_cast<const char*>(a.logits) + (seq * a.seq_stride + t * a.row_stride) * TI::kBytes;
+  const float m = a.row_max[r.at], ls = a.log_sum[r.at], h = a.dentropy ? a.entropy[r.at] : 0.f;
+  const float l2 = ls * kLog2e;
+  float A = -fmaf(gh, h, gl) * a.inv_tau;
+  const float B = -gh * kLn2 * a.inv_tau, at_token = gl * a.inv_tau;
+  if (!__builtin_isfinite(m) || !__builtin_isfinite(ls) || !__builtin_isfinite(A) || !__builtin_isfinite(B)) {
+    A = __builtin_nanf("");
+    if (tid == 0 && block == 0) raise_error(a.tok.err, kErrNonFinite);
+  }
+  const int y = static_cast<int>(r.id);
+  auto grad = [&](float x, int e) {
+    const float d = fmaxf(fmaf(x - m, a.k2, -l2), kLeastExp);
+    const float g = hw_exp2(d) * fmaf(B, d, A);
+    return e == y ? g + at_token : g;
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int e = e0 + u * (kBlock * N);
+    const char* xp = xrow + static_cast<int64_t>(e) * TI::kBytes;
+    u32x4* dp = reinterpret_cast<u32x4*>(drow + static_cast<int64_t>(e) * TO::kBytes);
+    if (e >= 0 && e + N <= V) {
+      uint32_t w[4] = {}, b[4] = {};
+      if constexpr (N * TI::kBytes == 16) {
+        const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(xp));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = v[i];
+      } else {
+        const u32x2 v = __builtin_nontemporal_load(reinterpret_cast<const u32x2_any*>(xp));
+        w[0] = v[0];
+        w[1] = v[1];
+      }
+      if constexpr (ACC) {
+        const u32x4 v = __builtin_nontemporal_load(dp);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) b[i] = v[i];
+      }
+      float o[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        o[j] = grad(TI::unpack(w, j), e + j);
+        if constexpr (ACC) o[j] += TO::unpack(b, j);
+      }
+      store_vals<TO, N, true>(dp, 0, o);
+    } else {
+      for (int j = max(-e, 0); j < min(N, V - e); ++j) {
+        float o = grad(TI::load1(xrow, e + j), e + j);
+        if constexpr (ACC) o += TO::load1(drow, e + j);
+        store1<TO>(drow, e + j, o);
+      }
+    }
+  }
+}
+
+template <typename TI, typename TO>
+hipError_t launch_grad(ScoreBwdArgs a, int64_t n_rows, bool accumulate, hipStream_t st) {
+  constexpr int N = 16 / TO::kBytes;
+  // The groups of a row that begins up to N - 1 elements past an aligned address.
+  const int64_t groups = (a.tok.vocab + N - 1 + N - 1) / N;
+  a.blocks = static_cast<int32_t>((groups + kBlock * kGradU - 1) / (kBlock * kGradU));
+  const int64_t rows = (int64_t(1) << 23) / a.blocks > 0 ? (int64_t(1) << 23) / a.blocks : 1;   // of a launch
+  for (int64_t r0 = 0; r0 < n_rows; r0 += rows) {
+    a.row0 = r0;
+    const unsigned grid = static_cast<unsigned>((n_rows - r0 < rows ? n_rows - r0 : rows) * a.blocks);
+    if (accumulate) score_grad_kernel<TI, TO, true><<<grid, kBlock, 0, st>>>(a);
+    else score_grad_kernel<TI, TO, false><<<grid, kBlock, 0, st>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+// ---- entry points -----------------------------------------------------------------------
+
+inline bool misaligned(const void* p, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & static_cast<uintptr_t>(size - 1)) != 0;
+}
+
+// Elements from the first to past the last of n_seq x rows rows (0 where there are none);
+// false where that overflows.
+bool extent_of(int64_t n_seq, int64_t rows, int64_t row_stride, int64_t seq_stride, int64_t vocab, int64_t* out) {
+  *out = 0;
+  if (n_seq == 0 || rows == 0) return true;
+  int64_t a, b, bytes;
+  if (mul_overflows(n_seq - 1, seq_stride, &a) || mul_overflows(rows - 1, row_stride, &b) ||
+      __builtin_add_overflow(a, b, &a) || __builtin_add_overflow(a, vocab, &a) || mul_overflows(a, 8, &bytes))
+    return false;
+  *out = a;
+  return true;
+}
+
+// What both calls check alike, and the token arrays that follow from it.
+template <typename Args>
+int score_common(pcp_ctx* ctx, const Args* a, TokenArrays* tok, float* k2) {
+  if (a->n_seq < 0) return fail(ctx, PCP_ERR_INVALID_ARG, "n_seq must be >= 0 (got %lld)", (long long)a->n_seq);
+  if (a->rows < 0) return fail(ctx, PCP_ERR_INVALID_ARG, "rows must be >= 0 (got %lld)", (long long)a->rows);
+  if (a->vocab < 1 || a->vocab > PCP_SCORE_MAX_VOCAB)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "vocab must be in [1, %d] (got %lld)", PCP_SCORE_MAX_VOCAB, (long long)a->vocab);
+  if (a->logits_dtype != PCP_BF16 && a->logits_dtype != PCP_F16 && a->logits_dtype != PCP_F32)
+    return fail(ctx, PCP_ERR_DTYPE, "logits dtype must be bf16, f16 or f32 (got %d)", a->logits_dtype);
+  if (a->ids && a->ids_dtype != PCP_I64 && a->ids_dtype != PCP_I32)
+    return fail(ctx, PCP_ERR_DTYPE, "ids dtype must be i64 or i32 (got %d)", a->ids_dtype);
+  if (a->mask && a->mask_dtype != PCP_F32 && a->mask_dtype != PCP_BOOL)
+    return fail(ctx, PCP_ERR_DTYPE, "mask dtype must be f32 or bool (got %d)", a->mask_dtype);
+  *k2 = static_cast<float>(1.4426950408889634074 / static_cast<double>(a->temperature));
+  if (!(a->temperature > 0.f) || !std::isfinite(a->temperature) || !std::isnormal(*k2))
+    return fail(ctx, PCP_ERR_INVALID_ARG, "temperature must be positive and finite (and its inverse a normal f32)");
+  if (a->flags & ~PCP_FLAG_ASYNC) return fail(ctx, PCP_ERR_INVALID_ARG, "only PCP_FLAG_ASYNC applies here");
+  const int64_t ts = a->tok_seq_stride ? a->tok_seq_stride : a->rows;
+  if (a->tok_offset < 0 || a->rows > ts || a->tok_offset > ts - a->rows)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "tok_offset + rows must fit in tok_seq_stride");
+  int64_t tmp;
+  if (mul_overflows(a->n_seq, ts, &tmp) || mul_overflows(tmp, 8 * PCP_SCORE_TOP_MAX, &tmp))
+    return fail(ctx, PCP_ERR_OVERFLOW, "token array size overflows int64");
+  if (misaligned(a->logits, dtype_bytes(a->logits_dtype)) || (a->ids && misaligned(a->ids, dtype_bytes(a->ids_dtype))) ||
+      (a->mask && a->mask_dtype == PCP_F32 && misaligned(a->mask, 4)))
+    return fail(ctx, PCP_ERR_INVALID_ARG, "pointers must be aligned to their element size");
+  *tok = TokenArrays{a->ids, a->mask, a->rows, ts, a->tok_offset, a->vocab, nullptr, a->ids_dtype == PCP_I64,
+                     a->mask_dtype == PCP_BOOL};
+  return PCP_OK;
+}
+
+int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
+  if (!a) return fail(ctx, PCP_ERR_INVALID_ARG, "args is NULL");
+  ScoreArgs t;
+  std::memset(&t, 0, sizeof(t));
+  const int rc0 = score_common(ctx, a, &t.tok, &t.k2);
+  if (rc0 != PCP_OK) return rc0;
+  if (a->k < 0 || a->k > PCP_SCORE_TOP_MAX || a->k > a->vocab)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "k must be in [0, min(vocab, %d)] (got %d)", PCP_SCORE_TOP_MAX, a->k);
+  t.row_stride = a->row_stride ? a->row_stride : a->vocab;
+  if (t.row_stride < a->vocab) return fail(ctx, PCP_ERR_INVALID_ARG, "row_stride (%lld) must be >= vocab", (long long)t.row_stride);
+  int64_t n_rows, extent;
+  if (mul_overflows(a->n_seq, a->rows, &n_rows) || n_rows > INT32_MAX)
+    return fail(ctx, PCP_ERR_OVERFLOW, "n_seq * rows exceeds 2^31-1 rows");
+  if (a->seq_stride) t.seq_stride = a->seq_stride;
+  else if (mul_overflows(a->rows, t.row_stride, &t.seq_stride)) return fail(ctx, PCP_ERR_OVERFLOW, "logits byte size overflows int64");
+  if (a->n_seq > 1 && a->rows > 0 && t.seq_stride < a->vocab)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "seq_stride (%lld) must be >= vocab", (long long)t.seq_stride);
+  if (!extent_of(a->n_seq, a->rows, t.row_stride, t.seq_stride, a->vocab, &extent))
+    return fail(ctx, PCP_ERR_OVERFLOW, "logits byte size overflows int64");
+  if (a->k > 0 && a->top_ids_dtype != PCP_I64 && a->top_ids_dtype != PCP_I32)
+    return fail(ctx, PCP_ERR_DTYPE, "top_ids dtype must be i64 or i32 (got %d)", a->top_ids_dtype);
+  if (n_rows > 0 && (!a->logits || (a->k > 0 && (!a->top_logp || !a->top_ids))))
+    return fail(ctx, PCP_ERR_INVALID_ARG, "logits, or top_logp / top_ids with k > 0, is NULL");
+  if (!a->ids && a->logp) return fail(ctx, PCP_ERR_INVALID_ARG, "logp needs ids");
+  if (misaligned(a->logp, 4) || misaligned(a->entropy, 4) || misaligned(a->row_max, 4) || misaligned(a->log_sum, 4) ||
+      (a->k > 0 && (misaligned(a->top_logp, 4) || misaligned(a->top_ids, dtype_bytes(a->top_ids_dtype)))))
+    return fail(ctx, PCP_ERR_INVALID_ARG, "pointers must be aligned to their element size");
+  if (!ctx) return fail(nullptr, PCP_ERR_INVALID_ARG, "context is NULL");
+  if (n_rows == 0) return PCP_OK;
+  const DeviceScope scope(ctx->device);
+  if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
+  hipStream_t st = static_cast<hipStream_t>(a->stream);
+
+  // Workgroups per row: as few rows' logits as would leave CUs idle are dealt to several, at least a batch each.
+  const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
+  const int64_t batches = nv > 0 ? (nv + kBlock * kU - 1) / (kBlock * kU) : 1;
+  int64_t parts = n_rows < kScoreTickets ? (2048 + n_rows - 1) / n_rows : 1;
+  if (parts > batches) parts = batches;
+  if (parts > 64) parts = 64;   // one wave merges their sums
+  const int64_t per_batches = (batches + parts - 1) / parts;
+  parts = (batches + per_batches - 1) / per_batches;
+  const int64_t part_cap = a->k > 0 ? a->k + 64 : 0;
+  const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(n_rows) * parts * part_cap : 0;
+  const size_t sums = parts > 1 ? sizeof(ScorePart) * static_cast<size_t>(n_rows) * parts + 16 : 0;
+  if (parts > 1) {
+    const int rc = ensure_scratch_on(ctx, keys + sums, st);
+    if (rc != PCP_OK) return rc;
+  }
+  t.tok.err = ctx->d_page->err;
+  t.logits = a->logits;
+  t.logp = a->logp;
+  t.entropy = a->entropy;
+  t.row_max = a->row_max;
+  t.log_sum = a->log_sum;
+  t.top_logp = a->top_logp;
+  t.top_ids = a->top_ids;
+  t.part_key = static_cast<uint64_t*>(ctx->scratch);
+  t.part = reinterpret_cast<ScorePart*>(static_cast<char*>(ctx->scratch) + ((keys + 15) & ~static_cast<size_t>(15)));
+  t.done = ctx->d_score_done;
+  t.inv_tau = 1. / static_cast<double>(a->temperature);
+  t.k = a->k;
+  t.top_i64 = a->top_ids_dtype == PCP_I64;
+  t.parts = static_cast<int32_t>(parts);
+  t.per = static_cast<int32_t>(per_batches * kBlock * kU);
+  t.part_cap = static_cast<int32_t>(part_cap);
+  const bool timed = prof_begin(ctx, st);
+  const hipError_t e = a->logits_dtype == PCP_F32    ? launch_score<F32T>(t, n_rows, st)
+                       : a->logits_dtype == PCP_BF16 ? launch_score<BF16T>(t, n_rows, st)
+                                                     : launch_score<F16T>(t, n_rows, st);
+  prof_end(ctx, st, timed);
+  if (e != hipSuccess) return hip_fail(ctx, e, "token scores launch");
+  return finish_call(ctx, a->flags, st);
+}
+
+int score_bwd(pcp_ctx* ctx, const pcp_score_bwd_args* a) {
+  if (!a) return fail(ctx, PCP_ERR_INVALID_ARG, "args is NULL");
+  ScoreBwdArgs t;
+  std::memset(&t, 0, sizeof(t));
+  const int rc0 = score_common(ctx, a, &t.tok, &t.k2);
+  if (rc0 != PCP_OK) return rc0;
+  if (a->dlogits_dtype != a->logits_dtype && a->dlogits_dtype != PCP_F32)
+    return fail(ctx, PCP_ERR_DTYPE, "dlogits dtype must equal the logits dtype or be f32");
+  t.logit_rows = a->logit_rows ? a->logit_rows : a->rows;
+  if (t.logit_rows < a->rows)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "logit_rows (%lld) must be >= rows", (long long)a->logit_rows);
+  t.row_stride = a->row_stride ? a->row_stride : a->vocab;
+  t.drow_stride = a->drow_stride ? a->drow_stride : a->vocab;
+  if (t.row_stride < a->vocab || t.drow_stride < a->vocab)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "row_stride and drow_stride must be >= vocab");
+  int64_t n_rows, extent, dextent;
+  if (mul_overflows(a->n_seq, t.logit_rows, &n_rows) || n_rows > INT32_MAX)
+    return fail(ctx, PCP_ERR_OVERFLOW, "n_seq * logit_rows exceeds 2^31-1 rows");
+  t.seq_stride = a->seq_stride;
+  t.dseq_stride = a->dseq_stride;
+  if ((!a->seq_stride && mul_overflows(t.logit_rows, t.row_stride, &t.seq_stride)) ||
+      (!a->dseq_stride && mul_overflows(t.logit_rows, t.drow_stride, &t.dseq_stride)))
+    return fail(ctx, PCP_ERR_OVERFLOW, "logits byte size overflows int64");
+  if (a->n_seq > 1 && n_rows > 0 && (t.seq_stride < a->vocab || t.dseq_stride < a->vocab))
+    return fail(ctx, PCP_ERR_INVALID_ARG, "seq_stride and dseq_stride must be >= vocab");
+  if (!extent_of(a->n_seq, a->rows, t.row_stride, t.seq_stride, a->vocab, &extent) ||
+      !extent_of(a->n_seq, t.logit_rows, t.drow_stride, t.dseq_stride, a->vocab, &dextent))
+    return fail(ctx, PCP_ERR_OVERFLOW, "logits byte size overflows int64");
+  {
+    // Rows of dlogits apart: sequences after one another, or row by row beside one another.
+    int64_t one = 0, all = 0;
+    (void)extent_of(1, t.logit_rows, t.drow_stride, t.dseq_stride, a->vocab, &one);
+    (void)extent_of(a->n_seq, 1, t.drow_stride, t.dseq_stride, a->vocab, &all);
+    if (a->n_seq > 1 && t.logit_rows > 1 && t.dseq_stride < one && t.drow_stride < all)
+      return fail(ctx, PCP_ERR_INVALID_ARG, "rows of dlogits overlap");
+  }
+  if (n_rows > 0 && !a->dlogits) return fail(ctx, PCP_ERR_INVALID_ARG, "dlogits is NULL");
+  if (extent > 0 && (!a->logits || !a->row_max || !a->log_sum))
+    return fail(ctx, PCP_ERR_INVALID_ARG, "logits / row_max / log_sum is NULL");
+  if (a->dlogp && !a->ids) return fail(ctx, PCP_ERR_INVALID_ARG, "dlogp needs ids");
+  if (a->dentropy && !a->entropy) return fail(ctx, PCP_ERR_INVALID_ARG, "dentropy needs the forward's entropy");
+  if (misaligned(a->dlogits, dtype_bytes(a->dlogits_dtype)) || misaligned(a->row_max, 4) || misaligned(a->log_sum, 4) ||
+      misaligned(a->entropy, 4) || misaligned(a->dlogp, 4) || misaligned(a->dentropy, 4))
+    return fail(ctx, PCP_ERR_INVALID_ARG, "pointers must be aligned to their element size");
+  {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a->logits), d = reinterpret_cast<uintptr_t>(a->dlogits);
+    const uintptr_t xn = static_cast<uintptr_t>(extent) * dtype_bytes(a->logits_dtype);
+    const uintptr_t dn = static_cast<uintptr_t>(dextent) * dtype_bytes(a->dlogits_dtype);
+    const bool same = x == d && a->logits_dtype == a->dlogits_dtype && t.row_stride == t.drow_stride && t.seq_stride == t.dseq_stride;
+    if (extent > 0 && !same && x < d + dn && d < x + xn)
+      return fail(ctx, PCP_ERR_INVALID_ARG, "dlogits overlap the logits without being the same rows");
+  }
+  if (!ctx) return fail(nullptr, PCP_ERR_INVALID_ARG, "context is NULL");
+  if (n_rows == 0) return PCP_OK;
+  const DeviceScope scope(ctx->device);
+  if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
+  hipStream_t st = static_cast<hipStream_t>(a->stream);
+  t.tok.err = ctx->d_page->err;
+  t.logits = a->logits;
+  t.dlogits = a->dlogits;
+  t.row_max = a->row_max;
+  t.log_sum = a->log_sum;
+  t.entropy = a->entropy;
+  t.dlogp = a->dlogp;
+  t.dentropy = a->dentropy;
+  t.inv_tau = static_cast<float>(1. / static_cast<double>(a->temperature));
+  const bool acc = a->accumulate != 0, wide = a->dlogits_dtype == PCP_F32;
+  const bool timed = prof_begin(ctx, st);
+  const hipError_t e = a->logits_dtype == PCP_F32 ? launch_grad<F32T, F32T>(t, n_rows, acc, st)
+                       : a->logits_dtype == PCP_BF16
+                           ? (wide ? launch_grad<BF16T, F32T>(t, n_rows, acc, st) : launch_grad<BF16T, BF16T>(t, n_rows, acc, st))
+                           : (wide ? launch_grad<F16T, F32T>(t, n_rows, acc, st) : launch_grad<F16T, F16T>(t, n_rows, acc, st));
+  prof_end(ctx, st, timed);
+  if (e != hipSuccess) return hip_fail(ctx, e, "token scores' gradient launch");
+  return finish_call(ctx, a->flags, st);
+}
+
+}  // namespace
+}  // namespace pcp
+
+using namespace pcp;
+
+extern "C" {
+
+void pcp_score_args_init(pcp_score_args* a) {
+  if (!a) return;
+  std::memset(a, 0, sizeof(*a));
+  a->logits_dtype = PCP_BF16;
+  a->ids_dtype = PCP_I64;
+  a->mask_dtype = PCP_F32;
+  a->top_ids_dtype = PCP_I32;
+  a->temperature = 1.f;
+}
+
+int pcp_score_fwd(pcp_ctx* ctx, const pcp_score_args* a) { return score_fwd(ctx, a); }
+
+void pcp_score_bwd_args_init(pcp_score_bwd_args* a) {
+  if (!a) return;
+  std::memset(a, 0, sizeof(*a));
+  a->logits_dtype = a->dlogits_dtype = PCP_BF16;
+  a->ids_dtype = PCP_I64;
+  a->mask_dtype = PCP_F32;
+  a->temperature = 1.f;
+}
+
+int pcp_score_bwd(pcp_ctx* ctx, const pcp_score_bwd_args* a) { return score_bwd(ctx, a); }
+
+}  // extern "C"

@@ -559,6 +559,11 @@ int pcp_nesterov_update_flat(pcp_nesterov* opt, float* params, const float* grad
   return sync_only(ctx, st);
 }
 
+float* pcp_nesterov_velocity(pcp_nesterov* opt, int index) {
+  if (!opt || index < 0 || index >= static_cast<int>(opt->counts.size()) || opt->counts[index] == 0) return nullptr;
+  return opt->vel + opt->offsets[index];
+}
+
 int64_t pcp_nesterov_total(const pcp_nesterov* opt) { return opt ? opt->total : PCP_ERR_INVALID_ARG; }
 
 int pcp_nesterov_serialize(pcp_nesterov* opt, void* host, size_t bytes) {

@@ -1,0 +1,162 @@
+"""Scores of given tokens over torch tensors in HBM (include/pcp_score.h): log-probs, entropy and the top
+alternatives of rows of logits, and the gradient of any function of the log-probs and entropies.
+
+The reference scores tokens inside its training graph alone (tools/export_qwen_forward.py:154-156). Token
+arrays, masks and the shifted layout are those of ``pcp_amd.grpo``; the arithmetic runs in libpcp_grpo.so.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from ._lib import PcpError, ScoreArgs, ScoreBwdArgs, check, lib
+from .grpo import Context, _ptr, call_scope, default_context, dtype_code
+from .step import _row_stride, _seq_stride
+
+
+@dataclass
+class TokenScores:
+    logp: torch.Tensor | None      # f32 [S, TS]; None without ids
+    entropy: torch.Tensor          # f32 [S, TS]
+    row_max: torch.Tensor          # f32 [S, TS]: the row's largest logit
+    log_sum: torch.Tensor          # f32 [S, TS]: log sum exp((x - row_max) / temperature)
+    top_logp: torch.Tensor | None  # f32 [S, TS, k], falling; None where k is 0
+    top_ids: torch.Tensor | None   # i32 / i64 [S, TS, k]
+
+
+def _tokens(logits, ids, mask, rows, tok_offset, tokens):
+    """(S, LS, V, TS, rows, tok_offset) of a call on logits [S, LS, V]."""
+    if logits.dim() != 3:
+        raise PcpError(-1, "logits must be [S, LS, V]")
+    S, LS, V = logits.shape
+    TS = LS if tokens is None else int(tokens)
+    for t, name in ((mask, "mask"), (ids, "ids")):
+        if t is not None:
+            if t.dim() != 2 or t.shape[0] != S:
+                raise PcpError(-1, f"{name} must be [S, TS]")
+            TS = t.shape[1]
+    if ids is not None and mask is not None and ids.shape != mask.shape:
+        raise PcpError(-1, "ids and mask must have the same shape")
+    rows, tok_offset = LS if rows is None else int(rows), int(tok_offset)
+    if rows < 0 or rows > LS:
+        raise PcpError(-1, f"{rows} rows of sequences of {LS}")
+    # (Token arrays of no tokens have no pointer and no stride: the C entry would take them for absent ones.)
+    if tok_offset < 0 or tok_offset + rows > TS:
+        raise PcpError(-1, f"{rows} rows from token {tok_offset} on do not fit in {TS} tokens")
+    return S, LS, V, TS, rows, tok_offset
+
+
+def _row_places(t: torch.Tensor, a, row: str, seq: str) -> None:
+    """The strides of [S, LS, V] rows into fields `row` and `seq` of a."""
+    step = _row_stride(t)
+    setattr(a, row, step)
+    setattr(a, seq, _seq_stride(t) or max(t.shape[1], 1) * step)
+
+
+def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: torch.Tensor | None = None, *, k: int = 0,
+                 temperature: float = 1.0, rows: int | None = None, tok_offset: int = 0, tokens: int | None = None,
+                 top_ids_dtype: torch.dtype = torch.int32, outputs: TokenScores | None = None, sync: bool = True,
+                 stream=None, ctx: Context | None = None) -> TokenScores:
+    """Log-probs of ids [S, TS] under logits [S, LS, V] (f32, bf16 or f16) at `temperature`, each row's entropy,
+    and its k largest logits as log-probs with their ids (equal logits by rising id): pcp_score_fwd. Row (s, t),
+    t < rows, scores token tok_offset + t; rows whose token weighs 0 in mask [S, TS] or is IGNORE_INDEX are
+    left out (zeros, ids IGNORE_INDEX). Without ids no log-probs are formed; without a mask too, `tokens`
+    (default LS) is TS. The logits may be views with contiguous rows, such as ``logits[:, -n:]``, rows of a padded
+    vocabulary or a stack of decode steps [n, S, V], transposed.
+
+    Pass ``outputs`` of an earlier call of the same shape to reuse its buffers; entries that no row addresses
+    keep their values (zeros in new ones). sync=False only enqueues."""
+    S, LS, V, TS, rows, tok_offset = _tokens(logits, ids, mask, rows, tok_offset, tokens)
+    k = int(k)
+    if not 0 <= k <= min(V, _lib.SCORE_TOP_MAX):
+        raise PcpError(-1, f"k must be in [0, {min(V, _lib.SCORE_TOP_MAX)}] (got {k})")
+    a = ScoreArgs()
+    lib().pcp_score_args_init(ctypes.byref(a))
+    _row_places(logits, a, "row_stride", "seq_stride")
+    ctx = ctx or default_context(logits.device.index or 0)
+    given = () if outputs is None else (outputs.logp, outputs.entropy, outputs.row_max, outputs.log_sum,
+                                        outputs.top_logp, outputs.top_ids)
+    with call_scope(ctx, stream, logits, ids, mask, *given) as handle:
+        if outputs is None:
+            f32 = dict(dtype=torch.float32, device=logits.device)
+            outputs = TokenScores(torch.zeros((S, TS), **f32) if ids is not None else None, torch.zeros((S, TS), **f32),
+                                  torch.zeros((S, TS), **f32), torch.zeros((S, TS), **f32),
+                                  torch.zeros((S, TS, k), **f32) if k else None,
+                                  torch.zeros((S, TS, k), dtype=top_ids_dtype, device=logits.device) if k else None)
+        o = outputs
+        for t, n in ((o.logp if ids is not None else None, 1), (o.entropy, 1), (o.row_max, 1), (o.log_sum, 1),
+                     (o.top_logp if k else None, k)):
+            if t is not None and (t.dtype != torch.float32 or t.numel() != S * TS * n):
+                raise PcpError(-1, "outputs do not fit the call: f32 [S, TS], top_logp f32 and top_ids [S, TS, k]")
+        if k and (o.top_logp is None or o.top_ids is None or o.top_ids.dtype != top_ids_dtype
+                  or o.top_ids.numel() != S * TS * k):
+            raise PcpError(-1, "outputs do not fit the call: f32 [S, TS], top_logp f32 and top_ids [S, TS, k]")
+        a.n_seq, a.rows, a.vocab, a.tok_seq_stride, a.tok_offset = S, rows, V, TS, tok_offset
+        a.k, a.temperature, a.logits_dtype = k, temperature, dtype_code(logits)
+        a.logits = logits.data_ptr()
+        _set_tokens(a, ids, mask)
+        a.logp = _ptr(o.logp) if ids is not None else None
+        a.entropy, a.row_max, a.log_sum = _ptr(o.entropy), _ptr(o.row_max), _ptr(o.log_sum)
+        if k:
+            a.top_logp, a.top_ids, a.top_ids_dtype = _ptr(o.top_logp), _ptr(o.top_ids), dtype_code(o.top_ids)
+        a.flags = 0 if sync else _lib.FLAG_ASYNC
+        a.stream = handle
+        check(lib().pcp_score_fwd(ctx.handle, ctypes.byref(a)), ctx.handle)
+    return outputs
+
+
+def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: torch.Tensor, log_sum: torch.Tensor,
+                     entropy: torch.Tensor | None = None, *, dlogp: torch.Tensor | None = None,
+                     dentropy: torch.Tensor | None = None, mask: torch.Tensor | None = None, temperature: float = 1.0,
+                     rows: int | None = None, tok_offset: int = 0, dlogits: torch.Tensor | None = None,
+                     dlogits_dtype: torch.dtype | None = None, accumulate: bool = False, sync: bool = True, stream=None,
+                     ctx: Context | None = None) -> torch.Tensor:
+    """dlogits [S, LS, V] of a function of ``token_scores``' logp and entropy, whose gradients are dlogp and
+    dentropy [S, TS] (f32, either may be None for 0): pcp_score_bwd. row_max, log_sum and (for dentropy) entropy are
+    the forward's, at the same temperature, rows and tok_offset. With accumulate the gradient is added to the
+    given dlogits (the loss head's, for an entropy bonus); rows that have none stay as they are, and are 0
+    otherwise. dlogits may be the logits themselves, and views with contiguous rows as the logits may."""
+    S, LS, V, TS, rows, tok_offset = _tokens(logits, ids, mask, rows, tok_offset, row_max.shape[1] if row_max.dim() == 2 else 0)
+    for t, name in ((row_max, "row_max"), (log_sum, "log_sum"), (entropy, "entropy"), (dlogp, "dlogp"),
+                    (dentropy, "dentropy")):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (S, TS)):
+            raise PcpError(-1, f"{name} must be f32 [S, TS]")
+    if dlogp is not None and ids is None:
+        raise PcpError(-1, "dlogp needs ids")
+    if dentropy is not None and entropy is None:
+        raise PcpError(-1, "dentropy needs the forward's entropy")
+    if dlogits is None and accumulate:
+        raise PcpError(-1, "accumulate needs dlogits")
+    if dlogits is not None and dlogits.shape != logits.shape:
+        raise PcpError(-1, "dlogits must have the logits' shape")
+    if dlogits is not None and dlogits_dtype is not None and dlogits.dtype != dlogits_dtype:
+        raise PcpError(-2, f"dlogits_dtype is {dlogits_dtype}, the given dlogits are {dlogits.dtype}")
+    a = ScoreBwdArgs()
+    lib().pcp_score_bwd_args_init(ctypes.byref(a))
+    _row_places(logits, a, "row_stride", "seq_stride")
+    ctx = ctx or default_context(logits.device.index or 0)
+    with call_scope(ctx, stream, logits, ids, mask, row_max, log_sum, entropy, dlogp, dentropy, dlogits) as handle:
+        if dlogits is None:
+            dlogits = torch.empty((S, LS, V), dtype=dlogits_dtype or logits.dtype, device=logits.device)
+        _row_places(dlogits, a, "drow_stride", "dseq_stride")
+        a.n_seq, a.rows, a.logit_rows, a.vocab, a.tok_seq_stride, a.tok_offset = S, rows, LS, V, TS, tok_offset
+        a.logits_dtype, a.dlogits_dtype, a.temperature = dtype_code(logits), dtype_code(dlogits), temperature
+        a.logits, a.dlogits = logits.data_ptr(), dlogits.data_ptr()
+        _set_tokens(a, ids, mask)
+        a.row_max, a.log_sum, a.entropy = _ptr(row_max), _ptr(log_sum), _ptr(entropy)
+        a.dlogp, a.dentropy = _ptr(dlogp), _ptr(dentropy)
+        a.accumulate = 1 if accumulate else 0
+        a.flags = 0 if sync else _lib.FLAG_ASYNC
+        a.stream = handle
+        check(lib().pcp_score_bwd(ctx.handle, ctypes.byref(a)), ctx.handle)
+    return dlogits
+
+
+def _set_tokens(a, ids, mask) -> None:
+    if ids is not None:
+        a.ids, a.ids_dtype = _ptr(ids), dtype_code(ids)
+    if mask is not None:
+        a.mask, a.mask_dtype = _ptr(mask), dtype_code(mask)

@@ -1,5 +1,5 @@
 """Device-resident work around the loss head in one training step (include/pcp_step.h):
-rollout packing, gradient statistics and the Nesterov update, over torch tensors in HBM.
+rollout packing, gradient statistics, norm and clipping, and the Nesterov update, over torch tensors in HBM.
 
 Mirrors RLShepherd.trainStep (src/nodes/controllers/rl_shepherd.zig:487-515 packing,
 :600-641 statistics, :643-682 update loop) and the host optimizer
@@ -13,7 +13,8 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from ._lib import FLAG_ASYNC, GradStats, NesterovMode, PcpError, VerifyArgs, check, lib
+from ._lib import (DType, FLAG_ASYNC, GradClipArgs, GradStats, NesterovManyArgs, NesterovMode, NormType, PcpError, VerifyArgs,
+                   check, lib)
 from .grpo import Context, _ptr, _stream_handle, call_scope, default_context, dtype_code
 
 
@@ -57,6 +58,137 @@ def grad_stats(grads, *, stream=None, ctx: Context | None = None) -> dict:
             "inf_count": st.inf_count, "elements": st.elements}
 
 
+@dataclass
+class GradNorm:
+    norm: torch.Tensor        # f32 scalar
+    coef: torch.Tensor        # f32 scalar: what brings the gradients down to max_norm, at most 1
+
+
+_GRAD_DTYPE = {torch.float32: int(DType.f32), torch.bfloat16: int(DType.bf16), torch.float16: int(DType.f16)}
+
+
+class _List:
+    """A list of tensors as the C entry points take it: host arrays of addresses, and of element types."""
+
+    __slots__ = ("ptrs", "types", "at", "types_at")
+
+    def __init__(self, tensors, what: str, dtype: torch.dtype | None = None):
+        n = len(tensors)
+        held = [t for t in tensors if t is not None]
+        try:
+            codes = [_GRAD_DTYPE[t.dtype] for t in held]
+        except KeyError:
+            raise PcpError(-2, f"{what} must be f32, bf16 or f16") from None
+        if dtype is not None and any([c != _GRAD_DTYPE[dtype] for c in codes]):
+            raise PcpError(-2, f"{what} must be {dtype}")
+        if not all([t.is_contiguous() for t in held]):
+            raise PcpError(-1, f"{what} must be contiguous")
+        self.ptrs = (ctypes.c_void_p * n)(*[None if t is None else t.data_ptr() for t in tensors])
+        self.types = (ctypes.c_int32 * len(codes))(*codes)
+        self.at, self.types_at = ctypes.addressof(self.ptrs), ctypes.addressof(self.types)
+
+
+def _counts(grads, *others):
+    counts = [t.numel() for t in grads]
+    for name, ts in others:
+        if ts is not None and (len(ts) != len(counts) or any([t is not None and t.numel() != c for t, c in zip(ts, counts)])):
+            raise PcpError(-12, f"{name} must hold as many tensors as the gradients, of the same sizes")
+    return (ctypes.c_int64 * len(counts))(*counts)
+
+
+def grad_norm(grads, max_norm: float = float("inf"), *, norm_type: int | str = NormType.l2,
+              outputs: GradNorm | None = None, sync: bool = True, stream=None, ctx: Context | None = None) -> GradNorm:
+    """The norm of all gradients together (a tensor or a list of them, f32, bf16 and f16 mixed) and the coefficient
+    that brings it down to max_norm, both left on the device (pcp_grad_clip without outputs): norm_type "l2" or "max".
+    ``Nesterov.update_many`` and ``nesterov_update_many`` take the coefficient there. A norm that is not finite is
+    reported, and its coefficient is NaN. sync=False only enqueues. An empty list needs a ctx or outputs."""
+    return _grad_clip(grads, max_norm, norm_type, None, outputs, sync, stream, ctx)
+
+
+def clip_grads(grads, max_norm: float, *, norm_type: int | str = NormType.l2, out=None, outputs: GradNorm | None = None,
+               sync: bool = True, stream=None, ctx: Context | None = None) -> GradNorm:
+    """``grad_norm``, and the gradients times its coefficient: in place, or into `out` (as many tensors of the same
+    sizes, of any of the three types, such as the pieces of the flat f32 buffer that ``Nesterov.update_flat`` takes).
+    Gradients whose norm is not finite are left (or copied) as they are."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    out = grads if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    return _grad_clip(grads, max_norm, norm_type, out, outputs, sync, stream, ctx)
+
+
+def _grad_clip(grads, max_norm, norm_type, out, outputs, sync, stream, ctx) -> GradNorm:
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if isinstance(norm_type, str):
+        try:
+            norm_type = NormType[norm_type]
+        except KeyError:
+            raise PcpError(-1, f"unknown norm_type {norm_type!r}") from None
+    ctx = ctx or default_context((grads[0] if grads else outputs.norm if outputs is not None else torch.empty(0)).device.index or 0)
+    g = _List(grads, "gradients")
+    counts = _counts(grads, ("out", out))
+    o = None if out is None else g if out is grads else _List(out, "out")
+    a = GradClipArgs()
+    lib().pcp_grad_clip_args_init(ctypes.byref(a))
+    given = () if outputs is None else (outputs.norm, outputs.coef)
+    with call_scope(ctx, stream, *grads, *(out if out is not None and out is not grads else ()), *given) as handle:
+        if outputs is None:
+            both = torch.empty(2, dtype=torch.float32, device=torch.device("cuda", ctx.device))
+            outputs = GradNorm(both[0], both[1])
+        if any(t.dtype != torch.float32 or t.numel() != 1 for t in (outputs.norm, outputs.coef)):
+            raise PcpError(-1, "outputs do not fit the call: norm and coef f32 scalars")
+        a.n_tensors, a.grads, a.counts, a.dtypes = len(grads), g.at, ctypes.addressof(counts), g.types_at
+        if o is not None:
+            a.out, a.out_dtypes = o.at, o.types_at
+        a.norm, a.coef, a.norm_type, a.max_norm = outputs.norm.data_ptr(), outputs.coef.data_ptr(), int(norm_type), max_norm
+        a.flags = 0 if sync else FLAG_ASYNC
+        a.stream = handle
+        check(lib().pcp_grad_clip(ctx.handle, ctypes.byref(a)), ctx.handle)
+    return outputs
+
+
+def nesterov_update_many(params, velocities, grads, param_copies=None, *, coef: torch.Tensor | None = None,
+                         learning_rate: float = 0.01, momentum: float = 0.9, mode: int | str = NesterovMode.sutskever,
+                         sync: bool = True, stream=None, ctx: Context | None = None) -> None:
+    """The Nesterov update of a list of parameters (f32) with their velocities (f32) and gradients (f32, bf16 or f16),
+    each where it lies (pcp_nesterov_update_many): the gradients times coef (a device scalar, ``grad_norm``'s; a
+    coefficient that is not finite skips the update), the updated weights also as bf16 into param_copies (a list of
+    tensors, None among them where there is no copy).
+    sync=False only enqueues."""
+    params, velocities, grads = list(params), list(velocities), list(grads)
+    copies = None if param_copies is None else list(param_copies)
+    if not params and not grads and not velocities:
+        return
+    ctx = ctx or default_context((params or grads or velocities)[0].device.index or 0)
+    v = _List(velocities, "velocities", torch.float32)
+    _update_many(ctx, params, v.at, grads, copies, coef, learning_rate, momentum, mode, sync, stream, velocities)
+
+
+def _update_many(ctx, params, velocities_at, grads, copies, coef, learning_rate, momentum, mode, sync, stream,
+                 velocities=None, counts=None):
+    if isinstance(mode, str):
+        try:
+            mode = NesterovMode[mode]
+        except KeyError:
+            raise PcpError(-1, f"unknown mode {mode!r}") from None
+    n = _counts(grads, ("params", params), ("velocities", velocities), ("param_copies", copies))
+    if counts is not None and list(n) != counts:
+        raise PcpError(-12, "the gradients must have the sizes of the optimizer's tensors")
+    if coef is not None and (coef.dtype != torch.float32 or coef.numel() != 1):
+        raise PcpError(-1, "coef must be an f32 scalar")
+    p, g = _List(params, "parameters", torch.float32), _List(grads, "gradients")
+    c = None if copies is None else _List(copies, "param_copies", torch.bfloat16)
+    a = NesterovManyArgs()
+    lib().pcp_nesterov_many_args_init(ctypes.byref(a))
+    with call_scope(ctx, stream, *params, *(velocities or ()), *grads, *(copies or ()), coef) as handle:
+        a.n_tensors, a.counts = len(grads), ctypes.addressof(n)
+        a.params, a.velocities, a.grads, a.dtypes = p.at, velocities_at, g.at, g.types_at
+        a.param_copies = None if c is None else c.at
+        a.coef = None if coef is None else coef.data_ptr()
+        a.learning_rate, a.momentum, a.mode = learning_rate, momentum, int(mode)
+        a.flags = 0 if sync else FLAG_ASYNC
+        a.stream = handle
+        check(lib().pcp_nesterov_update_many(ctx.handle, ctypes.byref(a)), ctx.handle)
+
+
 class Nesterov:
     """The reference's Nesterov optimizer (src/optimizers/nesterov.zig) with its
     velocities in HBM: init + initParameters -> __init__, update(index, param, grad),
@@ -72,6 +204,7 @@ class Nesterov:
         check(lib().pcp_nesterov_create(self.ctx.handle, float(learning_rate), float(momentum), int(mode),
                                         len(self.counts), arr, ctypes.byref(h)), self.ctx.handle)
         self.handle = h
+        self.learning_rate, self.momentum, self.mode = float(learning_rate), float(momentum), int(mode)
 
     @property
     def total(self) -> int:
@@ -91,6 +224,16 @@ class Nesterov:
             raise PcpError(-2, "param_bf16 must be bf16 with one element per parameter")
         check(lib().pcp_nesterov_update_flat(self.handle, _ptr(params), _ptr(grads), _ptr(param_bf16),
                                              _stream_handle(stream)), self.ctx.handle)
+
+    def update_many(self, params, grads, param_copies=None, *, coef: torch.Tensor | None = None, sync: bool = True,
+                    stream=None) -> None:
+        """``nesterov_update_many`` with this optimizer's velocities: params and grads in the order of its counts."""
+        params, grads = list(params), list(grads)
+        copies = None if param_copies is None else list(param_copies)
+        v = (ctypes.c_void_p * len(self.counts))(*[lib().pcp_nesterov_velocity(self.handle, i)
+                                                   for i in range(len(self.counts))])
+        _update_many(self.ctx, params, ctypes.addressof(v), grads, copies, coef, self.learning_rate, self.momentum,
+                     self.mode, sync, stream, counts=self.counts)
 
     def reset(self) -> None:
         check(lib().pcp_nesterov_reset(self.handle, None), self.ctx.handle)
