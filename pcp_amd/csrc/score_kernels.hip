@@ -34,14 +34,13 @@ struct ScoreRow {
 
 __device__ __forceinline__ ScoreRow score_row(const TokenArrays& a, int64_t s, int64_t t) {
   ScoreRow r{s * a.tok_stride + a.tok_offset + t, -1, true};
+  if (a.ids != nullptr)   // (read along with the mask: one latency for both)
+    r.id = a.ids_i64 ? static_cast<const int64_t*>(a.ids)[r.at] : static_cast<const int32_t*>(a.ids)[r.at];
   if (a.mask != nullptr)
     r.live = a.mask_u8 ? static_cast<const uint8_t*>(a.mask)[r.at] != 0 : static_cast<const float*>(a.mask)[r.at] != 0.f;
-  if (a.ids != nullptr && r.live) {
-    r.id = a.ids_i64 ? static_cast<const int64_t*>(a.ids)[r.at] : static_cast<const int32_t*>(a.ids)[r.at];
-    if (r.id < 0 || r.id >= a.vocab) {
-      if (r.id != PCP_IGNORE_INDEX && threadIdx.x == 0) raise_error(a.err, kErrTokenRange);
-      r.live = false;
-    }
+  if (a.ids != nullptr && r.live && (r.id < 0 || r.id >= a.vocab)) {
+    if (r.id != PCP_IGNORE_INDEX && threadIdx.x == 0) raise_error(a.err, kErrTokenRange);
+    r.live = false;
   }
   return r;
 }
@@ -93,12 +92,12 @@ struct ScoreSums {
   static constexpr bool kFresh = true;
   float k2, mx;
   double s, t;
+  bool masked;
 
-  template <typename TI, int U, typename Held>
-  __device__ __forceinline__ void fresh(const u32x4 (&x)[U], Held held, float bx) {
-    const float nm = fmaxf(mx, bx);
-    const TermScale ts = term_scale(nm, k2);
-    float s1 = 0.f, t1 = 0.f;
+  // CLAMP: exponents of -inf, or near it, may be among them (see terms).
+  template <typename TI, bool CLAMP, int U, typename Held>
+  __device__ __forceinline__ void terms(const u32x4 (&x)[U], Held held, const TermScale& ts, float& s1, float& t1) {
+    s1 = t1 = 0.f;
 #pragma unroll
     for (int q = 0; q < U; ++q)
       if (held(q)) {
@@ -108,9 +107,21 @@ struct ScoreSums {
           const float d = fmaf(TI::unpack(w, j), ts.k, -ts.ref);
           const float e = hw_exp2(d);
           s1 += e;
-          t1 = fmaf(e, fmaxf(d, kLeastExp), t1);
+          t1 = fmaf(e, CLAMP ? fmaxf(d, kLeastExp) : d, t1);
         }
       }
+  }
+  template <typename TI, int U, typename Held>
+  __device__ __forceinline__ void fresh(const u32x4 (&x)[U], Held held, float bx) {
+    const float nm = fmaxf(mx, bx);
+    const TermScale ts = term_scale(nm, k2);
+    float s1, t1;
+    // A masked element's product 0 * -inf makes t1 NaN: then once more, and from there on, with exponents clamped.
+    if (!masked) {
+      terms<TI, false>(x, held, ts, s1, t1);
+      masked = __any(t1 != t1);
+    }
+    if (masked) terms<TI, true>(x, held, ts, s1, t1);
     score_rebase(s, t, mx, nm, k2);
     const float r = term_residue(nm, ts), adj = hw_exp2(-r);
     s += static_cast<double>(s1 * adj);
@@ -120,6 +131,31 @@ struct ScoreSums {
   template <typename TI, int U, typename Held>
   __device__ __forceinline__ bool add(const u32x4 (&)[U], Held, float, bool (&)[U]) { return false; }
 };
+
+// The largest of m and a vector's elements. bf16: a word taken as an f32 orders by its upper element, whose
+// bits are then the maximum's upper half (an infinity there may read as NaN, which is left out: -inf is
+// no maximum, and a row with +inf is reported by its sum). f16: pairs at once.
+template <typename TI>
+__device__ __forceinline__ float score_max(float m, const u32x4& v) {
+  if constexpr (__is_same(TI, BF16T)) {
+    float hi = kNegInf;
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      // (Byte permutes, which the compiler does not merge with the sums' shifts: those would stay live.)
+      m = max3(m, __uint_as_float(__builtin_amdgcn_perm(v[i], 0u, 0x05040c0cu)),
+               __uint_as_float(__builtin_amdgcn_perm(v[i + 1], 0u, 0x05040c0cu)));
+      hi = max3(hi, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+    }
+    return fmaxf(m, __uint_as_float(__float_as_uint(hi) & 0xffff0000u));
+  } else if constexpr (__is_same(TI, F16T)) {
+    const f16x2 a = __builtin_elementwise_max(__builtin_bit_cast(f16x2, v[0]), __builtin_bit_cast(f16x2, v[1]));
+    const f16x2 b = __builtin_elementwise_max(__builtin_bit_cast(f16x2, v[2]), __builtin_bit_cast(f16x2, v[3]));
+    const f16x2 c = __builtin_elementwise_max(a, b);
+    return max3(m, static_cast<float>(c[0]), static_cast<float>(c[1]));
+  } else {
+    return vec_max<TI>(m, v);
+  }
+}
 
 // The merge of the first N lanes' sums, on every lane, in a fixed order.
 template <int N>
@@ -190,7 +226,7 @@ __global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
   const RowSpan sp = row_span<TI>(xrow, a.tok.vocab);
   const int v0 = part * a.per, end = min(v0 + a.per, sp.nv);
   const __amdgpu_buffer_rsrc_t xbuf = row_rsrc(sp.vec, static_cast<uint32_t>(max(end, 0)) * 16u);
-  ScoreSums sums{a.k2, kNegInf, 0., 0.};
+  ScoreSums sums{a.k2, kNegInf, 0., 0., false};
   Candidates c{sh, 0, kNegInf};
   if constexpr (TOP) {
     if (tid == 0) sh.count = 0;
@@ -213,17 +249,20 @@ __global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
     __syncthreads();
     n = sh.count;
   } else {
-    for (int base = v0; base < end; base += BLOCK * U) {
+    // Whole batches without a test for each vector, then what is left.
+    auto batch = [&](int base, auto held) {
       u32x4 x[U];
       const uint32_t off = static_cast<uint32_t>(base + tid) * 16u;
 #pragma unroll
       for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
-      auto held = [&](int q) { return base + q * BLOCK + tid < end; };
       float bx = kNegInf;
 #pragma unroll
-      for (int q = 0; q < U; ++q) bx = held(q) ? vec_max<TI>(bx, x[q]) : bx;
+      for (int q = 0; q < U; ++q) bx = held(q) ? score_max<TI>(bx, x[q]) : bx;
       sums.template fresh<TI>(x, held, bx);
-    }
+    };
+    int base = v0;
+    for (; base + BLOCK * U <= end; base += BLOCK * U) batch(base, [](int) { return true; });
+    if (base < end) batch(base, [&](int q) { return base + q * BLOCK + tid < end; });
   }
   float mx = sums.mx;
   double s = sums.s, tt = sums.t;
