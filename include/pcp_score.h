@@ -48,9 +48,9 @@ extern "C" {
  * 0; NaN ranks below every number. A finite mask of any size (-1e30, a type's lowest value)
  * is a logit like any other.
  *
- * Reported after the call (or by pcp_sync), with the outputs written: a token id outside
- * [0, V) on a row with weight (PCP_ERR_TOKEN_RANGE; the row counts as one without weight), and
- * a row whose row_max or log_sum is not finite (a NaN or +Inf logit, nothing above -Inf: PCP_ERR_NONFINITE).
+ * Reported after the call (or by pcp_sync): a token id outside [0, V) on a row with weight
+ * (PCP_ERR_TOKEN_RANGE; the row counts as one without weight), and a row whose row_max or log_sum is not finite
+ * (a NaN or +Inf logit, nothing above -Inf: PCP_ERR_NONFINITE; its outputs are written and mean nothing).
  * Rows are summed in a fixed order: the same call gives the same bits, but calls with other row
  * counts may deal a row to other numbers of workgroups.
  */

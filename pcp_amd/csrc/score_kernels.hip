@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <cstddef>
 #include <cstdint>
 #include <cstring>
 
@@ -72,6 +73,7 @@ struct ScoreArgs {
   double inv_tau;
   float k2;                // log2(e) / temperature
   int32_t k, top_i64, parts, per, part_cap;
+  int32_t group;           // batches per group (gather_top)
 };
 
 // An exponent this low is a term of 0, whose product with it then is 0 too (and not NaN at -inf).
@@ -86,15 +88,14 @@ __device__ __forceinline__ void score_rebase(double& s, double& t, float m, floa
 }
 
 // Of a lane: its largest logit mx, and against it the sum s of the terms 2^d, d = (x - mx) k, and the sum t of
-// 2^d d. The sums of a batch are f32 against the rounded product ref of mx and k, whose residue is
+// 2^d d. The sums of a batch are f32 against the rounded product ref of mx and k, whose residue r is
 // taken out once per batch: of terms 2^d it leaves 2^-r s and 2^-r (t - r s).
 struct ScoreSums {
-  static constexpr bool kFresh = true;
   float k2, mx;
   double s, t;
   bool masked;
 
-  // CLAMP: exponents of -inf, or near it, may be among them (see terms).
+  // CLAMP: exponents of -inf, or near it, may be among them, whose products would be NaN.
   template <typename TI, bool CLAMP, int U, typename Held>
   __device__ __forceinline__ void terms(const u32x4 (&x)[U], Held held, const TermScale& ts, float& s1, float& t1) {
     s1 = t1 = 0.f;
@@ -111,50 +112,260 @@ struct ScoreSums {
         }
       }
   }
+  // A batch whose largest logit is bx. A masked element's product 0 * -inf makes t1 NaN: then once more, and
+  // from there on, with exponents clamped.
   template <typename TI, int U, typename Held>
-  __device__ __forceinline__ void fresh(const u32x4 (&x)[U], Held held, float bx) {
+  __device__ __forceinline__ void add(const u32x4 (&x)[U], Held held, float bx) {
     const float nm = fmaxf(mx, bx);
     const TermScale ts = term_scale(nm, k2);
     float s1, t1;
-    // A masked element's product 0 * -inf makes t1 NaN: then once more, and from there on, with exponents clamped.
     if (!masked) {
       terms<TI, false>(x, held, ts, s1, t1);
       masked = __any(t1 != t1);
     }
-    if (masked) terms<TI, true>(x, held, ts, s1, t1);
+    if (masked) {
+      // Opaque copies: the compiler would else keep every exponent and term of the first pass for this one.
+      u32x4 y[U];
+#pragma unroll
+      for (int q = 0; q < U; ++q) {
+        y[q] = x[q];
+        asm volatile("" : "+v"(y[q]));
+      }
+      terms<TI, true>(y, held, ts, s1, t1);
+    }
     score_rebase(s, t, mx, nm, k2);
     const float r = term_residue(nm, ts), adj = hw_exp2(-r);
     s += static_cast<double>(s1 * adj);
     t += static_cast<double>(fmaf(-r, s1, t1) * adj);
     mx = nm;
   }
-  template <typename TI, int U, typename Held>
-  __device__ __forceinline__ bool add(const u32x4 (&)[U], Held, float, bool (&)[U]) { return false; }
 };
 
-// The largest of m and a vector's elements. bf16: a word taken as an f32 orders by its upper element, whose
-// bits are then the maximum's upper half (an infinity there may read as NaN, which is left out: -inf is
-// no maximum, and a row with +inf is reported by its sum). f16: pairs at once.
-template <typename TI>
-__device__ __forceinline__ float score_max(float m, const u32x4& v) {
+// The largest element of a batch, two 16-bit ones an instruction. bf16 values compare as 16-bit integers where one is
+// positive; a lane that holds negative ones alone (or none) makes its wave look again.
+template <typename TI, int U, typename Held>
+__device__ __forceinline__ float batch_max(const u32x4 (&x)[U], Held held) {
+  typedef short i16x2 __attribute__((ext_vector_type(2)));
+  float m = kNegInf;
   if constexpr (__is_same(TI, BF16T)) {
-    float hi = kNegInf;
+    i16x2 top = {-32768, -32768};
 #pragma unroll
-    for (int i = 0; i < 4; i += 2) {
-      // (Byte permutes, which the compiler does not merge with the sums' shifts: those would stay live.)
-      m = max3(m, __uint_as_float(__builtin_amdgcn_perm(v[i], 0u, 0x05040c0cu)),
-               __uint_as_float(__builtin_amdgcn_perm(v[i + 1], 0u, 0x05040c0cu)));
-      hi = max3(hi, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-    }
-    return fmaxf(m, __uint_as_float(__float_as_uint(hi) & 0xffff0000u));
+    for (int q = 0; q < U; ++q)
+      if (held(q)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = x[q][i];   // (a variable: __builtin_bit_cast of a vector's element takes the first one)
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(i16x2, w));
+        }
+      }
+    const uint32_t t = __builtin_bit_cast(uint32_t, top);
+    m = fmaxf(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u));
+    if (!__any(top[0] < 0 && top[1] < 0)) return m;
+    m = kNegInf;
+#pragma unroll
+    for (int q = 0; q < U; ++q) m = held(q) ? vec_max<TI>(m, x[q]) : m;
   } else if constexpr (__is_same(TI, F16T)) {
-    const f16x2 a = __builtin_elementwise_max(__builtin_bit_cast(f16x2, v[0]), __builtin_bit_cast(f16x2, v[1]));
-    const f16x2 b = __builtin_elementwise_max(__builtin_bit_cast(f16x2, v[2]), __builtin_bit_cast(f16x2, v[3]));
-    const f16x2 c = __builtin_elementwise_max(a, b);
-    return max3(m, static_cast<float>(c[0]), static_cast<float>(c[1]));
+    f16x2 top = {-__builtin_inff16(), -__builtin_inff16()};
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+      if (held(q)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t w = x[q][i];
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(f16x2, w));
+        }
+      }
+    m = fmaxf(static_cast<float>(top[0]), static_cast<float>(top[1]));
   } else {
-    return vec_max<TI>(m, v);
+#pragma unroll
+    for (int q = 0; q < U; ++q) m = held(q) ? vec_max<TI>(m, x[q]) : m;
   }
+  return m;
+}
+
+// ---- the k largest of a part ----
+// The pass over the part leaves each lane's largest logit of every group of batches (at most kGroups groups). What k of
+// those reach, k elements reach, each in a group of its own; so only groups that reach it are read again, about
+// k of a row's thousands, and what reaches it there are the candidates, few more than k.
+
+constexpr int kGroups = 16;
+
+struct PartShared {
+  union {
+    Shared sh;
+    float group[kGroups][kBlock];   // until the candidates are gathered
+  };
+};
+static_assert(offsetof(Shared, key) == 0 && sizeof(float) * kGroups * kBlock <= sizeof(uint64_t) * kCap,
+              "groups lie over the keys alone");
+
+// The part's candidates where values may be equal in any number: the exact k-th largest by its bits, eight a pass,
+// then those above it and as many of its equals as are missing, by rising id. Called by the whole workgroup with sh free;
+// returns their number, min(k, elements). Six passes: for parts of masks or of few values.
+template <typename TI>
+__device__ __forceinline__ int select_exact(const char* xrow, const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end,
+                                            bool edges, int k, Shared& sh) {
+  constexpr int EPV = 16 / TI::kBytes;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int total = max(end - v0, 0) * EPV + (edges ? sp.head + sp.tail : 0);
+  const int ek = edges ? edge_index<TI>(sp, tid) : -1;
+  const uint32_t edge = ek >= 0 ? order_bits(TI::load1(xrow, ek)) : 0u;
+  int need = min(k, total);
+  uint32_t prefix = 0;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kBlock) sh.bin[i] = 0;
+    __syncthreads();
+    auto count = [&](bool is, uint32_t b) {
+      const uint32_t rest = shift == 24 ? 0u : (b ^ prefix) >> (shift + 8);
+      const int bin = is && rest == 0 ? static_cast<int>(b >> shift & 255u) : -1;
+      // One lane for all where a wave's elements are alike, as masks are.
+      const int other = __builtin_amdgcn_readfirstlane(bin);
+      if (__all(bin == other)) {
+        if (lane == 0 && bin >= 0) atomicAdd(&sh.bin[bin], 64);
+      } else if (bin >= 0) {
+        atomicAdd(&sh.bin[bin], 1);
+      }
+    };
+    for (int base = v0; base < end; base += kBlock) {
+      const bool is = base + tid < end;
+      const u32x4 x = buf_ld16<false>(xbuf, static_cast<uint32_t>(base + tid) * 16u);
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) count(is, order_bits(TI::unpack(reinterpret_cast<const uint32_t*>(&x), j)));
+    }
+    if (ek >= 0) {
+      const uint32_t rest = shift == 24 ? 0u : (edge ^ prefix) >> (shift + 8);
+      if (rest == 0) atomicAdd(&sh.bin[edge >> shift & 255u], 1);
+    }
+    __syncthreads();
+    // Every wave finds the bin of the need-th largest: lane l has bins 4 (63 - l) .. + 3.
+    const int first = 4 * (63 - lane);
+    const int4 c = *reinterpret_cast<const int4*>(&sh.bin[first]);
+    const int all = c.x + c.y + c.z + c.w;
+    int above = lanes_scan(all) - all, at = first + 3;
+    const int counts[4] = {c.w, c.z, c.y, c.x};
+    const uint64_t who = __ballot(above + all >= need);
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (!found) {
+        if (above + counts[i] >= need) {
+          found = true;
+          at = first + 3 - i;
+        } else {
+          above += counts[i];
+        }
+      }
+    const int owner = __builtin_ctzll(who);
+    need -= __builtin_amdgcn_readlane(above, owner);
+    prefix |= static_cast<uint32_t>(__builtin_amdgcn_readlane(at, owner)) << shift;
+  }
+  // prefix: the k-th largest, need: its equals to take, by rising id: head, interior, tail.
+  __syncthreads();
+  if (tid == 0) sh.count = 0;
+  int taken = 0;
+  __syncthreads();
+  Candidates c{sh, 0, kNegInf};
+  auto step = [&](const u32x4& x, bool is, uint32_t id0, int n_el) {   // up to EPV elements of rising id per lane
+    uint32_t b[EPV];
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) {
+      b[j] = order_bits(TI::unpack(reinterpret_cast<const uint32_t*>(&x), j));
+      mine += is && j < n_el && b[j] == prefix;
+    }
+    const int incl = lanes_scan(mine);
+    if (lane == 63) sh.bin[wave] = incl;
+    __syncthreads();
+    int before = taken + incl - mine, sum = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      before += w < wave ? sh.bin[w] : 0;
+      sum += sh.bin[w];
+    }
+    __syncthreads();
+    taken += sum;
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) {
+      const bool there = is && j < n_el, same = there && b[j] == prefix;
+      c.add((there && b[j] > prefix) || (same && before < need),
+            static_cast<uint64_t>(b[j]) << 32 | (0xffffffffu - (id0 + static_cast<uint32_t>(j))));
+      before += same;
+    }
+  };
+  auto one = [&](int at) {
+    u32x4 x = {};
+    const float v = TI::load1(xrow, at);
+    x[0] = TI::kBytes == 4 ? __float_as_uint(v) : __is_same(TI, BF16T) ? __float_as_uint(v) >> 16 : pack2<F16T>(v, 0.f);
+    return x;
+  };
+  if (edges) step(one(min(tid, max(sp.head - 1, 0))), tid < sp.head, static_cast<uint32_t>(tid), 1);
+  for (int base = v0; base < end; base += kBlock)
+    step(buf_ld16<false>(xbuf, static_cast<uint32_t>(base + tid) * 16u), base + tid < end,
+         static_cast<uint32_t>(sp.head + (base + tid) * EPV), EPV);
+  const int tail0 = sp.head + sp.nv * EPV;
+  if (edges) step(one(tail0 + min(tid, max(sp.tail - 1, 0)) - (sp.tail == 0)), tid < sp.tail, static_cast<uint32_t>(tail0 + tid), 1);
+  __syncthreads();
+  return min(k, total);
+}
+
+// The candidates of a part whose lanes have left their groups' largest logits (batches: batches per group, groups:
+// how many), k or more of them where the part has as many elements. Called by the whole workgroup; ends with a barrier.
+template <typename TI>
+__device__ __forceinline__ int gather_top(const char* xrow, const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end,
+                                          bool edges, int k, int batches, int groups, PartShared& ps) {
+  constexpr int EPV = 16 / TI::kBytes, U = kU;
+  Shared& sh = ps.sh;
+  const int tid = threadIdx.x;
+  float v[kGroups], lane_max[1] = {kNegInf};
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    v[g] = g < groups ? ps.group[g][tid] : kNegInf;
+    lane_max[0] = fmaxf(lane_max[0], v[g]);
+  }
+  // Up to 64 of the lanes' own maxima are nearly as high as the groups', and 256 values sooner counted than 4096.
+  const float least = k <= 64 ? reached_by(sh, lane_max, k) : reached_by(sh, v, k);
+  uint32_t left = 0;
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) left |= g < groups && v[g] >= least ? 1u << g : 0u;
+  __syncthreads();
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  const int total = max(end - v0, 0) * EPV + (edges ? sp.head + sp.tail : 0);
+  const bool all = least == kNegInf;   // fewer than k values above masks: a short part's elements all
+  if (all && total > kCap) return select_exact<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
+  if (all) left = (1u << groups) - 1u;
+  Candidates c{sh, 0, least};
+  if (edges && tid < 64) {
+    const int ek = edge_index<TI>(sp, tid);
+    const float x = ek >= 0 ? TI::load1(xrow, ek) : kNegInf;
+    c.add(ek >= 0 && (x >= least || all), element_key(x, static_cast<uint32_t>(ek)));
+  }
+  while (__any(left != 0)) {
+    const bool mine = left != 0;
+    const int g = __builtin_ctz(left | 1u << kGroups);
+    left &= left - 1;
+    for (int b = 0; b < batches; ++b) {
+      const int at = v0 + (g * batches + b) * (kBlock * U) + tid;
+      u32x4 x[U];
+#pragma unroll
+      for (int q = 0; q < U; ++q) x[q] = buf_ld16<false>(xbuf, mine ? static_cast<uint32_t>(at + q * kBlock) * 16u : 0u);
+#pragma unroll
+      for (int q = 0; q < U; ++q) {
+        const bool is = mine && at + q * kBlock < end;
+        if (!__any(is && (vec_max<TI>(kNegInf, x[q]) >= least || all))) continue;
+#pragma unroll
+        for (int j = 0; j < EPV; ++j) {
+          const float e = TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j);
+          c.add(is && (e >= least || all), element_key(e, static_cast<uint32_t>(sp.head + (at + q * kBlock) * EPV + j)));
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = sh.count;
+  __syncthreads();
+  return n <= kCap ? n : select_exact<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
 }
 
 // The merge of the first N lanes' sums, on every lane, in a fixed order.
@@ -168,23 +379,24 @@ __device__ __forceinline__ void score_merge(float& mx, double& s, double& t, flo
   mx = M;
 }
 
-template <typename TI>
+// A row's outputs: the alternatives by the threads that rank them, the rest by thread 0.
+template <typename TI, bool TOP>
 __device__ __forceinline__ void score_write(const ScoreArgs& a, const ScoreRow& r, const char* xrow, Shared& sh, int n,
                                             float mx, double s, double t) {
   const double log_sum = ms_lse(0.f, static_cast<float>(s));
-  if (a.k > 0)
+  auto log_p = [&](float x) {
+    return static_cast<float>((static_cast<double>(x) - static_cast<double>(mx)) * a.inv_tau - log_sum);
+  };
+  if constexpr (TOP)
     rank_entries(sh, n, a.k, [&](int rank, float x, int64_t id) {
       const int64_t at = r.at * a.k + rank;
-      a.top_logp[at] = static_cast<float>((static_cast<double>(x) - static_cast<double>(mx)) * a.inv_tau - log_sum);
+      a.top_logp[at] = log_p(x);
       if (a.top_i64) static_cast<int64_t*>(a.top_ids)[at] = id;
       else static_cast<int32_t*>(a.top_ids)[at] = static_cast<int32_t>(id);
     });
   if (threadIdx.x != 0) return;
   if (!__builtin_isfinite(mx) || !__builtin_isfinite(log_sum)) raise_error(a.tok.err, kErrNonFinite);
-  if (a.logp) {
-    const double x = r.id < 0 ? static_cast<double>(mx) : static_cast<double>(TI::load1(xrow, r.id));
-    a.logp[r.at] = r.id < 0 ? 0.f : static_cast<float>((x - static_cast<double>(mx)) * a.inv_tau - log_sum);
-  }
+  if (a.logp) a.logp[r.at] = r.id < 0 ? 0.f : log_p(TI::load1(xrow, r.id));
   if (a.entropy) a.entropy[r.at] = static_cast<float>(log_sum - t / s * kLn2d);
   if (a.row_max) a.row_max[r.at] = mx;
   if (a.log_sum) a.log_sum[r.at] = static_cast<float>(log_sum);
@@ -205,9 +417,10 @@ __device__ __forceinline__ void score_dead(const ScoreArgs& a, const ScoreRow& r
 }
 
 template <typename TI, bool TOP>
-__global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
+__global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a) {
   constexpr int BLOCK = kBlock, U = kU;
-  __shared__ __align__(16) Shared sh;
+  __shared__ __align__(16) PartShared ps;
+  Shared& sh = ps.sh;
   __shared__ double wave_s[kWaves], wave_t[kWaves];
   __shared__ float wave_mx[kWaves];
   __shared__ unsigned turn;
@@ -227,43 +440,32 @@ __global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
   const int v0 = part * a.per, end = min(v0 + a.per, sp.nv);
   const __amdgpu_buffer_rsrc_t xbuf = row_rsrc(sp.vec, static_cast<uint32_t>(max(end, 0)) * 16u);
   ScoreSums sums{a.k2, kNegInf, 0., 0., false};
-  Candidates c{sh, 0, kNegInf};
-  if constexpr (TOP) {
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-  }
   if (part == 0 && tid < 64) {   // the elements outside the interior
     const int ek = edge_index<TI>(sp, tid);
-    float xe = kNegInf;
     if (ek >= 0) {
-      xe = TI::load1(xrow, ek);
-      sums.mx = fmaxf(sums.mx, xe);
-      sums.s = hw_exp2((xe - ms_ref(sums.mx)) * a.k2);
+      sums.mx = fmaxf(sums.mx, TI::load1(xrow, ek));
+      sums.s = hw_exp2((TI::load1(xrow, ek) - ms_ref(sums.mx)) * a.k2);
     }
-    if constexpr (TOP) c.add(ek >= 0, element_key(xe, static_cast<uint32_t>(ek)));
   }
-  int n = 0;
-  if constexpr (TOP) {
-    scan_part<TI>(sp, xbuf, v0, end, part == 0 ? sp.head + sp.tail : 0, a.k, a.parts == 1 ? a.k + 64 : a.part_cap, sums, c,
-                  sh);
-    __syncthreads();
-    n = sh.count;
-  } else {
-    // Whole batches without a test for each vector, then what is left.
-    auto batch = [&](int base, auto held) {
-      u32x4 x[U];
-      const uint32_t off = static_cast<uint32_t>(base + tid) * 16u;
+  // Whole batches without a test for each vector, then what is left.
+  float group = kNegInf;
+  int b = 0;
+  auto batch = [&](int base, auto held) {
+    u32x4 x[U];
+    const uint32_t off = static_cast<uint32_t>(base + tid) * 16u;
 #pragma unroll
-      for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
-      float bx = kNegInf;
-#pragma unroll
-      for (int q = 0; q < U; ++q) bx = held(q) ? score_max<TI>(bx, x[q]) : bx;
-      sums.template fresh<TI>(x, held, bx);
-    };
-    int base = v0;
-    for (; base + BLOCK * U <= end; base += BLOCK * U) batch(base, [](int) { return true; });
-    if (base < end) batch(base, [&](int q) { return base + q * BLOCK + tid < end; });
-  }
+    for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
+    const float bx = batch_max<TI>(x, held);
+    sums.template add<TI>(x, held, bx);
+    if constexpr (TOP) {
+      group = b % a.group == 0 ? bx : fmaxf(group, bx);
+      ps.group[b / a.group][tid] = group;
+      ++b;
+    }
+  };
+  int base = v0;
+  for (; base + BLOCK * U <= end; base += BLOCK * U) batch(base, [](int) { return true; });
+  if (base < end) batch(base, [&](int q) { return base + q * BLOCK + tid < end; });
   float mx = sums.mx;
   double s = sums.s, tt = sums.t;
   score_merge<64>(mx, s, tt, a.k2);
@@ -277,10 +479,14 @@ __global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
   s = wave_s[lane & (kWaves - 1)];
   tt = wave_t[lane & (kWaves - 1)];
   score_merge<kWaves>(mx, s, tt, a.k2);
+  int n = 0;
+  if constexpr (TOP) n = gather_top<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, a.group, (b + a.group - 1) / a.group, ps);
   if (a.parts == 1) {
-    score_write<TI>(a, r, xrow, sh, n, mx, s, tt);
+    score_write<TI, TOP>(a, r, xrow, sh, n, mx, s, tt);
     return;
   }
+  if constexpr (TOP)
+    if (n > a.part_cap) n = Candidates{sh, 0, kNegInf}.thin(n, a.k, a.part_cap);
   // The part's candidates and sums for the last of the row's workgroups to finish, which merges them.
   ScorePart* parts = a.part + static_cast<int64_t>(of) * a.parts;
   uint64_t* keys = a.part_key + static_cast<int64_t>(of) * a.parts * a.part_cap;
@@ -308,7 +514,7 @@ __global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
     tt = parts[lane].t;
   }
   score_merge<64>(mx, s, tt, a.k2);
-  score_write<TI>(a, r, xrow, sh, n, mx, s, tt);
+  score_write<TI, TOP>(a, r, xrow, sh, n, mx, s, tt);
 }
 
 template <typename TI>
@@ -539,14 +745,14 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
   hipStream_t st = static_cast<hipStream_t>(a->stream);
 
-  // Workgroups per row: as few rows' logits as would leave CUs idle are dealt to several, at least a batch each.
+  // Workgroups per row: as few rows' logits as would leave CUs idle are dealt to several, at least kLeastPart vectors each.
+  constexpr int64_t kLeastPart = 2 * kBlock;
   const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
-  const int64_t batches = nv > 0 ? (nv + kBlock * kU - 1) / (kBlock * kU) : 1;
   int64_t parts = n_rows < kScoreTickets ? (2048 + n_rows - 1) / n_rows : 1;
-  if (parts > batches) parts = batches;
   if (parts > 64) parts = 64;   // one wave merges their sums
-  const int64_t per_batches = (batches + parts - 1) / parts;
-  parts = (batches + per_batches - 1) / per_batches;
+  int64_t per = ((nv + parts - 1) / parts + kBlock - 1) / kBlock * kBlock;
+  if (per < kLeastPart) per = kLeastPart;
+  parts = nv > 0 ? (nv + per - 1) / per : 1;
   const int64_t part_cap = a->k > 0 ? a->k + 64 : 0;
   const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(n_rows) * parts * part_cap : 0;
   const size_t sums = parts > 1 ? sizeof(ScorePart) * static_cast<size_t>(n_rows) * parts + 16 : 0;
@@ -569,8 +775,9 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   t.k = a->k;
   t.top_i64 = a->top_ids_dtype == PCP_I64;
   t.parts = static_cast<int32_t>(parts);
-  t.per = static_cast<int32_t>(per_batches * kBlock * kU);
+  t.per = static_cast<int32_t>(per);
   t.part_cap = static_cast<int32_t>(part_cap);
+  t.group = static_cast<int32_t>((per + kBlock * kU * kGroups - 1) / (kBlock * kU * kGroups));
   const bool timed = prof_begin(ctx, st);
   const hipError_t e = a->logits_dtype == PCP_F32    ? launch_score<F32T>(t, n_rows, st)
                        : a->logits_dtype == PCP_BF16 ? launch_score<BF16T>(t, n_rows, st)
