@@ -76,6 +76,15 @@ struct ScoreArgs {
   int32_t group;           // batches per group (gather_top)
 };
 
+// Loads at agent scope (sc1), for what other workgroups have stored with store_coherent.
+constexpr int kBufAgent = 16;
+__device__ __forceinline__ u32x4 buf_ld16_coherent(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, kBufAgent));
+}
+__device__ __forceinline__ uint64_t buf_ld8_coherent(__amdgpu_buffer_rsrc_t r, uint32_t off) {
+  return __builtin_bit_cast(uint64_t, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, kBufAgent));
+}
+
 // An exponent this low is a term of 0, whose product with it then is 0 too (and not NaN at -inf).
 constexpr float kLeastExp = -1024.f;
 
@@ -350,18 +359,45 @@ __device__ __forceinline__ int gather_top(const char* xrow, const RowSpan& sp, _
       u32x4 x[U];
 #pragma unroll
       for (int q = 0; q < U; ++q) x[q] = buf_ld16<false>(xbuf, mine ? static_cast<uint32_t>(at + q * kBlock) * 16u : 0u);
+      uint32_t left_q = 0;
 #pragma unroll
-      for (int q = 0; q < U; ++q) {
-        const bool is = mine && at + q * kBlock < end;
-        if (!__any(is && (vec_max<TI>(kNegInf, x[q]) >= least || all))) continue;
-#pragma unroll
-        for (int j = 0; j < EPV; ++j) {
-          const float e = TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j);
-          c.add(is && (e >= least || all), element_key(e, static_cast<uint32_t>(sp.head + (at + q * kBlock) * EPV + j)));
-        }
-      }
+      for (int q = 0; q < U; ++q)
+        left_q |= mine && at + q * kBlock < end && (vec_max<TI>(kNegInf, x[q]) >= least || all) ? 1u << q : 0u;
+      take_vectors<TI>(c, x, left_q, static_cast<uint32_t>(sp.head + at * EPV), (1u << EPV) - 1u);
     }
   }
+  __syncthreads();
+  const int n = sh.count;
+  __syncthreads();
+  return n <= kCap ? n : select_exact<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
+}
+
+// The same for a part of one batch, which is still in x; lane_max: the lane's largest logit.
+template <typename TI, int U>
+__device__ __forceinline__ int gather_one(const char* xrow, const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end,
+                                          bool edges, int k, const u32x4 (&x)[U], float lane_max, Shared& sh) {
+  constexpr int EPV = 16 / TI::kBytes;
+  const int tid = threadIdx.x;
+  float v[U];
+#pragma unroll
+  for (int q = 0; q < U; ++q) v[q] = v0 + q * kBlock + tid < end ? vec_max<TI>(kNegInf, x[q]) : kNegInf;
+  const float own[1] = {lane_max};
+  const float least = k <= 64 ? reached_by(sh, own, k) : reached_by(sh, v, k);
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  const int total = max(end - v0, 0) * EPV + (edges ? sp.head + sp.tail : 0);
+  const bool all = least == kNegInf;
+  if (all && total > kCap) return select_exact<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
+  Candidates c{sh, 0, least};
+  if (edges && tid < 64) {
+    const int ek = edge_index<TI>(sp, tid);
+    const float e = ek >= 0 ? TI::load1(xrow, ek) : kNegInf;
+    c.add(ek >= 0 && (e >= least || all), element_key(e, static_cast<uint32_t>(ek)));
+  }
+  uint32_t left_q = 0;
+#pragma unroll
+  for (int q = 0; q < U; ++q) left_q |= v0 + q * kBlock + tid < end && (v[q] >= least || all) ? 1u << q : 0u;
+  take_vectors<TI>(c, x, left_q, static_cast<uint32_t>(sp.head + (v0 + tid) * EPV), (1u << EPV) - 1u);
   __syncthreads();
   const int n = sh.count;
   __syncthreads();
@@ -380,9 +416,9 @@ __device__ __forceinline__ void score_merge(float& mx, double& s, double& t, flo
 }
 
 // A row's outputs: the alternatives by the threads that rank them, the rest by thread 0.
-template <typename TI, bool TOP>
-__device__ __forceinline__ void score_write(const ScoreArgs& a, const ScoreRow& r, const char* xrow, Shared& sh, int n,
-                                            float mx, double s, double t) {
+template <bool TOP>
+__device__ __forceinline__ void score_write(const ScoreArgs& a, const ScoreRow& r, float token, Shared& sh, int n, float mx,
+                                            double s, double t) {
   const double log_sum = ms_lse(0.f, static_cast<float>(s));
   auto log_p = [&](float x) {
     return static_cast<float>((static_cast<double>(x) - static_cast<double>(mx)) * a.inv_tau - log_sum);
@@ -396,7 +432,7 @@ __device__ __forceinline__ void score_write(const ScoreArgs& a, const ScoreRow& 
     });
   if (threadIdx.x != 0) return;
   if (!__builtin_isfinite(mx) || !__builtin_isfinite(log_sum)) raise_error(a.tok.err, kErrNonFinite);
-  if (a.logp) a.logp[r.at] = r.id < 0 ? 0.f : log_p(TI::load1(xrow, r.id));
+  if (a.logp) a.logp[r.at] = r.id < 0 ? 0.f : log_p(token);
   if (a.entropy) a.entropy[r.at] = static_cast<float>(log_sum - t / s * kLn2d);
   if (a.row_max) a.row_max[r.at] = mx;
   if (a.log_sum) a.log_sum[r.at] = static_cast<float>(log_sum);
@@ -416,7 +452,8 @@ __device__ __forceinline__ void score_dead(const ScoreArgs& a, const ScoreRow& r
   if (a.log_sum) a.log_sum[r.at] = 0.f;
 }
 
-template <typename TI, bool TOP>
+// ONE: rows in parts of at most a batch each.
+template <typename TI, bool TOP, bool ONE>
 __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a) {
   constexpr int BLOCK = kBlock, U = kU;
   __shared__ __align__(16) PartShared ps;
@@ -424,6 +461,7 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
   __shared__ double wave_s[kWaves], wave_t[kWaves];
   __shared__ float wave_mx[kWaves];
   __shared__ unsigned turn;
+  __shared__ int counts[64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t of = blockIdx.x / static_cast<uint32_t>(a.parts);
   const int part = static_cast<int>(blockIdx.x - of * static_cast<uint32_t>(a.parts));
@@ -440,6 +478,7 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
   const int v0 = part * a.per, end = min(v0 + a.per, sp.nv);
   const __amdgpu_buffer_rsrc_t xbuf = row_rsrc(sp.vec, static_cast<uint32_t>(max(end, 0)) * 16u);
   ScoreSums sums{a.k2, kNegInf, 0., 0., false};
+  const float token = r.id >= 0 ? TI::load1(xrow, r.id) : 0.f;   // (ahead of the row: nothing waits for it at the end)
   if (part == 0 && tid < 64) {   // the elements outside the interior
     const int ek = edge_index<TI>(sp, tid);
     if (ek >= 0) {
@@ -447,25 +486,26 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
       sums.s = hw_exp2((TI::load1(xrow, ek) - ms_ref(sums.mx)) * a.k2);
     }
   }
-  // Whole batches without a test for each vector, then what is left.
-  float group = kNegInf;
+  u32x4 x[U];
+  float bx = kNegInf, group = kNegInf;
   int b = 0;
   auto batch = [&](int base, auto held) {
-    u32x4 x[U];
     const uint32_t off = static_cast<uint32_t>(base + tid) * 16u;
 #pragma unroll
     for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
-    const float bx = batch_max<TI>(x, held);
+    bx = batch_max<TI>(x, held);
     sums.template add<TI>(x, held, bx);
-    if constexpr (TOP) {
+    if constexpr (TOP && !ONE) {
       group = b % a.group == 0 ? bx : fmaxf(group, bx);
       ps.group[b / a.group][tid] = group;
       ++b;
     }
   };
+  // Whole batches without a test for each vector, then what is left.
   int base = v0;
-  for (; base + BLOCK * U <= end; base += BLOCK * U) batch(base, [](int) { return true; });
-  if (base < end) batch(base, [&](int q) { return base + q * BLOCK + tid < end; });
+  if constexpr (!ONE)
+    for (; base + BLOCK * U <= end; base += BLOCK * U) batch(base, [](int) { return true; });
+  if (base < end || ONE) batch(base, [&](int q) { return base + q * BLOCK + tid < end; });
   float mx = sums.mx;
   double s = sums.s, tt = sums.t;
   score_merge<64>(mx, s, tt, a.k2);
@@ -480,9 +520,11 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
   tt = wave_t[lane & (kWaves - 1)];
   score_merge<kWaves>(mx, s, tt, a.k2);
   int n = 0;
-  if constexpr (TOP) n = gather_top<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, a.group, (b + a.group - 1) / a.group, ps);
+  if constexpr (TOP && ONE) n = gather_one<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, x, bx, sh);
+  else if constexpr (TOP)
+    n = gather_top<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, a.group, (b + a.group - 1) / a.group, ps);
   if (a.parts == 1) {
-    score_write<TI, TOP>(a, r, xrow, sh, n, mx, s, tt);
+    score_write<TOP>(a, r, token, sh, n, mx, s, tt);
     return;
   }
   if constexpr (TOP)
@@ -503,18 +545,45 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
   if (tid == 0) turn = __hip_atomic_fetch_add(a.done + of, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (turn + 1 != static_cast<unsigned>(a.parts)) return;
-  acquire_coherent();
   if (tid == 0) store_coherent(a.done + of, 0u);
-  if constexpr (TOP) n = merge_parts(keys, a.parts, a.part_cap, a.k, [&](int p) { return parts[p].n; }, sh);
+  // Read at the level that the stores went to, past the caches, which then need no invalidation (an XCD's whole L2,
+  // for every row).
   mx = kNegInf;
   s = tt = 0.;
+  int left = 0;
   if (lane < a.parts) {
-    mx = parts[lane].mx;
-    s = parts[lane].s;
-    tt = parts[lane].t;
+    const __amdgpu_buffer_rsrc_t pbuf = row_rsrc(parts, static_cast<uint32_t>(a.parts) * sizeof(ScorePart));
+    const u32x4 p0 = buf_ld16_coherent(pbuf, lane * sizeof(ScorePart));
+    const u32x4 p1 = buf_ld16_coherent(pbuf, lane * sizeof(ScorePart) + 16);
+    s = __builtin_bit_cast(double, static_cast<uint64_t>(p0[1]) << 32 | p0[0]);
+    tt = __builtin_bit_cast(double, static_cast<uint64_t>(p0[3]) << 32 | p0[2]);
+    mx = __uint_as_float(p1[0]);
+    left = static_cast<int>(p1[1]);
+  }
+  if constexpr (TOP) {
+    const __amdgpu_buffer_rsrc_t kbuf = row_rsrc(keys, static_cast<uint32_t>(a.parts * a.part_cap) * 8u);
+    const int upto = lanes_scan(left), all = __builtin_amdgcn_readlane(upto, 63);
+    if (tid < 64) counts[tid] = all <= 2 * BLOCK ? upto - left : left;
+    __syncthreads();
+    auto key_at = [&](int i) { return buf_ld8_coherent(kbuf, static_cast<uint32_t>(i) * 8u); };
+    if (all <= 2 * BLOCK) {
+      // Few in all: ranked as they are, slot i from the part p that counts[p] <= i names.
+#pragma unroll
+      for (int i = tid; i < 2 * BLOCK; i += BLOCK)
+        if (i < all) {
+          int p = 0;
+#pragma unroll
+          for (int step = 32; step > 0; step >>= 1) p += p + step < a.parts && counts[p + step] <= i ? step : 0;
+          sh.key[i] = key_at(p * a.part_cap + i - counts[p]);
+        }
+      __syncthreads();
+      n = all;
+    } else {
+      n = merge_parts(key_at, a.parts, a.part_cap, a.k, [&](int p) { return counts[p]; }, sh);
+    }
   }
   score_merge<64>(mx, s, tt, a.k2);
-  score_write<TI, TOP>(a, r, xrow, sh, n, mx, s, tt);
+  score_write<TOP>(a, r, token, sh, n, mx, s, tt);
 }
 
 template <typename TI>
@@ -523,8 +592,11 @@ hipError_t launch_score(ScoreArgs a, int64_t n_rows, hipStream_t st) {
   for (int64_t r0 = 0; r0 < n_rows; r0 += kRows) {
     a.row0 = r0;
     const unsigned grid = static_cast<unsigned>((n_rows - r0 < kRows ? n_rows - r0 : kRows) * a.parts);
-    if (a.k > 0) score_kernel<TI, true><<<grid, kBlock, 0, st>>>(a);
-    else score_kernel<TI, false><<<grid, kBlock, 0, st>>>(a);
+    const bool one = a.parts > 1 && a.per <= kBlock * kU;
+    if (a.k > 0 && one) score_kernel<TI, true, true><<<grid, kBlock, 0, st>>>(a);
+    else if (a.k > 0) score_kernel<TI, true, false><<<grid, kBlock, 0, st>>>(a);
+    else if (one) score_kernel<TI, false, true><<<grid, kBlock, 0, st>>>(a);
+    else score_kernel<TI, false, false><<<grid, kBlock, 0, st>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
@@ -746,9 +818,9 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   hipStream_t st = static_cast<hipStream_t>(a->stream);
 
   // Workgroups per row: as few rows' logits as would leave CUs idle are dealt to several, at least kLeastPart vectors each.
-  constexpr int64_t kLeastPart = 2 * kBlock;
+  constexpr int64_t kLeastPart = 8 * kBlock;
   const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
-  int64_t parts = n_rows < kScoreTickets ? (2048 + n_rows - 1) / n_rows : 1;
+  int64_t parts = n_rows < kScoreTickets ? (1024 + n_rows - 1) / n_rows : 1;
   if (parts > 64) parts = 64;   // one wave merges their sums
   int64_t per = ((nv + parts - 1) / parts + kBlock - 1) / kBlock * kBlock;
   if (per < kLeastPart) per = kLeastPart;

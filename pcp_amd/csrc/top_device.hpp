@@ -203,6 +203,45 @@ __device__ __forceinline__ void rank_entries(Shared& sh, int n, int k, Put put) 
   }
 }
 
+// The elements of this lane's vectors left_q (bit q: x[q], whose first element is first + q kBlock EPV) that pass go into
+// the candidates, of those that keep has (bit EPV - 1 - j: element j). Each lane takes its own vectors one
+// after the other: about a dozen of a wave's 512 pass, so that two turns serve all. Called by every lane of a wave.
+template <typename TI, int U>
+__device__ __forceinline__ void take_vectors(Candidates& c, const u32x4 (&x)[U], uint32_t left_q, uint32_t first, uint32_t keep) {
+  constexpr int EPV = 16 / TI::kBytes;
+  // While nothing is ruled out NaN is taken too, which ranks below all.
+  const bool all = c.least_x == kNegInf;
+  while (__any(left_q != 0)) {
+    const int mine = __builtin_ctz(left_q | 1u << U);
+    u32x4 w = x[0];
+#pragma unroll
+    for (int q = 1; q < U; ++q)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = mine == q ? x[q][i] : w[i];
+    // Few lanes have any element that passes, fewer have two.
+    uint32_t bits = 0;
+#pragma unroll
+    for (int j = 0; j < EPV; ++j) {
+      const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&w), j);
+      bits = 2 * bits + ((v >= c.least_x || all) ? 1u : 0u);
+    }
+    if (left_q == 0) bits = 0;
+    left_q &= left_q - 1;
+    bits &= keep;
+    while (__any(bits != 0)) {
+      const int j = EPV - 32 + __builtin_clz(bits | 1u);   // the first that is left
+      uint32_t u = w[0];
+      const int word = TI::kBytes == 4 ? j : j >> 1;
+#pragma unroll
+      for (int i = 1; i < 4; ++i) u = word == i ? w[i] : u;
+      if constexpr (TI::kBytes == 2) u >>= 16 * (j & 1);
+      const uint64_t key = element_key(TI::unpack(&u, 0), first + static_cast<uint32_t>(mine * kBlock * EPV + j));
+      c.add(bits != 0 && key > c.least, key);
+      bits &= ~((1u << (EPV - 1)) >> j);
+    }
+  }
+}
+
 // The 16-byte vectors [v0, end) of a row interior (sp) through xbuf: every element goes into the lane's
 // sums, and those that may be among the k largest into the candidates, which hold `edges` elements
 // at the start and at most `left` (>= k) at the end, few more than k where the row lets them. Called by the whole
@@ -242,44 +281,13 @@ __device__ __forceinline__ void scan_part(const RowSpan& sp, __amdgpu_buffer_rsr
 #pragma unroll
       for (int q = 0; q < U; ++q) near[q] = held(q) && (vm[q] >= c.least_x || c.least_x == kNegInf);
     }
-    // While nothing is ruled out NaN is taken too, which ranks below all.
-    const bool all = c.least_x == kNegInf;
-    // Each lane takes its own vectors one after the other: about a dozen of a wave's 512 pass, so
-    // that two turns serve all.
     uint32_t left_q = 0;
 #pragma unroll
     for (int q = 0; q < U; ++q) left_q |= near[q] ? 1u << q : 0u;
     if (round >= 0) left_q &= 1u << (round / (EPV / 4));
-    while (__any(left_q != 0)) {
-      const int mine = __builtin_ctz(left_q | 1u << U);
-      u32x4 w = x[0];
-#pragma unroll
-      for (int q = 1; q < U; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = mine == q ? x[q][i] : w[i];
-      // Bit EPV - 1 - j: element j passes. Few lanes have any, fewer have two.
-      uint32_t bits = 0;
-#pragma unroll
-      for (int j = 0; j < EPV; ++j) {
-        const float v = TI::unpack(reinterpret_cast<const uint32_t*>(&w), j);
-        bits = 2 * bits + ((v >= c.least_x || all) ? 1u : 0u);
-      }
-      if (left_q == 0) bits = 0;
-      left_q &= left_q - 1;
-      if (round >= 0) bits &= 0xf0u >> (EPV == 4 ? 4 : 4 * (round % 2));
-      const uint32_t first = static_cast<uint32_t>(sp.head + (base + mine * BLOCK + tid) * EPV);
-      while (__any(bits != 0)) {
-        const int j = EPV - 32 + __builtin_clz(bits | 1u);   // the first that is left
-        uint32_t u = w[0];
-        const int word = TI::kBytes == 4 ? j : j >> 1;
-#pragma unroll
-        for (int i = 1; i < 4; ++i) u = word == i ? w[i] : u;
-        if constexpr (TI::kBytes == 2) u >>= 16 * (j & 1);
-        const uint64_t key = element_key(TI::unpack(&u, 0), first + j);
-        c.add(bits != 0 && key > c.least, key);
-        bits &= ~((1u << (EPV - 1)) >> j);
-      }
-    }
+    uint32_t keep = (1u << EPV) - 1u;
+    if (round >= 0) keep = 0xf0u >> (EPV == 4 ? 4 : 4 * (round % 2));
+    take_vectors<TI>(c, x, left_q, static_cast<uint32_t>(sp.head + (base + tid) * EPV), keep);
     __syncthreads();
     const int was = n;
     n = sh.count;
@@ -298,12 +306,12 @@ __device__ __forceinline__ void scan_part(const RowSpan& sp, __amdgpu_buffer_rsr
 }
 
 // The candidates of a row's parts, kMergeKeys per lane at a time: a histogram of the first ones finds what
-// k of them reach, as in the scan. n_of(part): what a part has left, part_cap keys apart in `in`. Leaves
-// them in sh, and returns their number; called by the whole workgroup with sh free.
+// k of them reach, as in the scan. n_of(part): what a part has left, part_cap keys apart, key_at(i) the i-th
+// of all. Leaves them in sh, and returns their number; called by the whole workgroup with sh free.
 constexpr int kMergeKeys = 12;
 
-template <typename NOf>
-__device__ __forceinline__ int merge_parts(const uint64_t* in, int parts, int part_cap, int k, NOf n_of, Shared& sh) {
+template <typename KeyAt, typename NOf>
+__device__ __forceinline__ int merge_parts(KeyAt key_at, int parts, int part_cap, int k, NOf n_of, Shared& sh) {
   constexpr int R = kMergeKeys, kPer = 4;   // keys per lane: of a round, of a cautious one
   static_assert(R % kPer == 0 && kBlock * kPer <= kCap - kCut, "cautious rounds fit");
   const int tid = threadIdx.x;
@@ -319,7 +327,7 @@ __device__ __forceinline__ int merge_parts(const uint64_t* in, int parts, int pa
     for (int i = 0; i < R; ++i) {
       const int at = base + i * kBlock + tid, p = at / part_cap;
       const bool is = at < total && at - p * part_cap < n_of(p);
-      key[i] = is ? in[at] : 0;   // no key is 0
+      key[i] = is ? key_at(at) : 0;   // no key is 0
     }
 #pragma unroll
     for (int i = 0; i < R; ++i) v[i] = key[i] ? from_order(static_cast<uint32_t>(key[i] >> 32)) : kNegInf;

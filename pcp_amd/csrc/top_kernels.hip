@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(kBlock) top_merge_kernel(TopArgs a) {
   const int tid = threadIdx.x;
   const int64_t row = a.row0 + blockIdx.x;
   const PartSum* sums = a.part_sum + row * a.parts;
-  const int n = merge_parts(a.part_key + row * a.parts * a.part_cap, a.parts, a.part_cap, a.k,
-                            [&](int p) { return sums[p].n; }, sh);
+  const uint64_t* in = a.part_key + row * a.parts * a.part_cap;
+  const int n = merge_parts([&](int i) { return in[i]; }, a.parts, a.part_cap, a.k, [&](int p) { return sums[p].n; }, sh);
   write_entries(a, row, sh, n);
   if (tid < 64) {
     float mx = kNegInf, s = 0.f;
