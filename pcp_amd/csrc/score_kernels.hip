@@ -52,8 +52,9 @@ __device__ __forceinline__ ScoreRow score_row(const TokenArrays& a, int64_t s, i
 struct alignas(16) ScorePart {
   double s, t;
   float mx;
-  int32_t n;
-  int64_t pad;
+  int32_t n;               // its candidates
+  float least;             // k of them reach this (-inf: not known)
+  int32_t pad;
 };
 
 struct ScoreArgs {
@@ -319,10 +320,11 @@ __device__ __forceinline__ int select_exact(const char* xrow, const RowSpan& sp,
 }
 
 // The candidates of a part whose lanes have left their groups' largest logits (batches: batches per group, groups:
-// how many), k or more of them where the part has as many elements. Called by the whole workgroup; ends with a barrier.
+// how many), k or more of them where the part has as many elements, and what k of them reach. Called by the whole
+// workgroup; ends with a barrier.
 template <typename TI>
 __device__ __forceinline__ int gather_top(const char* xrow, const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end,
-                                          bool edges, int k, int batches, int groups, PartShared& ps) {
+                                          bool edges, int k, int batches, int groups, PartShared& ps, float& least) {
   constexpr int EPV = 16 / TI::kBytes, U = kU;
   Shared& sh = ps.sh;
   const int tid = threadIdx.x;
@@ -333,7 +335,7 @@ __device__ __forceinline__ int gather_top(const char* xrow, const RowSpan& sp, _
     lane_max[0] = fmaxf(lane_max[0], v[g]);
   }
   // Up to 64 of the lanes' own maxima are nearly as high as the groups', and 256 values sooner counted than 4096.
-  const float least = k <= 64 ? reached_by(sh, lane_max, k) : reached_by(sh, v, k);
+  least = k <= 64 ? reached_by(sh, lane_max, k) : reached_by(sh, v, k);
   uint32_t left = 0;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) left |= g < groups && v[g] >= least ? 1u << g : 0u;
@@ -375,14 +377,15 @@ __device__ __forceinline__ int gather_top(const char* xrow, const RowSpan& sp, _
 // The same for a part of one batch, which is still in x; lane_max: the lane's largest logit.
 template <typename TI, int U>
 __device__ __forceinline__ int gather_one(const char* xrow, const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end,
-                                          bool edges, int k, const u32x4 (&x)[U], float lane_max, Shared& sh) {
+                                          bool edges, int k, const u32x4 (&x)[U], float lane_max, Shared& sh,
+                                          float& least) {
   constexpr int EPV = 16 / TI::kBytes;
   const int tid = threadIdx.x;
   float v[U];
 #pragma unroll
   for (int q = 0; q < U; ++q) v[q] = v0 + q * kBlock + tid < end ? vec_max<TI>(kNegInf, x[q]) : kNegInf;
   const float own[1] = {lane_max};
-  const float least = k <= 64 ? reached_by(sh, own, k) : reached_by(sh, v, k);
+  least = k <= 64 ? reached_by(sh, own, k) : reached_by(sh, v, k);
   if (tid == 0) sh.count = 0;
   __syncthreads();
   const int total = max(end - v0, 0) * EPV + (edges ? sp.head + sp.tail : 0);
@@ -520,9 +523,10 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
   tt = wave_t[lane & (kWaves - 1)];
   score_merge<kWaves>(mx, s, tt, a.k2);
   int n = 0;
-  if constexpr (TOP && ONE) n = gather_one<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, x, bx, sh);
+  float least = kNegInf;
+  if constexpr (TOP && ONE) n = gather_one<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, x, bx, sh, least);
   else if constexpr (TOP)
-    n = gather_top<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, a.group, (b + a.group - 1) / a.group, ps);
+    n = gather_top<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, a.group, (b + a.group - 1) / a.group, ps, least);
   if (a.parts == 1) {
     score_write<TOP>(a, r, token, sh, n, mx, s, tt);
     return;
@@ -539,6 +543,7 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
     store_coherent(&parts[part].t, tt);
     store_coherent(&parts[part].mx, mx);
     store_coherent(&parts[part].n, n);
+    store_coherent(&parts[part].least, least);
   }
   wait_stores();
   __syncthreads();
@@ -551,6 +556,7 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
   mx = kNegInf;
   s = tt = 0.;
   int left = 0;
+  least = kNegInf;
   if (lane < a.parts) {
     const __amdgpu_buffer_rsrc_t pbuf = row_rsrc(parts, static_cast<uint32_t>(a.parts) * sizeof(ScorePart));
     const u32x4 p0 = buf_ld16_coherent(pbuf, lane * sizeof(ScorePart));
@@ -559,26 +565,39 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
     tt = __builtin_bit_cast(double, static_cast<uint64_t>(p0[3]) << 32 | p0[2]);
     mx = __uint_as_float(p1[0]);
     left = static_cast<int>(p1[1]);
+    least = __uint_as_float(p1[2]);
   }
   if constexpr (TOP) {
     const __amdgpu_buffer_rsrc_t kbuf = row_rsrc(keys, static_cast<uint32_t>(a.parts * a.part_cap) * 8u);
-    const int upto = lanes_scan(left), all = __builtin_amdgcn_readlane(upto, 63);
-    if (tid < 64) counts[tid] = all <= 2 * BLOCK ? upto - left : left;
-    __syncthreads();
     auto key_at = [&](int i) { return buf_ld8_coherent(kbuf, static_cast<uint32_t>(i) * 8u); };
-    if (all <= 2 * BLOCK) {
-      // Few in all: ranked as they are, slot i from the part p that counts[p] <= i names.
+    const int upto = lanes_scan(left), all = __builtin_amdgcn_readlane(upto, 63);
+    // What one part's candidates reach, the row's k largest reach: few of the others' do.
+    Candidates c{sh, 0, lanes_max<64>(least)};
+    if (tid < 64) counts[tid] = upto - left;
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    constexpr int R = 4;
+    for (int base = 0; base < all; base += R * BLOCK) {
+      uint64_t key[R];
 #pragma unroll
-      for (int i = tid; i < 2 * BLOCK; i += BLOCK)
-        if (i < all) {
-          int p = 0;
+      for (int q = 0; q < R; ++q) {   // slot i: of the last part p with counts[p] <= i
+        const int i = base + q * BLOCK + tid;
+        int p = 0;
 #pragma unroll
-          for (int step = 32; step > 0; step >>= 1) p += p + step < a.parts && counts[p + step] <= i ? step : 0;
-          sh.key[i] = key_at(p * a.part_cap + i - counts[p]);
-        }
+        for (int step = 32; step > 0; step >>= 1) p += p + step < a.parts && counts[p + step] <= i ? step : 0;
+        key[q] = i < all ? key_at(p * a.part_cap + i - counts[p]) : 0;
+      }
+#pragma unroll
+      for (int q = 0; q < R; ++q)
+        if (base + q * BLOCK < all)
+          c.add(key[q] != 0 && (c.least_x == kNegInf || from_order(static_cast<uint32_t>(key[q] >> 32)) >= c.least_x), key[q]);
+    }
+    __syncthreads();
+    n = sh.count;
+    __syncthreads();
+    if (n > kCap) {
+      if (tid < 64) counts[tid] = left;
       __syncthreads();
-      n = all;
-    } else {
       n = merge_parts(key_at, a.parts, a.part_cap, a.k, [&](int p) { return counts[p]; }, sh);
     }
   }
@@ -823,7 +842,7 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   int64_t parts = n_rows < kScoreTickets ? (1024 + n_rows - 1) / n_rows : 1;
   if (parts > 64) parts = 64;   // one wave merges their sums
   int64_t per = ((nv + parts - 1) / parts + kBlock - 1) / kBlock * kBlock;
-  if (per < kLeastPart) per = kLeastPart;
+  if (per < kLeastPart || (per <= 2 * kLeastPart && nv <= 64 * kLeastPart)) per = kLeastPart;
   parts = nv > 0 ? (nv + per - 1) / per : 1;
   const int64_t part_cap = a->k > 0 ? a->k + 64 : 0;
   const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(n_rows) * parts * part_cap : 0;

@@ -184,19 +184,22 @@ struct Candidates {
 // number of larger ones, counted over LDS reads that every lane shares. put(rank, logit, id).
 template <typename Put>
 __device__ __forceinline__ void rank_entries(Shared& sh, int n, int k, Put put) {
+  constexpr int kRead = 8;   // keys read at once
   if (n > 2 * kBlock) {
     sort_falling(sh.key, n);
     n = k;
-  } else {
-    if (threadIdx.x == 0) sh.key[n] = 0;   // pairs below
-    __syncthreads();
   }
+  if (threadIdx.x < kRead && n + static_cast<int>(threadIdx.x) < kCap) sh.key[n + threadIdx.x] = 0;   // read below
+  __syncthreads();
   for (int i = threadIdx.x; i < n; i += kBlock) {
     const uint64_t v = sh.key[i];
     int rank = 0;
-    for (int o = 0; o < n; o += 2) {
-      const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(&sh.key[o]);
-      rank += (w.x > v) + (w.y > v);
+    for (int o = 0; o < n; o += kRead) {
+      ulonglong2 w[kRead / 2];
+#pragma unroll
+      for (int j = 0; j < kRead / 2; ++j) w[j] = *reinterpret_cast<const ulonglong2*>(&sh.key[o + 2 * j]);
+#pragma unroll
+      for (int j = 0; j < kRead / 2; ++j) rank += (w[j].x > v) + (w[j].y > v);
     }
     if (rank < k)
       put(rank, from_order(static_cast<uint32_t>(v >> 32)), static_cast<int64_t>(0xffffffffu - static_cast<uint32_t>(v)));
