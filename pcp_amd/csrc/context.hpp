@@ -19,7 +19,8 @@ struct HostStager;
 namespace pcp {
 // Rows of token scores that several workgroups may share, and workgroups of a gradient norm.
 constexpr int kScoreTickets = 512;
-constexpr int kNormBlocks = 2048;
+constexpr int kNormBlocks = 16384;
+constexpr int kNormGroups = 32, kNormApart = 16;   // its tickets: one for all and one a group, 64 bytes apart
 
 // What kernels hand back to the host: one pinned, coherent host page per context, written
 // by the device with plain system-scope stores and read by the host after the stream is
@@ -44,7 +45,7 @@ struct pcp_ctx {
   float4* d_logprob_parts = nullptr;  // and of log-probs: of the synchronous call that holds
   std::atomic<bool> logprob_parts_busy{false};   // this flag
   unsigned* d_score_done = nullptr;   // the token scores' tickets, kScoreTickets (same allocation; zero between launches)
-  unsigned* d_norm_done = nullptr;    // the gradient norm's ticket (the same)
+  unsigned* d_norm_done = nullptr;    // the gradient norm's tickets (the same)
   double* d_norm_parts = nullptr;     // and its partial results, kNormBlocks
   void* scratch = nullptr;       // per-call work buffers, grown on demand
   size_t scratch_bytes = 0;

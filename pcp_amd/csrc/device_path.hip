@@ -447,7 +447,8 @@ int pcp_init(int backend, int device_ordinal, pcp_ctx** out) {
   // losses and for log-probs. Held from the start, they add nothing to what a call needs.
   void* fixed = nullptr;
   // Behind them the tickets and the partial results of pcp_score_fwd and pcp_grad_clip.
-  constexpr size_t kTicketBytes = sizeof(unsigned) * (kScoreTickets + 64), kNormBytes = sizeof(double) * kNormBlocks;
+  constexpr size_t kTicketBytes = sizeof(unsigned) * (kScoreTickets + (1 + kNormGroups) * kNormApart);
+  constexpr size_t kNormBytes = sizeof(double) * kNormBlocks;
   e = hipMalloc(&fixed, 256 + 2 * kPartScratchBytes + kTicketBytes + kNormBytes);
   if (e != hipSuccess) {
     delete c;

@@ -57,16 +57,17 @@ __device__ __forceinline__ int piece_of(const int* first, int pieces, int c) {
 // ---- norm -------------------------------------------------------------------------------
 
 constexpr int kNormPieces = 240;
-constexpr int kNormChunk = 16384;
+constexpr int kNormChunk = 16384, kNormSmall = 4096;
+constexpr int kNormGrid = 2048;    // workgroups of a launch: eight on each CU
 
 struct NormArgs {
   const void* g[kNormPieces];
   uint32_t n[kNormPieces];
   int first[kNormPieces + 1];
   int pieces;
+  int chunk;              // elements
   int block0;             // workgroups of earlier launches
   int blocks;             // of all launches
-  int norm_type;
   float max_norm;
   double* parts;
   unsigned* done;
@@ -92,7 +93,7 @@ __device__ __forceinline__ void norm_add(double& s, uint32_t& top, const float (
 
 template <int TYPE, typename TI>
 __device__ __forceinline__ void norm_chunk(const char* g, int n, double& s, uint32_t& top) {
-  constexpr int EPV = 16 / TI::kBytes, U = 8;
+  constexpr int EPV = 16 / TI::kBytes, U = 4;
   const int nv = n / EPV;
   const u32x4_any* v = reinterpret_cast<const u32x4_any*>(g);
   int i = threadIdx.x;
@@ -149,28 +150,41 @@ __global__ void __launch_bounds__(kBlock) norm_kernel(NormArgs a) {
   const int c1 = static_cast<int>(static_cast<int64_t>(chunks) * (blockIdx.x + 1) / gridDim.x);
   double s = 0.;
   uint32_t top = 0;
+  // A workgroup's chunks lie one after another: what they have of a piece is read as one stretch, with no lookup (three
+  // dependent scalar loads) between chunks.
   if (c0 < c1) {
     int t = piece_of(a.first, a.pieces, c0);
-    for (int c = c0; c < c1; ++c) {
-      if (c == a.first[t + 1]) ++t;
+    for (int c = c0; c < c1; ++t) {
       const uint32_t word = a.n[t];
-      const int e0 = (c - a.first[t]) * kNormChunk, n = min(kNormChunk, static_cast<int>(word & kCount) - e0);
+      const int from = c - a.first[t], to = min(c1, a.first[t + 1]) - a.first[t];
+      const int64_t e0 = static_cast<int64_t>(from) * a.chunk;
+      const int n = static_cast<int>(min(static_cast<int64_t>(to) * a.chunk, static_cast<int64_t>(word & kCount)) - e0);
       with_type(word >> kTypeShift, [&](auto type) {
         using TI = decltype(type);
-        norm_chunk<TYPE, TI>(static_cast<const char*>(a.g[t]) + static_cast<int64_t>(e0) * TI::kBytes, n, s, top);
+        norm_chunk<TYPE, TI>(static_cast<const char*>(a.g[t]) + e0 * TI::kBytes, n, s, top);
       });
+      c += to - from;
     }
   }
   const double mine = norm_block<TYPE>(s, top, lds);
   if (threadIdx.x == 0) {
     store_coherent(a.parts + a.block0 + blockIdx.x, mine);
     wait_stores();
-    turn = __hip_atomic_fetch_add(a.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // The last of a group of workgroups counts for it: one counter for all of them would take an atomic after the other.
+    const int block = a.block0 + static_cast<int>(blockIdx.x), g = block % kNormGroups;
+    const unsigned of_group = static_cast<unsigned>((a.blocks - g + kNormGroups - 1) / kNormGroups);
+    const unsigned groups = static_cast<unsigned>(min(a.blocks, kNormGroups));
+    unsigned* const mine = a.done + (1 + g) * kNormApart;
+    turn = 0;
+    if (__hip_atomic_fetch_add(mine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == of_group) {
+      store_coherent(mine, 0u);
+      turn = __hip_atomic_fetch_add(a.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1 == groups;
+      if (turn) store_coherent(a.done, 0u);
+    }
   }
   __syncthreads();
-  if (turn + 1 != static_cast<unsigned>(a.blocks)) return;
+  if (!turn) return;
   acquire_coherent();
-  if (threadIdx.x == 0) store_coherent(a.done, 0u);
   s = 0.;
   top = 0;
   for (int i = threadIdx.x; i < a.blocks; i += kBlock) {
@@ -408,16 +422,18 @@ struct Pieces {
   }
 };
 
-hipError_t launch_norm(pcp_ctx* ctx, const pcp_grad_clip_args* a, hipStream_t st) {
+hipError_t launch_norm(pcp_ctx* ctx, const pcp_grad_clip_args* a, int64_t elements, hipStream_t st) {
   // The launches, and how many workgroups each may have: kNormBlocks in all.
   int64_t pieces = 0;
   for (Pieces p{a->counts, a->n_tensors}; p.next();) ++pieces;
   const int64_t launches = std::max<int64_t>(1, (pieces + kNormPieces - 1) / kNormPieces);
-  const int most = static_cast<int>(kNormBlocks / launches);
+  const int most = static_cast<int>(std::min<int64_t>(kNormGrid, kNormBlocks / launches));
+  // Chunks small enough that a small model's gradients occupy the chip, and large enough that a vector's loads are wide.
+  const int chunk = elements < int64_t(kNormGrid) * kNormChunk ? kNormSmall : kNormChunk;
   static_assert((PCP_GRAD_MAX_TENSORS + 65536) / kNormPieces + 1 <= kNormBlocks, "a workgroup for every launch");
   NormArgs b;
   std::memset(&b, 0, sizeof(b));
-  b.norm_type = a->norm_type;
+  b.chunk = chunk;
   b.max_norm = a->max_norm;
   b.parts = ctx->d_norm_parts;
   b.done = ctx->d_norm_done;
@@ -436,7 +452,7 @@ hipError_t launch_norm(pcp_ctx* ctx, const pcp_grad_clip_args* a, hipStream_t st
         const int dt = a->dtypes ? a->dtypes[p.tensor] : PCP_F32;
         b.g[b.pieces] = static_cast<const char*>(a->grads[p.tensor]) + p.from * dtype_bytes(dt);
         b.n[b.pieces] = static_cast<uint32_t>(p.size) | static_cast<uint32_t>(dt) << kTypeShift;
-        b.first[b.pieces + 1] = b.first[b.pieces] + static_cast<int>((p.size + kNormChunk - 1) / kNormChunk);
+        b.first[b.pieces + 1] = b.first[b.pieces] + static_cast<int>((p.size + chunk - 1) / chunk);
         ++b.pieces;
       }
       const int grid = std::max(1, std::min(most, b.first[b.pieces]));
@@ -530,7 +546,7 @@ int grad_clip(pcp_ctx* ctx, const pcp_grad_clip_args* a) {
   const DeviceScope scope(ctx->device);
   if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
   hipStream_t st = static_cast<hipStream_t>(a->stream);
-  hipError_t e = launch_norm(ctx, a, st);
+  hipError_t e = launch_norm(ctx, a, elements, st);
   if (e != hipSuccess) return hip_fail(ctx, e, "gradient norm launch");
   if (a->out && elements > 0 && (e = launch_clip(a, st)) != hipSuccess) return hip_fail(ctx, e, "gradient clipping launch");
   return finish_call(ctx, a->flags, st);
