@@ -201,21 +201,21 @@ class ScoreBwdArgs(ctypes.Structure):
 
 
 class GradClipArgs(ctypes.Structure):
-    """pcp_grad_clip_args (include/pcp_step.h); the lists as addresses of host arrays."""
+    """pcp_grad_clip_args (include/pcp_step.h); the lists as host arrays (bytes, or their addresses)."""
     _fields_ = [
-        ("n_tensors", ctypes.c_int64), ("grads", ctypes.c_void_p), ("counts", ctypes.c_void_p),
-        ("dtypes", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_dtypes", ctypes.c_void_p),
+        ("n_tensors", ctypes.c_int64), ("grads", ctypes.c_char_p), ("counts", ctypes.c_char_p),
+        ("dtypes", ctypes.c_char_p), ("out", ctypes.c_char_p), ("out_dtypes", ctypes.c_char_p),
         ("norm", ctypes.c_void_p), ("coef", ctypes.c_void_p), ("norm_type", ctypes.c_int32), ("max_norm", ctypes.c_float),
         ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
     ]
 
 
 class NesterovManyArgs(ctypes.Structure):
-    """pcp_nesterov_many_args (include/pcp_step.h); the lists as addresses of host arrays."""
+    """pcp_nesterov_many_args (include/pcp_step.h); the lists as host arrays (bytes, or their addresses)."""
     _fields_ = [
-        ("n_tensors", ctypes.c_int64), ("counts", ctypes.c_void_p), ("params", ctypes.c_void_p),
-        ("velocities", ctypes.c_void_p), ("grads", ctypes.c_void_p), ("dtypes", ctypes.c_void_p),
-        ("param_copies", ctypes.c_void_p), ("coef", ctypes.c_void_p),
+        ("n_tensors", ctypes.c_int64), ("counts", ctypes.c_char_p), ("params", ctypes.c_char_p),
+        ("velocities", ctypes.c_char_p), ("grads", ctypes.c_char_p), ("dtypes", ctypes.c_char_p),
+        ("param_copies", ctypes.c_char_p), ("coef", ctypes.c_void_p),
         ("learning_rate", ctypes.c_float), ("momentum", ctypes.c_float), ("mode", ctypes.c_int32),
         ("flags", ctypes.c_uint32), ("stream", ctypes.c_void_p),
     ]

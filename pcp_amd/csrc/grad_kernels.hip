@@ -205,7 +205,6 @@ __global__ void __launch_bounds__(kBlock) norm_kernel(NormArgs a) {
 // ---- clipping ---------------------------------------------------------------------------
 
 constexpr int kClipPieces = 160;
-constexpr int kClipU = 2;    // groups per lane
 
 struct ClipArgs {
   const void* g[kClipPieces];
@@ -218,9 +217,9 @@ struct ClipArgs {
 };
 static_assert(sizeof(ClipArgs) <= 4096, "kernel arguments");
 
-// Elements per lane and group: 16 bytes of the wider type.
-template <typename TI, typename TO>
-constexpr int clip_group() { return TI::kBytes == 4 || TO::kBytes == 4 ? 4 : 8; }
+// Elements per lane and group: 16 bytes of the wider type; and groups per lane.
+constexpr __host__ __device__ inline int clip_group(int from, int to) { return from == 4 || to == 4 ? 4 : 8; }
+constexpr __host__ __device__ inline int clip_unroll(int from, int to) { return from == 4 ? 1 : to == 4 ? 4 : 2; }
 
 // Chunks begin where out is aligned to its group: the first group of a tensor may begin before it.
 constexpr __host__ __device__ inline int clip_lead(uintptr_t out, int bytes, int group) {
@@ -251,17 +250,17 @@ __device__ __forceinline__ float f32_product(float a, float b) {
 
 template <typename TI, typename TO>
 __device__ __forceinline__ void clip_chunk(const char* g, char* out, int n, int c, float coef) {
-  constexpr int N = clip_group<TI, TO>();
+  constexpr int N = clip_group(TI::kBytes, TO::kBytes), U = clip_unroll(TI::kBytes, TO::kBytes);
   const int first = -clip_lead(reinterpret_cast<uintptr_t>(out), TO::kBytes, N);
-  const int e0 = first + (c * (kClipU * kBlock) + static_cast<int>(threadIdx.x)) * N;
-  float x[kClipU][N];
+  const int e0 = first + (c * (U * kBlock) + static_cast<int>(threadIdx.x)) * N;
+  float x[U][N];
 #pragma unroll
-  for (int u = 0; u < kClipU; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int e = e0 + u * kBlock * N;
     if (e >= 0 && e + N <= n) load_group<N, TI>(g + static_cast<int64_t>(e) * TI::kBytes, x[u]);
   }
 #pragma unroll
-  for (int u = 0; u < kClipU; ++u) {
+  for (int u = 0; u < U; ++u) {
     const int e = e0 + u * kBlock * N;
     if (e >= 0 && e + N <= n) {
 #pragma unroll
@@ -480,13 +479,13 @@ hipError_t launch_clip(const pcp_grad_clip_args* a, hipStream_t st) {
     b.first[0] = 0;
     for (; more && b.pieces < kClipPieces; more = p.next()) {
       const int from = a->dtypes ? a->dtypes[p.tensor] : PCP_F32, to = a->out_dtypes ? a->out_dtypes[p.tensor] : from;
-      const int group = from == PCP_F32 || to == PCP_F32 ? 4 : 8;
+      const int group = clip_group(dtype_bytes(from), dtype_bytes(to));
       char* out = static_cast<char*>(a->out[p.tensor]) + p.from * dtype_bytes(to);
       b.g[b.pieces] = static_cast<const char*>(a->grads[p.tensor]) + p.from * dtype_bytes(from);
       b.out[b.pieces] = out;
       b.n[b.pieces] = static_cast<uint32_t>(p.size) | static_cast<uint32_t>(to) << kTypeShift;
       b.from[b.pieces] = static_cast<uint8_t>(from);
-      const int64_t chunk = kClipU * kBlock * group;
+      const int64_t chunk = clip_unroll(dtype_bytes(from), dtype_bytes(to)) * kBlock * group;
       const int64_t span = p.size + clip_lead(reinterpret_cast<uintptr_t>(out), dtype_bytes(to), group);
       b.first[b.pieces + 1] = b.first[b.pieces] + static_cast<int>((span + chunk - 1) / chunk);
       ++b.pieces;

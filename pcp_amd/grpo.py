@@ -107,13 +107,29 @@ class call_scope:
         for t in tensors:
             if t is not None and t.get_device() != ctx.device:   # -1 on the CPU
                 raise PcpError(-1, f"tensor on {t.device}, context on device {ctx.device}")
+        self._enter_on(ctx, stream, tensors)
+
+    @classmethod
+    def of_described(cls, ctx: Context, stream, device: int, *lists):
+        """The same for lists of tensors (or None) that ``_tensors.describe`` has found on `device`."""
+        if device != ctx.device and device != -3:   # -3: no tensor
+            raise PcpError(-1, "tensors on several devices" if device == -2 else
+                           f"tensors on {'the CPU' if device < 0 else f'device {device}'}, context on device {ctx.device}")
+        self = cls.__new__(cls)
+        self._enter_on(ctx, stream, None if stream is None else [t for ts in lists for t in ts])
+        return self
+
+    def _enter_on(self, ctx, stream, tensors):
         self.inner = None
+        if stream is None:
+            self.handle = torch._C._cuda_getCurrentRawStream(ctx.device) or None
+            return
         current = torch.cuda.current_stream(ctx.device)
         if isinstance(stream, int):
             stream = (current if stream == current.cuda_stream
                       else torch.cuda.ExternalStream(stream, device=ctx.device) if stream
                       else torch.cuda.default_stream(ctx.device))
-        if stream is not None and stream.cuda_stream != current.cuda_stream:
+        if stream.cuda_stream != current.cuda_stream:
             self.inner = torch.cuda.stream(stream)
             for t in tensors:
                 if t is not None:

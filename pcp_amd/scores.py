@@ -11,9 +11,9 @@ from dataclasses import dataclass
 
 import torch
 
-from . import _lib
-from ._lib import PcpError, ScoreArgs, ScoreBwdArgs, check, lib
-from .grpo import Context, _ptr, call_scope, default_context, dtype_code
+from . import _lib, _tensors
+from ._lib import DType, PcpError, ScoreArgs, ScoreBwdArgs, check, lib
+from .grpo import _TORCH_DTYPE, Context, call_scope, default_context, dtype_code
 from .step import _row_stride, _seq_stride
 
 
@@ -77,35 +77,42 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: to
     lib().pcp_score_args_init(ctypes.byref(a))
     _row_places(logits, a, "row_stride", "seq_stride")
     ctx = ctx or default_context(logits.device.index or 0)
-    given = () if outputs is None else (outputs.logp, outputs.entropy, outputs.row_max, outputs.log_sum,
-                                        outputs.top_logp, outputs.top_ids)
-    with call_scope(ctx, stream, logits, ids, mask, *given) as handle:
-        if outputs is None:
-            f32 = dict(dtype=torch.float32, device=logits.device)
-            outputs = TokenScores(torch.zeros((S, TS), **f32) if ids is not None else None, torch.zeros((S, TS), **f32),
-                                  torch.zeros((S, TS), **f32), torch.zeros((S, TS), **f32),
-                                  torch.zeros((S, TS, k), **f32) if k else None,
-                                  torch.zeros((S, TS, k), dtype=top_ids_dtype, device=logits.device) if k else None)
-        o = outputs
-        for t, n in ((o.logp if ids is not None else None, 1), (o.entropy, 1), (o.row_max, 1), (o.log_sum, 1),
-                     (o.top_logp if k else None, k)):
-            if t is not None and (t.dtype != torch.float32 or t.numel() != S * TS * n):
-                raise PcpError(-1, "outputs do not fit the call: f32 [S, TS], top_logp f32 and top_ids [S, TS, k]")
-        if k and (o.top_logp is None or o.top_ids is None or o.top_ids.dtype != top_ids_dtype
-                  or o.top_ids.numel() != S * TS * k):
-            raise PcpError(-1, "outputs do not fit the call: f32 [S, TS], top_logp f32 and top_ids [S, TS, k]")
+    o = outputs
+    if o is None:
+        made = lambda *shape: torch.zeros(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
+    given = () if o is None else (o.logp if ids is not None else None, o.entropy, o.row_max, o.log_sum,
+                                  o.top_logp if k else None, o.top_ids if k else None)
+    known = (ids, mask, *given)
+    d = _tensors.describe((logits, *known))
+    _contiguous(d)
+    with call_scope.of_described(ctx, stream, d[4], (logits, *known)) as handle:
+        if o is None:
+            o = TokenScores(made(S, TS) if ids is not None else None, made(S, TS), made(S, TS), made(S, TS),
+                            made(S, TS, k) if k else None,
+                            torch.zeros((S, TS, k), dtype=top_ids_dtype, device=logits.device) if k else None)
+            known = (ids, mask, o.logp, o.entropy, o.row_max, o.log_sum, o.top_logp, o.top_ids)
+            d = _tensors.describe((logits, *known))
+        else:
+            n = memoryview(d[1]).cast("q")
+            t = memoryview(d[2]).cast("i")
+            top = int(_TORCH_DTYPE.get(top_ids_dtype, -2))
+            for i, want in ((3, S * TS if ids is not None else -1), (4, S * TS), (5, S * TS), (6, S * TS),
+                            (7, S * TS * k or -1), (8, S * TS * k or -1)):
+                wants = top if i == 8 else int(DType.f32)
+                # (Optional ones may be None: but logp with ids, and the alternatives with k.)
+                if (n[i] != want or t[i] != wants) and not (n[i] == -1 and (want <= 0 or 4 <= i <= 6)):
+                    raise PcpError(-1, "outputs do not fit the call: f32 [S, TS], top_logp f32 and top_ids [S, TS, k]")
+        at = memoryview(d[0]).cast("q")
         a.n_seq, a.rows, a.vocab, a.tok_seq_stride, a.tok_offset = S, rows, V, TS, tok_offset
-        a.k, a.temperature, a.logits_dtype = k, temperature, dtype_code(logits)
-        a.logits = logits.data_ptr()
-        _set_tokens(a, ids, mask)
-        a.logp = _ptr(o.logp) if ids is not None else None
-        a.entropy, a.row_max, a.log_sum = _ptr(o.entropy), _ptr(o.row_max), _ptr(o.log_sum)
+        a.k, a.temperature, a.logits_dtype, a.logits = k, temperature, dtype_code(logits), at[0]
+        _set_tokens(a, ids, mask, at)
+        a.logp, a.entropy, a.row_max, a.log_sum, a.top_logp, a.top_ids = at[3:]
         if k:
-            a.top_logp, a.top_ids, a.top_ids_dtype = _ptr(o.top_logp), _ptr(o.top_ids), dtype_code(o.top_ids)
+            a.top_ids_dtype = dtype_code(o.top_ids)
         a.flags = 0 if sync else _lib.FLAG_ASYNC
         a.stream = handle
         check(lib().pcp_score_fwd(ctx.handle, ctypes.byref(a)), ctx.handle)
-    return outputs
+    return o
 
 
 def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: torch.Tensor, log_sum: torch.Tensor,
@@ -138,16 +145,19 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: to
     lib().pcp_score_bwd_args_init(ctypes.byref(a))
     _row_places(logits, a, "row_stride", "seq_stride")
     ctx = ctx or default_context(logits.device.index or 0)
-    with call_scope(ctx, stream, logits, ids, mask, row_max, log_sum, entropy, dlogp, dentropy, dlogits) as handle:
+    known = (logits, ids, mask, row_max, log_sum, entropy, dlogp, dentropy)
+    d = _tensors.describe((*known, dlogits))
+    _contiguous(d, len(known))
+    with call_scope.of_described(ctx, stream, d[4], known, (dlogits,)) as handle:
         if dlogits is None:
             dlogits = torch.empty((S, LS, V), dtype=dlogits_dtype or logits.dtype, device=logits.device)
         _row_places(dlogits, a, "drow_stride", "dseq_stride")
+        at = memoryview(d[0]).cast("q")
         a.n_seq, a.rows, a.logit_rows, a.vocab, a.tok_seq_stride, a.tok_offset = S, rows, LS, V, TS, tok_offset
         a.logits_dtype, a.dlogits_dtype, a.temperature = dtype_code(logits), dtype_code(dlogits), temperature
-        a.logits, a.dlogits = logits.data_ptr(), dlogits.data_ptr()
-        _set_tokens(a, ids, mask)
-        a.row_max, a.log_sum, a.entropy = _ptr(row_max), _ptr(log_sum), _ptr(entropy)
-        a.dlogp, a.dentropy = _ptr(dlogp), _ptr(dentropy)
+        a.logits, a.dlogits = at[0], dlogits.data_ptr()
+        _set_tokens(a, ids, mask, at)
+        a.row_max, a.log_sum, a.entropy, a.dlogp, a.dentropy = at[3:8]
         a.accumulate = 1 if accumulate else 0
         a.flags = 0 if sync else _lib.FLAG_ASYNC
         a.stream = handle
@@ -155,8 +165,14 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: to
     return dlogits
 
 
-def _set_tokens(a, ids, mask) -> None:
+def _contiguous(d, n: int | None = None) -> None:
+    """The first n described tensors behind the logits are contiguous."""
+    if 0 in d[3][1:n]:
+        raise PcpError(-1, "token arrays and outputs must be contiguous")
+
+
+def _set_tokens(a, ids, mask, at) -> None:
     if ids is not None:
-        a.ids, a.ids_dtype = _ptr(ids), dtype_code(ids)
+        a.ids, a.ids_dtype = at[1], dtype_code(ids)
     if mask is not None:
-        a.mask, a.mask_dtype = _ptr(mask), dtype_code(mask)
+        a.mask, a.mask_dtype = at[2], dtype_code(mask)

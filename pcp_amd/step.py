@@ -7,15 +7,18 @@ Mirrors RLShepherd.trainStep (src/nodes/controllers/rl_shepherd.zig:487-515 pack
 """
 from __future__ import annotations
 
+import array
 import ctypes
+import sys
 from dataclasses import dataclass
 
 import numpy as np
 import torch
 
+from . import _tensors
 from ._lib import (DType, FLAG_ASYNC, GradClipArgs, GradStats, NesterovManyArgs, NesterovMode, NormType, PcpError, VerifyArgs,
                    check, lib)
-from .grpo import Context, _ptr, _stream_handle, call_scope, default_context, dtype_code
+from .grpo import _TORCH_DTYPE, Context, _ptr, _stream_handle, call_scope, default_context, dtype_code
 
 
 def pack_rollouts(prompt_tokens: torch.Tensor, prompt_offsets: torch.Tensor, completion_tokens: torch.Tensor,
@@ -64,36 +67,33 @@ class GradNorm:
     coef: torch.Tensor        # f32 scalar: what brings the gradients down to max_norm, at most 1
 
 
-_GRAD_DTYPE = {torch.float32: int(DType.f32), torch.bfloat16: int(DType.bf16), torch.float16: int(DType.f16)}
+def _described(tensors, what: str, dtype: DType | None = None):
+    """What ``_tensors.describe`` says of a list, its tensors contiguous and, with dtype, of that type (or None)."""
+    d = _tensors.describe(tensors)
+    if 0 in d[3]:
+        raise PcpError(-1, f"{what} must be contiguous")
+    if dtype is not None and d[2] != _code(dtype) * len(tensors):
+        if any(t is not None and int(_TORCH_DTYPE.get(t.dtype, -1)) != dtype for t in tensors):
+            raise PcpError(-2, f"{what} must be {dtype.name}")
+    return d
 
 
-class _List:
-    """A list of tensors as the C entry points take it: host arrays of addresses, and of element types."""
-
-    __slots__ = ("ptrs", "types", "at", "types_at")
-
-    def __init__(self, tensors, what: str, dtype: torch.dtype | None = None):
-        n = len(tensors)
-        held = [t for t in tensors if t is not None]
-        try:
-            codes = [_GRAD_DTYPE[t.dtype] for t in held]
-        except KeyError:
-            raise PcpError(-2, f"{what} must be f32, bf16 or f16") from None
-        if dtype is not None and any([c != _GRAD_DTYPE[dtype] for c in codes]):
-            raise PcpError(-2, f"{what} must be {dtype}")
-        if not all([t.is_contiguous() for t in held]):
-            raise PcpError(-1, f"{what} must be contiguous")
-        self.ptrs = (ctypes.c_void_p * n)(*[None if t is None else t.data_ptr() for t in tensors])
-        self.types = (ctypes.c_int32 * len(codes))(*codes)
-        self.at, self.types_at = ctypes.addressof(self.ptrs), ctypes.addressof(self.types)
+def _code(dtype: DType) -> bytes:
+    return int(dtype).to_bytes(4, sys.byteorder)
 
 
-def _counts(grads, *others):
-    counts = [t.numel() for t in grads]
-    for name, ts in others:
-        if ts is not None and (len(ts) != len(counts) or any([t is not None and t.numel() != c for t, c in zip(ts, counts)])):
-            raise PcpError(-12, f"{name} must hold as many tensors as the gradients, of the same sizes")
-    return (ctypes.c_int64 * len(counts))(*counts)
+def _same_sizes(grads, *others) -> None:
+    """The descriptions (name, description, tensors) hold the gradients' numbers of elements (or None)."""
+    for name, d, ts in others:
+        if d is not None and d[1] != grads[1]:
+            counts = memoryview(grads[1]).cast("q")
+            if len(ts) != len(counts) or any(t is not None and t.numel() != c for t, c in zip(ts, counts)):
+                raise PcpError(-12, f"{name} must hold as many tensors as the gradients, of the same sizes")
+
+
+def _one_device(*descriptions) -> int:
+    found = {d[4] for d in descriptions if d is not None and d[4] != -3}
+    return -3 if not found else found.pop() if len(found) == 1 else -2
 
 
 def grad_norm(grads, max_norm: float = float("inf"), *, norm_type: int | str = NormType.l2,
@@ -122,27 +122,35 @@ def _grad_clip(grads, max_norm, norm_type, out, outputs, sync, stream, ctx) -> G
             norm_type = NormType[norm_type]
         except KeyError:
             raise PcpError(-1, f"unknown norm_type {norm_type!r}") from None
-    ctx = ctx or default_context((grads[0] if grads else outputs.norm if outputs is not None else torch.empty(0)).device.index or 0)
-    g = _List(grads, "gradients")
-    counts = _counts(grads, ("out", out))
-    o = None if out is None else g if out is grads else _List(out, "out")
+    g = _described(grads, "gradients")
+    o = None if out is None else g if out is grads else _described(out, "out")
+    _same_sizes(g, ("out", o, out))
+    given = [] if outputs is None else [outputs.norm, outputs.coef]
+    e = _described(given, "outputs", DType.f32)
+    device = _one_device(g, o, e)
+    ctx = ctx or default_context(max(device, 0))
     a = GradClipArgs()
     lib().pcp_grad_clip_args_init(ctypes.byref(a))
-    given = () if outputs is None else (outputs.norm, outputs.coef)
-    with call_scope(ctx, stream, *grads, *(out if out is not None and out is not grads else ()), *given) as handle:
+    with call_scope.of_described(ctx, stream, device, grads, () if out is None or out is grads else out, given) as handle:
         if outputs is None:
             both = torch.empty(2, dtype=torch.float32, device=torch.device("cuda", ctx.device))
             outputs = GradNorm(both[0], both[1])
-        if any(t.dtype != torch.float32 or t.numel() != 1 for t in (outputs.norm, outputs.coef)):
-            raise PcpError(-1, "outputs do not fit the call: norm and coef f32 scalars")
-        a.n_tensors, a.grads, a.counts, a.dtypes = len(grads), g.at, ctypes.addressof(counts), g.types_at
+            a.norm, a.coef = both.data_ptr(), both.data_ptr() + 4
+        else:
+            if e[1] != _ONE + _ONE:
+                raise PcpError(-1, "outputs do not fit the call: norm and coef f32 scalars")
+            a.norm, a.coef = memoryview(e[0]).cast("q")
+        a.n_tensors, a.grads, a.counts, a.dtypes = len(grads), g[0], g[1], g[2]
         if o is not None:
-            a.out, a.out_dtypes = o.at, o.types_at
-        a.norm, a.coef, a.norm_type, a.max_norm = outputs.norm.data_ptr(), outputs.coef.data_ptr(), int(norm_type), max_norm
+            a.out, a.out_dtypes = o[0], o[2]
+        a.norm_type, a.max_norm = int(norm_type), max_norm
         a.flags = 0 if sync else FLAG_ASYNC
         a.stream = handle
         check(lib().pcp_grad_clip(ctx.handle, ctypes.byref(a)), ctx.handle)
     return outputs
+
+
+_ONE = (1).to_bytes(8, sys.byteorder)
 
 
 def nesterov_update_many(params, velocities, grads, param_copies=None, *, coef: torch.Tensor | None = None,
@@ -157,32 +165,36 @@ def nesterov_update_many(params, velocities, grads, param_copies=None, *, coef: 
     copies = None if param_copies is None else list(param_copies)
     if not params and not grads and not velocities:
         return
-    ctx = ctx or default_context((params or grads or velocities)[0].device.index or 0)
-    v = _List(velocities, "velocities", torch.float32)
-    _update_many(ctx, params, v.at, grads, copies, coef, learning_rate, momentum, mode, sync, stream, velocities)
+    v = _described(velocities, "velocities", DType.f32)
+    _update_many(ctx, params, v, velocities, grads, copies, coef, learning_rate, momentum, mode, sync, stream)
 
 
-def _update_many(ctx, params, velocities_at, grads, copies, coef, learning_rate, momentum, mode, sync, stream,
-                 velocities=None, counts=None):
+def _update_many(ctx, params, v, velocities, grads, copies, coef, learning_rate, momentum, mode, sync, stream):
+    """v: the velocities' description, or the addresses of an optimizer's own (velocities is None then)."""
     if isinstance(mode, str):
         try:
             mode = NesterovMode[mode]
         except KeyError:
             raise PcpError(-1, f"unknown mode {mode!r}") from None
-    n = _counts(grads, ("params", params), ("velocities", velocities), ("param_copies", copies))
-    if counts is not None and list(n) != counts:
-        raise PcpError(-12, "the gradients must have the sizes of the optimizer's tensors")
-    if coef is not None and (coef.dtype != torch.float32 or coef.numel() != 1):
+    g, p = _described(grads, "gradients"), _described(params, "parameters", DType.f32)
+    c = None if copies is None else _described(copies, "param_copies", DType.bf16)
+    _same_sizes(g, ("params", p, params), ("velocities", None if velocities is None else v, velocities),
+                ("param_copies", c, copies))
+    scale = [] if coef is None else [coef]
+    e = _described(scale, "coef", DType.f32)
+    if coef is not None and e[1] != _ONE:
         raise PcpError(-1, "coef must be an f32 scalar")
-    p, g = _List(params, "parameters", torch.float32), _List(grads, "gradients")
-    c = None if copies is None else _List(copies, "param_copies", torch.bfloat16)
+    device = _one_device(g, p, v if velocities is not None else None, c, e)
+    ctx = ctx or default_context(max(device, 0))
     a = NesterovManyArgs()
     lib().pcp_nesterov_many_args_init(ctypes.byref(a))
-    with call_scope(ctx, stream, *params, *(velocities or ()), *grads, *(copies or ()), coef) as handle:
-        a.n_tensors, a.counts = len(grads), ctypes.addressof(n)
-        a.params, a.velocities, a.grads, a.dtypes = p.at, velocities_at, g.at, g.types_at
-        a.param_copies = None if c is None else c.at
-        a.coef = None if coef is None else coef.data_ptr()
+    with call_scope.of_described(ctx, stream, device, params, velocities or (), grads, copies or (), scale) as handle:
+        a.n_tensors, a.counts, a.params, a.grads, a.dtypes = len(grads), g[1], p[0], g[0], g[2]
+        a.velocities = v if velocities is None else v[0]
+        if c is not None:
+            a.param_copies = c[0]
+        if coef is not None:
+            a.coef = memoryview(e[0]).cast("q")[0]
         a.learning_rate, a.momentum, a.mode = learning_rate, momentum, int(mode)
         a.flags = 0 if sync else FLAG_ASYNC
         a.stream = handle
@@ -230,10 +242,11 @@ class Nesterov:
         """``nesterov_update_many`` with this optimizer's velocities: params and grads in the order of its counts."""
         params, grads = list(params), list(grads)
         copies = None if param_copies is None else list(param_copies)
-        v = (ctypes.c_void_p * len(self.counts))(*[lib().pcp_nesterov_velocity(self.handle, i)
-                                                   for i in range(len(self.counts))])
-        _update_many(self.ctx, params, ctypes.addressof(v), grads, copies, coef, self.learning_rate, self.momentum,
-                     self.mode, sync, stream, counts=self.counts)
+        if [t.numel() for t in grads] != self.counts:
+            raise PcpError(-12, "the gradients must have the sizes of the optimizer's tensors")
+        v = [lib().pcp_nesterov_velocity(self.handle, i) or 0 for i in range(len(self.counts))]
+        _update_many(self.ctx, params, array.array("Q", v).tobytes(), None, grads, copies, coef, self.learning_rate,
+                     self.momentum, self.mode, sync, stream)
 
     def reset(self) -> None:
         check(lib().pcp_nesterov_reset(self.handle, None), self.ctx.handle)
