@@ -423,15 +423,17 @@ struct Pieces {
 
 hipError_t launch_norm(pcp_ctx* ctx, const pcp_grad_clip_args* a, int64_t elements, hipStream_t st) {
   // The launches, and how many workgroups each may have: kNormBlocks in all.
-  int64_t pieces = 0;
-  for (Pieces p{a->counts, a->n_tensors}; p.next();) ++pieces;
+  int64_t pieces = elements == 0 ? 0 : a->n_tensors;
+  if (elements > kPiece || pieces > kNormPieces) {
+    pieces = 0;
+    for (Pieces p{a->counts, a->n_tensors}; p.next();) ++pieces;
+  }
   const int64_t launches = std::max<int64_t>(1, (pieces + kNormPieces - 1) / kNormPieces);
   const int most = static_cast<int>(std::min<int64_t>(kNormGrid, kNormBlocks / launches));
   // Chunks small enough that a small model's gradients occupy the chip, and large enough that a vector's loads are wide.
   const int chunk = elements < int64_t(kNormGrid) * kNormChunk ? kNormSmall : kNormChunk;
   static_assert((PCP_GRAD_MAX_TENSORS + 65536) / kNormPieces + 1 <= kNormBlocks, "a workgroup for every launch");
   NormArgs b;
-  std::memset(&b, 0, sizeof(b));
   b.chunk = chunk;
   b.max_norm = a->max_norm;
   b.parts = ctx->d_norm_parts;
@@ -439,8 +441,8 @@ hipError_t launch_norm(pcp_ctx* ctx, const pcp_grad_clip_args* a, int64_t elemen
   b.norm = a->norm;
   b.coef = a->coef;
   b.err = ctx->d_page->err;
-  // Two walks: the workgroups are counted before the first launch, since each needs their number.
-  for (int launch = 0; launch < 2; ++launch) {
+  // With several launches two walks: the workgroups are counted before the first, since each needs their number.
+  for (int launch = launches > 1 ? 0 : 1; launch < 2; ++launch) {
     Pieces p{a->counts, a->n_tensors};
     bool more = p.next();
     int blocks = 0;
@@ -457,6 +459,7 @@ hipError_t launch_norm(pcp_ctx* ctx, const pcp_grad_clip_args* a, int64_t elemen
       const int grid = std::max(1, std::min(most, b.first[b.pieces]));
       if (launch == 1) {
         b.block0 = blocks;
+        if (launches == 1) b.blocks = grid;
         if (a->norm_type == PCP_NORM_L2) norm_kernel<PCP_NORM_L2><<<grid, kBlock, 0, st>>>(b);
         else norm_kernel<PCP_NORM_MAX><<<grid, kBlock, 0, st>>>(b);
         const hipError_t e = hipGetLastError();
@@ -471,7 +474,6 @@ hipError_t launch_norm(pcp_ctx* ctx, const pcp_grad_clip_args* a, int64_t elemen
 
 hipError_t launch_clip(const pcp_grad_clip_args* a, hipStream_t st) {
   ClipArgs b;
-  std::memset(&b, 0, sizeof(b));
   b.coef = a->coef;
   Pieces p{a->counts, a->n_tensors};
   for (bool more = p.next(); more;) {
@@ -598,7 +600,6 @@ int nesterov_many(pcp_ctx* ctx, const pcp_nesterov_many_args* a) {
   if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
   hipStream_t st = static_cast<hipStream_t>(a->stream);
   UpdateArgs b;
-  std::memset(&b, 0, sizeof(b));
   b.coef = a->coef;
   b.lr = a->learning_rate;
   b.mu = a->momentum;

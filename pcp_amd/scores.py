@@ -14,7 +14,6 @@ import torch
 from . import _lib, _tensors
 from ._lib import DType, PcpError, ScoreArgs, ScoreBwdArgs, check, lib
 from .grpo import _TORCH_DTYPE, Context, call_scope, default_context, dtype_code
-from .step import _row_stride, _seq_stride
 
 
 @dataclass
@@ -49,11 +48,19 @@ def _tokens(logits, ids, mask, rows, tok_offset, tokens):
     return S, LS, V, TS, rows, tok_offset
 
 
-def _row_places(t: torch.Tensor, a, row: str, seq: str) -> None:
-    """The strides of [S, LS, V] rows into fields `row` and `seq` of a."""
-    step = _row_stride(t)
-    setattr(a, row, step)
-    setattr(a, seq, _seq_stride(t) or max(t.shape[1], 1) * step)
+def _row_strides(t: torch.Tensor) -> tuple[int, int]:
+    """Elements between the rows and between the sequences of [S, LS, V]."""
+    S, m, V = t.shape
+    seq, row, one = t.stride()
+    if one != 1 and V > 1:
+        raise PcpError(-1, "logits rows must be contiguous")
+    if m <= 1:
+        row = V
+    if S <= 1 or m < 1:
+        seq = max(m, 1) * row
+    if row < V or seq < V:
+        raise PcpError(-1, "logits rows overlap: expand them with .contiguous()")
+    return row, seq
 
 
 def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: torch.Tensor | None = None, *, k: int = 0,
@@ -74,8 +81,7 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: to
     if not 0 <= k <= min(V, _lib.SCORE_TOP_MAX):
         raise PcpError(-1, f"k must be in [0, {min(V, _lib.SCORE_TOP_MAX)}] (got {k})")
     a = ScoreArgs()
-    lib().pcp_score_args_init(ctypes.byref(a))
-    _row_places(logits, a, "row_stride", "seq_stride")
+    a.row_stride, a.seq_stride = _row_strides(logits)
     ctx = ctx or default_context(logits.device.index or 0)
     o = outputs
     if o is None:
@@ -93,22 +99,22 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: to
             known = (ids, mask, o.logp, o.entropy, o.row_max, o.log_sum, o.top_logp, o.top_ids)
             d = _tensors.describe((logits, *known))
         else:
-            n = memoryview(d[1]).cast("q")
-            t = memoryview(d[2]).cast("i")
-            top = int(_TORCH_DTYPE.get(top_ids_dtype, -2))
-            for i, want in ((3, S * TS if ids is not None else -1), (4, S * TS), (5, S * TS), (6, S * TS),
-                            (7, S * TS * k or -1), (8, S * TS * k or -1)):
-                wants = top if i == 8 else int(DType.f32)
-                # (Optional ones may be None: but logp with ids, and the alternatives with k.)
-                if (n[i] != want or t[i] != wants) and not (n[i] == -1 and (want <= 0 or 4 <= i <= 6)):
-                    raise PcpError(-1, "outputs do not fit the call: f32 [S, TS], top_logp f32 and top_ids [S, TS, k]")
+            # (Optional ones may be None: but logp with ids, and the alternatives with k.)
+            f32, top = int(DType.f32), int(_TORCH_DTYPE.get(top_ids_dtype, -2))
+            n, t = memoryview(d[1]).cast("q")[3:].tolist(), memoryview(d[2]).cast("i")[3:].tolist()
+            N = S * TS
+            want = [N if ids is not None else -1, N, N, N, N * k if k else -1, N * k if k else -1]
+            types = [f32 if ids is not None else -1, f32, f32, f32, f32 if k else -1, top if k else -1]
+            if n != want or t != types:
+                for i in range(6):
+                    if (n[i] != want[i] or t[i] != types[i]) and not (n[i] == -1 and 1 <= i <= 3):
+                        raise PcpError(-1, "outputs do not fit the call: f32 [S, TS], top_logp f32 and top_ids [S, TS, k]")
         at = memoryview(d[0]).cast("q")
         a.n_seq, a.rows, a.vocab, a.tok_seq_stride, a.tok_offset = S, rows, V, TS, tok_offset
-        a.k, a.temperature, a.logits_dtype, a.logits = k, temperature, dtype_code(logits), at[0]
-        _set_tokens(a, ids, mask, at)
+        kinds = memoryview(d[2]).cast("i")
+        a.k, a.temperature, a.logits, a.ids, a.mask = k, temperature, at[0], at[1], at[2]
+        a.logits_dtype, a.ids_dtype, a.mask_dtype, a.top_ids_dtype = kinds[0], kinds[1], kinds[2], kinds[8]
         a.logp, a.entropy, a.row_max, a.log_sum, a.top_logp, a.top_ids = at[3:]
-        if k:
-            a.top_ids_dtype = dtype_code(o.top_ids)
         a.flags = 0 if sync else _lib.FLAG_ASYNC
         a.stream = handle
         check(lib().pcp_score_fwd(ctx.handle, ctypes.byref(a)), ctx.handle)
@@ -142,8 +148,7 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: to
     if dlogits is not None and dlogits_dtype is not None and dlogits.dtype != dlogits_dtype:
         raise PcpError(-2, f"dlogits_dtype is {dlogits_dtype}, the given dlogits are {dlogits.dtype}")
     a = ScoreBwdArgs()
-    lib().pcp_score_bwd_args_init(ctypes.byref(a))
-    _row_places(logits, a, "row_stride", "seq_stride")
+    a.row_stride, a.seq_stride = _row_strides(logits)
     ctx = ctx or default_context(logits.device.index or 0)
     known = (logits, ids, mask, row_max, log_sum, entropy, dlogp, dentropy)
     d = _tensors.describe((*known, dlogits))
@@ -151,12 +156,12 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: to
     with call_scope.of_described(ctx, stream, d[4], known, (dlogits,)) as handle:
         if dlogits is None:
             dlogits = torch.empty((S, LS, V), dtype=dlogits_dtype or logits.dtype, device=logits.device)
-        _row_places(dlogits, a, "drow_stride", "dseq_stride")
+        a.drow_stride, a.dseq_stride = _row_strides(dlogits)
         at = memoryview(d[0]).cast("q")
         a.n_seq, a.rows, a.logit_rows, a.vocab, a.tok_seq_stride, a.tok_offset = S, rows, LS, V, TS, tok_offset
-        a.logits_dtype, a.dlogits_dtype, a.temperature = dtype_code(logits), dtype_code(dlogits), temperature
-        a.logits, a.dlogits = at[0], dlogits.data_ptr()
-        _set_tokens(a, ids, mask, at)
+        kinds = memoryview(d[2]).cast("i")
+        a.logits_dtype, a.ids_dtype, a.mask_dtype, a.dlogits_dtype = kinds[0], kinds[1], kinds[2], dtype_code(dlogits)
+        a.temperature, a.logits, a.ids, a.mask, a.dlogits = temperature, at[0], at[1], at[2], dlogits.data_ptr()
         a.row_max, a.log_sum, a.entropy, a.dlogp, a.dentropy = at[3:8]
         a.accumulate = 1 if accumulate else 0
         a.flags = 0 if sync else _lib.FLAG_ASYNC
@@ -169,10 +174,3 @@ def _contiguous(d, n: int | None = None) -> None:
     """The first n described tensors behind the logits are contiguous."""
     if 0 in d[3][1:n]:
         raise PcpError(-1, "token arrays and outputs must be contiguous")
-
-
-def _set_tokens(a, ids, mask, at) -> None:
-    if ids is not None:
-        a.ids, a.ids_dtype = at[1], dtype_code(ids)
-    if mask is not None:
-        a.mask, a.mask_dtype = at[2], dtype_code(mask)
