@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstddef>
 #include <cstdint>
@@ -457,7 +458,7 @@ __device__ __forceinline__ void score_dead(const ScoreArgs& a, const ScoreRow& r
 
 // ONE: rows in parts of at most a batch each.
 template <typename TI, bool TOP, bool ONE>
-__global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a) {
+__global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
   constexpr int BLOCK = kBlock, U = kU;
   __shared__ __align__(16) PartShared ps;
   Shared& sh = ps.sh;
@@ -492,10 +493,12 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
   u32x4 x[U];
   float bx = kNegInf, group = kNegInf;
   int b = 0;
-  auto batch = [&](int base, auto held) {
+  auto load = [&](u32x4 (&to)[U], int base) {
     const uint32_t off = static_cast<uint32_t>(base + tid) * 16u;
 #pragma unroll
-    for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
+    for (int q = 0; q < U; ++q) to[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
+  };
+  auto batch = [&](auto held) {
     bx = batch_max<TI>(x, held);
     sums.template add<TI>(x, held, bx);
     if constexpr (TOP && !ONE) {
@@ -504,11 +507,18 @@ __global__ void __launch_bounds__(kBlock, TOP ? 5 : 8) score_kernel(ScoreArgs a)
       ++b;
     }
   };
-  // Whole batches without a test for each vector, then what is left.
+  // Whole batches without a test for each vector, then what is left; the next batch's loads go out ahead.
   int base = v0;
+  if (base < end || ONE) load(x, base);
   if constexpr (!ONE)
-    for (; base + BLOCK * U <= end; base += BLOCK * U) batch(base, [](int) { return true; });
-  if (base < end || ONE) batch(base, [&](int q) { return base + q * BLOCK + tid < end; });
+    for (; base + BLOCK * U <= end; base += BLOCK * U) {
+      u32x4 next[U];
+      load(next, base + BLOCK * U);
+      batch([](int) { return true; });
+#pragma unroll
+      for (int q = 0; q < U; ++q) x[q] = next[q];
+    }
+  if (base < end || ONE) batch([&](int q) { return base + q * BLOCK + tid < end; });
   float mx = sums.mx;
   double s = sums.s, tt = sums.t;
   score_merge<64>(mx, s, tt, a.k2);
@@ -643,13 +653,15 @@ struct ScoreBwdArgs {
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
 
-constexpr int kGradU = 2;    // groups per lane
+// Groups per lane: 16 bytes of dlogits each, so that 16-bit logits of f32 dlogits come 8 bytes a group.
+template <typename TI, typename TO>
+constexpr int grad_unroll() { return TI::kBytes == 2 && TO::kBytes == 4 ? 4 : 2; }
 
 // A row's gradient is one pass: dz = p (A + B d) with d = (x - m) k2 - log2 sum, p = 2^d, and the token's
 // own term.
 template <typename TI, typename TO, bool ACC>
 __global__ void __launch_bounds__(kBlock) score_grad_kernel(ScoreBwdArgs a) {
-  constexpr int N = 16 / TO::kBytes, U = kGradU;   // elements per group
+  constexpr int N = 16 / TO::kBytes, U = grad_unroll<TI, TO>();   // elements per group
   const int tid = threadIdx.x;
   const uint32_t of = blockIdx.x / static_cast<uint32_t>(a.blocks);
   const int block = static_cast<int>(blockIdx.x - of * static_cast<uint32_t>(a.blocks));
@@ -737,10 +749,10 @@ __global__ void __launch_bounds__(kBlock) score_grad_kernel(ScoreBwdArgs a) {
 
 template <typename TI, typename TO>
 hipError_t launch_grad(ScoreBwdArgs a, int64_t n_rows, bool accumulate, hipStream_t st) {
-  constexpr int N = 16 / TO::kBytes;
+  constexpr int N = 16 / TO::kBytes, U = grad_unroll<TI, TO>();
   // The groups of a row that begins up to N - 1 elements past an aligned address.
   const int64_t groups = (a.tok.vocab + N - 1 + N - 1) / N;
-  a.blocks = static_cast<int32_t>((groups + kBlock * kGradU - 1) / (kBlock * kGradU));
+  a.blocks = static_cast<int32_t>((groups + kBlock * U - 1) / (kBlock * U));
   const int64_t rows = (int64_t(1) << 23) / a.blocks > 0 ? (int64_t(1) << 23) / a.blocks : 1;   // of a launch
   for (int64_t r0 = 0; r0 < n_rows; r0 += rows) {
     a.row0 = r0;
@@ -839,11 +851,13 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   // Workgroups per row: as few rows' logits as would leave CUs idle are dealt to several, at least kLeastPart vectors each.
   constexpr int64_t kLeastPart = 8 * kBlock;
   const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
-  int64_t parts = n_rows < kScoreTickets ? (1024 + n_rows - 1) / n_rows : 1;
-  if (parts > 64) parts = 64;   // one wave merges their sums
-  int64_t per = ((nv + parts - 1) / parts + kBlock - 1) / kBlock * kBlock;
-  if (per < kLeastPart || (per <= 2 * kLeastPart && nv <= 64 * kLeastPart)) per = kLeastPart;
-  parts = nv > 0 ? (nv + per - 1) / per : 1;
+  int64_t parts = 1, per = (nv + kBlock - 1) / kBlock * kBlock;
+  if (n_rows < kScoreTickets && nv > kLeastPart) {   // (a ticket per row)
+    parts = std::min<int64_t>((1024 + n_rows - 1) / n_rows, 64);   // one wave merges their sums
+    per = ((nv + parts - 1) / parts + kBlock - 1) / kBlock * kBlock;
+    if (per <= 2 * kLeastPart && nv <= 64 * kLeastPart) per = kLeastPart;
+    parts = (nv + per - 1) / per;
+  }
   const int64_t part_cap = a->k > 0 ? a->k + 64 : 0;
   const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(n_rows) * parts * part_cap : 0;
   const size_t sums = parts > 1 ? sizeof(ScorePart) * static_cast<size_t>(n_rows) * parts + 16 : 0;
