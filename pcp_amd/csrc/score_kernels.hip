@@ -320,6 +320,66 @@ __device__ __forceinline__ int select_exact(const char* xrow, const RowSpan& sp,
   return min(k, total);
 }
 
+// The candidates of a part where fewer than k values lie above masks: those, and of the masked ones, if all are
+// equal, the first k elements of the part (at least as many as are missing are among them). Called by the whole
+// workgroup; ends with a barrier.
+template <typename TI>
+__device__ __forceinline__ int gather_masked(const char* xrow, const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end,
+                                             bool edges, int k, Shared& sh) {
+  constexpr int EPV = 16 / TI::kBytes, U = 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int total = max(end - v0, 0) * EPV + (edges ? sp.head + sp.tail : 0);
+  __syncthreads();
+  if (tid == 0) sh.count = 0;
+  __syncthreads();
+  Candidates c{sh, 0, kMasked + 0x1p-9f};   // the least f32 above kMasked
+  float lo = __builtin_inff(), hi = kNegInf;   // of the masked elements
+  auto masked = [&](bool is, float e) {
+    is = is && e <= kMasked;
+    lo = is ? fminf(lo, e) : lo;
+    hi = is ? fmaxf(hi, e) : hi;
+  };
+  if (edges && tid < 64) {
+    const int ek = edge_index<TI>(sp, tid);
+    const float e = ek >= 0 ? TI::load1(xrow, ek) : kNegInf;
+    masked(ek >= 0, e);
+    c.add(ek >= 0 && e >= c.least_x, element_key(e, static_cast<uint32_t>(ek)));
+  }
+  for (int base = v0; base < end; base += kBlock * U) {
+    u32x4 x[U];
+#pragma unroll
+    for (int q = 0; q < U; ++q) x[q] = buf_ld16<false>(xbuf, static_cast<uint32_t>(base + q * kBlock + tid) * 16u);
+    uint32_t left_q = 0;
+#pragma unroll
+    for (int q = 0; q < U; ++q) {
+      const bool is = base + q * kBlock + tid < end;
+#pragma unroll
+      for (int j = 0; j < EPV; ++j) masked(is, TI::unpack(reinterpret_cast<const uint32_t*>(&x[q]), j));
+      left_q |= is && vec_max<TI>(kNegInf, x[q]) >= c.least_x ? 1u << q : 0u;
+    }
+    take_vectors<TI>(c, x, left_q, static_cast<uint32_t>(sp.head + (base + tid) * EPV), (1u << EPV) - 1u);
+  }
+  lo = -lanes_max<64>(-lo);
+  hi = lanes_max<64>(hi);
+  if (lane == 0) {
+    sh.low[wave] = lo;
+    sh.high[wave] = hi;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    lo = fminf(lo, sh.low[w]);
+    hi = fmaxf(hi, sh.high[w]);
+  }
+  const int first = edges ? 0 : sp.head + v0 * EPV;
+  const float e = tid < min(k, total) ? TI::load1(xrow, first + tid) : 0.f;
+  c.add(tid < min(k, total) && e <= kMasked, element_key(e, static_cast<uint32_t>(first + tid)));
+  __syncthreads();
+  const int n = sh.count;
+  __syncthreads();
+  return n <= kCap && !(lo < hi) ? n : select_exact<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
+}
+
 // The candidates of a part whose lanes have left their groups' largest logits (batches: batches per group, groups:
 // how many), k or more of them where the part has as many elements, and what k of them reach. Called by the whole
 // workgroup; ends with a barrier.
@@ -345,7 +405,7 @@ __device__ __forceinline__ int gather_top(const char* xrow, const RowSpan& sp, _
   __syncthreads();
   const int total = max(end - v0, 0) * EPV + (edges ? sp.head + sp.tail : 0);
   const bool all = least == kNegInf;   // fewer than k values above masks: a short part's elements all
-  if (all && total > kCap) return select_exact<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
+  if (all && total > kCap) return gather_masked<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
   if (all) left = (1u << groups) - 1u;
   Candidates c{sh, 0, least};
   if (edges && tid < 64) {
@@ -391,7 +451,7 @@ __device__ __forceinline__ int gather_one(const char* xrow, const RowSpan& sp, _
   __syncthreads();
   const int total = max(end - v0, 0) * EPV + (edges ? sp.head + sp.tail : 0);
   const bool all = least == kNegInf;
-  if (all && total > kCap) return select_exact<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
+  if (all && total > kCap) return gather_masked<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
   Candidates c{sh, 0, least};
   if (edges && tid < 64) {
     const int ek = edge_index<TI>(sp, tid);
@@ -427,13 +487,16 @@ __device__ __forceinline__ void score_write(const ScoreArgs& a, const ScoreRow& 
   auto log_p = [&](float x) {
     return static_cast<float>((static_cast<double>(x) - static_cast<double>(mx)) * a.inv_tau - log_sum);
   };
-  if constexpr (TOP)
+  if constexpr (TOP) {
+    // (Sorted instead, 600 candidates of one row took 16 us more.)
+    if (n > 2 * kBlock) n = Candidates{sh, 0, kNegInf}.thin(n, a.k, 2 * kBlock);
     rank_entries(sh, n, a.k, [&](int rank, float x, int64_t id) {
       const int64_t at = r.at * a.k + rank;
       a.top_logp[at] = log_p(x);
       if (a.top_i64) static_cast<int64_t*>(a.top_ids)[at] = id;
       else static_cast<int32_t*>(a.top_ids)[at] = static_cast<int32_t>(id);
     });
+  }
   if (threadIdx.x != 0) return;
   if (!__builtin_isfinite(mx) || !__builtin_isfinite(log_sum)) raise_error(a.tok.err, kErrNonFinite);
   if (a.logp) a.logp[r.at] = r.id < 0 ? 0.f : log_p(token);

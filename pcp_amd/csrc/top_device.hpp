@@ -1,6 +1,5 @@
-// Finding the k largest logits of a row in one pass, beside sums over it: candidates in LDS, a
-// threshold that at least k of the elements seen reach, and the scan that feeds both (top_kernels.hip
-// says how; score_kernels.hip scans with sums of its own).
+// The k largest logits of a row: elements as 64-bit keys, candidates of them in LDS, a threshold that at least k
+// reach, and the ranking of what is left (top_kernels.hip and score_kernels.hip say how they come by them).
 #pragma once
 
 #include "grpo_device.hpp"
@@ -242,69 +241,6 @@ __device__ __forceinline__ void take_vectors(Candidates& c, const u32x4 (&x)[U],
       c.add(bits != 0 && key > c.least, key);
       bits &= ~((1u << (EPV - 1)) >> j);
     }
-  }
-}
-
-// The 16-byte vectors [v0, end) of a row interior (sp) through xbuf: every element goes into the lane's
-// sums, and those that may be among the k largest into the candidates, which hold `edges` elements
-// at the start and at most `left` (>= k) at the end, few more than k where the row lets them. Called by the whole
-// workgroup after a barrier; ends with one. Sums: mx the lane's largest logit (-inf: none yet), fresh() a
-// batch whose largest logit is bx, and, unless kFresh, add(), which may refuse a batch.
-template <typename TI, typename Sums>
-__device__ __forceinline__ void scan_part(const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end, int edges, int k,
-                                          int left, Sums& sums, Candidates& c, Shared& sh) {
-  constexpr int EPV = 16 / TI::kBytes, U = kU, BLOCK = kBlock;
-  const int tid = threadIdx.x;
-  // The candidates are thinned where they pass `limit`; after the last batch to about k.
-  const int room = min(kCut, 2 * k + 128);
-  constexpr int kRounds = U * EPV / 4;                   // of 4 elements per lane
-  int n = edges;                                         // candidates before the batch
-  int round = -1;                                        // >= 0: a batch taken in rounds
-  for (int base = v0; base < end;) {
-    u32x4 x[U];
-    const uint32_t off = static_cast<uint32_t>(base + tid) * 16u;
-#pragma unroll
-    for (int q = 0; q < U; ++q) x[q] = buf_ld16<true>(xbuf, off + q * (BLOCK * 16u));
-    auto held = [&](int q) { return base + q * BLOCK + tid < end; };
-    bool near[U];   // this lane's vector may hold an element that passes
-    bool fresh = Sums::kFresh || round >= 0 || base == v0 || __any(sums.mx == kNegInf);
-    if (!fresh) fresh = !sums.template add<TI>(x, held, c.least_x, near);
-    if (fresh) {
-      float vm[U], bx = kNegInf;
-#pragma unroll
-      for (int q = 0; q < U; ++q) {
-        vm[q] = held(q) ? vec_max<TI>(kNegInf, x[q]) : kNegInf;
-        bx = fmaxf(bx, vm[q]);
-      }
-      if (round < 0) {
-        sums.template fresh<TI>(x, held, bx);
-        // k vectors of the first batch reach this, each with one element at least.
-        if (base == v0) c.least_x = reached_by(sh, vm, k);
-      }
-#pragma unroll
-      for (int q = 0; q < U; ++q) near[q] = held(q) && (vm[q] >= c.least_x || c.least_x == kNegInf);
-    }
-    uint32_t left_q = 0;
-#pragma unroll
-    for (int q = 0; q < U; ++q) left_q |= near[q] ? 1u << q : 0u;
-    if (round >= 0) left_q &= 1u << (round / (EPV / 4));
-    uint32_t keep = (1u << EPV) - 1u;
-    if (round >= 0) keep = 0xf0u >> (EPV == 4 ? 4 : 4 * (round % 2));
-    take_vectors<TI>(c, x, left_q, static_cast<uint32_t>(sp.head + (base + tid) * EPV), keep);
-    __syncthreads();
-    const int was = n;
-    n = sh.count;
-    __syncthreads();
-    if (round < 0 && n > kCap) {   // too many at once: this batch again, in rounds that are sure to fit
-      if (tid == 0) sh.count = was;
-      n = was;
-      round = 0;
-    } else if (round < 0 || ++round == kRounds) {
-      round = -1;
-      base += BLOCK * U;
-    }
-    if (n > (base >= end ? left : round >= 0 ? kCut : room)) n = c.thin(n, k, base >= end ? left : kCut);
-    else __syncthreads();
   }
 }
 

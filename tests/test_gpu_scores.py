@@ -125,6 +125,24 @@ def test_scores_of_odd_rows(kind, dtype, R, V, k, tau):
     check_scores(x, ids, out, tau, k)
 
 
+@pytest.mark.parametrize("R,V,k,left", [(2, 40000, 20, 3), (600, 5000, 9, 2), (1, 151936, 64, 64), (520, 20000, 5, 0), (3, 300, 256, 1)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_fewer_tokens_left_than_alternatives(dtype, R, V, k, left):
+    """Rows of two kinds of masks, of one, and with the unmasked ones spread over every part."""
+    rng = np.random.default_rng(V + left)
+    x = np.full((R, V), -1e30, np.float32)
+    x[::2][rng.random(x[::2].shape) < 0.5] = -np.inf
+    if R == 1:
+        x[:] = -np.inf
+    for r in range(R):
+        n = max(left, 1)
+        x[r, rng.choice(V, n, replace=False)] = rng.standard_normal(n)
+    x = to_dev(x, dtype, 1)
+    ids = rng.integers(0, V, R)
+    out = scores.token_scores(x[:, None], dev(ids[:, None], torch.int64), k=k)
+    check_scores(x, ids, out, 1.0, k)
+
+
 @pytest.mark.parametrize("mask_dtype", [torch.float32, torch.bool])
 @pytest.mark.parametrize("S,T,V,k,shift", [(3, 9, 1003, 5, 1), (2, 5, 70000, 3, 0), (40, 20, 333, 0, 1), (64, 1, 30000, 2, 0)])
 def test_layout_masks_and_ignored_tokens(mask_dtype, S, T, V, k, shift):
@@ -332,6 +350,42 @@ def test_the_same_call_gives_the_same_bits(k, S, V):
         for n in ("logp", "entropy", "row_max", "log_sum", "top_logp", "top_ids"):
             if getattr(a, n) is not None:
                 assert torch.equal(getattr(a, n), getattr(b, n)), n
+
+
+def test_rows_beside_the_number_of_tickets():
+    """As many rows as may be dealt to several workgroups, and one more; the context's other buffers stay as they are."""
+    from pcp_amd import step
+    ctx = grpo.Context(0)
+    g = torch.randn(1 << 20, device=DEV)
+    want = step.grad_norm(g, ctx=ctx)
+    torch.manual_seed(1)
+    for rows in (511, 512, 4096):
+        x = torch.randn(rows, 1, 20000, device=DEV).to(torch.bfloat16)
+        ids = torch.randint(0, 20000, (rows, 1), device=DEV)
+        for _ in range(3):
+            out = scores.token_scores(x, ids, k=3, ctx=ctx)
+        picked = [0, rows // 2, rows - 1]
+        check_scores(x[picked, 0], ids[picked, 0].cpu().numpy(), scores.TokenScores(*(t[picked] for t in (
+            out.logp, out.entropy, out.row_max, out.log_sum, out.top_logp, out.top_ids))), 1.0, 3)
+        got = step.grad_norm(g, ctx=ctx)
+        assert torch.equal(got.norm, want.norm)
+
+
+@pytest.mark.parametrize("which", ["dlogp", "dentropy", "row_max", "entropy"])
+def test_a_gradient_or_statistic_that_is_not_finite_is_reported(which):
+    x, ids = bad_calls()
+    ctx = grpo.Context(0)
+    sc = scores.token_scores(x, ids, ctx=ctx)
+    a = dict(row_max=sc.row_max, log_sum=sc.log_sum, entropy=sc.entropy, dlogp=torch.ones(4, 6, device=DEV),
+             dentropy=torch.ones(4, 6, device=DEV))
+    a[which] = a[which].clone()
+    a[which][2, 1] = float("nan")
+    d = torch.zeros_like(x)
+    with pytest.raises(PcpError) as e:
+        scores.token_scores_bwd(x, ids, dlogits=d, ctx=ctx, **a)
+    assert e.value.code == -4 and torch.isnan(d[2, 1]).all()
+    d[2, 1] = 0
+    assert torch.isfinite(d).all()
 
 
 def test_captured_calls_and_other_streams():
