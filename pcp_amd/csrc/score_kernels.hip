@@ -54,8 +54,7 @@ struct alignas(16) ScorePart {
   double s, t;
   float mx;
   int32_t n;               // its candidates
-  float least;             // k of them reach this (-inf: not known)
-  int32_t pad;
+  int64_t pad;
 };
 
 struct ScoreArgs {
@@ -381,11 +380,10 @@ __device__ __forceinline__ int gather_masked(const char* xrow, const RowSpan& sp
 }
 
 // The candidates of a part whose lanes have left their groups' largest logits (batches: batches per group, groups:
-// how many), k or more of them where the part has as many elements, and what k of them reach. Called by the whole
-// workgroup; ends with a barrier.
+// how many), k or more of them where the part has as many elements. Called by the whole workgroup; ends with a barrier.
 template <typename TI>
 __device__ __forceinline__ int gather_top(const char* xrow, const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end,
-                                          bool edges, int k, int batches, int groups, PartShared& ps, float& least) {
+                                          bool edges, int k, int batches, int groups, PartShared& ps) {
   constexpr int EPV = 16 / TI::kBytes, U = kU;
   Shared& sh = ps.sh;
   const int tid = threadIdx.x;
@@ -396,7 +394,7 @@ __device__ __forceinline__ int gather_top(const char* xrow, const RowSpan& sp, _
     lane_max[0] = fmaxf(lane_max[0], v[g]);
   }
   // Up to 64 of the lanes' own maxima are nearly as high as the groups', and 256 values sooner counted than 4096.
-  least = k <= 64 ? reached_by(sh, lane_max, k) : reached_by(sh, v, k);
+  const float least = k <= 64 ? reached_by(sh, lane_max, k) : reached_by(sh, v, k);
   uint32_t left = 0;
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) left |= g < groups && v[g] >= least ? 1u << g : 0u;
@@ -438,15 +436,14 @@ __device__ __forceinline__ int gather_top(const char* xrow, const RowSpan& sp, _
 // The same for a part of one batch, which is still in x; lane_max: the lane's largest logit.
 template <typename TI, int U>
 __device__ __forceinline__ int gather_one(const char* xrow, const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end,
-                                          bool edges, int k, const u32x4 (&x)[U], float lane_max, Shared& sh,
-                                          float& least) {
+                                          bool edges, int k, const u32x4 (&x)[U], float lane_max, Shared& sh) {
   constexpr int EPV = 16 / TI::kBytes;
   const int tid = threadIdx.x;
   float v[U];
 #pragma unroll
   for (int q = 0; q < U; ++q) v[q] = v0 + q * kBlock + tid < end ? vec_max<TI>(kNegInf, x[q]) : kNegInf;
   const float own[1] = {lane_max};
-  least = k <= 64 ? reached_by(sh, own, k) : reached_by(sh, v, k);
+  const float least = k <= 64 ? reached_by(sh, own, k) : reached_by(sh, v, k);
   if (tid == 0) sh.count = 0;
   __syncthreads();
   const int total = max(end - v0, 0) * EPV + (edges ? sp.head + sp.tail : 0);
@@ -596,10 +593,9 @@ __global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
   tt = wave_t[lane & (kWaves - 1)];
   score_merge<kWaves>(mx, s, tt, a.k2);
   int n = 0;
-  float least = kNegInf;
-  if constexpr (TOP && ONE) n = gather_one<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, x, bx, sh, least);
+  if constexpr (TOP && ONE) n = gather_one<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, x, bx, sh);
   else if constexpr (TOP)
-    n = gather_top<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, a.group, (b + a.group - 1) / a.group, ps, least);
+    n = gather_top<TI>(xrow, sp, xbuf, v0, end, part == 0, a.k, a.group, (b + a.group - 1) / a.group, ps);
   if (a.parts == 1) {
     score_write<TOP>(a, r, token, sh, n, mx, s, tt);
     return;
@@ -616,7 +612,6 @@ __global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
     store_coherent(&parts[part].t, tt);
     store_coherent(&parts[part].mx, mx);
     store_coherent(&parts[part].n, n);
-    store_coherent(&parts[part].least, least);
   }
   wait_stores();
   __syncthreads();
@@ -625,52 +620,46 @@ __global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
   if (turn + 1 != static_cast<unsigned>(a.parts)) return;
   if (tid == 0) store_coherent(a.done + of, 0u);
   // Read at the level that the stores went to, past the caches, which then need no invalidation (an XCD's whole L2,
-  // for every row).
-  mx = kNegInf;
-  s = tt = 0.;
-  int left = 0;
-  least = kNegInf;
-  if (lane < a.parts) {
-    const __amdgpu_buffer_rsrc_t pbuf = row_rsrc(parts, static_cast<uint32_t>(a.parts) * sizeof(ScorePart));
-    const u32x4 p0 = buf_ld16_coherent(pbuf, lane * sizeof(ScorePart));
-    const u32x4 p1 = buf_ld16_coherent(pbuf, lane * sizeof(ScorePart) + 16);
-    s = __builtin_bit_cast(double, static_cast<uint64_t>(p0[1]) << 32 | p0[0]);
-    tt = __builtin_bit_cast(double, static_cast<uint64_t>(p0[3]) << 32 | p0[2]);
-    mx = __uint_as_float(p1[0]);
-    left = static_cast<int>(p1[1]);
-    least = __uint_as_float(p1[2]);
+  // for every row: 400 rows of 50,257 in four parts each took 50 us instead of 16).
+  const __amdgpu_buffer_rsrc_t pbuf = row_rsrc(parts, static_cast<uint32_t>(a.parts) * sizeof(ScorePart));
+  const __amdgpu_buffer_rsrc_t kbuf = row_rsrc(keys, static_cast<uint32_t>(a.parts * a.part_cap) * 8u);
+  auto key_at = [&](int i) { return buf_ld8_coherent(kbuf, static_cast<uint32_t>(i) * 8u); };
+  // Few slots are read along with the parts' counts, whatever they hold.
+  constexpr int R = 4;
+  const int slots = TOP ? a.parts * a.part_cap : 0;
+  uint64_t key[R] = {};
+  if (TOP && slots <= R * BLOCK) {
+#pragma unroll
+    for (int q = 0; q < R; ++q) key[q] = key_at(q * BLOCK + tid);   // (past the last: 0)
   }
+  const u32x4 p0 = buf_ld16_coherent(pbuf, lane * sizeof(ScorePart));
+  const u32x4 p1 = buf_ld16_coherent(pbuf, lane * sizeof(ScorePart) + 16);
+  const bool is = lane < a.parts;
+  s = is ? __builtin_bit_cast(double, static_cast<uint64_t>(p0[1]) << 32 | p0[0]) : 0.;
+  tt = is ? __builtin_bit_cast(double, static_cast<uint64_t>(p0[3]) << 32 | p0[2]) : 0.;
+  mx = is ? __uint_as_float(p1[0]) : kNegInf;
   if constexpr (TOP) {
-    const __amdgpu_buffer_rsrc_t kbuf = row_rsrc(keys, static_cast<uint32_t>(a.parts * a.part_cap) * 8u);
-    auto key_at = [&](int i) { return buf_ld8_coherent(kbuf, static_cast<uint32_t>(i) * 8u); };
-    const int upto = lanes_scan(left), all = __builtin_amdgcn_readlane(upto, 63);
-    // What one part's candidates reach, the row's k largest reach: few of the others' do.
-    Candidates c{sh, 0, lanes_max<64>(least)};
-    if (tid < 64) counts[tid] = upto - left;
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    constexpr int R = 4;
-    for (int base = 0; base < all; base += R * BLOCK) {
-      uint64_t key[R];
+    const int left = is ? static_cast<int>(p1[1]) : 0;
+    if (tid < 64) counts[tid] = left;
+    if (slots <= R * BLOCK) {
+      __syncthreads();
+      float v[R];
 #pragma unroll
-      for (int q = 0; q < R; ++q) {   // slot i: of the last part p with counts[p] <= i
-        const int i = base + q * BLOCK + tid;
-        int p = 0;
-#pragma unroll
-        for (int step = 32; step > 0; step >>= 1) p += p + step < a.parts && counts[p + step] <= i ? step : 0;
-        key[q] = i < all ? key_at(p * a.part_cap + i - counts[p]) : 0;
+      for (int q = 0; q < R; ++q) {
+        const int at = q * BLOCK + tid, p = at / a.part_cap;
+        key[q] = at < slots && at - p * a.part_cap < counts[p] ? key[q] : 0;   // no key is 0
+        v[q] = key[q] ? from_order(static_cast<uint32_t>(key[q] >> 32)) : kNegInf;
       }
+      Candidates c{sh, 0, reached_by(sh, v, a.k, (slots + BLOCK - 1) / BLOCK)};
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
 #pragma unroll
       for (int q = 0; q < R; ++q)
-        if (base + q * BLOCK < all)
-          c.add(key[q] != 0 && (c.least_x == kNegInf || from_order(static_cast<uint32_t>(key[q] >> 32)) >= c.least_x), key[q]);
-    }
-    __syncthreads();
-    n = sh.count;
-    __syncthreads();
-    if (n > kCap) {
-      if (tid < 64) counts[tid] = left;
+        if (q * BLOCK < slots) c.add(key[q] != 0 && (v[q] >= c.least_x || c.least_x == kNegInf), key[q]);
       __syncthreads();
+      n = sh.count;
+      __syncthreads();
+    } else {
       n = merge_parts(key_at, a.parts, a.part_cap, a.k, [&](int p) { return counts[p]; }, sh);
     }
   }
@@ -921,7 +910,7 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
     if (per <= 2 * kLeastPart && nv <= 64 * kLeastPart) per = kLeastPart;
     parts = (nv + per - 1) / per;
   }
-  const int64_t part_cap = a->k > 0 ? a->k + 64 : 0;
+  const int64_t part_cap = a->k > 0 ? a->k + 16 + a->k / 4 : 0;   // a part seldom has more (see gather_one), and is thinned then
   const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(n_rows) * parts * part_cap : 0;
   const size_t sums = parts > 1 ? sizeof(ScorePart) * static_cast<size_t>(n_rows) * parts + 16 : 0;
   if (parts > 1) {

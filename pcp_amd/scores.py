@@ -15,6 +15,8 @@ from . import _lib, _tensors
 from ._lib import DType, PcpError, ScoreArgs, ScoreBwdArgs, check, lib
 from .grpo import _TORCH_DTYPE, Context, call_scope, default_context, dtype_code
 
+_F32 = int(DType.f32)
+
 
 @dataclass
 class TokenScores:
@@ -100,7 +102,7 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: to
             d = _tensors.describe((logits, *known))
         else:
             # (Optional ones may be None: but logp with ids, and the alternatives with k.)
-            f32, top = int(DType.f32), int(_TORCH_DTYPE.get(top_ids_dtype, -2))
+            f32, top = _F32, int(_TORCH_DTYPE.get(top_ids_dtype, -2))
             n, t = memoryview(d[1]).cast("q")[3:].tolist(), memoryview(d[2]).cast("i")[3:].tolist()
             N = S * TS
             want = [N if ids is not None else -1, N, N, N, N * k if k else -1, N * k if k else -1]
@@ -133,10 +135,6 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: to
     given dlogits (the loss head's, for an entropy bonus); rows that have none stay as they are, and are 0
     otherwise. dlogits may be the logits themselves, and views with contiguous rows as the logits may."""
     S, LS, V, TS, rows, tok_offset = _tokens(logits, ids, mask, rows, tok_offset, row_max.shape[1] if row_max.dim() == 2 else 0)
-    for t, name in ((row_max, "row_max"), (log_sum, "log_sum"), (entropy, "entropy"), (dlogp, "dlogp"),
-                    (dentropy, "dentropy")):
-        if t is not None and (t.dtype != torch.float32 or t.shape != (S, TS)):
-            raise PcpError(-1, f"{name} must be f32 [S, TS]")
     if dlogp is not None and ids is None:
         raise PcpError(-1, "dlogp needs ids")
     if dentropy is not None and entropy is None:
@@ -153,14 +151,18 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: to
     known = (logits, ids, mask, row_max, log_sum, entropy, dlogp, dentropy)
     d = _tensors.describe((*known, dlogits))
     _contiguous(d, len(known))
+    counts, kinds = memoryview(d[1]).cast("q").tolist(), memoryview(d[2]).cast("i").tolist()
+    if counts[3:5] != [S * TS] * 2 or any([n != S * TS and n != -1 for n in counts[5:8]]):
+        raise PcpError(-1, "row_max, log_sum, entropy, dlogp and dentropy must be [S, TS]")
+    if kinds[3:5] != [_F32, _F32] or any([t != _F32 and t != -1 for t in kinds[5:8]]):
+        raise PcpError(-2, "row_max, log_sum, entropy, dlogp and dentropy must be f32")
     with call_scope.of_described(ctx, stream, d[4], known, (dlogits,)) as handle:
         if dlogits is None:
             dlogits = torch.empty((S, LS, V), dtype=dlogits_dtype or logits.dtype, device=logits.device)
         a.drow_stride, a.dseq_stride = _row_strides(dlogits)
         at = memoryview(d[0]).cast("q")
         a.n_seq, a.rows, a.logit_rows, a.vocab, a.tok_seq_stride, a.tok_offset = S, rows, LS, V, TS, tok_offset
-        kinds = memoryview(d[2]).cast("i")
-        a.logits_dtype, a.ids_dtype, a.mask_dtype, a.dlogits_dtype = kinds[0], kinds[1], kinds[2], dtype_code(dlogits)
+        a.logits_dtype, a.ids_dtype, a.mask_dtype, a.dlogits_dtype = *kinds[:3], dtype_code(dlogits)
         a.temperature, a.logits, a.ids, a.mask, a.dlogits = temperature, at[0], at[1], at[2], dlogits.data_ptr()
         a.row_max, a.log_sum, a.entropy, a.dlogp, a.dentropy = at[3:8]
         a.accumulate = 1 if accumulate else 0
