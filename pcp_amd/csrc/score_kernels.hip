@@ -1,5 +1,22 @@
 // Scores of given tokens (pcp_score.h): log-probs, entropy and the top alternatives of rows of
 // logits, and the gradient of a function of the log-probs and entropies.
+//
+// Forward: one read of a row. With m the largest logit, d = (x - m) log2(e) / temperature, s = sum 2^d and
+// t = sum 2^d d, the log-sum-exp is m / temperature + ln s and the entropy ln s - ln 2 t / s, two parts of one sign, so
+// that nothing cancels where a row has one likely token. A batch of eight 16-byte vectors a lane gives a lane's maximum
+// (two 16-bit elements an instruction), then s and t against it; the next batch's loads are out meanwhile. The
+// alternatives come after the pass: the lanes have kept their groups' maxima, what k of those reach rules out all
+// but about k groups, and these are read again. Few rows are cut into parts, whose sums and candidates the
+// last part to finish merges; there a part is one batch, and its candidates come from its registers.
+//
+// Bound by HBM with many rows, and by their last ones: 4096 rows of 151,936 bf16 187 us (6.7 TB/s, 65% of the VALU's
+// time), with 5/8 of them live 128 (6.1 TB/s), with k = 20 204 and 139. By latency with few: one row 6.4 us, with
+// k = 20 11.1 (meta data 0.4, the pass 1.6, sums 0.6, candidates 2.3, stores and ticket 1.0, merge 3, ranking 1); 64
+// f32 rows 16 and with k = 5 20. Rows of masks with fewer than k tokens left take one more pass (4096 such rows
+// 408 us; by select_exact, as first written, 2097), rows of a few equal values six (select_exact).
+//
+// Backward: one read of the logits, one write (or update) of dlogits, elementwise from the forward's
+// statistics; 4096 rows of 151,936 bf16, 5/8 of them live, 350 us (5.8 TB/s), added to what was there 399 (5.8).
 
 #include <hip/hip_runtime.h>
 
@@ -314,7 +331,8 @@ __device__ __forceinline__ int select_exact(const char* xrow, const RowSpan& sp,
     step(buf_ld16<false>(xbuf, static_cast<uint32_t>(base + tid) * 16u), base + tid < end,
          static_cast<uint32_t>(sp.head + (base + tid) * EPV), EPV);
   const int tail0 = sp.head + sp.nv * EPV;
-  if (edges) step(one(tail0 + min(tid, max(sp.tail - 1, 0)) - (sp.tail == 0)), tid < sp.tail, static_cast<uint32_t>(tail0 + tid), 1);
+  if (edges)
+    step(one(tail0 + min(tid, max(sp.tail - 1, 0)) - (sp.tail == 0)), tid < sp.tail, static_cast<uint32_t>(tail0 + tid), 1);
   __syncthreads();
   return min(k, total);
 }
@@ -705,11 +723,14 @@ struct ScoreBwdArgs {
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
 
-// Groups per lane: 16 bytes of dlogits each, so that 16-bit logits of f32 dlogits come 8 bytes a group.
+// Groups per lane: 16 bytes of dlogits each, so that 16-bit logits of f32 dlogits come 8 bytes a group. us with 1 | 2 | 4:
+//   bf16 -> f32, 2048 rows of 50,257   142 | 112 | 105        f32 -> f32, 1024 rows of 151,936   197 | 172 | 183
+//   bf16 -> bf16, 4096 rows of 151,936 452 | 350 | 354, added 432 | 399 | 414
 template <typename TI, typename TO>
 constexpr int grad_unroll() { return TI::kBytes == 2 && TO::kBytes == 4 ? 4 : 2; }
 
-// A row's gradient is one pass: dz = p (A + B d) with d = (x - m) k2 - log2 sum, p = 2^d, and the token's
+// Stores at system scope (sc0 sc1), which suit the whole-model updates, took 400 us for 399 here and, on rows off 16
+// bytes, 87 for 68. A row's gradient is one pass: dz = p (A + B d) with d = (x - m) k2 - log2 sum, p = 2^d, and the token's
 // own term.
 template <typename TI, typename TO, bool ACC>
 __global__ void __launch_bounds__(kBlock) score_grad_kernel(ScoreBwdArgs a) {
@@ -876,12 +897,14 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   if (a->k < 0 || a->k > PCP_SCORE_TOP_MAX || a->k > a->vocab)
     return fail(ctx, PCP_ERR_INVALID_ARG, "k must be in [0, min(vocab, %d)] (got %d)", PCP_SCORE_TOP_MAX, a->k);
   t.row_stride = a->row_stride ? a->row_stride : a->vocab;
-  if (t.row_stride < a->vocab) return fail(ctx, PCP_ERR_INVALID_ARG, "row_stride (%lld) must be >= vocab", (long long)t.row_stride);
+  if (t.row_stride < a->vocab)
+    return fail(ctx, PCP_ERR_INVALID_ARG, "row_stride (%lld) must be >= vocab", (long long)t.row_stride);
   int64_t n_rows, extent;
   if (mul_overflows(a->n_seq, a->rows, &n_rows) || n_rows > INT32_MAX)
     return fail(ctx, PCP_ERR_OVERFLOW, "n_seq * rows exceeds 2^31-1 rows");
   if (a->seq_stride) t.seq_stride = a->seq_stride;
-  else if (mul_overflows(a->rows, t.row_stride, &t.seq_stride)) return fail(ctx, PCP_ERR_OVERFLOW, "logits byte size overflows int64");
+  else if (mul_overflows(a->rows, t.row_stride, &t.seq_stride))
+    return fail(ctx, PCP_ERR_OVERFLOW, "logits byte size overflows int64");
   if (a->n_seq > 1 && a->rows > 0 && t.seq_stride < a->vocab)
     return fail(ctx, PCP_ERR_INVALID_ARG, "seq_stride (%lld) must be >= vocab", (long long)t.seq_stride);
   if (!extent_of(a->n_seq, a->rows, t.row_stride, t.seq_stride, a->vocab, &extent))
@@ -900,7 +923,12 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
   hipStream_t st = static_cast<hipStream_t>(a->stream);
 
-  // Workgroups per row: as few rows' logits as would leave CUs idle are dealt to several, at least kLeastPart vectors each.
+  // Workgroups per row: few rows' logits are dealt to about 1024 in all, kLeastPart vectors (a batch) each or more. us for
+  // 2048 workgroups in all | 1024 | 1024 of half a batch:
+  //   one bf16 row of 151,936, k 20   12.2 | 12.1 | 19.4     64 f32 rows of 151,936, k 0   16.3 | 14.8 | 15.0
+  //   200 bf16 rows, k 0              22.3 | 18.2 | 18.5     400 bf16 rows of 50,257, k 0  16.1 | 15.4 | 15.9
+  // From kScoreTickets rows on each has one workgroup: dealt to 4096 or 8192 in all, 1520 f16 rows of 50,257 took 25 us
+  // instead of 26, but 1024 bf16 rows of 151,936 62 instead of 54 and 4096 of them 133 instead of 129.
   constexpr int64_t kLeastPart = 8 * kBlock;
   const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
   int64_t parts = 1, per = (nv + kBlock - 1) / kBlock * kBlock;
@@ -910,7 +938,7 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
     if (per <= 2 * kLeastPart && nv <= 64 * kLeastPart) per = kLeastPart;
     parts = (nv + per - 1) / per;
   }
-  const int64_t part_cap = a->k > 0 ? a->k + 16 + a->k / 4 : 0;   // a part seldom has more (see gather_one), and is thinned then
+  const int64_t part_cap = a->k > 0 ? a->k + 16 + a->k / 4 : 0;   // a part seldom has more, and is thinned then
   const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(n_rows) * parts * part_cap : 0;
   const size_t sums = parts > 1 ? sizeof(ScorePart) * static_cast<size_t>(n_rows) * parts + 16 : 0;
   if (parts > 1) {
@@ -992,7 +1020,8 @@ int score_bwd(pcp_ctx* ctx, const pcp_score_bwd_args* a) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a->logits), d = reinterpret_cast<uintptr_t>(a->dlogits);
     const uintptr_t xn = static_cast<uintptr_t>(extent) * dtype_bytes(a->logits_dtype);
     const uintptr_t dn = static_cast<uintptr_t>(dextent) * dtype_bytes(a->dlogits_dtype);
-    const bool same = x == d && a->logits_dtype == a->dlogits_dtype && t.row_stride == t.drow_stride && t.seq_stride == t.dseq_stride;
+    const bool same = x == d && a->logits_dtype == a->dlogits_dtype && t.row_stride == t.drow_stride &&
+                      t.seq_stride == t.dseq_stride;
     if (extent > 0 && !same && x < d + dn && d < x + xn)
       return fail(ctx, PCP_ERR_INVALID_ARG, "dlogits overlap the logits without being the same rows");
   }

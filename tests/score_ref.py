@@ -8,10 +8,10 @@ The logarithm of the sum is therefore off by less than 5e-6 + 2^-23 H, the entro
 temperature (at most H), by as much of itself and 2^-24 more: REL = 1e-5 of (1 + 2 H) covers them. Outputs are
 rounded to f32 once.
 
-Backward. dz = p (A + B d): p from the given row_max and log_sum has the relative error of d, (2^-24 |d| for the fma, for k2, for
-log_sum's product with log2 e and for its rounding, natural units: 2^-22 |log p| and 2^-22 |log_sum|), and 2^-23 for the exponential;
-the products and sums 2^-22 of the terms' magnitudes; the forward's errors of log_sum (REL) and of the entropy (REL (1 + 2 H)
-dentropy p) add. A result rounded to 16 bits moves by half a step.
+Backward. dz = p (A + B d): p from the given row_max and log_sum has the relative error of d, (2^-24 |d| for the fma,
+for k2, for log_sum's product with log2 e and for its rounding, natural units: 2^-22 |log p| and 2^-22 |log_sum|), and
+2^-23 for the exponential; the products and sums 2^-22 of the terms' magnitudes; the forward's errors of log_sum (REL) and of
+the entropy (REL (1 + 2 H) dentropy p) add. A result rounded to 16 bits moves by half a step.
 """
 import numpy as np
 
