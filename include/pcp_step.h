@@ -79,7 +79,8 @@ int pcp_grad_stats_compute_many(pcp_ctx* ctx, int n_tensors, const float* const*
  * element's address. Every out[i] is either grads[i] in the same type (in place) or overlaps
  * no gradient and no other output. A gradient may stand in the list twice where there is no
  * output. Synchronous unless PCP_FLAG_ASYNC is set. The call allocates no device memory, and can be
- * captured in a HIP graph, with the pointers that it was given. */
+ * captured in a HIP graph, with the pointers that it was given. It uses a part of the context's
+ * memory: calls (and replayed graphs) that may overlap need separate contexts. */
 typedef enum {
   PCP_NORM_L2 = 0,
   PCP_NORM_MAX = 1
@@ -147,8 +148,8 @@ int pcp_nesterov_update_flat(pcp_nesterov* opt, float* params, const float* grad
  *
  * The arrays are host memory, read during the call. params[i], velocities[i] and param_copies[i]
  * overlap nothing else in the lists. Synchronous unless PCP_FLAG_ASYNC is set. The call allocates
- * no device memory, and can be captured in a HIP graph, with the pointers that it was given.
- * pcp_nesterov_velocity gives the place of an optimizer's velocities, so that its tensors can be
+ * no device memory and uses none of the context's, and can be captured in a HIP graph, with the
+ * pointers that it was given. pcp_nesterov_velocity gives the place of an optimizer's velocities, so that its tensors can be
  * updated in this way too and still be serialized. */
 typedef struct pcp_nesterov_many_args {
   int64_t n_tensors;            /* 0 .. PCP_GRAD_MAX_TENSORS                              */

@@ -124,7 +124,8 @@ int collect_device_errors(pcp_ctx* ctx) {
     return fail(ctx, PCP_ERR_INVALID_ARG, "a row uses one teacher id twice");
   if (h & kErrDraftLen)
     return fail(ctx, PCP_ERR_INVALID_ARG, "a sequence's draft length is outside [0, n_draft]");
-  return fail(ctx, PCP_ERR_NONFINITE, "a live row has a non-finite log-sum-exp (NaN/Inf logits)");
+  return fail(ctx, PCP_ERR_NONFINITE, "a live row has a non-finite log-sum-exp (NaN/Inf logits), or a gradient or its "
+                                      "norm is not finite");
 }
 
 // Work buffers of pcp_grpo_loss_fwd_bwd_noalloc: one array per GPU, which holds it

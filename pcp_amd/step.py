@@ -16,8 +16,8 @@ import numpy as np
 import torch
 
 from . import _tensors
-from ._lib import (DType, FLAG_ASYNC, GradClipArgs, GradStats, NesterovManyArgs, NesterovMode, NormType, PcpError, VerifyArgs,
-                   check, lib)
+from ._lib import (DType, FLAG_ASYNC, GradClipArgs, GradStats, NesterovManyArgs, NesterovMode, NormType, PcpError,
+                   VerifyArgs, check, lib)
 from .grpo import _TORCH_DTYPE, Context, _ptr, _stream_handle, call_scope, default_context, dtype_code
 
 
@@ -102,6 +102,7 @@ def grad_norm(grads, max_norm: float = float("inf"), *, norm_type: int | str = N
     that brings it down to max_norm, both left on the device (pcp_grad_clip without outputs): norm_type "l2" or "max".
     ``Nesterov.update_many`` and ``nesterov_update_many`` take the coefficient there. A norm that is not finite is
     reported, and its coefficient is NaN. sync=False only enqueues. An empty list needs a ctx or outputs."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     return _grad_clip(grads, max_norm, norm_type, None, outputs, sync, stream, ctx)
 
 
@@ -116,7 +117,6 @@ def clip_grads(grads, max_norm: float, *, norm_type: int | str = NormType.l2, ou
 
 
 def _grad_clip(grads, max_norm, norm_type, out, outputs, sync, stream, ctx) -> GradNorm:
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if isinstance(norm_type, str):
         try:
             norm_type = NormType[norm_type]

@@ -64,7 +64,7 @@ def check_scores(x, ids, out, tau, k, live=None):
 SHAPES = [("f32", 1, 1, 1), ("bf16", 3, 7, 7), ("f16", 5, 64, 64), ("f32", 4, 255, 20), ("bf16", 6, 1000, 256),
           ("bf16", 2, 1003, 65), ("f32", 3, 8191, 128), ("bf16", 5, 16385, 256), ("f16", 2, 50257, 33),
           ("f32", 2, 50257, 256), ("bf16", 1, 151936, 20), ("bf16", 300, 16000, 8), ("f32", 511, 9000, 3),
-          ("f32", 512, 9000, 3), ("bf16", 513, 20000, 1), ("bf16", 2, 262144, 256), ("f16", 2049, 4096, 64)]
+          ("f32", 512, 9000, 3), ("bf16", 513, 20000, 1), ("bf16", 2, 262144, 256), ("f16", 2049, 4096, 64), ("f32", 515, 151936, 30)]
 
 
 @pytest.mark.parametrize("dtype,R,V,k", SHAPES)
@@ -169,6 +169,22 @@ def test_layout_masks_and_ignored_tokens(mask_dtype, S, T, V, k, shift):
     check_scores(x[:, :rows].reshape(S * rows, V), ids[:, sel].reshape(-1), part, 1.0, k, live)
     for t in (out.logp, out.entropy, out.row_max, out.log_sum) + ((out.top_logp, out.top_ids) if k else ()):
         assert (t[:, :off] == 7).all() and (t[:, off + rows:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype,R,V,k", [("bf16", 1, 1 << 24, 40), ("f32", 520, 600000, 70), ("f16", 3, 5000001, 256)])
+def test_long_rows(dtype, R, V, k):
+    """Groups of several batches a lane, and the largest vocabulary; a few rows are checked."""
+    g = torch.Generator(device=DEV).manual_seed(R)
+    x = torch.empty((R, V), dtype=DT[dtype], device=DEV)
+    for r in range(R):
+        x[r] = (torch.randn(V, generator=g, device=DEV) * 2).to(DT[dtype])
+    x[:, V // 3] = 11.0
+    x[:, V - 1] = 10.5
+    ids = torch.randint(0, V, (R, 1), generator=g, device=DEV)
+    out = scores.token_scores(x[:, None], ids, k=k)
+    picked = sorted({0, R // 2, R - 1})
+    check_scores(x[picked], ids[picked, 0].cpu().numpy(), scores.TokenScores(*(t[picked] for t in (
+        out.logp, out.entropy, out.row_max, out.log_sum, out.top_logp, out.top_ids))), 1.0, k)
 
 
 def test_views_and_entropy_alone():
