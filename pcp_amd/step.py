@@ -130,7 +130,6 @@ def _grad_clip(grads, max_norm, norm_type, out, outputs, sync, stream, ctx) -> G
     device = _one_device(g, o, e)
     ctx = ctx or default_context(max(device, 0))
     a = GradClipArgs()
-    lib().pcp_grad_clip_args_init(ctypes.byref(a))
     with call_scope.of_described(ctx, stream, device, grads, () if out is None or out is grads else out, given) as handle:
         if outputs is None:
             both = torch.empty(2, dtype=torch.float32, device=torch.device("cuda", ctx.device))
@@ -187,7 +186,6 @@ def _update_many(ctx, params, v, velocities, grads, copies, coef, learning_rate,
     device = _one_device(g, p, v if velocities is not None else None, c, e)
     ctx = ctx or default_context(max(device, 0))
     a = NesterovManyArgs()
-    lib().pcp_nesterov_many_args_init(ctypes.byref(a))
     with call_scope.of_described(ctx, stream, device, params, velocities or (), grads, copies or (), scale) as handle:
         a.n_tensors, a.counts, a.params, a.grads, a.dtypes = len(grads), g[1], p[0], g[0], g[2]
         a.velocities = v if velocities is None else v[0]

@@ -268,3 +268,33 @@ def test_reference_gradient_against_differences(tau):
         assert abs((f(hi) - f(lo)) / 2e-5 - g[r, v]) < 1e-8
     m, log_sum, log_p = softmax_parts(x, tau)
     assert np.allclose(np.exp(log_p).sum(1), 1) and (entropy_of(log_p) <= np.log(9) + 1e-12).all()
+
+
+def test_overlaps_are_found_in_any_order():
+    """Random lists of ranges, rising or shuffled, against every pair of them."""
+    rng = np.random.default_rng(11)
+    L = _lib.lib()
+    seen = set()
+    for turn in range(400):
+        n = int(rng.integers(1, 6))
+        counts = rng.integers(0, 6, n)
+        room = int(rng.choice([60, 400, 4000]))
+        cols = {k: rng.integers(1, room, n) * 4 + 0x1000 for k in ("params", "velocities", "grads", "param_copies")}
+        if turn % 2:                                       # pieces of flat buffers, at times one over another
+            base = 0x1000
+            for k in cols:
+                cols[k] = base + np.concatenate([[0], np.cumsum(counts[:-1])]) * 4
+                base += int(counts.sum()) * 4 - (8 if rng.random() < 0.2 else 0)
+        size = {"params": 4, "velocities": 4, "grads": 4, "param_copies": 2}
+        spans = [(int(cols[k][i]), int(cols[k][i]) + int(counts[i]) * size[k], k != "grads")
+                 for k in cols for i in range(n) if counts[i]]
+        meet = any(a[0] < b[1] and b[0] < a[1] and (a[2] or b[2]) for i, a in enumerate(spans) for b in spans[:i])
+        keep = lists(n, counts=[int(c) for c in counts], **{k: [int(x) for x in v] for k, v in cols.items()})
+        a = filled(_lib.NesterovManyArgs, "pcp_nesterov_many_args_init")
+        a.n_tensors = n
+        for k, v in keep.items():
+            setattr(a, k, ctypes.addressof(v))
+        assert L.pcp_nesterov_update_many(None, ctypes.byref(a)) == -1
+        assert ("overlaps" if meet else "context is NULL") in L.pcp_last_error(None).decode(), (spans, meet)
+        seen.add((turn % 2, meet))
+    assert len(seen) == 4
