@@ -17,8 +17,9 @@ struct HostStager;
 }
 
 namespace pcp {
-// Rows of token scores that several workgroups may share, and workgroups of a gradient norm.
-constexpr int kScoreTickets = 512;
+// Token scores of fewer rows than this may share a row between workgroups (a ticket each), about as many of those in all: the
+// CUs; and workgroups of a gradient norm.
+constexpr int kScoreTickets = 256;
 constexpr int kNormBlocks = 16384;
 constexpr int kNormGroups = 32, kNormApart = 16;   // its tickets: one for all and one a group, 64 bytes apart
 

@@ -12,7 +12,7 @@
 // Bound by HBM with many rows, and by their last ones: 4096 rows of 151,936 bf16 187 us (6.7 TB/s, 65% of the VALU's
 // time), with 5/8 of them live 128 (6.1 TB/s), with k = 20 204 and 139. By latency with few: one row 6.4 us, with
 // k = 20 11.1 (meta data 0.4, the pass 1.6, sums 0.6, candidates 2.3, stores and ticket 1.0, merge 3, ranking 1); 64
-// f32 rows 16 and with k = 5 20. Rows of masks with fewer than k tokens left take one more pass (4096 such rows
+// f32 rows 12 and with k = 5 17. Rows of masks with fewer than k tokens left take one more pass (4096 such rows
 // 408 us; by select_exact, as first written, 2097), rows of a few equal values six (select_exact).
 //
 // Backward: one read of the logits, one write (or update) of dlogits, elementwise from the forward's
@@ -923,19 +923,21 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
   hipStream_t st = static_cast<hipStream_t>(a->stream);
 
-  // Workgroups per row: few rows' logits are dealt to about 1024 in all, kLeastPart vectors (a batch) each or more. us for
-  // 2048 workgroups in all | 1024 | 1024 of half a batch:
-  //   one bf16 row of 151,936, k 20   12.2 | 12.1 | 19.4     64 f32 rows of 151,936, k 0   16.3 | 14.8 | 15.0
-  //   200 bf16 rows, k 0              22.3 | 18.2 | 18.5     400 bf16 rows of 50,257, k 0  16.1 | 15.4 | 15.9
-  // From kScoreTickets rows on each has one workgroup: dealt to 4096 or 8192 in all, 1520 f16 rows of 50,257 took 25 us
-  // instead of 26, but 1024 bf16 rows of 151,936 62 instead of 54 and 4096 of them 133 instead of 129.
-  constexpr int64_t kLeastPart = 8 * kBlock;
+  // Workgroups per row: about one on each CU in all, so that few wait for the ticket at a time, and a batch (kLeastPart vectors) each
+  // or more. us with 1024 workgroups in all | 512 | 256, by then of several batches each:
+  //   64 f32 rows of 151,936, k 0   16.0 | 12.7 | 12.0     k 5   19.8 | 18.3 | 17.0     100 bf16 rows, k 0   12.4 | 12.8 | 14.4
+  //   200 bf16 rows                 18.8 | 19.1 | 18.3           27.5 | 25.9 | 24.2     500 bf16 rows        36.3 | 34.8 | 31.9
+  // Half a batch each took one bf16 row of 151,936 with k = 20 from 12 to 19 us. 1520 f16 rows of 50,257 in 8192 took 25 us for 26,
+  // but 1024 bf16 rows of 151,936 62 for 54 and 4096 of them 133 for 129.
+  constexpr int64_t kLeastPart = kU * kBlock;
   const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
   int64_t parts = 1, per = (nv + kBlock - 1) / kBlock * kBlock;
   if (n_rows < kScoreTickets && nv > kLeastPart) {   // (a ticket per row)
-    parts = std::min<int64_t>((1024 + n_rows - 1) / n_rows, 64);   // one wave merges their sums
+    parts = std::min<int64_t>((kScoreTickets + n_rows - 1) / n_rows, 64);   // one wave merges their sums
     per = ((nv + parts - 1) / parts + kBlock - 1) / kBlock * kBlock;
-    if (per <= 2 * kLeastPart && nv <= 64 * kLeastPart) per = kLeastPart;
+    // A part of one batch is gathered from registers: as long as that leaves no CU two.
+    const int64_t ones = (nv + kLeastPart - 1) / kLeastPart;
+    if (per < kLeastPart || (per <= 2 * kLeastPart && ones <= 64 && n_rows * ones <= kScoreTickets)) per = kLeastPart;
     parts = (nv + per - 1) / per;
   }
   const int64_t part_cap = a->k > 0 ? a->k + 16 + a->k / 4 : 0;   // a part seldom has more, and is thinned then

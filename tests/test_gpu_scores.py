@@ -64,7 +64,8 @@ def check_scores(x, ids, out, tau, k, live=None):
 SHAPES = [("f32", 1, 1, 1), ("bf16", 3, 7, 7), ("f16", 5, 64, 64), ("f32", 4, 255, 20), ("bf16", 6, 1000, 256),
           ("bf16", 2, 1003, 65), ("f32", 3, 8191, 128), ("bf16", 5, 16385, 256), ("f16", 2, 50257, 33),
           ("f32", 2, 50257, 256), ("bf16", 1, 151936, 20), ("bf16", 300, 16000, 8), ("f32", 511, 9000, 3),
-          ("f32", 512, 9000, 3), ("bf16", 513, 20000, 1), ("bf16", 2, 262144, 256), ("f16", 2049, 4096, 64), ("f32", 515, 151936, 30)]
+          ("f32", 512, 9000, 3), ("bf16", 513, 20000, 1), ("bf16", 2, 262144, 256), ("f16", 2049, 4096, 64), ("f32", 515, 151936, 30), ("f32", 64, 151936, 5), ("bf16", 100, 151936, 33),
+          ("f16", 255, 50257, 17), ("bf16", 128, 32768, 0), ("f32", 3, 600000, 77)]
 
 
 @pytest.mark.parametrize("dtype,R,V,k", SHAPES)
@@ -375,7 +376,7 @@ def test_rows_beside_the_number_of_tickets():
     g = torch.randn(1 << 20, device=DEV)
     want = step.grad_norm(g, ctx=ctx)
     torch.manual_seed(1)
-    for rows in (511, 512, 4096):
+    for rows in (1, 100, 255, 256, 257, 511, 512, 4096):
         x = torch.randn(rows, 1, 20000, device=DEV).to(torch.bfloat16)
         ids = torch.randint(0, 20000, (rows, 1), device=DEV)
         for _ in range(3):
