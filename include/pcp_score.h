@@ -44,8 +44,9 @@ extern "C" {
  *   top     = the k largest logits by falling logit, equal ones by rising id, as log p and id
  * each at index i (top_*: i * k + rank). Rows whose token weighs 0 or is PCP_IGNORE_INDEX
  * have zero outputs and alternatives with the id PCP_IGNORE_INDEX; entries that no row
- * addresses are not written. Tokens of probability 0 add nothing to the entropy. -0 counts as
- * 0; NaN ranks below every number. A finite mask of any size (-1e30, a type's lowest value)
+ * addresses are not written. Tokens of probability 0 add nothing to the entropy. No log-prob is
+ * above 0, no entropy and no log_sum below 0 (of rows that are not reported). -0 counts as 0;
+ * NaN ranks below every number. A finite mask of any size (-1e30, a type's lowest value)
  * is a logit like any other.
  *
  * Reported after the call (or by pcp_sync): a token id outside [0, V) on a row with weight

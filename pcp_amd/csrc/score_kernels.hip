@@ -2,12 +2,12 @@
 // logits, and the gradient of a function of the log-probs and entropies.
 //
 // Forward: one read of a row. With m the largest logit, d = (x - m) log2(e) / temperature, s = sum 2^d and
-// t = sum 2^d d, the log-sum-exp is m / temperature + ln s and the entropy ln s - ln 2 t / s, two parts of one sign, so
-// that nothing cancels where a row has one likely token. A batch of eight 16-byte vectors a lane gives a lane's maximum
-// (two 16-bit elements an instruction), then s and t against it; the next batch's loads are out meanwhile. The
-// alternatives come after the pass: the lanes have kept their groups' maxima, what k of those reach rules out all
-// but about k groups, and these are read again. Few rows are cut into parts, whose sums and candidates the
-// last part to finish merges; there a part is one batch, and its candidates come from its registers.
+// t = sum 2^d d, the log-sum-exp is m / temperature + ln s and the entropy ln s - ln 2 t / s, two parts that are not
+// negative: a row with one likely token keeps its entropy to 2^-24, the rounding of its largest term. A batch of eight
+// 16-byte vectors a lane gives a lane's maximum (two 16-bit elements an instruction), then s and t against it; the next
+// batch's loads are out meanwhile. The alternatives come after the pass: the lanes have kept their groups' maxima, what k
+// of those reach rules out all but about k groups, and these are read again. Few rows are cut into parts, whose sums and
+// candidates the last part to finish merges; there a part is one batch, and its candidates come from its registers.
 //
 // Bound by HBM with many rows, and by their last ones: 4096 rows of 151,936 bf16 187 us (6.7 TB/s, 65% of the VALU's
 // time), with 5/8 of them live 128 (6.1 TB/s), with k = 20 204 and 139. By latency with few: one row 6.4 us, with
@@ -494,11 +494,29 @@ __device__ __forceinline__ void score_merge(float& mx, double& s, double& t, flo
   mx = M;
 }
 
+// ln s, s >= 1, to 2^-24 and near 1 to a few 2^-24 of itself: s = 2^k m with m in [1/sqrt 2, sqrt 2), of which f32 has the
+// logarithm of the nearest f32 f, and (m - f) / f is added. f64's logarithm took 0.9 us more of the 30 of 1520 f16 rows of
+// 50,257 with k = 8.
+__device__ __forceinline__ double score_log(double s) {
+  int k = __builtin_amdgcn_frexp_exp(s);
+  double m = __builtin_amdgcn_frexp_mant(s);
+  if (m < 0.70710678118654752440) {
+    m += m;
+    k -= 1;
+  }
+  const float f = static_cast<float>(m), rest = static_cast<float>(m - static_cast<double>(f));
+  return static_cast<double>(k) * kLn2d + static_cast<double>(logf(f) + rest * __builtin_amdgcn_rcpf(f));
+}
+
 // A row's outputs: the alternatives by the threads that rank them, the rest by thread 0.
 template <bool TOP>
 __device__ __forceinline__ void score_write(const ScoreArgs& a, const ScoreRow& r, float token, Shared& sh, int n, float mx,
                                             double s, double t) {
-  const double log_sum = ms_lse(0.f, static_cast<float>(s));
+  // The largest logit's own term is 1 and no exponent is above 0. Rounding misses either by 2^-24, and a row of one
+  // likely token would have a positive log-prob and a negative entropy. (NaN, and a sum of 0, stay and are reported.)
+  if (s > 0. && s < 1.) s = 1.;
+  if (t > 0.) t = 0.;
+  const double log_sum = score_log(s);
   auto log_p = [&](float x) {
     return static_cast<float>((static_cast<double>(x) - static_cast<double>(mx)) * a.inv_tau - log_sum);
   };
