@@ -338,8 +338,8 @@ __device__ __forceinline__ int select_exact(const char* xrow, const RowSpan& sp,
 }
 
 // The candidates of a part where fewer than k values lie above masks: those, and of the masked ones, if all are
-// equal, the first k elements of the part (at least as many as are missing are among them). Called by the whole
-// workgroup; ends with a barrier.
+// equal, the first k elements of the part (at least as many as are missing are among them, unless some are NaN). Called by
+// the whole workgroup; ends with a barrier.
 template <typename TI>
 __device__ __forceinline__ int gather_masked(const char* xrow, const RowSpan& sp, __amdgpu_buffer_rsrc_t xbuf, int v0, int end,
                                              bool edges, int k, Shared& sh) {
@@ -394,7 +394,7 @@ __device__ __forceinline__ int gather_masked(const char* xrow, const RowSpan& sp
   __syncthreads();
   const int n = sh.count;
   __syncthreads();
-  return n <= kCap && !(lo < hi) ? n : select_exact<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
+  return n >= min(k, total) && n <= kCap && !(lo < hi) ? n : select_exact<TI>(xrow, sp, xbuf, v0, end, edges, k, sh);
 }
 
 // The candidates of a part whose lanes have left their groups' largest logits (batches: batches per group, groups:
