@@ -169,7 +169,8 @@ struct ScoreSums {
 };
 
 // The largest element of a batch, two 16-bit ones an instruction. bf16 values compare as 16-bit integers where one is
-// positive; a lane that holds negative ones alone (or none) makes its wave look again.
+// positive; a lane that holds negative ones alone (or none), or a NaN, which is above all as an integer, makes its wave
+// look again.
 template <typename TI, int U, typename Held>
 __device__ __forceinline__ float batch_max(const u32x4 (&x)[U], Held held) {
   typedef short i16x2 __attribute__((ext_vector_type(2)));
@@ -186,8 +187,8 @@ __device__ __forceinline__ float batch_max(const u32x4 (&x)[U], Held held) {
         }
       }
     const uint32_t t = __builtin_bit_cast(uint32_t, top);
-    m = fmaxf(__uint_as_float(t << 16), __uint_as_float(t & 0xffff0000u));
-    if (!__any(top[0] < 0 && top[1] < 0)) return m;
+    const float even = __uint_as_float(t << 16), odd = __uint_as_float(t & 0xffff0000u);
+    if (!__any((top[0] < 0 && top[1] < 0) || __builtin_isunordered(even, odd))) return fmaxf(even, odd);
     m = kNegInf;
 #pragma unroll
     for (int q = 0; q < U; ++q) m = held(q) ? vec_max<TI>(m, x[q]) : m;

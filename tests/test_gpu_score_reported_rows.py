@@ -10,6 +10,8 @@ from pcp_amd._lib import PcpError
 pytestmark = pytest.mark.gpu
 
 DEV = torch.device("cuda:0")
+QUIET = {"bf16": torch.tensor([0x7fc0, -0x40], dtype=torch.int16), "f16": torch.tensor([0x7e00, -0x200], dtype=torch.int16),
+         "f32": torch.tensor([0x7fc00000, -0x400000], dtype=torch.int32)}
 DT = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
 
 
@@ -58,3 +60,31 @@ def test_every_alternative_of_a_row_of_nan_is_written(dtype, R, V, k, numbers):
     if good.any():
         want = scores.token_scores(x[good][:, None], ids[good], k=k)
         assert torch.equal(out.top_ids[good], want.top_ids)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("R,V,k", [(300, 20003, 5), (300, 20003, 100), (3, 20003, 5), (2, 151936, 77), (20, 50257, 0), (4, 8192, 9)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_nan_hides_no_number(dtype, R, V, k, sign):
+    """A NaN of either sign a few elements from the largest logits, which mostly are the same lane's: they are found all the same."""
+    rng = np.random.default_rng(R + V + k)
+    x = rng.standard_normal((R, V)).astype(np.float32) * 3
+    rows = np.arange(R)
+    at = rng.integers(0, V - 32, R)
+    for step in (2, 4, 6):             # distinct logits, all above the rest, at places of the same parity
+        x[rows, at + step] = 40 + step
+    d = torch.from_numpy(x).to(DT[dtype])
+    for i in (at, at + 12):            # by their bits: a conversion may give any NaN
+        d[rows, i] = QUIET[dtype][0 if sign > 0 else 1].view(DT[dtype])
+    assert torch.isnan(d[rows, at]).all()
+    d = d.to(DEV)
+    ctx = grpo.Context(0)
+    out = scores.token_scores(d[:, None], torch.zeros((R, 1), dtype=torch.int64, device=DEV), k=k, sync=False, ctx=ctx)
+    with pytest.raises(PcpError) as e:
+        ctx.sync()
+    assert e.value.code == -4
+    assert torch.isnan(out.entropy).all() and torch.isnan(out.log_sum).all()
+    if k:
+        host = d.double().cpu().numpy()
+        order = np.lexsort((np.broadcast_to(np.arange(V), host.shape), -np.nan_to_num(host, nan=0.0), np.isnan(host)))[:, :k]
+        assert np.array_equal(out.top_ids[:, 0].cpu().numpy(), order)
