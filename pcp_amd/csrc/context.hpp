@@ -17,11 +17,9 @@ struct HostStager;
 }
 
 namespace pcp {
-// Token scores of fewer rows than this may share a row between workgroups (a ticket each), about as many of those in all: the
-// CUs; and workgroups of a gradient norm.
-constexpr int kScoreTickets = 256;
+// Most workgroups of a gradient norm, and its tickets: one for all and one a group, 64 bytes apart.
 constexpr int kNormBlocks = 16384;
-constexpr int kNormGroups = 32, kNormApart = 16;   // its tickets: one for all and one a group, 64 bytes apart
+constexpr int kNormGroups = 32, kNormApart = 16;
 
 // What kernels hand back to the host: one pinned, coherent host page per context, written
 // by the device with plain system-scope stores and read by the host after the stream is

@@ -18,6 +18,7 @@
 #include "grpo_device.hpp"
 #include "grpo_launch.hpp"
 #include "pcp_grpo.h"
+#include "score_split.hpp"
 
 namespace pcp {
 

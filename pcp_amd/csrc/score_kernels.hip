@@ -29,6 +29,7 @@
 #include "context.hpp"
 #include "grpo_device.hpp"
 #include "pcp_score.h"
+#include "score_split.hpp"
 #include "top_device.hpp"
 
 namespace pcp {
@@ -216,7 +217,8 @@ __device__ __forceinline__ float batch_max(const u32x4 (&x)[U], Held held) {
 // those reach, k elements reach, each in a group of its own; so only groups that reach it are read again, about
 // k of a row's thousands, and what reaches it there are the candidates, few more than k.
 
-constexpr int kGroups = 16;
+constexpr int kGroups = kScoreGroups;
+static_assert(kBlock == kScoreBlock && kU == kScoreU, "score_split.hpp");
 
 struct PartShared {
   union {
@@ -562,7 +564,7 @@ __global__ void __launch_bounds__(kBlock, 5) score_kernel(ScoreArgs a) {
   __shared__ double wave_s[kWaves], wave_t[kWaves];
   __shared__ float wave_mx[kWaves];
   __shared__ unsigned turn;
-  __shared__ int counts[64];
+  __shared__ int counts[kScoreParts];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t of = blockIdx.x / static_cast<uint32_t>(a.parts);
   const int part = static_cast<int>(blockIdx.x - of * static_cast<uint32_t>(a.parts));
@@ -942,23 +944,8 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   if (scope.error() != hipSuccess) return hip_fail(ctx, scope.error(), "making the context's device current");
   hipStream_t st = static_cast<hipStream_t>(a->stream);
 
-  // Workgroups per row: about one on each CU in all, so that few wait for the ticket at a time, and a batch (kLeastPart vectors) each
-  // or more. us with 1024 workgroups in all | 512 | 256, by then of several batches each:
-  //   64 f32 rows of 151,936, k 0   16.0 | 12.7 | 12.0     k 5   19.8 | 18.3 | 17.0     100 bf16 rows, k 0   12.4 | 12.8 | 14.4
-  //   200 bf16 rows                 18.8 | 19.1 | 18.3           27.5 | 25.9 | 24.2     500 bf16 rows        36.3 | 34.8 | 31.9
-  // Half a batch each took one bf16 row of 151,936 with k = 20 from 12 to 19 us. 1520 f16 rows of 50,257 in 8192 took 25 us for 26,
-  // but 1024 bf16 rows of 151,936 62 for 54 and 4096 of them 133 for 129.
-  constexpr int64_t kLeastPart = kU * kBlock;
-  const int64_t nv = a->vocab * dtype_bytes(a->logits_dtype) / 16;
-  int64_t parts = 1, per = (nv + kBlock - 1) / kBlock * kBlock;
-  if (n_rows < kScoreTickets && nv > kLeastPart) {   // (a ticket per row)
-    parts = std::min<int64_t>((kScoreTickets + n_rows - 1) / n_rows, 64);   // one wave merges their sums
-    per = ((nv + parts - 1) / parts + kBlock - 1) / kBlock * kBlock;
-    // A part of one batch is gathered from registers: as long as that leaves no CU two.
-    const int64_t ones = (nv + kLeastPart - 1) / kLeastPart;
-    if (per < kLeastPart || (per <= 2 * kLeastPart && ones <= 64 && n_rows * ones <= kScoreTickets)) per = kLeastPart;
-    parts = (nv + per - 1) / per;
-  }
+  const ScoreSplit split = score_split(n_rows, a->vocab, dtype_bytes(a->logits_dtype));
+  const int64_t parts = split.parts;
   const int64_t part_cap = a->k > 0 ? a->k + 16 + a->k / 4 : 0;   // a part seldom has more, and is thinned then
   const size_t keys = parts > 1 ? sizeof(uint64_t) * static_cast<size_t>(n_rows) * parts * part_cap : 0;
   const size_t sums = parts > 1 ? sizeof(ScorePart) * static_cast<size_t>(n_rows) * parts + 16 : 0;
@@ -981,9 +968,9 @@ int score_fwd(pcp_ctx* ctx, const pcp_score_args* a) {
   t.k = a->k;
   t.top_i64 = a->top_ids_dtype == PCP_I64;
   t.parts = static_cast<int32_t>(parts);
-  t.per = static_cast<int32_t>(per);
+  t.per = static_cast<int32_t>(split.per);
   t.part_cap = static_cast<int32_t>(part_cap);
-  t.group = static_cast<int32_t>((per + kBlock * kU * kGroups - 1) / (kBlock * kU * kGroups));
+  t.group = split.group;
   const bool timed = prof_begin(ctx, st);
   const hipError_t e = a->logits_dtype == PCP_F32    ? launch_score<F32T>(t, n_rows, st)
                        : a->logits_dtype == PCP_BF16 ? launch_score<BF16T>(t, n_rows, st)

@@ -1,9 +1,10 @@
-"""Token scores where the definition bounds them: signs of peaked rows."""
+"""Token scores where the definition bounds them: signs of peaked rows, the smallest vocabularies."""
 import numpy as np
 import pytest
 import torch
 
 from pcp_amd import scores
+from score_ref import bars, close, score_ref
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +35,26 @@ def test_signs_of_peaked_rows(dtype, R, V, k, tau, second):
     assert torch.isfinite(out.entropy.sqrt()).all() and not torch.isnan(torch.log1p(-out.logp.exp())).any()
     if k:
         assert (out.top_logp <= 0).all() and torch.equal(out.top_ids[:, 0, 0].long(), ids[:, 0])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32", "f16"])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("R", [1, 300])
+def test_smallest_vocabularies(dtype, offset, R):
+    """Rows without a whole 16-byte vector, or with one or two: every k there is."""
+    rng = np.random.default_rng(R)
+    for V in range(1, 19):
+        host = torch.from_numpy(rng.standard_normal((R, V)) * 3).to(DT[dtype])
+        buf = torch.empty(R * V + offset, dtype=DT[dtype], device=DEV)
+        x = buf[offset:].view(R, V)
+        x.copy_(host)
+        ids = rng.integers(0, V, R)
+        for k in range(V + 1):
+            out = scores.token_scores(x[:, None], torch.from_numpy(ids[:, None]).to(DEV), k=k)
+            logp, h, m, log_sum, tlp, tid = score_ref(host.double().numpy(), ids, 1.0, k)
+            for got, want, bar in ((out.logp, logp, bars(h)), (out.entropy, h, bars(h)), (out.log_sum, log_sum, bars(h)),
+                                   (out.row_max, m, 0.0)):
+                close(got.cpu().numpy()[:, 0], want, bar)
+            if k:
+                assert np.array_equal(out.top_ids.cpu().numpy()[:, 0], tid), (V, k)
+                close(out.top_logp.cpu().numpy()[:, 0], tlp, bars(h)[:, None])
