@@ -77,10 +77,11 @@ int pcp_grad_stats_compute_many(pcp_ctx* ctx, int n_tensors, const float* const*
  *
  * The arrays are host memory, read during the call; what they point to is device memory, at any
  * element's address. Every out[i] is either grads[i] in the same type (in place) or overlaps
- * no gradient and no other output. A gradient may stand in the list twice where there is no
- * output. Synchronous unless PCP_FLAG_ASYNC is set. The call allocates no device memory, and can be
- * captured in a HIP graph, with the pointers that it was given. It uses a part of the context's
- * memory: calls (and replayed graphs) that may overlap need separate contexts. */
+ * no gradient and no other output; norm and coef are outputs too. A gradient may stand in the
+ * list twice where there is no out. Synchronous unless PCP_FLAG_ASYNC is set. The call allocates
+ * no device memory, and can be captured in a HIP graph, with the pointers that it was given. It
+ * uses a part of the context's memory: calls (and replayed graphs) that may overlap need separate
+ * contexts. */
 typedef enum {
   PCP_NORM_L2 = 0,
   PCP_NORM_MAX = 1

@@ -565,6 +565,15 @@ int grad_clip(pcp_ctx* ctx, const pcp_grad_clip_args* a) {
     if (misaligned(a->grads[i], dtype_bytes(from)) || (a->out && misaligned(a->out[i], dtype_bytes(to))))
       return fail(ctx, PCP_ERR_INVALID_ARG, "pointers must be aligned to their element size");
   }
+  const uintptr_t norm = reinterpret_cast<uintptr_t>(a->norm), coef = reinterpret_cast<uintptr_t>(a->coef);
+  bool scalars = norm < coef + 4 && coef < norm + 4;
+  if (!a->out)   // (with outputs their ranges are among the lists': below. Gradients may overlap one another here.)
+    for (int64_t i = 0; i < a->n_tensors; ++i) {
+      const uintptr_t g = reinterpret_cast<uintptr_t>(a->grads[i]);
+      const uintptr_t end = g + static_cast<uintptr_t>(a->counts[i]) * dtype_bytes(a->dtypes ? a->dtypes[i] : PCP_F32);
+      scalars = scalars || (norm < end && g < norm + 4 && g < end) || (coef < end && g < coef + 4 && g < end);
+    }
+  if (scalars) return fail(ctx, PCP_ERR_INVALID_ARG, "norm or coef overlaps a gradient, or one the other");
   try {
     const bool meet = a->out && ranges_meet([&](auto add) {
       for (int64_t i = 0; i < a->n_tensors; ++i) {
