@@ -326,22 +326,19 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
-_ext = None
-
-
-def tensors():
-    """The extension that describes lists of tensors (raises if it has not been built for this interpreter and torch)."""
-    global _ext
-    if _ext is None:
-        import torch  # noqa: F401  (whose libraries it needs)
-        try:
-            from . import _tensors
-        except ImportError as e:
-            raise ImportError(
-                "pcp_amd/_tensors.so is missing or of another Python or torch: build it first (make -C pcp_amd/csrc python "
-                "PYTHON=<interpreter>, or __graft_entry__.build())") from e
-        _ext = _tensors
-    return _ext
+def describe(tensors):
+    """What the extension says of a list of tensors (tensor_lists.cpp), which the first call loads and puts in this
+    function's place (raises if it has not been built for this interpreter and torch)."""
+    global describe
+    import torch  # noqa: F401  (whose libraries it needs)
+    try:
+        from . import _tensors
+    except ImportError as e:
+        raise ImportError(
+            "pcp_amd/_tensors.so is missing or of another Python or torch: build it first (make -C pcp_amd/csrc python "
+            "PYTHON=<interpreter>, or __graft_entry__.build())") from e
+    describe = _tensors.describe
+    return describe(tensors)
 
 
 def check(rc: int, ctx=None) -> None:

@@ -19,12 +19,17 @@ struct ScoreSplit {
   int32_t group;   // batches of a group, 1 or more
 };
 
-// Workgroups per row: about one on each CU in all, so that few wait for the ticket at a time, and a batch (kLeastPart vectors) each
-// or more. us with 1024 workgroups in all | 512 | 256, by then of several batches each:
-//   64 f32 rows of 151,936, k 0   16.0 | 12.7 | 12.0     k 5   19.8 | 18.3 | 17.0     100 bf16 rows, k 0   12.4 | 12.8 | 14.4
-//   200 bf16 rows                 18.8 | 19.1 | 18.3           27.5 | 25.9 | 24.2     500 bf16 rows        36.3 | 34.8 | 31.9
-// Half a batch each took one bf16 row of 151,936 with k = 20 from 12 to 19 us. 1520 f16 rows of 50,257 in 8192 took 25 us for 26,
-// but 1024 bf16 rows of 151,936 62 for 54 and 4096 of them 133 for 129.
+// Workgroups per row: about one on each CU in all, so that few wait for the ticket at a time, and a batch (kLeastPart vectors)
+// each or more. us of rows of 151,936 with 1024 workgroups in all | 512 | 256, by then of several batches each:
+//   64 f32 rows     k 0   14.0 | 12.4 | 11.9     k 5   19.4 | 17.8 | 17.1
+//   32 bf16 rows           8.9 |  9.0 |  8.8           12.9 | 12.9 | 14.0
+//   64 bf16 rows          10.5 | 10.4 | 10.1           15.2 | 16.2 | 15.7
+//   100 bf16 rows         11.9 | 12.5 | 14.3           17.5 | 19.3 | 20.5
+//   200 bf16 rows         16.9 | 18.7 | 17.8           25.1 | 25.8 | 24.2
+//   255 bf16 rows         19.6 | 19.6 | 18.4           27.1 | 26.9 | 24.8     (256, one part each: 16.5, 20.8)
+// It suits numbers of rows that divide the CUs; the 300 workgroups of 100 rows and the 510 of 255 leave some CUs one more than
+// others. Half a batch each took one bf16 row of 151,936 with k = 20 from 12 to 19 us. 1520 f16 rows of 50,257 in 8192 took
+// 25 us for 26, but 1024 bf16 rows of 151,936 62 for 54 and 4096 of them 133 for 129.
 inline ScoreSplit score_split(int64_t n_rows, int64_t vocab, int elem_bytes) {
   constexpr int64_t kBlock = kScoreBlock, kLeastPart = kScoreU * kBlock;
   const int64_t nv = vocab * elem_bytes / 16;

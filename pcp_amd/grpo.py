@@ -111,7 +111,7 @@ class call_scope:
 
     @classmethod
     def of_described(cls, ctx: Context, stream, device: int, *lists):
-        """The same for lists of tensors (or None) that ``_tensors.describe`` has found on `device`."""
+        """The same for lists of tensors (or None) that ``_lib.describe`` has found on `device`."""
         if device != ctx.device and device != -3:   # -3: no tensor
             raise PcpError(-1, "tensors on several devices" if device == -2 else
                            f"tensors on {'the CPU' if device < 0 else f'device {device}'}, context on device {ctx.device}")

@@ -91,7 +91,7 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: to
     given = () if o is None else (o.logp if ids is not None else None, o.entropy, o.row_max, o.log_sum,
                                   o.top_logp if k else None, o.top_ids if k else None)
     known = (ids, mask, *given)
-    d = _lib.tensors().describe((logits, *known))
+    d = _lib.describe((logits, *known))
     _contiguous(d)
     with call_scope.of_described(ctx, stream, d[4], (logits, *known)) as handle:
         if o is None:
@@ -99,7 +99,7 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: to
                             made(S, TS, k) if k else None,
                             torch.zeros((S, TS, k), dtype=top_ids_dtype, device=logits.device) if k else None)
             known = (ids, mask, o.logp, o.entropy, o.row_max, o.log_sum, o.top_logp, o.top_ids)
-            d = _lib.tensors().describe((logits, *known))
+            d = _lib.describe((logits, *known))
         else:
             # (Optional ones may be None: but logp with ids, and the alternatives with k.)
             f32, top = _F32, int(_TORCH_DTYPE.get(top_ids_dtype, -2))
@@ -149,7 +149,7 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: to
     a.row_stride, a.seq_stride = _row_strides(logits)
     ctx = ctx or default_context(logits.device.index or 0)
     known = (logits, ids, mask, row_max, log_sum, entropy, dlogp, dentropy)
-    d = _lib.tensors().describe((*known, dlogits))
+    d = _lib.describe((*known, dlogits))
     _contiguous(d, len(known))
     counts, kinds = memoryview(d[1]).cast("q").tolist(), memoryview(d[2]).cast("i").tolist()
     if counts[3:5] != [S * TS] * 2 or any([n != S * TS and n != -1 for n in counts[5:8]]):

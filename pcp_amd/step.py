@@ -15,8 +15,9 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
+from . import _lib
 from ._lib import (DType, FLAG_ASYNC, GradClipArgs, GradStats, NesterovManyArgs, NesterovMode, NormType, PcpError,
-                   VerifyArgs, check, lib, tensors as _tensors)
+                   VerifyArgs, check, lib)
 from .grpo import _TORCH_DTYPE, Context, _ptr, _stream_handle, call_scope, default_context, dtype_code
 
 
@@ -67,8 +68,8 @@ class GradNorm:
 
 
 def _described(tensors, what: str, dtype: DType | None = None):
-    """What ``_tensors.describe`` says of a list, its tensors contiguous and, with dtype, of that type (or None)."""
-    d = _tensors().describe(tensors)
+    """What ``_lib.describe`` says of a list, its tensors contiguous and, with dtype, of that type (or None)."""
+    d = _lib.describe(tensors)
     if 0 in d[3]:
         raise PcpError(-1, f"{what} must be contiguous")
     if dtype is not None and d[2] != _code(dtype) * len(tensors):
