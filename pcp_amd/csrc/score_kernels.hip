@@ -9,14 +9,14 @@
 // of those reach rules out all but about k groups, and these are read again. Few rows are cut into parts, whose sums and
 // candidates the last part to finish merges; there a part is one batch, and its candidates come from its registers.
 //
-// Bound by HBM with many rows, and by their last ones: 4096 rows of 151,936 bf16 187 us (6.7 TB/s, 65% of the VALU's
-// time), with 5/8 of them live 128 (6.1 TB/s), with k = 20 204 and 139. By latency with few: one row 6.4 us, with
+// Bound by HBM with many rows, and by their last ones: 4096 rows of 151,936 bf16 192 us (6.5 TB/s, 65% of the VALU's
+// time), with 5/8 of them live 126 (6.2 TB/s), with k = 20 207 and 139. By latency with few: one row 7.9 us, with
 // k = 20 11.1 (meta data 0.4, the pass 1.6, sums 0.6, candidates 2.3, stores and ticket 1.0, merge 3, ranking 1); 64
 // f32 rows 12 and with k = 5 17. Rows of masks with fewer than k tokens left take one more pass (4096 such rows
-// 408 us; by select_exact, as first written, 2097), rows of a few equal values six (select_exact).
+// 393 us; by select_exact, as first written, 2097), rows of a few equal values six (select_exact, 2490).
 //
 // Backward: one read of the logits, one write (or update) of dlogits, elementwise from the forward's
-// statistics; 4096 rows of 151,936 bf16, 5/8 of them live, 350 us (5.8 TB/s), added to what was there 399 (5.8).
+// statistics; 4096 rows of 151,936 bf16, 5/8 of them live, 349 us (5.8 TB/s), added to what was there 384 (6.1).
 
 #include <hip/hip_runtime.h>
 
@@ -744,14 +744,15 @@ struct ScoreBwdArgs {
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 typedef u32x2 u32x2_any __attribute__((aligned(2)));
 
-// Groups per lane: 16 bytes of dlogits each, so that 16-bit logits of f32 dlogits come 8 bytes a group. us with 1 | 2 | 4:
-//   bf16 -> f32, 2048 rows of 50,257   142 | 112 | 105        f32 -> f32, 1024 rows of 151,936   197 | 172 | 183
-//   bf16 -> bf16, 4096 rows of 151,936 452 | 350 | 354, added 432 | 399 | 414
+// Groups per lane: 16 bytes of dlogits each, so that 16-bit logits of f32 dlogits come 8 bytes a group. us with 1 | 2 | 4, 5/8
+// of the rows live:
+//   bf16 -> f32, 2048 rows of 50,257   142 | 112 | 104        f32 -> f32, 1024 rows of 151,936   209 | 169 | 176
+//   bf16 -> bf16, 4096 rows of 151,936 466 | 349 | 347, added 427 | 384 | 410
 template <typename TI, typename TO>
 constexpr int grad_unroll() { return TI::kBytes == 2 && TO::kBytes == 4 ? 4 : 2; }
 
-// Stores at system scope (sc0 sc1), which suit the whole-model updates, took 400 us for 399 here and, on rows off 16
-// bytes, 87 for 68. A row's gradient is one pass: dz = p (A + B d) with d = (x - m) k2 - log2 sum, p = 2^d, and the token's
+// Stores at system scope (sc0 sc1), which suit the whole-model updates, took as long here and, on rows off 16 bytes, 87 us
+// for 68. A row's gradient is one pass: dz = p (A + B d) with d = (x - m) k2 - log2 sum, p = 2^d, and the token's
 // own term.
 template <typename TI, typename TO, bool ACC>
 __global__ void __launch_bounds__(kBlock) score_grad_kernel(ScoreBwdArgs a) {
