@@ -326,10 +326,10 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
-def describe(tensors):
-    """What the extension says of a list of tensors (tensor_lists.cpp), which the first call loads and puts in this
-    function's place (raises if it has not been built for this interpreter and torch)."""
-    global describe
+def _load_tensors():
+    """The extension of tensor_lists.cpp, whose functions take the place of `describe` and `fit` (raises if it has not been
+    built for this interpreter and torch)."""
+    global describe, fit
     import torch  # noqa: F401  (whose libraries it needs)
     try:
         from . import _tensors
@@ -337,8 +337,18 @@ def describe(tensors):
         raise ImportError(
             "pcp_amd/_tensors.so is missing or of another Python or torch: build it first (make -C pcp_amd/csrc python "
             "PYTHON=<interpreter>, or __graft_entry__.build())") from e
-    describe = _tensors.describe
-    return describe(tensors)
+    describe, fit = _tensors.describe, _tensors.fit
+    return _tensors
+
+
+def describe(tensors):
+    """(addresses, counts, types, contiguous, device) of a list of tensors."""
+    return _load_tensors().describe(tensors)
+
+
+def fit(tensors, *sizes):
+    """Whether every tensor of a list (None among them) has those sizes."""
+    return _load_tensors().fit(tensors, *sizes)
 
 
 def check(rc: int, ctx=None) -> None:

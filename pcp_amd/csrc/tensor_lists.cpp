@@ -78,8 +78,43 @@ PyObject* describe(PyObject*, PyObject* arg) {
   return result;
 }
 
+// fit(tensors, sizes...) -> whether every tensor of a list (None among them) has those sizes.
+PyObject* fit(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  constexpr Py_ssize_t kMost = 8;
+  if (n_args < 1 || n_args - 1 > kMost) {
+    PyErr_SetString(PyExc_TypeError, "fit(tensors, sizes...) of at most 8 dimensions");
+    return nullptr;
+  }
+  int64_t sizes[kMost];
+  for (Py_ssize_t i = 1; i < n_args; ++i) {
+    sizes[i - 1] = PyLong_AsLongLong(args[i]);
+    if (sizes[i - 1] == -1 && PyErr_Occurred()) return nullptr;
+  }
+  PyObject* seq = PySequence_Fast(args[0], "a list or tuple of tensors is wanted");
+  if (!seq) return nullptr;
+  bool fits = true, fine = true;
+  try {
+    for (Py_ssize_t i = 0; fits && i < PySequence_Fast_GET_SIZE(seq); ++i) {
+      PyObject* const o = PySequence_Fast_GET_ITEM(seq, i);
+      if (o == Py_None) continue;
+      if (!THPVariable_Check(o)) {
+        PyErr_Format(PyExc_TypeError, "entry %zd is no tensor", i);
+        fine = false;
+        break;
+      }
+      fits = THPVariable_Unpack(o).sizes() == at::IntArrayRef(sizes, n_args - 1);
+    }
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    fine = false;
+  }
+  Py_DECREF(seq);
+  return fine ? PyBool_FromLong(fits) : nullptr;
+}
+
 PyMethodDef methods[] = {
     {"describe", describe, METH_O, "describe(tensors) -> (addresses, counts, types, contiguous, device)"},
+    {"fit", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fit)), METH_FASTCALL, "fit(tensors, sizes...) -> bool"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensors", "Lists of tensors as host arrays.", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};

@@ -16,6 +16,7 @@ from ._lib import DType, PcpError, ScoreArgs, ScoreBwdArgs, check, lib
 from .grpo import _TORCH_DTYPE, Context, call_scope, default_context, dtype_code
 
 _F32 = int(DType.f32)
+_NO_FIT = "outputs do not fit the call: f32 [S, TS], top_logp f32 and top_ids [S, TS, k]"
 
 
 @dataclass
@@ -84,8 +85,11 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: to
         raise PcpError(-1, f"k must be in [0, {min(V, _lib.SCORE_TOP_MAX)}] (got {k})")
     a = ScoreArgs()
     a.row_stride, a.seq_stride = _row_strides(logits)
-    ctx = ctx or default_context(logits.device.index or 0)
     o = outputs
+    if o is not None and not (_lib.fit((o.logp if ids is not None else None, o.entropy, o.row_max, o.log_sum), S, TS)
+                              and (k == 0 or _lib.fit((o.top_logp, o.top_ids), S, TS, k))):
+        raise PcpError(-1, _NO_FIT)
+    ctx = ctx or default_context(logits.device.index or 0)
     if o is None:
         made = lambda *shape: torch.zeros(shape, dtype=torch.float32, device=logits.device)  # noqa: E731
     given = () if o is None else (o.logp if ids is not None else None, o.entropy, o.row_max, o.log_sum,
@@ -110,7 +114,7 @@ def token_scores(logits: torch.Tensor, ids: torch.Tensor | None = None, mask: to
             if n != want or t != types:
                 for i in range(6):
                     if (n[i] != want[i] or t[i] != types[i]) and not (n[i] == -1 and 1 <= i <= 3):
-                        raise PcpError(-1, "outputs do not fit the call: f32 [S, TS], top_logp f32 and top_ids [S, TS, k]")
+                        raise PcpError(-1, _NO_FIT)
         at = memoryview(d[0]).cast("q")
         a.n_seq, a.rows, a.vocab, a.tok_seq_stride, a.tok_offset = S, rows, V, TS, tok_offset
         kinds = memoryview(d[2]).cast("i")
@@ -147,13 +151,13 @@ def token_scores_bwd(logits: torch.Tensor, ids: torch.Tensor | None, row_max: to
         raise PcpError(-2, f"dlogits_dtype is {dlogits_dtype}, the given dlogits are {dlogits.dtype}")
     a = ScoreBwdArgs()
     a.row_stride, a.seq_stride = _row_strides(logits)
-    ctx = ctx or default_context(logits.device.index or 0)
     known = (logits, ids, mask, row_max, log_sum, entropy, dlogp, dentropy)
+    if row_max is None or log_sum is None or not _lib.fit(known[3:], S, TS):
+        raise PcpError(-1, "row_max, log_sum, entropy, dlogp and dentropy must be [S, TS]")
+    ctx = ctx or default_context(logits.device.index or 0)
     d = _lib.describe((*known, dlogits))
     _contiguous(d, len(known))
-    counts, kinds = memoryview(d[1]).cast("q").tolist(), memoryview(d[2]).cast("i").tolist()
-    if counts[3:5] != [S * TS] * 2 or any([n != S * TS and n != -1 for n in counts[5:8]]):
-        raise PcpError(-1, "row_max, log_sum, entropy, dlogp and dentropy must be [S, TS]")
+    kinds = memoryview(d[2]).cast("i").tolist()
     if kinds[3:5] != [_F32, _F32] or any([t != _F32 and t != -1 for t in kinds[5:8]]):
         raise PcpError(-2, "row_max, log_sum, entropy, dlogp and dentropy must be f32")
     with call_scope.of_described(ctx, stream, d[4], known, (dlogits,)) as handle:
