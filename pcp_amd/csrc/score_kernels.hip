@@ -117,7 +117,9 @@ __device__ __forceinline__ void score_rebase(double& s, double& t, float m, floa
 
 // Of a lane: its largest logit mx, and against it the sum s of the terms 2^d, d = (x - mx) k, and the sum t of
 // 2^d d. The sums of a batch are f32 against the rounded product ref of mx and k, whose residue r is
-// taken out once per batch: of terms 2^d it leaves 2^-r s and 2^-r (t - r s).
+// taken out once per batch: of terms 2^d it leaves 2^-r s and 2^-r (t - r s). A batch has 64 terms at most, so that f32 loses
+// less than 4e-6 of them at worst (measured against 64 bits: 2e-7), and f64 would take a conversion and two adds of half the rate
+// per term of a kernel whose VALU is 65% busy; everything above a batch is f64.
 struct ScoreSums {
   float k2, mx;
   double s, t;

@@ -99,9 +99,11 @@ def _one_device(*descriptions) -> int:
 def grad_norm(grads, max_norm: float = float("inf"), *, norm_type: int | str = NormType.l2,
               outputs: GradNorm | None = None, sync: bool = True, stream=None, ctx: Context | None = None) -> GradNorm:
     """The norm of all gradients together (a tensor or a list of them, f32, bf16 and f16 mixed) and the coefficient
-    that brings it down to max_norm, both left on the device (pcp_grad_clip without outputs): norm_type "l2" or "max".
+    that brings it down to max_norm (rounded to f32), both left on the device (pcp_grad_clip without outputs): norm_type "l2"
+    or "max".
     ``Nesterov.update_many`` and ``nesterov_update_many`` take the coefficient there. A norm that is not finite is
-    reported, and its coefficient is NaN. sync=False only enqueues. An empty list needs a ctx or outputs."""
+    reported, and its coefficient is NaN. sync=False only enqueues. An empty list's results are on the
+    ctx's device, or device 0."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     return _grad_clip(grads, max_norm, norm_type, None, outputs, sync, stream, ctx)
 
